@@ -403,8 +403,98 @@ void indexed_moe_bf16(const void* in, const void* w, void* out, const uint32_t* 
 void indexed_moe_f16(const void* in, const void* w, void* out, const uint32_t* idx, int N,
                      int K, int M, int batch, int topk, int num_experts, void* stream);
 /* Synchronizes `stream`, returns and clears the device-side index-error flag
- * (4) raised by moe_align_block_size / the MoE GEMMs. */
+ * (4) raised by moe_align_block_size, the MoE GEMMs and the operators of a
+ * paged cache below. */
 int ubridge_device_error(void* stream);
+
+/* ------------------------------------------------ attention block of a decoder
+ * No counterpart in the reference's quantized-matmul path: the operators its
+ * host runs between those products. */
+/* int8 W8A8 linear: y[m, n] = T((sum_k a[m, k] w[n, k]) sa[m] sw[n] + bias[n]),
+ * x T [M, K] quantized per row by the call (sa = amax / 127, 1 for a row of
+ * zeros; codes rounded to even; a row with an infinity or a NaN gives NaN), w
+ * int8 [N, ld], 16-byte aligned, rows padded with zeros to ld, a multiple of
+ * 128; sw, bias f32 [N] (bias may be NULL); dtype 0 f32, 1 f16, 2 bf16.  K <=
+ * 132104, where the int32 sum stays exact.  Scratch: M (ld + 4) bytes. */
+int ubridge_int8_linear(const void* x, int dtype, const int8_t* w, const float* sw,
+                        const float* bias, void* y, int M, int K, int N, int ld, void* stream);
+
+/* Rotary positions.  q [T, Hq, D] and k [T, Hkv, D] (last dim contiguous,
+ * strides in elements of st per token and sh per head), turned to contiguous
+ * q_out and k_out: pair i (x[i], x[i + rot / 2]), or (x[2 i], x[2 i + 1]) when
+ * interleaved, turns by 2 pi positions[t] turns[i] (turns f64 [rot / 2],
+ * positions int32, or int64 with pos64) and is scaled by factor; elements from
+ * rot on pass through.  inverse: by minus the angle, the gradient.
+ * ubridge_rope_append: q to q_out; the turned k and v [T, Hkv, D] to slot
+ * slots[t] (page slot / S, place slot % S; negative: nowhere) of k_pages and
+ * v_pages [P, Hkv, S, D], page_stride elements apart, k_out unused.  Slots of
+ * one call differ.  cache_dtype is dtype, or 3 (e4m3): x / scale[head],
+ * saturating, k_scale / v_scale f32 [Hkv] or NULL for 1.  rot = 0: no
+ * rotation (positions, turns, and with Hq = 0 q, are not read).  A slot past the
+ * cache raises the flag of ubridge_device_error and is not stored. */
+typedef struct {
+  const void *q, *k, *v;
+  void *q_out, *k_out;
+  const void* positions;
+  const double* turns;
+  void *k_pages, *v_pages;
+  const int64_t* slots;
+  const float *k_scale, *v_scale;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, page_stride;
+  int32_t T, Hq, Hkv, D, rot, interleaved, inverse, pos64, dtype, cache_dtype, P, S;
+  float factor;
+  int32_t pad;
+} UbridgeRopeArgs;
+int ubridge_rope(const UbridgeRopeArgs* args, void* stream);
+int ubridge_rope_append(const UbridgeRopeArgs* args, void* stream);
+
+/* Attention of one new token per sequence over a paged cache.  q [B, Hq, D] f16
+ * or bf16, out [B, Hq, D] contiguous, lse f32 [B, Hq] or NULL; k_pages, v_pages
+ * [P, Hkv, S, D] of q's type or e4m3 (cache_dtype 3), strides in elements of sp
+ * per page, sh per head and ss per slot; tables int32 [B, width], table_stride
+ * apart, lens int32 [B].  Query head i reads kv head i / (Hq / Hkv).  scale is
+ * the factor on q . k, softcap c > 0 makes a score c tanh(x / c), slopes f32
+ * [Hq] add slope (t - (len - 1)), window > 0 keeps the last window tokens,
+ * k_scale / v_scale f32 [Hkv] multiply the stored values (each may be NULL).
+ * D is a multiple of 8 up to 256.  A sequence of length 0 gives zeros and lse
+ * -inf.  A length past width S is cut, a page outside [0, P) gives NaN; both
+ * raise the flag of ubridge_device_error.  Scratch: where a sequence is split,
+ * f32 partial outputs. */
+typedef struct {
+  const void* q;
+  void* out;
+  float* lse;
+  const void *k_pages, *v_pages;
+  const int32_t *tables, *lens;
+  const float *slopes, *k_scale, *v_scale;
+  int64_t q_sb, q_sh, k_sp, k_sh, k_ss, v_sp, v_sh, v_ss, table_stride;
+  int32_t B, Hq, Hkv, D, S, P, width, window, dtype, cache_dtype;
+  float scale, softcap;
+} UbridgePagedDecodeArgs;
+int ubridge_paged_decode(const UbridgePagedDecodeArgs* args, void* stream);
+
+/* Pages of a cache [L, 2, P, page_bytes] (layers, keys / values), counted in refs
+ * int32 [P] and listed by tables int32 [rows, width] (-1: none) with lens int32
+ * [rows] tokens, S to a page.  All state stays on the device.
+ * free: the rows named lose their pages and become empty.
+ * fork: row dst[i], empty, becomes a sample of row src[i]: whole pages are
+ * shared, a part-filled last page is copied to the lowest free page, in the
+ * order of i; new_pages[i] receives it, else -1.  Rows dst differ; a row that is
+ * not empty, out of range or for which no page is left is not changed, gives -1
+ * and raises the flag of ubridge_device_error.  n <= 65535.  Scratch: 12 n bytes.
+ * compact: with u pages in use, the k-th used page from u on moves to the k-th
+ * free page below u, tables and refs with it; n_used[0] = u.  Scratch: 8 P + 8
+ * bytes. */
+typedef struct {
+  void* kv;
+  int32_t *refs, *lens, *tables;
+  int64_t page_bytes;
+  int32_t L, P, S, rows, width, pad;
+} UbridgeKvPool;
+int ubridge_kv_free(const UbridgeKvPool* pool, const int32_t* rows, int n, void* stream);
+int ubridge_kv_fork(const UbridgeKvPool* pool, const int32_t* src, const int32_t* dst, int n,
+                    int32_t* new_pages, void* stream);
+int ubridge_kv_compact(const UbridgeKvPool* pool, int32_t* n_used, void* stream);
 
 /* ------------------------------------------------ name-keyed kernel launch
  * Replaces GcuDevice::get_or_load_func(func, module) (src/gcu_device.rs:160-183,

@@ -22,6 +22,9 @@ enum {
 };
 int ub_set_error(int code, const char* fmt, ...);
 int ub_check_launch(const char* what);
+// Device flag (UB_ERR_*) that kernels raise for an index out of range and
+// ubridge_device_error() reads; null: not available (moe.hip).
+int* ub_error_flag();
 
 // Launch-shape knobs (runtime.cpp): 0 = the automatic shape rule of the
 // launcher that reads it; set through ubridge_tune_set() or, at first use,
@@ -130,7 +133,7 @@ __device__ __forceinline__ uint16_t ub_f32_to_f16(float f) {
   return __half_as_ushort(__float2half_rn(f));
 }
 
-enum { UB_F32 = 0, UB_F16 = 1, UB_BF16 = 2 };
+enum { UB_F32 = 0, UB_F16 = 1, UB_BF16 = 2, UB_E4M3 = 3 };  // (e4m3: cache pages only)
 // GGML type ids.
 enum { UB_Q4_0 = 2, UB_Q8_0 = 8, UB_Q4_K = 12 };
 

@@ -855,24 +855,6 @@ void moe_gemm_launch(int path, const MoeArgs& a, int max_blocks, hipStream_t s) 
   }
 }
 
-// Address of g_device_error on the current device (null: not available).
-int* error_flag() {
-  static std::atomic<int*> cache[64];
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return nullptr;
-  int* p = cache[dev].load(std::memory_order_acquire);
-  if (!p) {
-    void* q = nullptr;
-    if (hipGetSymbolAddress(&q, HIP_SYMBOL(g_device_error)) != hipSuccess) {
-      (void)hipGetLastError();
-      return nullptr;
-    }
-    p = (int*)q;
-    cache[dev].store(p, std::memory_order_release);
-  }
-  return p;
-}
-
 int moe_gemm(const char* nm, int dt, bool q8, void* C, const void* A, const void* B,
              const void* Bscale, const void* bias, const float* tw, const int* sorted,
              const int* eids, const int* ntpp, int M, int K, int N, int E, int tis, int top_k,
@@ -897,10 +879,10 @@ int moe_gemm(const char* nm, int dt, bool q8, void* C, const void* A, const void
   const int max_blocks = (tis + E * (bs - 1)) / bs;
   hipStream_t s = ub_stream(stream);
   const int path = ub_tune(UB_TUNE_MOE_GEMM_PATH);
-  if ((path == 13 || (path == 0 && ub_moe_stream_pays(a, q8))) && ub_moe_stream(a, dt, q8, error_flag(), s))
+  if ((path == 13 || (path == 0 && ub_moe_stream_pays(a, q8))) && ub_moe_stream(a, dt, q8, ub_error_flag(), s))
     return ub_check_launch(nm);
   const int rows = path == 0 ? ub_moe_tile_rows(a, q8) : path == 10 ? 128 : path == 11 ? 64 : path == 12 && q8 ? 32 : 0;
-  if (rows && ub_moe_tile(a, rows, dt, q8, error_flag(), s)) return ub_check_launch(nm);
+  if (rows && ub_moe_tile(a, rows, dt, q8, ub_error_flag(), s)) return ub_check_launch(nm);
   if (dt == UB_BF16) {
     if (q8) moe_gemm_launch<UB_BF16, true>(path, a, max_blocks, s);
     else moe_gemm_launch<UB_BF16, false>(path, a, max_blocks, s);
@@ -1027,6 +1009,24 @@ int grid1(size_t n) { return (int)((n + 255) / 256 < 65536 ? (n + 255) / 256 : 6
 
 }  // namespace
 
+// Address of g_device_error on the current device (null: not available).
+int* ub_error_flag() {
+  static std::atomic<int*> cache[64];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return nullptr;
+  int* p = cache[dev].load(std::memory_order_acquire);
+  if (!p) {
+    void* q = nullptr;
+    if (hipGetSymbolAddress(&q, HIP_SYMBOL(g_device_error)) != hipSuccess) {
+      (void)hipGetLastError();
+      return nullptr;
+    }
+    p = (int*)q;
+    cache[dev].store(p, std::memory_order_release);
+  }
+  return p;
+}
+
 // ======================================================================= ABI
 UB_API int ubridge_device_error(void* stream) {
   int v = 0;
@@ -1037,7 +1037,7 @@ UB_API int ubridge_device_error(void* stream) {
   if (v) {
     const int zero = 0;
     (void)hipMemcpyToSymbol(HIP_SYMBOL(g_device_error), &zero, sizeof(int));
-    ub_set_error(v, "device-side index out of range (expert id / real_token_num)");
+    ub_set_error(v, "device-side index out of range (expert id, real_token_num, or a cache's page, slot, row or length)");
   }
   return v;
 }
