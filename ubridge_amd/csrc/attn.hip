@@ -5,78 +5,516 @@
 //   o = v_scale[h] sum_t softmax(x)[t] v[t],  lse = log sum_t exp(x[t])
 //
 // for each query head, h its key / value head, n the tokens of its sequence.
-// A sequence that sees nothing gives zeros and lse = -inf.  Scores, the
-// running maximum and sum, and the output's sum are f32.
+// A sequence that sees nothing gives zeros and lse = -inf.
+//
+// The work is a stream of the cache (2 D values a token and kv head against 4 D
+// G flops, G query heads to a kv head), so the kernel is shaped for bytes in
+// flight and for an even share of them per CU:
+//
+//  * All query heads of a kv head are taken together, as the 16 columns of MFMA
+//    tiles, so the cache is read once.  Keys and values go from memory
+//    straight into the registers that the MFMAs read: no LDS, no barrier in
+//    the loop, every wavefront walks its own tokens.
+//  * A step is 32 tokens.  Scores are S^T = K Q^T in two 16 x 16 x 32 products
+//    whose rows are dealt so that lane (c, g) ends with head c and the eight
+//    tokens 8 g .. 8 g + 7 -- which is the layout of the second product's right
+//    operand, O^T = V^T P^T over 32 tokens, so the weights never leave their
+//    lane.  A lane reads its eight values rows of V 16 bytes each (8 dims) and
+//    swaps tokens against dims with one byte permute a dword.
+//  * The steps of all (sequence, kv head) rows, whose number only the device
+//    knows, are laid end to end and cut into equal shares, one a workgroup.  A row
+//    inside one share is finished there; a row that is cut leaves f32 partial
+//    sums, which k_join adds in the order of the shares.
+//
+// Numerics.  Scores, the running maximum and sum, and the output's sum are f32.
+// The weights exp(x - m) enter the second product as the sum of two 16-bit
+// numbers (16 bits for bf16, 22 for f16; f16 weights are scaled by 2^14 so that
+// those far below the maximum keep them): one number would cost as much as the
+// output's own rounding, and the products are not what bounds the kernel.
+// e4m3 values are exact in both types.
 #include "common.h"
 
 namespace {
 
-template <int CT>
-__device__ __forceinline__ float ldc(const void* p, long i) {
-  if constexpr (CT == UB_E4M3) return __builtin_amdgcn_cvt_f32_fp8(((const uint8_t*)p)[i], 0);
-  else return ub_load<CT>(p, i);
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr float kInf = __builtin_inff();
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int W = 4;         // wavefronts of a workgroup
+constexpr int kMinSteps = 8;  // of a share
+
+template <int DT>
+__device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
+  if constexpr (DT == UB_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// One workgroup per (sequence, query head): four wavefronts, each a quarter of
-// the tokens, a lane the dims lane, lane + 64, ...
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const f32x2 v = {lo, hi};
+  if constexpr (DT == UB_BF16) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+  } else {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+  }
+}
+template <int DT>
+__device__ __forceinline__ float half_of(uint32_t w, int hi) {
+  if constexpr (DT == UB_BF16) return __uint_as_float(hi ? w & 0xffff0000u : w << 16);
+  else return ub_f16_to_f32((uint16_t)(hi ? w >> 16 : w));
+}
+
+// two e4m3 bytes (the low or the high two of w) as two T
+template <int DT, bool HI>
+__device__ __forceinline__ uint32_t from_e4m3(uint32_t w) {
+  if constexpr (DT == UB_BF16)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.0f, HI));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, HI));
+}
+
+// 8 stored values (element-aligned: gfx950 loads 16 bytes from there)
+template <int CT> struct Raw { typedef uint4 T; static constexpr int B = 2; };
+template <> struct Raw<UB_E4M3> { typedef uint2 T; static constexpr int B = 1; };
+template <int CT>
+__device__ __forceinline__ typename Raw<CT>::T ld8(const uint8_t* p) {
+  typename Raw<CT>::T v;
+  __builtin_memcpy(&v, p, sizeof(v));
+  return v;
+}
 template <int DT, int CT>
-__global__ void __launch_bounds__(256) k_decode(const UbridgePagedDecodeArgs a, int* err) {
-  __shared__ float sm[4], sl[4], so[4][256];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int b = blockIdx.x / a.Hq, hq = blockIdx.x - b * a.Hq, h = hq / (a.Hq / a.Hkv);
-  int n = a.lens[b];
-  if (n > (long)a.width * a.S || (n > 0 && a.P == 0)) {
-    if (tid == 0) *err = UB_ERR_INDEX;
-    n = a.P == 0 ? 0 : a.width * a.S;
+__device__ __forceinline__ uint4 widen(const typename Raw<CT>::T& v) {
+  if constexpr (CT == UB_E4M3)
+    return make_uint4(from_e4m3<DT, false>(v.x), from_e4m3<DT, true>(v.x),
+                      from_e4m3<DT, false>(v.y), from_e4m3<DT, true>(v.y));
+  else
+    return v;
+}
+
+struct Dev {
+  UbridgePagedDecodeArgs a;
+  int G, HG;     // query heads of a kv head; head groups of it (rows of one sequence: Hkv HG)
+  int shares;    // workgroups of k_decode
+  float* po;     // [2 shares][heads of a group][D] partial sums, relative to the maximum
+  float* pml;    // [2 shares][heads of a group][2] maximum (log2) and sum
+  int2* info;    // [B Hkv HG] first share and number of shares of a row
+  int* err;
+};
+
+// tokens [first, n) of sequence b, its steps; lengths past the table are cut
+struct Span { int first, n, steps; };
+__device__ __forceinline__ Span span(const Dev& d, int b) {
+  const UbridgePagedDecodeArgs& a = d.a;
+  Span s;
+  s.n = max(a.lens[b], 0);
+  const int top = a.P == 0 ? 0 : a.width * a.S;
+  if (s.n > top) {
+    *d.err = UB_ERR_INDEX;
+    s.n = top;
   }
-  const int first = a.window > 0 && n > a.window ? n - a.window : 0;
-  const float slope = a.slopes ? a.slopes[hq] : 0.f;
-  const float ks = a.scale * (a.k_scale ? a.k_scale[h] : 1.f);
-  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f};
+  s.first = a.window > 0 && s.n > a.window ? s.n - a.window : 0;
+  s.steps = s.n > s.first ? (s.n + 31) / 32 - s.first / 32 : 0;
+  return s;
+}
+
+__device__ __forceinline__ long shfl_up_l(long v, int o) { return __shfl_up((long long)v, o, 64); }
+
+// DK: 32-dim pieces of a head; PG8: S is a multiple of 8, so eight tokens 8 i
+// .. 8 i + 7 share a page; HT: tiles of 16 query heads.
+template <int DT, int CT, int DK, bool PG8, int HT>
+__global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(DK * HT > 4 ? 1 : 2)))
+k_decode(const Dev d) {
+  constexpr int NB = (DK + 3) / 4;      // 128-dim blocks of a head
+  constexpr int NP = PG8 ? 1 : 2, NV = PG8 ? 1 : 8;  // pages a lane looks up for K and V
+  constexpr int EB = Raw<CT>::B;
+  constexpr int kLeastD = DK == 2 ? 8 : DK == 3 ? 72 : DK == 4 ? 104 : DK == 6 ? 136 : 200;  // that takes this DK
+  constexpr int DP = 32 * DK + 4;
+  constexpr float kOff = DT == UB_F16 ? 14.f : 0.f;
+  typedef typename Raw<CT>::T R;
+  __shared__ float so[16 * HT][DP];
+  __shared__ float sm[W][16 * HT], sl[W][16 * HT];
+  __shared__ long wsum[W];
+  __shared__ long where[2];
+  const UbridgePagedDecodeArgs& a = d.a;
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int Hh = a.Hkv * d.HG;
+
+  // ---- this workgroup's share [cur, end) of the steps of all rows
+  long tot = 0;
+  for (int b = tid; b < a.B; b += 64 * W) tot += span(d, b).steps;
 #pragma unroll
-  for (int j = 0; j < 4; j++)
-    q[j] = lane + 64 * j < a.D ? ub_load<DT>(a.q, b * a.q_sb + hq * a.q_sh + lane + 64 * j) : 0.f;
-  float m = -__builtin_inff(), l = 0.f;
-  for (int t = first + wave; t < n; t += 4) {
-    int page = a.tables[b * a.table_stride + t / a.S];
-    const bool bad = page < 0 || page >= a.P;
-    if (bad) {
-      page = 0;
-      *err = UB_ERR_INDEX;
-    }
-    const long ko = page * a.k_sp + h * a.k_sh + (t % a.S) * a.k_ss;
-    const long vo = page * a.v_sp + h * a.v_sh + (t % a.S) * a.v_ss;
-    float x = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-      if (lane + 64 * j < a.D) x += q[j] * ldc<CT>(a.k_pages, ko + lane + 64 * j);
-    x = ub_wave_sum(x) * ks;
-    if (a.softcap > 0.f) x = a.softcap * tanhf(x / a.softcap);
-    x += slope * (float)(t - (n - 1));
-    if (bad) x = __builtin_nanf("");
-    const float mn = fmaxf(m, x), ms = mn == -__builtin_inff() ? 0.f : mn;  // (a NaN score: p is NaN)
-    const float al = expf(m - ms), p = expf(x - ms);
-    l = l * al + p;
-    m = mn;
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-      if (lane + 64 * j < a.D) o[j] = o[j] * al + p * ldc<CT>(a.v_pages, vo + lane + 64 * j);
-  }
-  if (lane == 0) sm[wave] = m, sl[wave] = l;
-#pragma unroll
-  for (int j = 0; j < 4; j++) so[wave][lane + 64 * j] = o[j];
+  for (int o = 32; o >= 1; o >>= 1) tot += __shfl_xor((long long)tot, o, 64);
+  if (lane == 0) wsum[wave] = tot;
   __syncthreads();
-  const float M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  float L = 0.f, O = 0.f;
-  for (int w = 0; w < 4; w++) {
-    const float f = expf(sm[w] - (M == -__builtin_inff() ? 0.f : M));
-    L += f * sl[w];
-    O += f * so[w][tid];
+  tot = (wsum[0] + wsum[1] + wsum[2] + wsum[3]) * Hh;
+  const long chunk = max((long)kMinSteps, (tot + d.shares - 1) / d.shares);
+  long cur = blockIdx.x * chunk;
+  const long end = min(tot, cur + chunk);
+  if (cur >= end) return;
+  long before = 0;
+  for (int b0 = 0;; b0 += 64 * W) {
+    const int b = b0 + tid;
+    const long s = b < a.B ? (long)span(d, b).steps * Hh : 0;
+    long x = s;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const long y = shfl_up_l(x, o);
+      if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) wsum[wave] = x;
+    __syncthreads();
+    x += before;
+    for (int w = 0; w < wave; w++) x += wsum[w];
+    if (cur >= x - s && cur < x) {
+      where[0] = b;
+      where[1] = cur - (x - s);
+    }
+    before += wsum[0] + wsum[1] + wsum[2] + wsum[3];
+    if (cur < before) break;  // (the same in every thread)
   }
+  __syncthreads();
+  int b = (int)where[0];
+  Span sp = span(d, b);
+  int hh = (int)(where[1] / sp.steps), st = (int)(where[1] - (long)hh * sp.steps);
+
+  const float cap = a.softcap;
+  const uint8_t* const kbase = (const uint8_t*)a.k_pages;
+  const uint8_t* const vbase = (const uint8_t*)a.v_pages;
+  // dims of this lane's pieces; a piece past D reads the head's first dims
+  // instead (in bounds) and counts for nothing
+  bool kin[DK];
+#pragma unroll
+  for (int j = 0; j < DK; j++) kin[j] = 32 * j + 8 * g < a.D;
+  int vdim[NB];
+#pragma unroll
+  for (int nb = 0; nb < NB; nb++) vdim[nb] = 128 * nb + 8 * c < a.D ? 128 * nb + 8 * c : 0;
+
+  while (cur < end) {
+    // ---- one row, or the part of it that lies in the share
+    const int h = hh / d.HG, hg = hh - h * d.HG;
+    const int q0 = hg * 16 * HT, nq = min(d.G - q0, 16 * HT);  // its query heads
+    const long left = end - cur;
+    const int s1 = left < sp.steps - st ? st + (int)left : sp.steps;
+    const int base = sp.first / 32;
+    const int* tb = a.tables + b * a.table_stride;
+
+    uint4 qf[HT][DK];
+    float slope[HT];
+#pragma unroll
+    for (int t = 0; t < HT; t++) {
+      const bool live = 16 * t + c < nq;
+      const int hq = h * d.G + q0 + 16 * t + c;
+      const uint16_t* p = (const uint16_t*)a.q + b * a.q_sb + (live ? hq : 0) * a.q_sh;
+#pragma unroll
+      for (int j = 0; j < DK; j++) {
+        qf[t][j] = make_uint4(0, 0, 0, 0);
+        if (live && kin[j]) __builtin_memcpy(&qf[t][j], p + 32 * j + 8 * g, 16);
+      }
+      slope[t] = live && a.slopes ? a.slopes[hq] * kLog2e : 0.f;
+    }
+    const float ks = a.scale * (a.k_scale ? a.k_scale[h] : 1.f);
+    const float kx = cap > 0.f ? 2.f * kLog2e * ks / cap : ks * kLog2e;  // on q . k
+
+    f32x4 o[HT][NB][8];
+    float m[HT], l[HT];
+#pragma unroll
+    for (int t = 0; t < HT; t++) {
+      m[t] = -kInf;
+      l[t] = 0.f;
+#pragma unroll
+      for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) o[t][nb][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+
+    R kf[2][DK], vf[NB][8];
+    int pk[NP], pv[NV];
+    // tokens that a lane reads keys of (tau = 0, 1) and values of (e = 0..7),
+    // kept inside [first, n); with PG8 the page of a group of eight, whose
+    // unseen tokens lie in the page too
+    auto tok = [&](int s, int i) {
+      const int t = 32 * (base + s) + i;
+      return PG8 ? min(max(t, sp.first & ~7), (sp.n - 1) & ~7) : min(max(t, sp.first), sp.n - 1);
+    };
+    auto lookup = [&](int s) {
+      if constexpr (PG8) {
+        pk[0] = tb[tok(s, 8 * (c >> 2)) / a.S];
+        pv[0] = tb[tok(s, 8 * g) / a.S];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; i++) pk[i] = tb[tok(s, 8 * (c >> 2) + 4 * i + (c & 3)) / a.S];
+#pragma unroll
+        for (int e = 0; e < 8; e++) pv[e] = tb[tok(s, 8 * g + e) / a.S];
+      }
+    };
+    auto page = [&](int p) { return (unsigned)p < (unsigned)a.P ? p : 0; };
+    auto load_k = [&](int s) {
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const int t = tok(s, 8 * (c >> 2) + (PG8 ? 0 : 4 * i + (c & 3)));
+        const int at = t % a.S + (PG8 ? 4 * i + (c & 3) : 0);
+        const uint8_t* p = kbase + EB * (page(pk[PG8 ? 0 : i]) * a.k_sp + h * a.k_sh + at * a.k_ss);
+#pragma unroll
+        for (int j = 0; j < DK; j++) kf[i][j] = ld8<CT>(p + EB * (kin[j] ? 32 * j + 8 * g : 0));
+      }
+    };
+    unsigned bad = 0;  // of the values being multiplied: tokens whose page is not there
+    unsigned bad_next = 0;
+    auto load_v = [&](int s) {
+      bad_next = 0;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const int t = tok(s, 8 * g + (PG8 ? 0 : e));
+        const int at = t % a.S + (PG8 ? e : 0);
+        const int pg = pv[PG8 ? 0 : e];
+        if ((unsigned)pg >= (unsigned)a.P) bad_next |= 1u << e;
+        const uint8_t* p = vbase + EB * (page(pg) * a.v_sp + h * a.v_sh + at * a.v_ss);
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) vf[nb][e] = ld8<CT>(p + EB * vdim[nb]);
+      }
+    };
+
+    int s = st + wave;
+    if (s < s1) {
+      lookup(s);
+      load_k(s);
+      load_v(s);
+      bad = bad_next;
+      if (s + W < s1) lookup(s + W);
+    }
+    for (; s < s1; s += W) {
+      const int t0 = 32 * (base + s) + 8 * g;  // this lane's first token
+      const bool edge = 32 * (base + s) < sp.first || 32 * (base + s) + 32 > sp.n;
+      // scores: x[t][tau * 4 + i] of head c, token t0 + 4 tau + i
+      f32x4 acc[HT][2];
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+#pragma unroll
+        for (int t = 0; t < HT; t++) acc[t][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < DK; j++) {
+          uint4 k = widen<DT, CT>(kf[i][j]);
+          if (32 * (j + 1) > kLeastD && !kin[j]) k = make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int t = 0; t < HT; t++) acc[t][i] = mfma<DT>(k, qf[t][j], acc[t][i]);
+        }
+      }
+      const int sn = s + W;
+      if (sn < s1) {
+        load_k(sn);
+      }
+      if (bad) *d.err = UB_ERR_INDEX;
+      uint4 ph[HT], pl[HT];
+#pragma unroll
+      for (int t = 0; t < HT; t++) {
+        float x[8], mx = -kInf;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          float v = acc[t][e >> 2][e & 3] * kx;
+          if (cap > 0.f)  // tanh z = 1 - 2 / (exp(2 z) + 1)
+            v = cap * kLog2e * (1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(v) + 1.f));
+          v += slope[t] * (float)(t0 + e - (sp.n - 1));
+          if (bad >> e & 1) v = __builtin_nanf("");
+          if (edge && (t0 + e < sp.first || t0 + e >= sp.n)) v = -kInf;
+          x[e] = v;
+          mx = fmaxf(mx, v);
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float mn = fmaxf(m[t], mx), ms = mn == -kInf ? 0.f : mn;  // (a NaN score: its weight is NaN)
+        const float al = __builtin_amdgcn_exp2f(m[t] - ms);
+        m[t] = mn;
+        float p[8], sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          p[e] = __builtin_amdgcn_exp2f(x[e] - ms + kOff);
+          sum += p[e];
+        }
+        l[t] = l[t] * al + sum;
+        uint32_t* hi = (uint32_t*)&ph[t];
+        uint32_t* lo = (uint32_t*)&pl[t];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          hi[q] = pack2<DT>(p[2 * q], p[2 * q + 1]);
+          lo[q] = pack2<DT>(p[2 * q] - half_of<DT>(hi[q], 0), p[2 * q + 1] - half_of<DT>(hi[q], 1));
+        }
+        if (__any(al != 1.f)) {
+#pragma unroll
+          for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) o[t][nb][j] *= al;
+        }
+      }
+      if (edge) {  // what lies behind a masked place may be anything
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (t0 + e < sp.first || t0 + e >= sp.n)
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) vf[nb][e] = R{};
+      }
+#pragma unroll
+      for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          uint32_t v0[4], v1[4];  // dims j and j + 1, two tokens a dword
+#pragma unroll
+          for (int q = 0; q < 4; q++) {
+            if constexpr (CT == UB_E4M3) {
+              const uint32_t x0 = j < 4 ? vf[nb][2 * q].x : vf[nb][2 * q].y;
+              const uint32_t x1 = j < 4 ? vf[nb][2 * q + 1].x : vf[nb][2 * q + 1].y;
+              const uint32_t w = __builtin_amdgcn_perm(x1, x0, j & 2 ? 0x07030602u : 0x05010400u);
+              v0[q] = from_e4m3<DT, false>(w);
+              v1[q] = from_e4m3<DT, true>(w);
+            } else {
+              const uint32_t x0 = ((const uint32_t*)&vf[nb][2 * q])[j / 2];
+              const uint32_t x1 = ((const uint32_t*)&vf[nb][2 * q + 1])[j / 2];
+              v0[q] = __builtin_amdgcn_perm(x1, x0, 0x05040100u);
+              v1[q] = __builtin_amdgcn_perm(x1, x0, 0x07060302u);
+            }
+          }
+          const uint4 w0 = make_uint4(v0[0], v0[1], v0[2], v0[3]), w1 = make_uint4(v1[0], v1[1], v1[2], v1[3]);
+#pragma unroll
+          for (int t = 0; t < HT; t++) {
+            o[t][nb][j] = mfma<DT>(w0, ph[t], o[t][nb][j]);
+            o[t][nb][j + 1] = mfma<DT>(w1, ph[t], o[t][nb][j + 1]);
+            o[t][nb][j] = mfma<DT>(w0, pl[t], o[t][nb][j]);
+            o[t][nb][j + 1] = mfma<DT>(w1, pl[t], o[t][nb][j + 1]);
+          }
+        }
+      if (sn < s1) {
+        load_v(sn);
+        bad = bad_next;
+        if (sn + W < s1) lookup(sn + W);
+      }
+    }
+
+    // ---- the wavefronts' sums meet in LDS, in their order
+#pragma unroll
+    for (int t = 0; t < HT; t++) {
+      l[t] += __shfl_xor(l[t], 16, 64);
+      l[t] += __shfl_xor(l[t], 32, 64);
+      if (g == 0) {
+        sm[wave][16 * t + c] = m[t];
+        sl[wave][16 * t + c] = l[t];
+      }
+    }
+    __syncthreads();
+    for (int w = 0; w < W; w++) {
+      if (w == wave) {
+#pragma unroll
+        for (int t = 0; t < HT; t++) {
+          if (16 * t + c >= nq) continue;
+          float M = -kInf;
+          for (int v = 0; v < W; v++) M = fmaxf(M, sm[v][16 * t + c]);
+          const float f = __builtin_amdgcn_exp2f(m[t] - (M == -kInf ? 0.f : M));
+#pragma unroll
+          for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              if (128 * nb + 32 * g + 8 * i >= 32 * DK) continue;
+              float* p = &so[16 * t + c][128 * nb + 32 * g + 8 * i];
+#pragma unroll
+              for (int j = 0; j < 8; j++) p[j] = (w ? p[j] : 0.f) + o[t][nb][j][i] * f;
+            }
+        }
+      }
+      __syncthreads();
+    }
+    const long slot = 2 * (long)blockIdx.x + (st == 0);
+    const bool whole = st == 0 && s1 == sp.steps;
+    for (int i = tid; i < nq * a.D; i += 64 * W) {
+      const int q = i / a.D, dim = i - q * a.D;
+      float M = -kInf, L = 0.f;
+      for (int w = 0; w < W; w++) M = fmaxf(M, sm[w][q]);
+      for (int w = 0; w < W; w++) L += __builtin_amdgcn_exp2f(sm[w][q] - (M == -kInf ? 0.f : M)) * sl[w][q];
+      if (whole) {
+        const size_t row = (size_t)b * a.Hq + h * d.G + q0 + q;
+        const float vs = a.v_scale ? a.v_scale[h] : 1.f;
+        ub_store<DT>(a.out, row * a.D + dim, L == 0.f ? 0.f : so[q][dim] / L * vs);
+        if (dim == 0 && a.lse) a.lse[row] = M == -kInf ? M + L : (M - kOff + __log2f(L)) * kLn2;
+      } else {
+        d.po[(slot * 16 * HT + q) * a.D + dim] = so[q][dim];
+        if (dim == 0) {
+          d.pml[(slot * 16 * HT + q) * 2] = M;
+          d.pml[(slot * 16 * HT + q) * 2 + 1] = L;
+        }
+      }
+    }
+    if (tid == 0 && st == 0)
+      d.info[(long)b * Hh + hh] = make_int2(blockIdx.x, (int)((cur + sp.steps - 1) / chunk) - (int)blockIdx.x + 1);
+    __syncthreads();
+
+    cur += s1 - st;
+    st = 0;
+    if (cur < end && ++hh == Hh) {
+      hh = 0;
+      do sp = span(d, ++b);
+      while (sp.steps == 0);
+    }
+  }
+}
+
+// One workgroup per (sequence, query head): the partial sums of a row that was
+// cut, in the order of the shares; zeros for a row without tokens.
+template <int DT>
+__global__ void __launch_bounds__(256) k_join(const Dev d, int heads) {
+  constexpr float kOff = DT == UB_F16 ? 14.f : 0.f;
+  const UbridgePagedDecodeArgs& a = d.a;
+  const int b = blockIdx.x / a.Hq, hq = blockIdx.x - b * a.Hq, h = hq / d.G;
+  const int hg = (hq - h * d.G) / heads, q = hq - h * d.G - hg * heads;
+  const int dim = threadIdx.x;
   const size_t row = (size_t)b * a.Hq + hq;
-  if (tid < a.D)
-    ub_store<DT>(a.out, row * a.D + tid, L == 0.f ? 0.f : O / L * (a.v_scale ? a.v_scale[h] : 1.f));
-  if (tid == 0 && a.lse) a.lse[row] = M + logf(L);
+  if (span(d, b).steps == 0) {
+    if (dim < a.D) ub_store<DT>(a.out, row * a.D + dim, 0.f);
+    if (dim == 0 && a.lse) a.lse[row] = -kInf;
+    return;
+  }
+  const int2 in = d.info[((long)b * a.Hkv + h) * d.HG + hg];
+  if (in.y == 1) return;  // (k_decode has written it)
+  auto slot = [&](int p) { return (long)(2 * (in.x + p) + (p == 0)) * heads + q; };
+  float M = -kInf, L = 0.f, O = 0.f;
+  for (int p = 0; p < in.y; p++) M = fmaxf(M, d.pml[2 * slot(p)]);
+  const float Ms = M == -kInf ? 0.f : M;
+  for (int p = 0; p < in.y; p++) {
+    const float f = __builtin_amdgcn_exp2f(d.pml[2 * slot(p)] - Ms);
+    L += f * d.pml[2 * slot(p) + 1];
+    if (dim < a.D) O += f * d.po[slot(p) * a.D + dim];
+  }
+  const float vs = a.v_scale ? a.v_scale[h] : 1.f;
+  if (dim < a.D) ub_store<DT>(a.out, row * a.D + dim, L == 0.f ? 0.f : O / L * vs);
+  if (dim == 0 && a.lse) a.lse[row] = M == -kInf ? M + L : (M - kOff + __log2f(L)) * kLn2;
+}
+
+template <int DT, int CT, int DK, bool PG8>
+void decode(const Dev& d, int HT, hipStream_t s) {
+  if (HT == 1) k_decode<DT, CT, DK, PG8, 1><<<d.shares, 64 * W, 0, s>>>(d);
+  else k_decode<DT, CT, DK, PG8, 2><<<d.shares, 64 * W, 0, s>>>(d);
+}
+template <int DT, int CT, int DK>
+void decode(const Dev& d, int HT, hipStream_t s) {
+  if (d.a.S % 8 == 0) decode<DT, CT, DK, true>(d, HT, s);
+  else decode<DT, CT, DK, false>(d, HT, s);
+}
+template <int DT, int CT>
+void decode(const Dev& d, int HT, hipStream_t s) {
+  if (d.a.D <= 64) decode<DT, CT, 2>(d, HT, s);
+  else if (d.a.D <= 96) decode<DT, CT, 3>(d, HT, s);
+  else if (d.a.D <= 128) decode<DT, CT, 4>(d, HT, s);
+  else if (d.a.D <= 192) decode<DT, CT, 6>(d, HT, s);
+  else decode<DT, CT, 8>(d, HT, s);
+  k_join<DT><<<d.a.B * d.a.Hq, 256, 0, s>>>(d, 16 * HT);
 }
 
 }  // namespace
@@ -91,20 +529,32 @@ UB_API int ubridge_paged_decode(const UbridgePagedDecodeArgs* p, void* stream) {
   UB_REQUIRE(a.B >= 0 && a.Hq >= 0 && a.Hkv > 0 && a.Hq % a.Hkv == 0,
              "%s: B=%d Hq=%d (a multiple of Hkv=%d)", nm, a.B, a.Hq, a.Hkv);
   UB_REQUIRE(a.D > 0 && a.D % 8 == 0 && a.D <= 256, "%s: D=%d (a multiple of 8, at most 256)", nm, a.D);
-  UB_REQUIRE(a.S > 0 && a.P >= 0 && a.width >= 0 && (int64_t)a.width * a.S <= 0x7fffffff,
+  UB_REQUIRE(a.S > 0 && a.P >= 0 && a.width >= 0 && (int64_t)a.width * a.S <= 0x7fffffc0,
              "%s: S=%d P=%d width=%d", nm, a.S, a.P, a.width);
   UB_REQUIRE(a.window >= 0 && a.softcap >= 0.f, "%s: window=%d softcap=%g", nm, a.window, a.softcap);
   if (a.B == 0 || a.Hq == 0) return UB_OK;
   UB_REQUIRE(a.q && a.out && a.lens && (a.tables || a.width == 0), "%s: null pointer", nm);
   UB_REQUIRE(a.P == 0 || (a.k_pages && a.v_pages), "%s: null pages", nm);
   UB_REQUIRE((int64_t)a.B * a.Hq < 1 << 23, "%s: B=%d Hq=%d", nm, a.B, a.Hq);
-  int* err = ub_error_flag();
-  UB_REQUIRE(err, "%s: no device flag", nm);
+  Dev d;
+  d.a = a;
+  d.G = a.Hq / a.Hkv;
+  d.err = ub_error_flag();
+  UB_REQUIRE(d.err, "%s: no device flag", nm);
+  const int HT = d.G > 16 ? 2 : 1, heads = 16 * HT;
+  d.HG = ub_cdiv(d.G, heads);
+  d.shares = 512;
+  const size_t rows = (size_t)a.B * a.Hkv * d.HG;
+  const size_t nml = sizeof(float) * 2 * d.shares * heads * 2, no = nml / 2 * a.D;
   hipStream_t s = ub_stream(stream);
-  const int grid = a.B * a.Hq;
-  if (a.dtype == UB_BF16 && a.cache_dtype == UB_BF16) k_decode<UB_BF16, UB_BF16><<<grid, 256, 0, s>>>(a, err);
-  else if (a.dtype == UB_BF16) k_decode<UB_BF16, UB_E4M3><<<grid, 256, 0, s>>>(a, err);
-  else if (a.cache_dtype == UB_F16) k_decode<UB_F16, UB_F16><<<grid, 256, 0, s>>>(a, err);
-  else k_decode<UB_F16, UB_E4M3><<<grid, 256, 0, s>>>(a, err);
+  UbScratch ws(s, no + nml + sizeof(int2) * rows);
+  if (!ws.get()) return ub_set_error(UB_ERR_LAUNCH, "%s: no workspace", nm);
+  d.po = (float*)ws.get();
+  d.pml = d.po + no / sizeof(float);
+  d.info = (int2*)((char*)ws.get() + no + nml);
+  if (a.dtype == UB_BF16 && a.cache_dtype == UB_BF16) decode<UB_BF16, UB_BF16>(d, HT, s);
+  else if (a.dtype == UB_BF16) decode<UB_BF16, UB_E4M3>(d, HT, s);
+  else if (a.cache_dtype == UB_F16) decode<UB_F16, UB_F16>(d, HT, s);
+  else decode<UB_F16, UB_E4M3>(d, HT, s);
   return ub_check_launch(nm);
 }
