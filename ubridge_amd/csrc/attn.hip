@@ -44,7 +44,8 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int W = 4;         // wavefronts of a workgroup
-constexpr int kMinSteps = 8;  // of a share
+constexpr int kMinShare = 4;  // least cost of a share
+constexpr int kRowCost = 2;
 
 template <int DT>
 __device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
@@ -103,11 +104,13 @@ __device__ __forceinline__ uint4 widen(const typename Raw<CT>::T& v) {
 
 struct Dev {
   UbridgePagedDecodeArgs a;
-  int G, HG;     // query heads of a kv head; head groups of it (rows of one sequence: Hkv HG)
-  int shares;    // workgroups of k_decode
-  float* po;     // [2 shares][heads of a group][D] partial sums, relative to the maximum
-  float* pml;    // [2 shares][heads of a group][2] maximum (log2) and sum
-  int2* info;    // [B Hkv HG] first share and number of shares of a row
+  int G, HG;       // query heads of a kv head; head groups of it (rows of one sequence: Hkv HG)
+  int lg_shares;   // log2 of the wavefronts of k_decode
+  uint64_t s_mul;  // t / S = t s_mul >> s_shift for 0 <= t < 2^31
+  int s_shift;
+  float* po;       // [2 shares][heads of a group][D] partial sums, relative to the maximum
+  float* pml;      // [2 shares][heads of a group][2] maximum (log2) and sum
+  int2* info;      // [B Hkv HG] first share and number of shares of a row
   int* err;
 };
 
@@ -126,8 +129,8 @@ __device__ __forceinline__ Span span(const Dev& d, int b) {
   s.steps = s.n > s.first ? (s.n + 31) / 32 - s.first / 32 : 0;
   return s;
 }
-
-__device__ __forceinline__ long shfl_up_l(long v, int o) { return __shfl_up((long long)v, o, 64); }
+// what a row costs, in steps: its own and the latency of its first loads
+__device__ __forceinline__ int cost(const Span& s) { return s.steps ? s.steps + kRowCost : 0; }
 
 // DK: 32-dim pieces of a head; PG8: S is a multiple of 8, so eight tokens 8 i
 // .. 8 i + 7 share a page; HT: tiles of 16 query heads.
@@ -138,38 +141,34 @@ k_decode(const Dev d) {
   constexpr int NP = PG8 ? 1 : 2, NV = PG8 ? 1 : 8;  // pages a lane looks up for K and V
   constexpr int EB = Raw<CT>::B;
   constexpr int kLeastD = DK == 2 ? 8 : DK == 3 ? 72 : DK == 4 ? 104 : DK == 6 ? 136 : 200;  // that takes this DK
-  constexpr int DP = 32 * DK + 4;
   constexpr float kOff = DT == UB_F16 ? 14.f : 0.f;
   typedef typename Raw<CT>::T R;
-  __shared__ float so[16 * HT][DP];
-  __shared__ float sm[W][16 * HT], sl[W][16 * HT];
-  __shared__ long wsum[W];
-  __shared__ long where[2];
+  __shared__ int wsum[W];
+  __shared__ int where[W][2];
   const UbridgePagedDecodeArgs& a = d.a;
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int Hh = a.Hkv * d.HG;
 
-  // ---- this workgroup's share [cur, end) of the steps of all rows
-  long tot = 0;
-  for (int b = tid; b < a.B; b += 64 * W) tot += span(d, b).steps;
+  // ---- the wavefronts' shares [cur, end) of the costs of all rows
+  int tot = 0;
+  for (int b = tid; b < a.B; b += 64 * W) tot += cost(span(d, b));
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) tot += __shfl_xor((long long)tot, o, 64);
+  for (int o = 32; o >= 1; o >>= 1) tot += __shfl_xor(tot, o, 64);
   if (lane == 0) wsum[wave] = tot;
   __syncthreads();
   tot = (wsum[0] + wsum[1] + wsum[2] + wsum[3]) * Hh;
-  const long chunk = max((long)kMinSteps, (tot + d.shares - 1) / d.shares);
-  long cur = blockIdx.x * chunk;
-  const long end = min(tot, cur + chunk);
-  if (cur >= end) return;
-  long before = 0;
+  const int chunk = max(kMinShare, (int)(((int64_t)tot + (1 << d.lg_shares) - 1) >> d.lg_shares));
+  const int64_t blk = (int64_t)blockIdx.x * W * chunk;  // the workgroup's first
+  if (blk >= tot) return;
+  int before = 0;
   for (int b0 = 0;; b0 += 64 * W) {
     const int b = b0 + tid;
-    const long s = b < a.B ? (long)span(d, b).steps * Hh : 0;
-    long x = s;
+    const int s = b < a.B ? cost(span(d, b)) * Hh : 0;
+    int x = s;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-      const long y = shfl_up_l(x, o);
+      const int y = __shfl_up(x, o, 64);
       if (lane >= o) x += y;
     }
     __syncthreads();
@@ -177,17 +176,27 @@ k_decode(const Dev d) {
     __syncthreads();
     x += before;
     for (int w = 0; w < wave; w++) x += wsum[w];
-    if (cur >= x - s && cur < x) {
-      where[0] = b;
-      where[1] = cur - (x - s);
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+      const int64_t p = blk + (int64_t)w * chunk;
+      if (p >= x - s && p < x) {
+        where[w][0] = b;
+        where[w][1] = (int)p - (x - s);
+      }
     }
     before += wsum[0] + wsum[1] + wsum[2] + wsum[3];
-    if (cur < before) break;  // (the same in every thread)
+    if (blk + (int64_t)(W - 1) * chunk < before || before == tot) break;  // (the same in every thread)
   }
   __syncthreads();
-  int b = (int)where[0];
+  const int share = blockIdx.x * W + wave;
+  if (blk + (int64_t)wave * chunk >= tot) return;  // (no barrier below)
+  int cur = (int)blk + wave * chunk;
+  const int end = (int)min((int64_t)tot, (int64_t)cur + chunk);
+  int b = __builtin_amdgcn_readfirstlane(where[wave][0]);
+  int at_row = __builtin_amdgcn_readfirstlane(where[wave][1]);
   Span sp = span(d, b);
-  int hh = (int)(where[1] / sp.steps), st = (int)(where[1] - (long)hh * sp.steps);
+  int hh = at_row / cost(sp);
+  at_row -= hh * cost(sp);  // the share starts this far into the row
 
   const float cap = a.softcap;
   const uint8_t* const kbase = (const uint8_t*)a.k_pages;
@@ -203,12 +212,22 @@ k_decode(const Dev d) {
 
   while (cur < end) {
     // ---- one row, or the part of it that lies in the share
+    const int len = min(end - cur, cost(sp) - at_row);
+    const int st = max(at_row - kRowCost, 0), s1 = at_row + len - kRowCost;
+    cur += len;
     const int h = hh / d.HG, hg = hh - h * d.HG;
+    const int row_of_b = hh, bb = b;
+    const Span sq = sp;
+    at_row = 0;
+    if (cur < end && ++hh == Hh) {
+      hh = 0;
+      do sp = span(d, ++b);
+      while (sp.steps == 0);
+    }
+    if (s1 <= st) continue;  // (only the row's head)
     const int q0 = hg * 16 * HT, nq = min(d.G - q0, 16 * HT);  // its query heads
-    const long left = end - cur;
-    const int s1 = left < sp.steps - st ? st + (int)left : sp.steps;
-    const int base = sp.first / 32;
-    const int* tb = a.tables + b * a.table_stride;
+    const int base = sq.first / 32;
+    const int* tb = a.tables + bb * a.table_stride;
 
     uint4 qf[HT][DK];
     float slope[HT];
@@ -216,7 +235,7 @@ k_decode(const Dev d) {
     for (int t = 0; t < HT; t++) {
       const bool live = 16 * t + c < nq;
       const int hq = h * d.G + q0 + 16 * t + c;
-      const uint16_t* p = (const uint16_t*)a.q + b * a.q_sb + (live ? hq : 0) * a.q_sh;
+      const uint16_t* p = (const uint16_t*)a.q + bb * a.q_sb + (live ? hq : 0) * a.q_sh;
 #pragma unroll
       for (int j = 0; j < DK; j++) {
         qf[t][j] = make_uint4(0, 0, 0, 0);
@@ -246,17 +265,18 @@ k_decode(const Dev d) {
     // unseen tokens lie in the page too
     auto tok = [&](int s, int i) {
       const int t = 32 * (base + s) + i;
-      return PG8 ? min(max(t, sp.first & ~7), (sp.n - 1) & ~7) : min(max(t, sp.first), sp.n - 1);
+      return PG8 ? min(max(t, sq.first & ~7), (sq.n - 1) & ~7) : min(max(t, sq.first), sq.n - 1);
     };
+    auto quo = [&](int t) { return (int)((uint64_t)t * d.s_mul >> d.s_shift); };  // t / S
     auto lookup = [&](int s) {
       if constexpr (PG8) {
-        pk[0] = tb[tok(s, 8 * (c >> 2)) / a.S];
-        pv[0] = tb[tok(s, 8 * g) / a.S];
+        pk[0] = tb[quo(tok(s, 8 * (c >> 2)))];
+        pv[0] = tb[quo(tok(s, 8 * g))];
       } else {
 #pragma unroll
-        for (int i = 0; i < 2; i++) pk[i] = tb[tok(s, 8 * (c >> 2) + 4 * i + (c & 3)) / a.S];
+        for (int i = 0; i < 2; i++) pk[i] = tb[quo(tok(s, 8 * (c >> 2) + 4 * i + (c & 3)))];
 #pragma unroll
-        for (int e = 0; e < 8; e++) pv[e] = tb[tok(s, 8 * g + e) / a.S];
+        for (int e = 0; e < 8; e++) pv[e] = tb[quo(tok(s, 8 * g + e))];
       }
     };
     auto page = [&](int p) { return (unsigned)p < (unsigned)a.P ? p : 0; };
@@ -264,7 +284,7 @@ k_decode(const Dev d) {
 #pragma unroll
       for (int i = 0; i < 2; i++) {
         const int t = tok(s, 8 * (c >> 2) + (PG8 ? 0 : 4 * i + (c & 3)));
-        const int at = t % a.S + (PG8 ? 4 * i + (c & 3) : 0);
+        const int at = t - quo(t) * a.S + (PG8 ? 4 * i + (c & 3) : 0);
         const uint8_t* p = kbase + EB * (page(pk[PG8 ? 0 : i]) * a.k_sp + h * a.k_sh + at * a.k_ss);
 #pragma unroll
         for (int j = 0; j < DK; j++) kf[i][j] = ld8<CT>(p + EB * (kin[j] ? 32 * j + 8 * g : 0));
@@ -277,7 +297,7 @@ k_decode(const Dev d) {
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         const int t = tok(s, 8 * g + (PG8 ? 0 : e));
-        const int at = t % a.S + (PG8 ? e : 0);
+        const int at = t - quo(t) * a.S + (PG8 ? e : 0);
         const int pg = pv[PG8 ? 0 : e];
         if ((unsigned)pg >= (unsigned)a.P) bad_next |= 1u << e;
         const uint8_t* p = vbase + EB * (page(pg) * a.v_sp + h * a.v_sh + at * a.v_ss);
@@ -286,17 +306,17 @@ k_decode(const Dev d) {
       }
     };
 
-    int s = st + wave;
+    int s = st;
     if (s < s1) {
       lookup(s);
       load_k(s);
       load_v(s);
       bad = bad_next;
-      if (s + W < s1) lookup(s + W);
+      if (s + 1 < s1) lookup(s + 1);
     }
-    for (; s < s1; s += W) {
+    for (; s < s1; s++) {
       const int t0 = 32 * (base + s) + 8 * g;  // this lane's first token
-      const bool edge = 32 * (base + s) < sp.first || 32 * (base + s) + 32 > sp.n;
+      const bool edge = 32 * (base + s) < sq.first || 32 * (base + s) + 32 > sq.n;
       // scores: x[t][tau * 4 + i] of head c, token t0 + 4 tau + i
       f32x4 acc[HT][2];
 #pragma unroll
@@ -311,7 +331,7 @@ k_decode(const Dev d) {
           for (int t = 0; t < HT; t++) acc[t][i] = mfma<DT>(k, qf[t][j], acc[t][i]);
         }
       }
-      const int sn = s + W;
+      const int sn = s + 1;
       if (sn < s1) {
         load_k(sn);
       }
@@ -325,9 +345,9 @@ k_decode(const Dev d) {
           float v = acc[t][e >> 2][e & 3] * kx;
           if (cap > 0.f)  // tanh z = 1 - 2 / (exp(2 z) + 1)
             v = cap * kLog2e * (1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(v) + 1.f));
-          v += slope[t] * (float)(t0 + e - (sp.n - 1));
+          v += slope[t] * (float)(t0 + e - (sq.n - 1));
           if (bad >> e & 1) v = __builtin_nanf("");
-          if (edge && (t0 + e < sp.first || t0 + e >= sp.n)) v = -kInf;
+          if (edge && (t0 + e < sq.first || t0 + e >= sq.n)) v = -kInf;
           x[e] = v;
           mx = fmaxf(mx, v);
         }
@@ -360,7 +380,7 @@ k_decode(const Dev d) {
       if (edge) {  // what lies behind a masked place may be anything
 #pragma unroll
         for (int e = 0; e < 8; e++)
-          if (t0 + e < sp.first || t0 + e >= sp.n)
+          if (t0 + e < sq.first || t0 + e >= sq.n)
 #pragma unroll
             for (int nb = 0; nb < NB; nb++) vf[nb][e] = R{};
       }
@@ -396,111 +416,128 @@ k_decode(const Dev d) {
       if (sn < s1) {
         load_v(sn);
         bad = bad_next;
-        if (sn + W < s1) lookup(sn + W);
+        if (sn + 1 < s1) lookup(sn + 1);
       }
     }
 
-    // ---- the wavefronts' sums meet in LDS, in their order
+    // ---- a whole row is finished here; a part leaves its sums
+    const bool whole = st == 0 && s1 == sq.steps;
+    const int slot = 2 * share + (st == 0);
+    const float vs = a.v_scale ? a.v_scale[h] : 1.f;
 #pragma unroll
     for (int t = 0; t < HT; t++) {
       l[t] += __shfl_xor(l[t], 16, 64);
       l[t] += __shfl_xor(l[t], 32, 64);
-      if (g == 0) {
-        sm[wave][16 * t + c] = m[t];
-        sl[wave][16 * t + c] = l[t];
-      }
-    }
-    __syncthreads();
-    for (int w = 0; w < W; w++) {
-      if (w == wave) {
-#pragma unroll
-        for (int t = 0; t < HT; t++) {
-          if (16 * t + c >= nq) continue;
-          float M = -kInf;
-          for (int v = 0; v < W; v++) M = fmaxf(M, sm[v][16 * t + c]);
-          const float f = __builtin_amdgcn_exp2f(m[t] - (M == -kInf ? 0.f : M));
-#pragma unroll
-          for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-              if (128 * nb + 32 * g + 8 * i >= 32 * DK) continue;
-              float* p = &so[16 * t + c][128 * nb + 32 * g + 8 * i];
-#pragma unroll
-              for (int j = 0; j < 8; j++) p[j] = (w ? p[j] : 0.f) + o[t][nb][j][i] * f;
-            }
-        }
-      }
-      __syncthreads();
-    }
-    const long slot = 2 * (long)blockIdx.x + (st == 0);
-    const bool whole = st == 0 && s1 == sp.steps;
-    for (int i = tid; i < nq * a.D; i += 64 * W) {
-      const int q = i / a.D, dim = i - q * a.D;
-      float M = -kInf, L = 0.f;
-      for (int w = 0; w < W; w++) M = fmaxf(M, sm[w][q]);
-      for (int w = 0; w < W; w++) L += __builtin_amdgcn_exp2f(sm[w][q] - (M == -kInf ? 0.f : M)) * sl[w][q];
+      const int q = 16 * t + c;
+      if (q >= nq) continue;
       if (whole) {
-        const size_t row = (size_t)b * a.Hq + h * d.G + q0 + q;
-        const float vs = a.v_scale ? a.v_scale[h] : 1.f;
-        ub_store<DT>(a.out, row * a.D + dim, L == 0.f ? 0.f : so[q][dim] / L * vs);
-        if (dim == 0 && a.lse) a.lse[row] = M == -kInf ? M + L : (M - kOff + __log2f(L)) * kLn2;
+        const size_t row = (size_t)bb * a.Hq + h * d.G + q0 + q;
+        const float f = l[t] == 0.f ? 0.f : vs / l[t];
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int dim = 128 * nb + 32 * g + 8 * i;
+            if (dim >= a.D) continue;
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[j] = pack2<DT>(o[t][nb][2 * j][i] * f, o[t][nb][2 * j + 1][i] * f);
+            __builtin_memcpy((uint16_t*)a.out + row * a.D + dim, w, 16);
+          }
+        if (g == 0 && a.lse) a.lse[row] = m[t] == -kInf ? m[t] + l[t] : (m[t] - kOff + __log2f(l[t])) * kLn2;
       } else {
-        d.po[(slot * 16 * HT + q) * a.D + dim] = so[q][dim];
-        if (dim == 0) {
-          d.pml[(slot * 16 * HT + q) * 2] = M;
-          d.pml[(slot * 16 * HT + q) * 2 + 1] = L;
-        }
+        float* po = d.po + ((size_t)slot * 16 * HT + q) * a.D;
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int dim = 128 * nb + 32 * g + 8 * i;
+            if (dim >= a.D) continue;
+#pragma unroll
+            for (int j = 0; j < 8; j += 4)
+              *(float4*)(po + dim + j) = make_float4(o[t][nb][j][i], o[t][nb][j + 1][i], o[t][nb][j + 2][i], o[t][nb][j + 3][i]);
+          }
+        if (g == 0) *(float2*)(d.pml + ((size_t)slot * 16 * HT + q) * 2) = make_float2(m[t], l[t]);
       }
     }
-    if (tid == 0 && st == 0)
-      d.info[(long)b * Hh + hh] = make_int2(blockIdx.x, (int)((cur + sp.steps - 1) / chunk) - (int)blockIdx.x + 1);
-    __syncthreads();
-
-    cur += s1 - st;
-    st = 0;
-    if (cur < end && ++hh == Hh) {
-      hh = 0;
-      do sp = span(d, ++b);
-      while (sp.steps == 0);
-    }
+    if (st == 0 && lane == 0)
+      d.info[(size_t)bb * Hh + row_of_b] =
+          make_int2(share, whole ? 1 : 1 + (int)(((unsigned)(sq.steps - s1) + chunk - 1) / (unsigned)chunk));
   }
 }
 
 // One workgroup per (sequence, query head): the partial sums of a row that was
-// cut, in the order of the shares; zeros for a row without tokens.
+// cut, in the order of the shares; zeros for a row without tokens.  Thread (dim
+// / 4, r) adds every R-th share, the R sums meet in LDS.
 template <int DT>
 __global__ void __launch_bounds__(256) k_join(const Dev d, int heads) {
   constexpr float kOff = DT == UB_F16 ? 14.f : 0.f;
+  __shared__ float wt[256], red[4];
+  __shared__ float4 part[256];
   const UbridgePagedDecodeArgs& a = d.a;
   const int b = blockIdx.x / a.Hq, hq = blockIdx.x - b * a.Hq, h = hq / d.G;
   const int hg = (hq - h * d.G) / heads, q = hq - h * d.G - hg * heads;
-  const int dim = threadIdx.x;
+  const int tid = threadIdx.x;
   const size_t row = (size_t)b * a.Hq + hq;
+  const int2 in = d.info[((size_t)b * a.Hkv + h) * d.HG + hg];  // (read ahead of the test below)
   if (span(d, b).steps == 0) {
-    if (dim < a.D) ub_store<DT>(a.out, row * a.D + dim, 0.f);
-    if (dim == 0 && a.lse) a.lse[row] = -kInf;
+    if (tid < a.D) ub_store<DT>(a.out, row * a.D + tid, 0.f);
+    if (tid == 0 && a.lse) a.lse[row] = -kInf;
     return;
   }
-  const int2 in = d.info[((long)b * a.Hkv + h) * d.HG + hg];
   if (in.y == 1) return;  // (k_decode has written it)
-  auto slot = [&](int p) { return (long)(2 * (in.x + p) + (p == 0)) * heads + q; };
-  float M = -kInf, L = 0.f, O = 0.f;
-  for (int p = 0; p < in.y; p++) M = fmaxf(M, d.pml[2 * slot(p)]);
+  auto slot = [&](int p) { return (size_t)(2 * (in.x + p) + (p == 0)) * heads + q; };
+  auto all = [&](float v, bool mx) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+      const float y = __shfl_xor(v, o, 64);
+      v = mx ? fmaxf(v, y) : v + y;
+    }
+    __syncthreads();
+    if ((tid & 63) == 0) red[tid >> 6] = v;
+    __syncthreads();
+    return mx ? fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])) : red[0] + red[1] + red[2] + red[3];
+  };
+  float M = -kInf, L = 0.f;
+  for (int p = tid; p < in.y; p += 256) M = fmaxf(M, d.pml[2 * slot(p)]);
+  M = all(M, true);
   const float Ms = M == -kInf ? 0.f : M;
-  for (int p = 0; p < in.y; p++) {
-    const float f = __builtin_amdgcn_exp2f(d.pml[2 * slot(p)] - Ms);
-    L += f * d.pml[2 * slot(p) + 1];
-    if (dim < a.D) O += f * d.po[slot(p) * a.D + dim];
+  const int V = a.D / 4, R = 256 / V;  // (D / 4 >= 2 threads a share)
+  const int v = tid % V, r = tid / V;
+  float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p0 = 0; p0 < in.y; p0 += 256) {
+    float w = 0.f;
+    if (p0 + tid < in.y) {
+      const float2 ml = *(const float2*)(d.pml + 2 * slot(p0 + tid));
+      w = __builtin_amdgcn_exp2f(ml.x - Ms);
+      L += w * ml.y;
+    }
+    __syncthreads();
+    wt[tid] = w;
+    __syncthreads();
+    if (r < R)
+      for (int p = r; p < min(256, in.y - p0); p += R) {
+        const float4 x = *(const float4*)(d.po + slot(p0 + p) * a.D + 4 * v);
+        const float f = wt[p];
+        O.x += f * x.x, O.y += f * x.y, O.z += f * x.z, O.w += f * x.w;
+      }
   }
-  const float vs = a.v_scale ? a.v_scale[h] : 1.f;
-  if (dim < a.D) ub_store<DT>(a.out, row * a.D + dim, L == 0.f ? 0.f : O / L * vs);
-  if (dim == 0 && a.lse) a.lse[row] = M == -kInf ? M + L : (M - kOff + __log2f(L)) * kLn2;
+  L = all(L, false);
+  part[tid] = O;
+  __syncthreads();
+  const float f = L == 0.f ? 0.f : (a.v_scale ? a.v_scale[h] : 1.f) / L;
+  if (tid < a.D) {
+    float s = 0.f;
+    for (int i = 0; i < R; i++) s += ((const float*)&part[i * V + tid / 4])[tid % 4];
+    ub_store<DT>(a.out, row * a.D + tid, s * f);
+  }
+  if (tid == 0 && a.lse) a.lse[row] = M == -kInf ? M + L : (M - kOff + __log2f(L)) * kLn2;
 }
 
 template <int DT, int CT, int DK, bool PG8>
 void decode(const Dev& d, int HT, hipStream_t s) {
-  if (HT == 1) k_decode<DT, CT, DK, PG8, 1><<<d.shares, 64 * W, 0, s>>>(d);
-  else k_decode<DT, CT, DK, PG8, 2><<<d.shares, 64 * W, 0, s>>>(d);
+  if (HT == 1) k_decode<DT, CT, DK, PG8, 1><<<(1 << d.lg_shares) / W, 64 * W, 0, s>>>(d);
+  else k_decode<DT, CT, DK, PG8, 2><<<(1 << d.lg_shares) / W, 64 * W, 0, s>>>(d);
 }
 template <int DT, int CT, int DK>
 void decode(const Dev& d, int HT, hipStream_t s) {
@@ -543,9 +580,14 @@ UB_API int ubridge_paged_decode(const UbridgePagedDecodeArgs* p, void* stream) {
   UB_REQUIRE(d.err, "%s: no device flag", nm);
   const int HT = d.G > 16 ? 2 : 1, heads = 16 * HT;
   d.HG = ub_cdiv(d.G, heads);
-  d.shares = 512;
-  const size_t rows = (size_t)a.B * a.Hkv * d.HG;
-  const size_t nml = sizeof(float) * 2 * d.shares * heads * 2, no = nml / 2 * a.D;
+  const int64_t rows = (int64_t)a.B * a.Hkv * d.HG;
+  UB_REQUIRE(rows * ((int64_t)a.width * a.S / 32 + 1 + kRowCost) < 0x7fffffff,
+             "%s: %ld rows of %ld tokens", nm, (long)rows, (long)a.width * a.S);
+  d.s_shift = 31;
+  while ((1ll << (d.s_shift - 31)) < a.S) d.s_shift++;
+  d.s_mul = (1ull << d.s_shift) / a.S + 1;
+  d.lg_shares = 11;
+  const size_t nml = sizeof(float) * 4 * heads << d.lg_shares, no = nml / 2 * a.D;
   hipStream_t s = ub_stream(stream);
   UbScratch ws(s, no + nml + sizeof(int2) * rows);
   if (!ws.get()) return ub_set_error(UB_ERR_LAUNCH, "%s: no workspace", nm);
