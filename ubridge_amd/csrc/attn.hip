@@ -44,8 +44,8 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int W = 4;         // wavefronts of a workgroup
-constexpr int kMinShare = 4;  // least cost of a share
-constexpr int kRowCost = 2;
+constexpr int kRowCost = 2;  // steps that the first loads of a row are worth
+constexpr int kShares = 2048;  // two wavefronts a SIMD
 
 template <int DT>
 __device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
@@ -105,12 +105,12 @@ __device__ __forceinline__ uint4 widen(const typename Raw<CT>::T& v) {
 struct Dev {
   UbridgePagedDecodeArgs a;
   int G, HG;       // query heads of a kv head; head groups of it (rows of one sequence: Hkv HG)
-  int lg_shares;   // log2 of the wavefronts of k_decode
+  int shares;      // wavefronts of k_decode
   uint64_t s_mul;  // t / S = t s_mul >> s_shift for 0 <= t < 2^31
   int s_shift;
   float* po;       // [2 shares][heads of a group][D] partial sums, relative to the maximum
   float* pml;      // [2 shares][heads of a group][2] maximum (log2) and sum
-  int2* info;      // [B Hkv HG] first share and number of shares of a row
+  int2* cut;       // [shares] the row that starts in a share and ends past it (-1: none), and its shares
   int* err;
 };
 
@@ -132,6 +132,12 @@ __device__ __forceinline__ Span span(const Dev& d, int b) {
 // what a row costs, in steps: its own and the latency of its first loads
 __device__ __forceinline__ int cost(const Span& s) { return s.steps ? s.steps + kRowCost : 0; }
 
+// m (log2) and l of a row -> log of the sum
+template <int DT>
+__device__ __forceinline__ float lse_of(float m, float l) {
+  return m == -kInf ? m + l : (m - (DT == UB_F16 ? 14.f : 0.f) + __log2f(l)) * kLn2;
+}
+
 // DK: 32-dim pieces of a head; PG8: S is a multiple of 8, so eight tokens 8 i
 // .. 8 i + 7 share a page; HT: tiles of 16 query heads.
 template <int DT, int CT, int DK, bool PG8, int HT>
@@ -143,59 +149,72 @@ k_decode(const Dev d) {
   constexpr int kLeastD = DK == 2 ? 8 : DK == 3 ? 72 : DK == 4 ? 104 : DK == 6 ? 136 : 200;  // that takes this DK
   constexpr float kOff = DT == UB_F16 ? 14.f : 0.f;
   typedef typename Raw<CT>::T R;
-  __shared__ int wsum[W];
-  __shared__ int where[W][2];
   const UbridgePagedDecodeArgs& a = d.a;
-  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int Hh = a.Hkv * d.HG;
 
-  // ---- the wavefronts' shares [cur, end) of the costs of all rows
-  int tot = 0;
-  for (int b = tid; b < a.B; b += 64 * W) tot += cost(span(d, b));
+  // ---- this wavefront's share [cur, end) of the costs of all rows: the sum
+  // over the sequences (lane: four neighbours of every 256), then the place
+  int four[4], tot = 0;
+  auto costs = [&](int b0) {
+    int s = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int b = b0 + 4 * lane + i;
+      four[i] = b < a.B ? cost(span(d, b)) : 0;
+      s += four[i];
+    }
+    return s;
+  };
+  for (int b0 = (a.B - 1) & ~255; b0 >= 0; b0 -= 256) tot += costs(b0);
+  int x = 0, mine = 0, b0 = 0;  // (four holds the first 256)
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) tot += __shfl_xor(tot, o, 64);
-  if (lane == 0) wsum[wave] = tot;
-  __syncthreads();
-  tot = (wsum[0] + wsum[1] + wsum[2] + wsum[3]) * Hh;
-  const int chunk = max(kMinShare, (int)(((int64_t)tot + (1 << d.lg_shares) - 1) >> d.lg_shares));
-  const int64_t blk = (int64_t)blockIdx.x * W * chunk;  // the workgroup's first
-  if (blk >= tot) return;
-  int before = 0;
-  for (int b0 = 0;; b0 += 64 * W) {
-    const int b = b0 + tid;
-    const int s = b < a.B ? cost(span(d, b)) * Hh : 0;
-    int x = s;
+  tot = __builtin_amdgcn_readfirstlane(tot) * Hh;
+  const int chunk = max(1, (int)(((unsigned)tot + d.shares - 1) / (unsigned)d.shares));
+  const int share = blockIdx.x * W + wave;
+  for (int i = share; i < a.B; i += d.shares)  // rows without tokens are nobody's share
+    if (span(d, i).steps == 0) {
+      const uint4 z = make_uint4(0, 0, 0, 0);
+      uint16_t* p = (uint16_t*)a.out + (size_t)i * a.Hq * a.D;
+      for (int e = 8 * lane; e < a.Hq * a.D; e += 512) __builtin_memcpy(p + e, &z, 16);
+      if (a.lse)
+        for (int e = lane; e < a.Hq; e += 64) a.lse[(size_t)i * a.Hq + e] = -kInf;
+    }
+  int2 cut = make_int2(-1, 0);
+  if ((int64_t)share * chunk >= tot) {
+    if (lane == 0) d.cut[share] = cut;
+    return;
+  }
+  int cur = share * chunk;
+  const int end = (int)min((int64_t)tot, (int64_t)cur + chunk);
+  for (int before = 0;; b0 += 256) {
+    if (b0) (void)costs(b0);
+    mine = (four[0] + four[1] + four[2] + four[3]) * Hh;
+    x = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const int y = __shfl_up(x, o, 64);
       if (lane >= o) x += y;
     }
-    __syncthreads();
-    if (lane == 63) wsum[wave] = x;
-    __syncthreads();
     x += before;
-    for (int w = 0; w < wave; w++) x += wsum[w];
-#pragma unroll
-    for (int w = 0; w < W; w++) {
-      const int64_t p = blk + (int64_t)w * chunk;
-      if (p >= x - s && p < x) {
-        where[w][0] = b;
-        where[w][1] = (int)p - (x - s);
-      }
-    }
-    before += wsum[0] + wsum[1] + wsum[2] + wsum[3];
-    if (blk + (int64_t)(W - 1) * chunk < before || before == tot) break;  // (the same in every thread)
+    before = __builtin_amdgcn_readlane(x, 63);
+    if (cur < before) break;
   }
-  __syncthreads();
-  const int share = blockIdx.x * W + wave;
-  if (blk + (int64_t)wave * chunk >= tot) return;  // (no barrier below)
-  int cur = (int)blk + wave * chunk;
-  const int end = (int)min((int64_t)tot, (int64_t)cur + chunk);
-  int b = __builtin_amdgcn_readfirstlane(where[wave][0]);
-  int at_row = __builtin_amdgcn_readfirstlane(where[wave][1]);
+  const int owner = __builtin_ctzll(__ballot(cur < x));  // the lane whose sequences hold cur
+  int at_row = cur - __builtin_amdgcn_readlane(x - mine, owner);
+  int b = b0 + 4 * owner;
+#pragma unroll
+  for (int i = 0; i < 3; i++) {
+    const int s = __builtin_amdgcn_readlane(four[i], owner) * Hh;
+    if (b == b0 + 4 * owner + i && at_row >= s) {
+      at_row -= s;
+      b++;
+    }
+  }
   Span sp = span(d, b);
-  int hh = at_row / cost(sp);
+  int hh = (int)((unsigned)at_row / (unsigned)cost(sp));
   at_row -= hh * cost(sp);  // the share starts this far into the row
 
   const float cap = a.softcap;
@@ -424,6 +443,7 @@ k_decode(const Dev d) {
     const bool whole = st == 0 && s1 == sq.steps;
     const int slot = 2 * share + (st == 0);
     const float vs = a.v_scale ? a.v_scale[h] : 1.f;
+    const size_t row0 = (size_t)bb * a.Hq + h * d.G + q0;
 #pragma unroll
     for (int t = 0; t < HT; t++) {
       l[t] += __shfl_xor(l[t], 16, 64);
@@ -431,7 +451,6 @@ k_decode(const Dev d) {
       const int q = 16 * t + c;
       if (q >= nq) continue;
       if (whole) {
-        const size_t row = (size_t)bb * a.Hq + h * d.G + q0 + q;
         const float f = l[t] == 0.f ? 0.f : vs / l[t];
 #pragma unroll
         for (int nb = 0; nb < NB; nb++)
@@ -442,9 +461,9 @@ k_decode(const Dev d) {
             uint32_t w[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) w[j] = pack2<DT>(o[t][nb][2 * j][i] * f, o[t][nb][2 * j + 1][i] * f);
-            __builtin_memcpy((uint16_t*)a.out + row * a.D + dim, w, 16);
+            __builtin_memcpy((uint16_t*)a.out + (row0 + q) * a.D + dim, w, 16);
           }
-        if (g == 0 && a.lse) a.lse[row] = m[t] == -kInf ? m[t] + l[t] : (m[t] - kOff + __log2f(l[t])) * kLn2;
+        if (g == 0 && a.lse) a.lse[row0 + q] = lse_of<DT>(m[t], l[t]);
       } else {
         float* po = d.po + ((size_t)slot * 16 * HT + q) * a.D;
 #pragma unroll
@@ -460,84 +479,92 @@ k_decode(const Dev d) {
         if (g == 0) *(float2*)(d.pml + ((size_t)slot * 16 * HT + q) * 2) = make_float2(m[t], l[t]);
       }
     }
-    if (st == 0 && lane == 0)
-      d.info[(size_t)bb * Hh + row_of_b] =
-          make_int2(share, whole ? 1 : 1 + (int)(((unsigned)(sq.steps - s1) + chunk - 1) / (unsigned)chunk));
+    if (st == 0 && !whole)
+      cut = make_int2(bb * Hh + row_of_b, 1 + (int)(((unsigned)(sq.steps - s1) + chunk - 1) / (unsigned)chunk));
   }
+  if (lane == 0) d.cut[share] = cut;
 }
 
-// One workgroup per (sequence, query head): the partial sums of a row that was
-// cut, in the order of the shares; zeros for a row without tokens.  Thread (dim
-// / 4, r) adds every R-th share, the R sums meet in LDS.
+// Workgroup i: the row that starts in share i and is cut, if there is one.
+// Thread (u, column) adds four dims of one head over every U-th of the row's
+// shares, four of them in flight, under a running maximum; the U sums meet in
+// LDS, in order.
 template <int DT>
-__global__ void __launch_bounds__(256) k_join(const Dev d, int heads) {
-  constexpr float kOff = DT == UB_F16 ? 14.f : 0.f;
-  __shared__ float wt[256], red[4];
-  __shared__ float4 part[256];
+__global__ void __launch_bounds__(512) k_join(const Dev d, int heads) {
+  __shared__ float4 so[512];
+  __shared__ float2 sml[512];
   const UbridgePagedDecodeArgs& a = d.a;
-  const int b = blockIdx.x / a.Hq, hq = blockIdx.x - b * a.Hq, h = hq / d.G;
-  const int hg = (hq - h * d.G) / heads, q = hq - h * d.G - hg * heads;
-  const int tid = threadIdx.x;
-  const size_t row = (size_t)b * a.Hq + hq;
-  const int2 in = d.info[((size_t)b * a.Hkv + h) * d.HG + hg];  // (read ahead of the test below)
-  if (span(d, b).steps == 0) {
-    if (tid < a.D) ub_store<DT>(a.out, row * a.D + tid, 0.f);
-    if (tid == 0 && a.lse) a.lse[row] = -kInf;
-    return;
-  }
-  if (in.y == 1) return;  // (k_decode has written it)
-  auto slot = [&](int p) { return (size_t)(2 * (in.x + p) + (p == 0)) * heads + q; };
-  auto all = [&](float v, bool mx) {
+  const int2 cut = d.cut[blockIdx.x];
+  if (cut.x < 0) return;
+  const int Hh = a.Hkv * d.HG, b = cut.x / Hh, hh = cut.x - b * Hh;
+  const int h = hh / d.HG, q0 = (hh - h * d.HG) * heads;
+  const int V = a.D / 4, cols = min(d.G - q0, heads) * V;
+  const int U = cols < 512 ? 512 / cols : 1;
+  const float vs = a.v_scale ? a.v_scale[h] : 1.f;
+  for (int c0 = 0; c0 < cols; c0 += 512) {
+    const int u = (int)threadIdx.x / cols, col = c0 + (int)threadIdx.x - u * cols;
+    const int q = col / V, v = col - q * V;
+    const bool live = u < U && col < cols;
+    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+    float M = -kInf, L = 0.f;
+    if (live)
+      for (int p0 = u; p0 < cut.y; p0 += 4 * U) {
+        float2 ml[4];
+        float4 x[4];
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-      const float y = __shfl_xor(v, o, 64);
-      v = mx ? fmaxf(v, y) : v + y;
-    }
-    __syncthreads();
-    if ((tid & 63) == 0) red[tid >> 6] = v;
-    __syncthreads();
-    return mx ? fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])) : red[0] + red[1] + red[2] + red[3];
-  };
-  float M = -kInf, L = 0.f;
-  for (int p = tid; p < in.y; p += 256) M = fmaxf(M, d.pml[2 * slot(p)]);
-  M = all(M, true);
-  const float Ms = M == -kInf ? 0.f : M;
-  const int V = a.D / 4, R = 256 / V;  // (D / 4 >= 2 threads a share)
-  const int v = tid % V, r = tid / V;
-  float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int p0 = 0; p0 < in.y; p0 += 256) {
-    float w = 0.f;
-    if (p0 + tid < in.y) {
-      const float2 ml = *(const float2*)(d.pml + 2 * slot(p0 + tid));
-      w = __builtin_amdgcn_exp2f(ml.x - Ms);
-      L += w * ml.y;
-    }
-    __syncthreads();
-    wt[tid] = w;
-    __syncthreads();
-    if (r < R)
-      for (int p = r; p < min(256, in.y - p0); p += R) {
-        const float4 x = *(const float4*)(d.po + slot(p0 + p) * a.D + 4 * v);
-        const float f = wt[p];
-        O.x += f * x.x, O.y += f * x.y, O.z += f * x.z, O.w += f * x.w;
+        for (int i = 0; i < 4; i++) {
+          const int p = min(p0 + i * U, cut.y - 1);
+          const size_t slot = (size_t)(2 * ((int)blockIdx.x + p) + (p == 0)) * heads + q;
+          ml[i] = *(const float2*)(d.pml + 2 * slot);
+          x[i] = *(const float4*)(d.po + slot * a.D + 4 * v);
+        }
+        float mn = M;
+#pragma unroll
+        for (int i = 0; i < 4; i++) mn = fmaxf(mn, ml[i].x);
+        const float ms = mn == -kInf ? 0.f : mn, al = __builtin_amdgcn_exp2f(M - ms);
+        M = mn;
+        O.x *= al, O.y *= al, O.z *= al, O.w *= al, L *= al;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          if (p0 + i * U >= cut.y) continue;
+          const float w = __builtin_amdgcn_exp2f(ml[i].x - ms);
+          O.x += w * x[i].x, O.y += w * x[i].y, O.z += w * x[i].z, O.w += w * x[i].w;
+          L += w * ml[i].y;
+        }
       }
+    if (U > 1) {
+      so[threadIdx.x] = O;
+      sml[threadIdx.x] = make_float2(M, L);
+      __syncthreads();
+      if (u == 0) {
+        float mn = M;
+        for (int i = 1; i < U; i++) mn = fmaxf(mn, sml[threadIdx.x + i * cols].x);
+        const float ms = mn == -kInf ? 0.f : mn, al = __builtin_amdgcn_exp2f(M - ms);
+        M = mn;
+        O.x *= al, O.y *= al, O.z *= al, O.w *= al, L *= al;
+        for (int i = 1; i < U; i++) {
+          const float2 ml = sml[threadIdx.x + i * cols];
+          const float4 x = so[threadIdx.x + i * cols];
+          const float w = __builtin_amdgcn_exp2f(ml.x - ms);
+          O.x += w * x.x, O.y += w * x.y, O.z += w * x.z, O.w += w * x.w;
+          L += w * ml.y;
+        }
+      }
+    }
+    if (live && u == 0) {
+      const size_t row = (size_t)b * a.Hq + h * d.G + q0 + q;
+      const float f = L == 0.f ? 0.f : vs / L;
+      const uint32_t w[2] = {pack2<DT>(O.x * f, O.y * f), pack2<DT>(O.z * f, O.w * f)};
+      __builtin_memcpy((uint16_t*)a.out + row * a.D + 4 * v, w, 8);
+      if (v == 0 && a.lse) a.lse[row] = lse_of<DT>(M, L);
+    }
   }
-  L = all(L, false);
-  part[tid] = O;
-  __syncthreads();
-  const float f = L == 0.f ? 0.f : (a.v_scale ? a.v_scale[h] : 1.f) / L;
-  if (tid < a.D) {
-    float s = 0.f;
-    for (int i = 0; i < R; i++) s += ((const float*)&part[i * V + tid / 4])[tid % 4];
-    ub_store<DT>(a.out, row * a.D + tid, s * f);
-  }
-  if (tid == 0 && a.lse) a.lse[row] = M == -kInf ? M + L : (M - kOff + __log2f(L)) * kLn2;
 }
 
 template <int DT, int CT, int DK, bool PG8>
 void decode(const Dev& d, int HT, hipStream_t s) {
-  if (HT == 1) k_decode<DT, CT, DK, PG8, 1><<<(1 << d.lg_shares) / W, 64 * W, 0, s>>>(d);
-  else k_decode<DT, CT, DK, PG8, 2><<<(1 << d.lg_shares) / W, 64 * W, 0, s>>>(d);
+  if (HT == 1) k_decode<DT, CT, DK, PG8, 1><<<d.shares / W, 64 * W, 0, s>>>(d);
+  else k_decode<DT, CT, DK, PG8, 2><<<d.shares / W, 64 * W, 0, s>>>(d);
 }
 template <int DT, int CT, int DK>
 void decode(const Dev& d, int HT, hipStream_t s) {
@@ -551,7 +578,7 @@ void decode(const Dev& d, int HT, hipStream_t s) {
   else if (d.a.D <= 128) decode<DT, CT, 4>(d, HT, s);
   else if (d.a.D <= 192) decode<DT, CT, 6>(d, HT, s);
   else decode<DT, CT, 8>(d, HT, s);
-  k_join<DT><<<d.a.B * d.a.Hq, 256, 0, s>>>(d, 16 * HT);
+  k_join<DT><<<d.shares, 512, 0, s>>>(d, 16 * HT);
 }
 
 }  // namespace
@@ -581,19 +608,19 @@ UB_API int ubridge_paged_decode(const UbridgePagedDecodeArgs* p, void* stream) {
   const int HT = d.G > 16 ? 2 : 1, heads = 16 * HT;
   d.HG = ub_cdiv(d.G, heads);
   const int64_t rows = (int64_t)a.B * a.Hkv * d.HG;
-  UB_REQUIRE(rows * ((int64_t)a.width * a.S / 32 + 1 + kRowCost) < 0x7fffffff,
-             "%s: %ld rows of %ld tokens", nm, (long)rows, (long)a.width * a.S);
+  const int64_t most = rows * ((int64_t)a.width * a.S / 32 + 1 + kRowCost);  // the costs of all rows
+  UB_REQUIRE(most < 0x7fffffff, "%s: %ld rows of %ld tokens", nm, (long)rows, (long)a.width * a.S);
   d.s_shift = 31;
   while ((1ll << (d.s_shift - 31)) < a.S) d.s_shift++;
   d.s_mul = (1ull << d.s_shift) / a.S + 1;
-  d.lg_shares = 11;
-  const size_t nml = sizeof(float) * 4 * heads << d.lg_shares, no = nml / 2 * a.D;
+  d.shares = most >= kShares ? kShares : ub_cdiv(most, W) * W;
+  const size_t nml = sizeof(float) * 4 * heads * d.shares, no = nml / 2 * a.D;
   hipStream_t s = ub_stream(stream);
-  UbScratch ws(s, no + nml + sizeof(int2) * rows);
+  UbScratch ws(s, no + nml + sizeof(int2) * d.shares);
   if (!ws.get()) return ub_set_error(UB_ERR_LAUNCH, "%s: no workspace", nm);
   d.po = (float*)ws.get();
   d.pml = d.po + no / sizeof(float);
-  d.info = (int2*)((char*)ws.get() + no + nml);
+  d.cut = (int2*)((char*)ws.get() + no + nml);
   if (a.dtype == UB_BF16 && a.cache_dtype == UB_BF16) decode<UB_BF16, UB_BF16>(d, HT, s);
   else if (a.dtype == UB_BF16) decode<UB_BF16, UB_E4M3>(d, HT, s);
   else if (a.cache_dtype == UB_F16) decode<UB_F16, UB_F16>(d, HT, s);
