@@ -1,92 +1,472 @@
 // int8.hip -- int8 W8A8 linear on gfx950:
 //
-//   y[m, n] = T( (sum_k a[m, k] w[n, k]) sa[m] sw[n] + bias[n] )
+//   y[m, n] = T( (sum_k a[m, k] w[n, k]) sw[n] sa[m] + bias[n] )
 //
 // a[m, k] = round(x[m, k] / sa[m]) (ties to even), sa[m] = max_k |x[m, k]| /
 // 127, or 1 for a row of zeros; sw one f32 scale an output channel.  The dot is
 // exact in int32 (|a w| <= 127 * 128, so K <= 132104), the epilogue f32, and
 // the sum rounds once, to x's type T.  The weight's scale is multiplied in first:
-// sa reaches both ends of f32, and with it first rows near the top overflowed.  A row that holds an infinity or a NaN
-// has no scale and gives a row of NaN.
+// sa reaches both ends of f32, and with it first rows near the top overflowed.  A
+// row that holds an infinity or a NaN has no scale and gives a row of NaN.
 //
 // Rows of a and w are padded with zeros to ld bytes, a multiple of 128.
+//
+// Up to 16 tokens the product is a stream of the weight and one kernel does it
+// all (k_i8_dec); beyond, k_quant makes the codes and k_i8_gemm multiplies them.
 #include "common.h"
+#include "lds_dma.h"
+
+#include <type_traits>
 
 namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
 
+template <int DT> struct Elem { typedef uint16_t T; static constexpr int E = 8; };  // 16-byte units
+template <> struct Elem<UB_F32> { typedef float T; static constexpr int E = 4; };
+
+// element e of a unit
 template <int DT>
-__device__ __forceinline__ float row_scale(float amax) {
-  // (an infinite or NaN maximum: no scale)
-  return !(amax < __builtin_inff()) ? __builtin_nanf("") : amax > 0.f ? __fdiv_rn(amax, 127.0f) : 1.0f;
+__device__ __forceinline__ float get(const uint4& w, int e) {
+  const uint32_t p[4] = {w.x, w.y, w.z, w.w};
+  if constexpr (DT == UB_F32) return __uint_as_float(p[e]);
+  else if constexpr (DT == UB_F16) return ub_f16_to_f32((uint16_t)(p[e >> 1] >> (16 * (e & 1))));
+  else return __uint_as_float((e & 1) ? p[e >> 1] & 0xffff0000u : p[e >> 1] << 16);
 }
 
-// code of x under scale s: |x / s| <= 127 up to the rounding of s, which for
-// a denormal s is as large as s (hence the clamp); 0 where s is NaN or 0
-__device__ __forceinline__ int code(float x, float s) {
-  const float q = rintf(__fdiv_rn(x, s));
-  return q == q ? (int)fminf(fmaxf(q, -127.f), 127.f) : 0;
+// Unit i of a row of K elements at p, zeros past its end.  The row may start
+// at any element: gfx950 loads 16 bytes from there.
+template <int DT>
+__device__ __forceinline__ uint4 unit(const typename Elem<DT>::T* p, int i, int K) {
+  constexpr int E = Elem<DT>::E;
+  uint4 v = make_uint4(0, 0, 0, 0);
+  const int n = K - i * E;
+  if (n >= E) {
+    __builtin_memcpy(&v, p + i * E, 16);
+  } else if (n > 0) {
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < E; e++)
+      if (e < n) {
+        if constexpr (DT == UB_F32) w[e] = __float_as_uint(p[i * E + e]);
+        else w[e >> 1] |= (uint32_t)p[i * E + e] << (16 * (e & 1));
+      }
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return v;
 }
 
-// One workgroup a row.
+// A row's maximum is taken over bit patterns without sign, which order like
+// the values and put infinities and NaN on top.
 template <int DT>
-__global__ void __launch_bounds__(256) k_quant(const void* __restrict__ x, int8_t* __restrict__ q,
-                                               float* __restrict__ scale, int K, int ld) {
-  __shared__ float wm[4];
+__device__ __forceinline__ uint32_t top_of(const uint4& u, uint32_t t) {
+#pragma unroll
+  for (int e = 0; e < Elem<DT>::E; e++) t = max(t, __float_as_uint(get<DT>(u, e)) & 0x7fffffffu);
+  return t;
+}
+__device__ __forceinline__ float scale_of(uint32_t top) {
+  return top >= 0x7f800000u ? __builtin_nanf("") : top == 0 ? 1.0f : __fdiv_rn(__uint_as_float(top), 127.0f);
+}
+
+// The codes of a unit under scale s.  The quotient is x r (r = 1 / s) corrected
+// twice by its exact residual x - q s (Markstein's division: the second
+// correction gives the correctly rounded x / s), 5 operations where the IEEE
+// divide takes 11; for s outside [2^-60, 2^60], where residuals underflow, it
+// divides (plain = true).  Adding 1.5 2^23 rounds to an integer, ties to even,
+// in the low bits.  |x / s| <= 127, but for a denormal s, whose own rounding is
+// as large as s (hence the clamp); a NaN or zero s has codes 0.
+template <int DT>
+__device__ __forceinline__ void codes(const uint4& u, float s, float r, bool plain, uint32_t (&o)[Elem<DT>::E / 4]) {
+  constexpr int E = Elem<DT>::E;
+  uint32_t c[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const float v = get<DT>(u, e);
+    float q;
+    if (plain) {
+      q = __fdiv_rn(v, s);
+      q = q == q ? fminf(fmaxf(q, -127.f), 127.f) : 0.f;
+    } else {
+      q = v * r;
+      q = __builtin_fmaf(__builtin_fmaf(-q, s, v), r, q);
+      q = __builtin_fmaf(__builtin_fmaf(-q, s, v), r, q);
+    }
+    c[e] = __float_as_uint(q + 12582912.f);
+  }
+#pragma unroll
+  for (int h = 0; h < E / 4; h++)
+    o[h] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[4 * h + 3], c[4 * h + 2], 0x0c0c0400u),
+                                 __builtin_amdgcn_perm(c[4 * h + 1], c[4 * h], 0x0c0c0400u), 0x05040100u);
+}
+__device__ __forceinline__ bool plain_scale(float s) { return !(s >= 0x1p-60f && s <= 0x1p60f); }
+
+// One workgroup of NT threads a row; a thread keeps NV units of it in registers,
+// so the row is read once.  NV = 0: rows of any length, read twice.
+template <int DT, int NT, int NV>
+__global__ void __launch_bounds__(NT) k_quant(const void* __restrict__ x, int8_t* __restrict__ q,
+                                              float* __restrict__ scale, int K, int ld) {
+  constexpr int E = Elem<DT>::E, N = NV ? NV : 1;
+  __shared__ uint32_t wm[NT / 64];
   const int tid = threadIdx.x;
-  const size_t r = blockIdx.x;
-  float amax = 0.f;
-  bool bad = false;
-  for (int c = tid; c < K; c += 256) {
-    const float v = fabsf(ub_load<DT>(x, r * K + c));
-    bad |= !(v < __builtin_inff());
-    amax = fmaxf(amax, v);
-  }
-  if (bad) amax = __builtin_inff();
+  const size_t row = blockIdx.x;
+  const typename Elem<DT>::T* p = (const typename Elem<DT>::T*)x + row * K;
+  uint4 u[N];
+  uint32_t top = 0;
+  if constexpr (NV > 0) {
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
-  if ((tid & 63) == 0) wm[tid >> 6] = amax;
+    for (int j = 0; j < NV; j++) u[j] = unit<DT>(p, tid + j * NT, K);
+#pragma unroll
+    for (int j = 0; j < NV; j++) top = top_of<DT>(u[j], top);
+  } else {
+    for (int i = tid; i * E < K; i += NT) top = top_of<DT>(unit<DT>(p, i, K), top);
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+  if ((tid & 63) == 0) wm[tid >> 6] = top;
   __syncthreads();
-  amax = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
-  const float s = row_scale<DT>(amax);
-  for (int c = tid; c < ld; c += 256)
-    q[r * ld + c] = c < K ? (int8_t)code(ub_load<DT>(x, r * K + c), s) : (int8_t)0;
-  if (tid == 0) scale[r] = s;
-}
-
-// One wavefront per 16 x 16 outputs: v_mfma_i32_16x16x64_i8 on fragments
-// straight from memory.
-template <int DT>
-__global__ void __launch_bounds__(64) k_i8_gemm(const int8_t* __restrict__ a,
-                                                const float* __restrict__ sa,
-                                                const int8_t* __restrict__ w,
-                                                const float* __restrict__ sw,
-                                                const float* __restrict__ bias,
-                                                void* __restrict__ y, int M, int N, int ld) {
-  const int lane = threadIdx.x, r = lane & 15, h = lane >> 4;
-  const int m0 = blockIdx.y * 16, n0 = blockIdx.x * 16;
-  const int8_t* pa = a + (size_t)min(m0 + r, M - 1) * ld + 16 * h;
-  const int8_t* pw = w + (size_t)min(n0 + r, N - 1) * ld + 16 * h;
-  i32x4 acc = {0, 0, 0, 0};
-  for (int k = 0; k < ld; k += 64)
-    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const i32x4*)(pa + k), *(const i32x4*)(pw + k), acc,
-                                                0, 0, 0);
-  const int n = n0 + r;
-  if (n >= N) return;
-  const float s = sw[n], b = bias ? bias[n] : 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const int m = m0 + 4 * h + i;
-    if (m < M) ub_store<DT>(y, (size_t)m * N + n, (float)acc[i] * s * sa[m] + b);
+  for (int w = 0; w < NT / 64; w++) top = max(top, wm[w]);
+  const float s = scale_of(top);
+  if (tid == 0) scale[row] = s;
+  const bool plain = plain_scale(s);
+  const float r = plain ? 0.f : __fdiv_rn(1.0f, s);
+  auto store = [&](const uint4& v, int i) {
+    uint32_t o[E / 4];
+    codes<DT>(v, s, r, plain, o);
+    if constexpr (E == 4) ((uint32_t*)(q + row * ld))[i] = o[0];
+    else ((uint2*)(q + row * ld))[i] = make_uint2(o[0], o[1]);
+  };
+  if constexpr (NV > 0) {
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+      if ((tid + j * NT) * E < ld) store(u[j], tid + j * NT);
+  } else {
+    for (int i = tid; i * E < ld; i += NT) store(unit<DT>(p, i, K), i);
   }
 }
 
 template <int DT>
-void linear(const void* x, const int8_t* w, const float* sw, const float* bias, void* y, int8_t* q,
-            float* sa, int M, int K, int N, int ld, hipStream_t s) {
-  k_quant<DT><<<M, 256, 0, s>>>(x, q, sa, K, ld);
-  k_i8_gemm<DT><<<dim3(ub_cdiv(N, 16), ub_cdiv(M, 16)), 64, 0, s>>>(q, sa, w, sw, bias, y, M, N, ld);
+__device__ __forceinline__ void put(void* y, size_t i, int acc, float sa, float sw, float b) {
+  ub_store<DT>(y, i, (float)acc * sw * sa + b);
+}
+
+// ------------------------------------------------------------------ tiles
+// WM x WN wavefronts of 32 TM x 32 TN outputs each, v_mfma_i32_32x32x32_i8.  The
+// operands reach LDS by direct loads in 64-byte halves of a 128-byte K-step,
+// each row of 64 bytes swizzled in 16-byte units (unit u of row r at u ^ ((r >>
+// 2) & 3)) so that the 16 rows of a fragment read lie in distinct banks.  Two
+// steps are in LDS: the products of a step's first half run on fragments
+// read before while the second half is read; then the next step is waited
+// for, the barrier frees this step's buffers for the loads of the one after,
+// and the second half's products run while the next first half is read.
+template <int DT, int WM, int WN, int TM, int TN, int OCC>
+__global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
+k_i8_gemm(const int8_t* __restrict__ A, const float* __restrict__ sa, const int8_t* __restrict__ B,
+          const float* __restrict__ sw, const float* __restrict__ bias, void* __restrict__ y, int M,
+          int N, int ld) {
+  constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN, NW = WM * WN;
+  constexpr int NA = BM / 16 / NW, NB = BN / 16 / NW;  // load instructions of a wavefront and half
+  constexpr int AB = BM * 64, HALF = (BM + BN) * 64;   // bytes
+  static_assert(NA * NW * 16 == BM && NB * NW * 16 == BN, "whole load instructions");
+  __shared__ __attribute__((aligned(16))) uint8_t h0[HALF], h1[HALF], h2[HALF], h3[HALF];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  int tile_m, tile_n;
+  ub_tile_order((M + BM - 1) / BM, (N + BN - 1) / BN, 8, tile_m, tile_n);
+  const int n0 = tile_n * BN, m0 = tile_m * BM;
+  // rows past the end lie past the buffers: zeros
+  const ub_u32x4 ra = ub_desc(A + (size_t)m0 * ld, (uint64_t)min(BM, M - m0) * ld);
+  const ub_u32x4 rb = ub_desc(B + (size_t)n0 * ld, (uint64_t)min(BN, N - n0) * ld);
+  uint32_t va[NA], vb[NB];
+#pragma unroll
+  for (int i = 0; i < NA; i++) {
+    const int u = (i * NW + wave) * 64 + lane, row = u >> 2;
+    va[i] = (uint32_t)row * (uint32_t)ld + 16 * ((u & 3) ^ ((row >> 2) & 3));
+  }
+#pragma unroll
+  for (int i = 0; i < NB; i++) {
+    const int u = (i * NW + wave) * 64 + lane, row = u >> 2;
+    vb[i] = (uint32_t)row * (uint32_t)ld + 16 * ((u & 3) ^ ((row >> 2) & 3));
+  }
+  auto issue = [&](int kt, uint8_t* st) {
+    const uint32_t sb = ub_lds_addr(st), k0 = (uint32_t)(kt * 64);
+#pragma unroll
+    for (int i = 0; i < NA; i++) ub_lds_load16_at(ra, sb + (i * NW + wave) * 1024, va[i], k0);
+#pragma unroll
+    for (int i = 0; i < NB; i++) ub_lds_load16_at(rb, sb + AB + (i * NW + wave) * 1024, vb[i], k0);
+  };
+  i32x16 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; i++)
+#pragma unroll
+    for (int j = 0; j < TN; j++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[i][j][r] = 0;
+  const int l32 = lane & 31, kh = lane >> 5;
+  // units 2 kh and 2 kh + 1 of a row: a lane's part of two products
+  i32x4 af[2][TM][2], bf[2][TN][2];
+  auto frag = [&](i32x4 (&f)[2], const uint8_t* t, int row) {
+    const int sz = (row >> 2) & 3;
+    f[0] = *(const i32x4*)(t + row * 64 + (((2 * kh) ^ sz) * 16));
+    f[1] = *(const i32x4*)(t + row * 64 + (((2 * kh + 1) ^ sz) * 16));
+  };
+  auto read_frags = [&](const uint8_t* st, int b) {
+#pragma unroll
+    for (int i = 0; i < TM; i++) frag(af[b][i], st, wm * 32 * TM + 32 * i + l32);
+#pragma unroll
+    for (int j = 0; j < TN; j++) frag(bf[b][j], st + AB, wn * 32 * TN + 32 * j + l32);
+  };
+  auto mfmas = [&](int b) {
+#pragma unroll
+    for (int q = 0; q < 2; q++)
+#pragma unroll
+      for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int i = 0; i < TM; i++)
+          acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(af[b][i][q], bf[b][j][q], acc[i][j], 0, 0, 0);
+  };
+  auto interleave = [&]() {
+#pragma unroll
+    for (int q = 0; q < 2 * TM * TN; q++) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // 1 MFMA
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // 1 DS read
+    }
+  };
+  const int nks = ld / 128;
+  auto stage = [&](auto Pc, int j) {
+    constexpr int P = decltype(Pc)::value;
+    uint8_t* a0 = P ? h2 : h0;
+    uint8_t* a1 = P ? h3 : h1;
+    uint8_t* nx = P ? h0 : h2;
+    mfmas(0);
+    read_frags(a1, 1);
+    interleave();
+    if (j + 1 < nks) {
+      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this step's fragments are read
+      ub_wait_vmcnt<0>();                  // the next step has landed
+      ub_barrier();
+      if (j + 2 < nks) {
+        issue(2 * (j + 2), a0);
+        issue(2 * (j + 2) + 1, a1);
+      }
+    }
+    mfmas(1);
+    read_frags(nx, 0);  // (after the last step: stale, not used)
+    interleave();
+  };
+  issue(0, h0);
+  issue(1, h1);
+  if (nks > 1) {
+    issue(2, h2);
+    issue(3, h3);
+    ub_wait_vmcnt<2 * (NA + NB)>();
+  } else {
+    ub_wait_vmcnt<0>();
+  }
+  ub_barrier();
+  read_frags(h0, 0);
+  for (int j = 0; j < nks; j += 2) {
+    stage(std::integral_constant<int, 0>{}, j);
+    if (j + 1 < nks) stage(std::integral_constant<int, 1>{}, j + 1);
+  }
+#pragma unroll
+  for (int j = 0; j < TN; j++) {
+    const int n = n0 + wn * 32 * TN + 32 * j + l32;
+    if (n >= N) continue;
+    const float s = sw[n], b = bias ? bias[n] : 0.f;
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const int m = m0 + wm * 32 * TM + 32 * i + 8 * (r >> 2) + 4 * kh + (r & 3);
+        if (m < M) put<DT>(y, (size_t)m * N + n, acc[i][j][r], sa[m], s, b);
+      }
+  }
+}
+
+// ----------------------------------------------------------- few tokens
+// Up to 16 tokens: HBM-bound, so shaped for bytes in flight.  A persistent grid
+// of one 16-wavefront workgroup a CU walks tiles of 16 weight rows; the
+// wavefronts split K in 64-byte steps (wavefront w the steps w, w + 16, ...),
+// SP of which they load at once straight into registers, and the next SP are
+// in flight while these are multiplied: v_mfma_i32_16x16x64_i8, tokens as A
+// rows.  The codes of the activations lie in LDS for the whole launch, rows 16
+// bytes further apart than they are long, so that the 16 rows of a fragment
+// read spread over the banks.  Each workgroup makes them itself, one wavefront a
+// row, after its first weight loads are on their way: a launch less, and
+// quantizing M K values hides behind the stream.  The wavefronts' sums meet
+// in LDS.
+constexpr int DW = 16;
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* base, uint64_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
+}
+
+template <int DT, int SP>
+__global__ void __launch_bounds__(64 * DW) k_i8_dec(const void* __restrict__ x, const int8_t* __restrict__ W,
+                                                    const float* __restrict__ sw, const float* __restrict__ bias,
+                                                    void* __restrict__ y, int M, int K, int N, int ld) {
+  constexpr int E = Elem<DT>::E;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  int* red = (int*)lds;                       // [16 wavefronts][M][17]
+  float* ssa = (float*)(red + DW * M * 17);   // [16]
+  uint8_t* a = (uint8_t*)(ssa + 16);          // [M][ld + 16]
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, h = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int steps = ld / 64, nc = (steps + DW * SP - 1) / (DW * SP), nt = (N + 15) / 16;
+  const int pitch = ld + 16;
+  const uint32_t row = (uint32_t)r * (uint32_t)ld + 16u * h;
+  i32x4 b0[SP], b1[SP];
+  // piece c of tile t; past the last tile or K: zeros
+  auto load = [&](i32x4 (&b)[SP], int t, int c) {
+    const int rows = t < nt ? min(16, N - 16 * t) : 0;
+    const __amdgpu_buffer_rsrc_t rw = rsrc(W + (size_t)16 * min(t, nt - 1) * ld, (uint64_t)rows * ld);
+#pragma unroll
+    for (int i = 0; i < SP; i++) {
+      const int s = (c * SP + i) * DW + wave;
+      b[i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rw, (int)(s < steps ? row + 64u * s : 0x80000000u), 0, 0));
+    }
+  };
+  int t = blockIdx.x, c = 0;  // the piece being multiplied
+  auto next = [&](int& t, int& c) {
+    if (++c == nc) {
+      c = 0;
+      t += gridDim.x;
+    }
+  };
+  int tn = t, cn = c;
+  load(b0, tn, cn);
+  next(tn, cn);
+  load(b1, tn, cn);
+  next(tn, cn);
+  for (int m = wave; m < M; m += DW) {
+    const typename Elem<DT>::T* p = (const typename Elem<DT>::T*)x + (size_t)m * K;
+    uint32_t top = 0;
+    for (int i = lane; i * E < K; i += 64) top = top_of<DT>(unit<DT>(p, i, K), top);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+    const float s = scale_of(top);
+    const bool plain = plain_scale(s);
+    const float rs = plain ? 0.f : __fdiv_rn(1.0f, s);
+    if (lane == 0) ssa[m] = s;
+    for (int i = lane; i * E < ld; i += 64) {
+      uint32_t o[E / 4];
+      codes<DT>(unit<DT>(p, i, K), s, rs, plain, o);
+      if constexpr (E == 4) *(uint32_t*)(a + m * pitch + 4 * i) = o[0];
+      else *(uint2*)(a + m * pitch + 8 * i) = make_uint2(o[0], o[1]);
+    }
+  }
+  __syncthreads();
+  i32x4 acc = {0, 0, 0, 0};
+  const uint8_t* ar = a + min(r, M - 1) * pitch + 16 * h;  // (tokens past M: not used)
+  auto work = [&](i32x4 (&b)[SP]) {
+#pragma unroll
+    for (int i = 0; i < SP; i++) {
+      const int s = min((c * SP + i) * DW + wave, steps - 1);  // (past K: times zeros)
+      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const i32x4*)(ar + 64 * s), b[i], acc, 0, 0, 0);
+    }
+    load(b, tn, cn);
+    next(tn, cn);
+    if (c == nc - 1) {
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (4 * h + i < M) red[(wave * M + 4 * h + i) * 17 + r] = acc[i];
+      acc = (i32x4){0, 0, 0, 0};
+      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0); the weight loads stay in flight
+      ub_barrier();
+      const int m = tid >> 4, n = 16 * t + (tid & 15);
+      if (m < M) {
+        int v = 0;
+#pragma unroll
+        for (int w = 0; w < DW; w++) v += red[(w * M + m) * 17 + (tid & 15)];
+        if (n < N) put<DT>(y, (size_t)m * N + n, v, ssa[m], sw[n], bias ? bias[n] : 0.f);
+      }
+      __builtin_amdgcn_s_waitcnt(0xC07F);
+      ub_barrier();
+    }
+    next(t, c);
+  };
+  while (t < nt) {
+    work(b0);
+    if (t >= nt) break;
+    work(b1);
+  }
+}
+
+constexpr int kLds = 160 * 1024;  // of a CU
+size_t dec_lds(int M, int ld) { return sizeof(int) * DW * M * 17 + 64 + (size_t)M * (ld + 16); }
+
+template <int DT, int SP>
+void dec(const void* x, const int8_t* w, const float* sw, const float* bias, void* y, int M, int K, int N, int ld,
+         hipStream_t s) {
+  static const hipError_t once =  // (beyond 64 KiB)
+      hipFuncSetAttribute((const void*)k_i8_dec<DT, SP>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+  (void)once;
+  const int nt = ub_cdiv(N, 16);
+  k_i8_dec<DT, SP><<<nt < 256 ? nt : 256, 64 * DW, dec_lds(M, ld), s>>>(x, w, sw, bias, y, M, K, N, ld);
+}
+// SP: a wavefront's steps, evened out over as few pieces of at most eight
+template <int DT>
+void dec(const void* x, const int8_t* w, const float* sw, const float* bias, void* y, int M, int K, int N, int ld,
+         hipStream_t s) {
+  const int per = ub_cdiv(ld / 64, DW), sp = ub_cdiv(per, ub_cdiv(per, 8));
+  if (sp <= 1) dec<DT, 1>(x, w, sw, bias, y, M, K, N, ld, s);
+  else if (sp <= 2) dec<DT, 2>(x, w, sw, bias, y, M, K, N, ld, s);
+  else if (sp <= 4) dec<DT, 4>(x, w, sw, bias, y, M, K, N, ld, s);
+  else if (sp <= 6) dec<DT, 6>(x, w, sw, bias, y, M, K, N, ld, s);
+  else dec<DT, 8>(x, w, sw, bias, y, M, K, N, ld, s);
+}
+
+template <int DT, int NT>
+bool quant(const void* x, int8_t* q, float* sa, int M, int K, int ld, hipStream_t s) {
+  const int nv = ub_cdiv(ld / Elem<DT>::E, NT);
+  if (nv <= 1) k_quant<DT, NT, 1><<<M, NT, 0, s>>>(x, q, sa, K, ld);
+  else if (nv <= 2) k_quant<DT, NT, 2><<<M, NT, 0, s>>>(x, q, sa, K, ld);
+  else if (nv <= 4) k_quant<DT, NT, 4><<<M, NT, 0, s>>>(x, q, sa, K, ld);
+  else if (nv <= 8) k_quant<DT, NT, 8><<<M, NT, 0, s>>>(x, q, sa, K, ld);
+  else return false;
+  return true;
+}
+
+template <int DT>
+void gemm(const int8_t* q, const float* sa, const int8_t* w, const float* sw, const float* bias, void* y, int M, int N,
+          int ld, hipStream_t s) {
+#define UB_TILE(WM, WN, TM, TN, OCC)                                                                     \
+  k_i8_gemm<DT, WM, WN, TM, TN, OCC><<<ub_cdiv(M, 32 * WM * TM) * ub_cdiv(N, 32 * WN * TN), 64 * WM * WN, 0, s>>>( \
+      q, sa, w, sw, bias, y, M, N, ld)
+  const int knob = ub_tune(UB_TUNE_GEMM_TILE);
+  switch (knob) {
+    case 11: UB_TILE(2, 4, 4, 2, 2); return;
+    case 12: UB_TILE(2, 2, 2, 2, 2); return;
+    case 13: UB_TILE(2, 2, 2, 1, 2); return;
+    case 14: UB_TILE(2, 2, 1, 2, 2); return;
+    case 15: UB_TILE(2, 2, 1, 1, 2); return;
+    case 16: UB_TILE(4, 2, 2, 2, 2); return;
+    case 17: UB_TILE(2, 4, 2, 2, 2); return;
+  }
+  const long t256 = (long)ub_cdiv(M, 256) * ub_cdiv(N, 256);
+  if (t256 >= 256) UB_TILE(2, 4, 4, 2, 2);
+  else UB_TILE(2, 2, 2, 2, 2);
+#undef UB_TILE
+}
+
+template <int DT>
+int linear(const char* nm, const void* x, const int8_t* w, const float* sw, const float* bias, void* y, int M, int K,
+           int N, int ld, hipStream_t s) {
+  if (M <= 16 && dec_lds(M, ld) <= kLds) {
+    dec<DT>(x, w, sw, bias, y, M, K, N, ld, s);
+    return UB_OK;
+  }
+  UbScratch ws(s, (size_t)M * ld + sizeof(float) * (size_t)M);
+  int8_t* q = (int8_t*)ws.get();
+  if (!q) return ub_set_error(UB_ERR_LAUNCH, "%s: no workspace", nm);
+  float* sa = (float*)(q + (size_t)M * ld);
+  if (!((M >= 512 || ld <= 2048) && quant<DT, 256>(x, q, sa, M, K, ld, s)) && !quant<DT, 1024>(x, q, sa, M, K, ld, s))
+    k_quant<DT, 1024, 0><<<M, 1024, 0, s>>>(x, q, sa, K, ld);
+  gemm<DT>(q, sa, w, sw, bias, y, M, N, ld, s);
+  return UB_OK;
 }
 
 }  // namespace
@@ -101,13 +481,10 @@ UB_API int ubridge_int8_linear(const void* x, int dtype, const int8_t* w, const 
   if ((size_t)M * N == 0) return UB_OK;
   UB_REQUIRE(x && w && sw && y, "%s: null pointer", nm);
   UB_REQUIRE(((uintptr_t)w & 15) == 0, "%s: weight not 16-byte aligned", nm);
+  UB_REQUIRE(M < 1 << 22, "%s: M=%d", nm, M);  // (a launch has fewer than 2^32 threads)
   hipStream_t s = ub_stream(stream);
-  UbScratch ws(s, (size_t)M * ld + sizeof(float) * (size_t)M);
-  int8_t* q = (int8_t*)ws.get();
-  if (!q) return ub_set_error(UB_ERR_LAUNCH, "%s: no workspace", nm);
-  float* sa = (float*)(q + (size_t)M * ld);
-  if (dtype == UB_F32) linear<UB_F32>(x, w, sw, bias, y, q, sa, M, K, N, ld, s);
-  else if (dtype == UB_F16) linear<UB_F16>(x, w, sw, bias, y, q, sa, M, K, N, ld, s);
-  else linear<UB_BF16>(x, w, sw, bias, y, q, sa, M, K, N, ld, s);
-  return ub_check_launch(nm);
+  const int e = dtype == UB_F32   ? linear<UB_F32>(nm, x, w, sw, bias, y, M, K, N, ld, s)
+                : dtype == UB_F16 ? linear<UB_F16>(nm, x, w, sw, bias, y, M, K, N, ld, s)
+                                  : linear<UB_BF16>(nm, x, w, sw, bias, y, M, K, N, ld, s);
+  return e ? e : ub_check_launch(nm);
 }
