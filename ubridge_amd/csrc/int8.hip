@@ -152,24 +152,80 @@ __device__ __forceinline__ void put(void* y, size_t i, int acc, float sa, float 
 }
 
 // ------------------------------------------------------------------ tiles
+// A wavefront's 32 TM x 32 TN outputs, through its part of LDS (kStage bytes a
+// wavefront, free by now) in rows, so that a store instruction writes whole runs
+// of a row.  The weights are the products' left operand: lane (c, kh) holds row m
+// = c and columns 8 q + 4 kh .. + 3 of a 32 x 32 tile, four to an LDS write.
+template <int DT, int TM, int TN>
+struct Epilogue {
+  typedef typename Elem<DT>::T T;
+  static constexpr int kPitch = 32 * TN * sizeof(T) + 16, kStage = 32 * kPitch;
+  static __device__ __forceinline__ void run(const i32x16 (&acc)[TM][TN], uint8_t* st, const float* sa, const float* sw,
+                                             const float* bias, void* y, int M, int N, int m0, int n0) {
+    constexpr int E = Elem<DT>::E, LR = 32 * TN / E, RI = 64 / LR;  // lanes a row, rows an instruction
+    const int lane = threadIdx.x & 63, c = lane & 31, kh = lane >> 5;
+    float s[TN][16], b[TN][16];
+#pragma unroll
+    for (int j = 0; j < TN; j++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const int n = min(n0 + 32 * j + 8 * (r >> 2) + 4 * kh + (r & 3), N - 1);
+        s[j][r] = sw[n];
+        b[j][r] = bias ? bias[n] : 0.f;
+      }
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+      const float a = sa[min(m0 + 32 * i + c, M - 1)];
+#pragma unroll
+      for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          T v[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) put<DT>(v, e, acc[i][j][4 * q + e], a, s[j][4 * q + e], b[j][4 * q + e]);
+          __builtin_memcpy(st + c * kPitch + (32 * j + 8 * q + 4 * kh) * sizeof(T), v, sizeof(v));
+        }
+#pragma unroll
+      for (int k = 0; k < 32; k += RI) {
+        const int row = k + lane / LR, col = (lane % LR) * E;
+        const uint4 v = *(const uint4*)(st + row * kPitch + col * sizeof(T));
+        const int m = m0 + 32 * i + row, n = n0 + col;
+        if (m < M && row < 32) {
+          T* p = (T*)y + (size_t)m * N + n;
+          if (n + E <= N) {
+            __builtin_memcpy(p, &v, 16);
+          } else {
+            T w[E];
+            __builtin_memcpy(w, &v, 16);
+#pragma unroll
+            for (int e = 0; e < E; e++)
+              if (n + e < N) p[e] = w[e];
+          }
+        }
+      }
+    }
+  }
+};
+
 // WM x WN wavefronts of 32 TM x 32 TN outputs each, v_mfma_i32_32x32x32_i8.  The
-// operands reach LDS by direct loads in 64-byte halves of a 128-byte K-step,
-// each row of 64 bytes swizzled in 16-byte units (unit u of row r at u ^ ((r >>
-// 2) & 3)) so that the 16 rows of a fragment read lie in distinct banks.  Two
-// steps are in LDS: the products of a step's first half run on fragments
-// read before while the second half is read; then the next step is waited
-// for, the barrier frees this step's buffers for the loads of the one after,
-// and the second half's products run while the next first half is read.
-template <int DT, int WM, int WN, int TM, int TN, int OCC>
+// operands reach LDS by direct loads in a ring of NS 64-byte K-steps, each row of
+// 64 bytes swizzled in 16-byte units (unit u of row r at u ^ ((r >> 2) & 3)) so
+// that the 16 rows of a fragment read lie in distinct banks.  Fragments live in
+// registers, two sets: step k multiplies those read during step k - 1 while
+// step k + 1's are read, and sends for step k + NS into the slot whose reading
+// ended with the barrier; NS - 1 steps are in flight.
+template <int DT, int WM, int WN, int TM, int TN, int NS, int OCC>
 __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
 k_i8_gemm(const int8_t* __restrict__ A, const float* __restrict__ sa, const int8_t* __restrict__ B,
           const float* __restrict__ sw, const float* __restrict__ bias, void* __restrict__ y, int M,
           int N, int ld) {
   constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN, NW = WM * WN;
-  constexpr int NA = BM / 16 / NW, NB = BN / 16 / NW;  // load instructions of a wavefront and half
-  constexpr int AB = BM * 64, HALF = (BM + BN) * 64;   // bytes
+  constexpr int NA = BM / 16 / NW, NB = BN / 16 / NW;  // load instructions of a wavefront and step
+  constexpr int AB = BM * 64, ST = (BM + BN) * 64;     // bytes
+  typedef Epilogue<DT, TM, TN> Out;
   static_assert(NA * NW * 16 == BM && NB * NW * 16 == BN, "whole load instructions");
-  __shared__ __attribute__((aligned(16))) uint8_t h0[HALF], h1[HALF], h2[HALF], h3[HALF];
+  static_assert(NW * Out::kStage <= NS * ST, "epilogue fits");
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
@@ -179,6 +235,7 @@ k_i8_gemm(const int8_t* __restrict__ A, const float* __restrict__ sa, const int8
   // rows past the end lie past the buffers: zeros
   const ub_u32x4 ra = ub_desc(A + (size_t)m0 * ld, (uint64_t)min(BM, M - m0) * ld);
   const ub_u32x4 rb = ub_desc(B + (size_t)n0 * ld, (uint64_t)min(BN, N - n0) * ld);
+  const uint32_t base = ub_lds_addr(lds);
   uint32_t va[NA], vb[NB];
 #pragma unroll
   for (int i = 0; i < NA; i++) {
@@ -190,12 +247,13 @@ k_i8_gemm(const int8_t* __restrict__ A, const float* __restrict__ sa, const int8
     const int u = (i * NW + wave) * 64 + lane, row = u >> 2;
     vb[i] = (uint32_t)row * (uint32_t)ld + 16 * ((u & 3) ^ ((row >> 2) & 3));
   }
-  auto issue = [&](int kt, uint8_t* st) {
-    const uint32_t sb = ub_lds_addr(st), k0 = (uint32_t)(kt * 64);
+  const int nk = ld / 64;
+  auto issue = [&](int k, uint32_t off) {  // (steps past K: the last again, not used)
+    const uint32_t k0 = (uint32_t)(min(k, nk - 1) * 64), sb = base + off + wave * 1024;
 #pragma unroll
-    for (int i = 0; i < NA; i++) ub_lds_load16_at(ra, sb + (i * NW + wave) * 1024, va[i], k0);
+    for (int i = 0; i < NA; i++) ub_lds_load16_at(ra, sb + i * NW * 1024, va[i], k0);
 #pragma unroll
-    for (int i = 0; i < NB; i++) ub_lds_load16_at(rb, sb + AB + (i * NW + wave) * 1024, vb[i], k0);
+    for (int i = 0; i < NB; i++) ub_lds_load16_at(rb, sb + AB + i * NW * 1024, vb[i], k0);
   };
   i32x16 acc[TM][TN];
 #pragma unroll
@@ -205,85 +263,143 @@ k_i8_gemm(const int8_t* __restrict__ A, const float* __restrict__ sa, const int8
 #pragma unroll
       for (int r = 0; r < 16; r++) acc[i][j][r] = 0;
   const int l32 = lane & 31, kh = lane >> 5;
-  // units 2 kh and 2 kh + 1 of a row: a lane's part of two products
+  // units 2 kh and 2 kh + 1 of a row: a lane's part of two products; the swizzle
+  // depends on the lane alone, tiles being 32 rows
+  const uint32_t u0 = l32 * 64 + (((2 * kh) ^ ((l32 >> 2) & 3)) * 16);
+  const uint32_t u1 = l32 * 64 + (((2 * kh + 1) ^ ((l32 >> 2) & 3)) * 16);
+  const uint32_t fa = wm * 32 * TM * 64, fb = AB + wn * 32 * TN * 64;
   i32x4 af[2][TM][2], bf[2][TN][2];
-  auto frag = [&](i32x4 (&f)[2], const uint8_t* t, int row) {
-    const int sz = (row >> 2) & 3;
-    f[0] = *(const i32x4*)(t + row * 64 + (((2 * kh) ^ sz) * 16));
-    f[1] = *(const i32x4*)(t + row * 64 + (((2 * kh + 1) ^ sz) * 16));
-  };
-  auto read_frags = [&](const uint8_t* st, int b) {
+  auto read_frags = [&](uint32_t off, int b) {
+    const uint8_t* p0 = lds + off + u0;
+    const uint8_t* p1 = lds + off + u1;
 #pragma unroll
-    for (int i = 0; i < TM; i++) frag(af[b][i], st, wm * 32 * TM + 32 * i + l32);
+    for (int j = 0; j < TN; j++) {
+      bf[b][j][0] = *(const i32x4*)(p0 + fb + j * 2048);
+      bf[b][j][1] = *(const i32x4*)(p1 + fb + j * 2048);
+    }
 #pragma unroll
-    for (int j = 0; j < TN; j++) frag(bf[b][j], st + AB, wn * 32 * TN + 32 * j + l32);
+    for (int i = 0; i < TM; i++) {
+      af[b][i][0] = *(const i32x4*)(p0 + fa + i * 2048);
+      af[b][i][1] = *(const i32x4*)(p1 + fa + i * 2048);
+    }
   };
-  auto mfmas = [&](int b) {
+  uint32_t off = 0;  // of step k's slot
+  auto step = [&](auto Bc, int k) {
+    constexpr int Bf = decltype(Bc)::value;
+    __builtin_amdgcn_s_waitcnt(0xC07F);     // lgkmcnt(0): this step's fragments are read
+    ub_wait_vmcnt<(NS - 2) * (NA + NB)>();  // the next step has landed
+    ub_barrier();
+    issue(k + NS, off);
+    off = off == (NS - 1) * ST ? 0 : off + ST;
+    read_frags(off, Bf ^ 1);  // (after the last step: not used)
 #pragma unroll
     for (int q = 0; q < 2; q++)
 #pragma unroll
       for (int j = 0; j < TN; j++)
 #pragma unroll
         for (int i = 0; i < TM; i++)
-          acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(af[b][i][q], bf[b][j][q], acc[i][j], 0, 0, 0);
-  };
-  auto interleave = [&]() {
+          acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(bf[Bf][j][q], af[Bf][i][q], acc[i][j], 0, 0, 0);
 #pragma unroll
     for (int q = 0; q < 2 * TM * TN; q++) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // 1 MFMA
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // 1 DS read
     }
   };
-  const int nks = ld / 128;
-  auto stage = [&](auto Pc, int j) {
-    constexpr int P = decltype(Pc)::value;
-    uint8_t* a0 = P ? h2 : h0;
-    uint8_t* a1 = P ? h3 : h1;
-    uint8_t* nx = P ? h0 : h2;
-    mfmas(0);
-    read_frags(a1, 1);
-    interleave();
-    if (j + 1 < nks) {
-      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this step's fragments are read
-      ub_wait_vmcnt<0>();                  // the next step has landed
-      ub_barrier();
-      if (j + 2 < nks) {
-        issue(2 * (j + 2), a0);
-        issue(2 * (j + 2) + 1, a1);
+#pragma unroll
+  for (int k = 0; k < NS; k++) issue(k, k * ST);
+  ub_wait_vmcnt<(NS - 1) * (NA + NB)>();
+  ub_barrier();
+  read_frags(0, 0);
+  for (int k = 0; k < nk; k += 2) {  // (nk is even)
+    step(std::integral_constant<int, 0>{}, k);
+    step(std::integral_constant<int, 1>{}, k + 1);
+  }
+  __builtin_amdgcn_s_waitcnt(0xC07F);
+  ub_wait_vmcnt<0>();
+  ub_barrier();
+  Out::run(acc, lds + wave * Out::kStage, sa, sw, bias, y, M, N, m0 + wm * 32 * TM, n0 + wn * 32 * TN);
+}
+
+// The same product for grids that leave a workgroup or less to a CU, where the
+// latency of a K-step's loads is what costs: a ring of NS 128-byte steps in LDS,
+// NS - 1 of them in flight, one barrier a step.  Rows of 128 bytes, unit u of row
+// r at u ^ (r & 7).
+template <int DT, int WM, int WN, int TM, int TN, int NS>
+__global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2, 2)))
+k_i8_ring(const int8_t* __restrict__ A, const float* __restrict__ sa, const int8_t* __restrict__ B,
+          const float* __restrict__ sw, const float* __restrict__ bias, void* __restrict__ y, int M,
+          int N, int ld) {
+  constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN, NW = WM * WN;
+  constexpr int NL = (BM + BN) / 8 / NW;  // load instructions of a wavefront and step: 8 rows each
+  constexpr int ST = (BM + BN) * 128;
+  static_assert(NL * NW * 8 == BM + BN && (BM / 8) % NW == 0, "whole load instructions");
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  int tile_m, tile_n;
+  ub_tile_order((M + BM - 1) / BM, (N + BN - 1) / BN, 8, tile_m, tile_n);
+  const int n0 = tile_n * BN, m0 = tile_m * BM;
+  const ub_u32x4 ra = ub_desc(A + (size_t)m0 * ld, (uint64_t)min(BM, M - m0) * ld);
+  const ub_u32x4 rb = ub_desc(B + (size_t)n0 * ld, (uint64_t)min(BN, N - n0) * ld);
+  const uint32_t base = ub_lds_addr(lds);
+  uint32_t v[NL];
+#pragma unroll
+  for (int i = 0; i < NL; i++) {
+    const int row = (i * NW + wave) * 8 + (lane >> 3);  // of A, then of B
+    v[i] = (uint32_t)(row < BM ? row : row - BM) * (uint32_t)ld + 16 * ((lane & 7) ^ (row & 7));
+  }
+  auto issue = [&](int k, int slot) {
+#pragma unroll
+    for (int i = 0; i < NL; i++)
+      ub_lds_load16_at(i * NW * 8 < BM ? ra : rb, base + slot * ST + (i * NW + wave) * 1024, v[i], (uint32_t)k * 128);
+  };
+  i32x16 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; i++)
+#pragma unroll
+    for (int j = 0; j < TN; j++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[i][j][r] = 0;
+  const int l32 = lane & 31, kh = lane >> 5;
+  const int nk = ld / 128;
+#pragma unroll
+  for (int k = 0; k < NS - 1; k++) issue(min(k, nk - 1), k);  // (past K: loaded again, not used)
+  int slot = 0;
+  for (int k = 0; k < nk; k++) {
+    ub_wait_vmcnt<(NS - 2) * NL>();  // step k has landed
+    ub_barrier();                    // for everyone, and step k - 1 is read
+    issue(min(k + NS - 1, nk - 1), slot == 0 ? NS - 1 : slot - 1);
+    const uint8_t* st = lds + slot * ST;
+    i32x4 af[TM][4], bf[TN][4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+#pragma unroll
+      for (int i = 0; i < TM; i++) {
+        const int row = wm * 32 * TM + 32 * i + l32;
+        af[i][q] = *(const i32x4*)(st + row * 128 + 16 * ((2 * q + kh) ^ (row & 7)));
+      }
+#pragma unroll
+      for (int j = 0; j < TN; j++) {
+        const int row = BM + wn * 32 * TN + 32 * j + l32;
+        bf[j][q] = *(const i32x4*)(st + row * 128 + 16 * ((2 * q + kh) ^ (row & 7)));
       }
     }
-    mfmas(1);
-    read_frags(nx, 0);  // (after the last step: stale, not used)
-    interleave();
-  };
-  issue(0, h0);
-  issue(1, h1);
-  if (nks > 1) {
-    issue(2, h2);
-    issue(3, h3);
-    ub_wait_vmcnt<2 * (NA + NB)>();
-  } else {
-    ub_wait_vmcnt<0>();
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+#pragma unroll
+      for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int i = 0; i < TM; i++)
+          acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(bf[j][q], af[i][q], acc[i][j], 0, 0, 0);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this step is read
+    slot = slot == NS - 1 ? 0 : slot + 1;
   }
+  ub_wait_vmcnt<0>();
   ub_barrier();
-  read_frags(h0, 0);
-  for (int j = 0; j < nks; j += 2) {
-    stage(std::integral_constant<int, 0>{}, j);
-    if (j + 1 < nks) stage(std::integral_constant<int, 1>{}, j + 1);
-  }
-#pragma unroll
-  for (int j = 0; j < TN; j++) {
-    const int n = n0 + wn * 32 * TN + 32 * j + l32;
-    if (n >= N) continue;
-    const float s = sw[n], b = bias ? bias[n] : 0.f;
-#pragma unroll
-    for (int i = 0; i < TM; i++)
-#pragma unroll
-      for (int r = 0; r < 16; r++) {
-        const int m = m0 + wm * 32 * TM + 32 * i + 8 * (r >> 2) + 4 * kh + (r & 3);
-        if (m < M) put<DT>(y, (size_t)m * N + n, acc[i][j][r], sa[m], s, b);
-      }
-  }
+  typedef Epilogue<DT, TM, TN> Out;
+  static_assert(NW * Out::kStage <= NS * ST, "epilogue fits");
+  Out::run(acc, lds + wave * Out::kStage, sa, sw, bias, y, M, N, m0 + wm * 32 * TM, n0 + wn * 32 * TN);
 }
 
 // ----------------------------------------------------------- few tokens
@@ -294,9 +410,9 @@ k_i8_gemm(const int8_t* __restrict__ A, const float* __restrict__ sa, const int8
 // in flight while these are multiplied: v_mfma_i32_16x16x64_i8, tokens as A
 // rows.  The codes of the activations lie in LDS for the whole launch, rows 16
 // bytes further apart than they are long, so that the 16 rows of a fragment
-// read spread over the banks.  Each workgroup makes them itself, one wavefront a
-// row, after its first weight loads are on their way: a launch less, and
-// quantizing M K values hides behind the stream.  The wavefronts' sums meet
+// read spread over the banks.  Each workgroup makes them itself, while its first
+// weight loads are on their way: a launch less, and quantizing M K values hides
+// behind the stream.  The wavefronts' sums meet
 // in LDS.
 constexpr int DW = 16;
 
@@ -308,7 +424,7 @@ template <int DT, int SP>
 __global__ void __launch_bounds__(64 * DW) k_i8_dec(const void* __restrict__ x, const int8_t* __restrict__ W,
                                                     const float* __restrict__ sw, const float* __restrict__ bias,
                                                     void* __restrict__ y, int M, int K, int N, int ld) {
-  constexpr int E = Elem<DT>::E;
+  constexpr int E = Elem<DT>::E, XU = SP > 4 ? 4 : 8;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   int* red = (int*)lds;                       // [16 wavefronts][M][17]
   float* ssa = (float*)(red + DW * M * 17);   // [16]
@@ -329,6 +445,15 @@ __global__ void __launch_bounds__(64 * DW) k_i8_dec(const void* __restrict__ x, 
       b[i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rw, (int)(s < steps ? row + 64u * s : 0x80000000u), 0, 0));
     }
   };
+  // ---- codes: 16 / P wavefronts a row, P the power of two from M on.  A lane's
+  // first XU units are asked for ahead of the weights (loads return in order)
+  // and stay in registers; longer rows are read again.
+  const int lg = M > 8 ? 0 : M > 4 ? 1 : M > 2 ? 2 : M > 1 ? 3 : 4;  // log2 of the wavefronts
+  const int m = wave >> lg, u0 = ((wave & ((1 << lg) - 1)) << 6) + lane, us = 64 << lg;
+  const typename Elem<DT>::T* p = (const typename Elem<DT>::T*)x + (size_t)min(m, M - 1) * K;
+  uint4 xu[XU];
+#pragma unroll
+  for (int j = 0; j < XU; j++) xu[j] = unit<DT>(p, u0 + j * us, K);
   int t = blockIdx.x, c = 0;  // the piece being multiplied
   auto next = [&](int& t, int& c) {
     if (++c == nc) {
@@ -341,22 +466,31 @@ __global__ void __launch_bounds__(64 * DW) k_i8_dec(const void* __restrict__ x, 
   next(tn, cn);
   load(b1, tn, cn);
   next(tn, cn);
-  for (int m = wave; m < M; m += DW) {
-    const typename Elem<DT>::T* p = (const typename Elem<DT>::T*)x + (size_t)m * K;
+  {
     uint32_t top = 0;
-    for (int i = lane; i * E < K; i += 64) top = top_of<DT>(unit<DT>(p, i, K), top);
+#pragma unroll
+    for (int j = 0; j < XU; j++) top = top_of<DT>(xu[j], top);
+    for (int i = u0 + XU * us; i * E < K; i += us) top = top_of<DT>(unit<DT>(p, i, K), top);
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+    if (lane == 0) red[wave] = (int)top;
+    __syncthreads();
+    for (int w = 0; w < 1 << lg; w++) top = max(top, (uint32_t)red[(m << lg) + w]);
+    __syncthreads();
     const float s = scale_of(top);
     const bool plain = plain_scale(s);
     const float rs = plain ? 0.f : __fdiv_rn(1.0f, s);
-    if (lane == 0) ssa[m] = s;
-    for (int i = lane; i * E < ld; i += 64) {
+    if (lane == 0 && m < M) ssa[m] = s;
+    auto store = [&](const uint4& v, int i) {
+      if (i * E >= ld || m >= M) return;
       uint32_t o[E / 4];
-      codes<DT>(unit<DT>(p, i, K), s, rs, plain, o);
+      codes<DT>(v, s, rs, plain, o);
       if constexpr (E == 4) *(uint32_t*)(a + m * pitch + 4 * i) = o[0];
       else *(uint2*)(a + m * pitch + 8 * i) = make_uint2(o[0], o[1]);
-    }
+    };
+#pragma unroll
+    for (int j = 0; j < XU; j++) store(xu[j], u0 + j * us);
+    for (int i = u0 + XU * us; i * E < ld; i += us) store(unit<DT>(p, i, K), i);
   }
   __syncthreads();
   i32x4 acc = {0, 0, 0, 0};
@@ -433,23 +567,56 @@ bool quant(const void* x, int8_t* q, float* sa, int M, int K, int ld, hipStream_
 template <int DT>
 void gemm(const int8_t* q, const float* sa, const int8_t* w, const float* sw, const float* bias, void* y, int M, int N,
           int ld, hipStream_t s) {
-#define UB_TILE(WM, WN, TM, TN, OCC)                                                                     \
-  k_i8_gemm<DT, WM, WN, TM, TN, OCC><<<ub_cdiv(M, 32 * WM * TM) * ub_cdiv(N, 32 * WN * TN), 64 * WM * WN, 0, s>>>( \
-      q, sa, w, sw, bias, y, M, N, ld)
+#define UB_TILE(WM, WN, TM, TN, NS, OCC)                                                                 \
+  {                                                                                                      \
+    constexpr int lds = NS * 64 * 32 * (WM * TM + WN * TN);                                              \
+    static const hipError_t once = hipFuncSetAttribute((const void*)k_i8_gemm<DT, WM, WN, TM, TN, NS, OCC>, \
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds); \
+    (void)once;                                                                                          \
+    k_i8_gemm<DT, WM, WN, TM, TN, NS, OCC><<<ub_cdiv(M, 32 * WM * TM) * ub_cdiv(N, 32 * WN * TN), 64 * WM * WN, lds, s>>>( \
+        q, sa, w, sw, bias, y, M, N, ld);                                                                \
+    return;                                                                                              \
+  }
+#define UB_RING(WM, WN, TM, TN, NS)                                                                      \
+  {                                                                                                      \
+    constexpr int lds = NS * 128 * 32 * (WM * TM + WN * TN);                                             \
+    static const hipError_t once = hipFuncSetAttribute((const void*)k_i8_ring<DT, WM, WN, TM, TN, NS>,   \
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds); \
+    (void)once;                                                                                          \
+    k_i8_ring<DT, WM, WN, TM, TN, NS><<<ub_cdiv(M, 32 * WM * TM) * ub_cdiv(N, 32 * WN * TN), 64 * WM * WN, lds, s>>>( \
+        q, sa, w, sw, bias, y, M, N, ld);                                                                \
+    return;                                                                                              \
+  }
   const int knob = ub_tune(UB_TUNE_GEMM_TILE);
   switch (knob) {
-    case 11: UB_TILE(2, 4, 4, 2, 2); return;
-    case 12: UB_TILE(2, 2, 2, 2, 2); return;
-    case 13: UB_TILE(2, 2, 2, 1, 2); return;
-    case 14: UB_TILE(2, 2, 1, 2, 2); return;
-    case 15: UB_TILE(2, 2, 1, 1, 2); return;
-    case 16: UB_TILE(4, 2, 2, 2, 2); return;
-    case 17: UB_TILE(2, 4, 2, 2, 2); return;
+    case 21: UB_RING(2, 2, 1, 1, 4)   // 64 x 64
+    case 22: UB_RING(2, 2, 1, 1, 8)
+    case 23: UB_RING(2, 2, 2, 1, 3)   // 128 x 64
+    case 24: UB_RING(2, 2, 2, 1, 6)
+    case 25: UB_RING(2, 2, 2, 2, 4)   // 128 x 128
+    case 26: UB_RING(4, 2, 2, 2, 3)   // 256 x 128
+    case 27: UB_RING(2, 4, 2, 1, 4)   // 128 x 128, 8 waves
+    case 28: UB_RING(2, 1, 1, 1, 4)   // 64 x 32
+    case 29: UB_RING(2, 1, 1, 1, 6)
+    case 30: UB_RING(1, 2, 1, 1, 6)   // 32 x 64
+    case 31: UB_RING(1, 4, 1, 1, 6)   // 32 x 128
+    case 32: UB_RING(4, 2, 1, 1, 6)   // 128 x 64, 8 waves
+  }
+  switch (knob) {
+    case 11: UB_TILE(2, 4, 4, 2, 4, 2)  // 256 x 256
+    case 12: UB_TILE(2, 4, 4, 2, 5, 2)
+    case 13: UB_TILE(2, 4, 4, 1, 6, 2)  // 256 x 128
+    case 14: UB_TILE(2, 2, 4, 2, 6, 1)  // 256 x 128, 4 waves
+    case 15: UB_TILE(2, 2, 2, 2, 4, 2)  // 128 x 128
+    case 16: UB_TILE(2, 2, 2, 2, 5, 2)
+    case 17: UB_TILE(2, 4, 2, 2, 6, 2)  // 128 x 256
+    case 18: UB_TILE(2, 2, 4, 4, 5, 1)  // 256 x 256, 4 waves
   }
   const long t256 = (long)ub_cdiv(M, 256) * ub_cdiv(N, 256);
-  if (t256 >= 256) UB_TILE(2, 4, 4, 2, 2);
-  else UB_TILE(2, 2, 2, 2, 2);
+  if (t256 >= 224) UB_TILE(2, 4, 4, 2, 4, 2)
+  UB_RING(2, 2, 1, 1, 4)
 #undef UB_TILE
+#undef UB_RING
 }
 
 template <int DT>
