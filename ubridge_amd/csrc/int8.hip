@@ -214,24 +214,18 @@ struct Epilogue {
 // registers, two sets: step k multiplies those read during step k - 1 while
 // step k + 1's are read, and sends for step k + NS into the slot whose reading
 // ended with the barrier; NS - 1 steps are in flight.
-template <int DT, int WM, int WN, int TM, int TN, int NS, int OCC>
-__global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
-k_i8_gemm(const int8_t* __restrict__ A, const float* __restrict__ sa, const int8_t* __restrict__ B,
-          const float* __restrict__ sw, const float* __restrict__ bias, void* __restrict__ y, int M,
-          int N, int ld) {
+template <int DT, int WM, int WN, int TM, int TN, int NS>
+__device__ __forceinline__ void i8_tile(const int8_t* A, const float* sa, const int8_t* B, const float* sw, const float* bias,
+                                        void* y, int M, int N, int ld, int m0, int n0, uint8_t* lds) {
   constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN, NW = WM * WN;
   constexpr int NA = BM / 16 / NW, NB = BN / 16 / NW;  // load instructions of a wavefront and step
   constexpr int AB = BM * 64, ST = (BM + BN) * 64;     // bytes
   typedef Epilogue<DT, TM, TN> Out;
   static_assert(NA * NW * 16 == BM && NB * NW * 16 == BN, "whole load instructions");
   static_assert(NW * Out::kStage <= NS * ST, "epilogue fits");
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
-  int tile_m, tile_n;
-  ub_tile_order((M + BM - 1) / BM, (N + BN - 1) / BN, 8, tile_m, tile_n);
-  const int n0 = tile_n * BN, m0 = tile_m * BM;
   // rows past the end lie past the buffers: zeros
   const ub_u32x4 ra = ub_desc(A + (size_t)m0 * ld, (uint64_t)min(BM, M - m0) * ld);
   const ub_u32x4 rb = ub_desc(B + (size_t)n0 * ld, (uint64_t)min(BN, N - n0) * ld);
@@ -318,6 +312,30 @@ k_i8_gemm(const int8_t* __restrict__ A, const float* __restrict__ sa, const int8
   ub_wait_vmcnt<0>();
   ub_barrier();
   Out::run(acc, lds + wave * Out::kStage, sa, sw, bias, y, M, N, m0 + wm * 32 * TM, n0 + wn * 32 * TN);
+}
+
+// The tiles in ub_tile_order; from tile `full` on (a multiple of the CUs) a tile is
+// two workgroups, its upper and its lower half: the last round, where at most
+// half the CUs had a tile, then takes about half as long.  full = all tiles
+// otherwise, as for tiles of one product's height (TM = 1).
+template <int DT, int WM, int WN, int TM, int TN, int NS>
+__global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2, 2)))
+k_i8_gemm(const int8_t* __restrict__ A, const float* __restrict__ sa, const int8_t* __restrict__ B,
+          const float* __restrict__ sw, const float* __restrict__ bias, void* __restrict__ y, int M,
+          int N, int ld, int full) {
+  constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int tm = (M + BM - 1) / BM, tn = (N + BN - 1) / BN;
+  const int b = (int)blockIdx.x;
+  int tile_m, tile_n;
+  if (TM == 1 || b < full) {
+    ub_tile_at(b, full, tm, tn, 8, tile_m, tile_n);
+    i8_tile<DT, WM, WN, TM, TN, NS>(A, sa, B, sw, bias, y, M, N, ld, tile_m * BM, tile_n * BN, lds);
+  } else if constexpr (TM > 1) {
+    ub_tile_at(full + ((b - full) >> 1), 0, tm, tn, 8, tile_m, tile_n);
+    const int m0 = tile_m * BM + ((b - full) & 1) * (BM / 2);
+    if (m0 < M) i8_tile<DT, WM, WN, TM / 2, TN, NS>(A, sa, B, sw, bias, y, M, N, ld, m0, tile_n * BN, lds);
+  }
 }
 
 // The same product for grids that leave a workgroup or less to a CU, where the
@@ -564,17 +582,39 @@ bool quant(const void* x, int8_t* q, float* sa, int M, int K, int ld, hipStream_
   return true;
 }
 
+// The tile that takes least, by its measured time for 128 bytes of K (0.01 us) on
+// a CU that has one workgroup of it, and for each of several (larger grids leave
+// that many to a CU, side by side or in turn): 256 x 256 205 / 205, 128 x 128 68 /
+// 62, 64 x 128 57 / 50, 64 x 64 34 / 29, 64 x 32 30 / 22.  us in a graph, with the
+// quantizing launch, M x K x N: 64 x 4096 x 6144 on these 32 / - / 20 / 15 / 13.7,
+// 201 x 3520 x 9001 40 / 24 / 38 / 32 / 33, 512 x 4096 x 4096 36 / 27 / 23 / 23 /
+// 32, 1024 x 2048 x 2048 25 / 20 / 17 / 16 / 22, 1024 x 4096 x 14336 75 / 97 / ...
+int tile_for(int M, int N) {
+  static const struct { int m, n, one, each; } t[5] = {
+      {256, 256, 205, 205}, {128, 128, 68, 62}, {64, 128, 57, 50}, {64, 64, 34, 29}, {64, 32, 30, 22}};
+  int best = 0;
+  double least = 0;
+  for (int i = 0; i < 5; i++) {
+    const int64_t tiles = (int64_t)ub_cdiv(M, t[i].m) * ub_cdiv(N, t[i].n), per = (tiles + 255) / 256;
+    double cost = per == 1 ? t[i].one : (double)per * t[i].each;
+    if (i == 0 && per > 1 && tiles % 256 && tiles % 256 <= 128) cost -= 0.45 * t[i].each;  // (halves)
+    if (i == 0 || cost < least) best = i, least = cost;
+  }
+  return best;
+}
+
 template <int DT>
 void gemm(const int8_t* q, const float* sa, const int8_t* w, const float* sw, const float* bias, void* y, int M, int N,
           int ld, hipStream_t s) {
-#define UB_TILE(WM, WN, TM, TN, NS, OCC)                                                                 \
+#define UB_TILE(WM, WN, TM, TN, NS)                                                                      \
   {                                                                                                      \
     constexpr int lds = NS * 64 * 32 * (WM * TM + WN * TN);                                              \
-    static const hipError_t once = hipFuncSetAttribute((const void*)k_i8_gemm<DT, WM, WN, TM, TN, NS, OCC>, \
+    static const hipError_t once = hipFuncSetAttribute((const void*)k_i8_gemm<DT, WM, WN, TM, TN, NS>,   \
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, lds); \
     (void)once;                                                                                          \
-    k_i8_gemm<DT, WM, WN, TM, TN, NS, OCC><<<ub_cdiv(M, 32 * WM * TM) * ub_cdiv(N, 32 * WN * TN), 64 * WM * WN, lds, s>>>( \
-        q, sa, w, sw, bias, y, M, N, ld);                                                                \
+    const int tiles = ub_cdiv(M, 32 * WM * TM) * ub_cdiv(N, 32 * WN * TN), rest = tiles % 256;           \
+    const int full = TM > 1 && tiles > 256 && rest <= 128 ? tiles - rest : tiles;                                  \
+    k_i8_gemm<DT, WM, WN, TM, TN, NS><<<2 * tiles - full, 64 * WM * WN, lds, s>>>(q, sa, w, sw, bias, y, M, N, ld, full); \
     return;                                                                                              \
   }
 #define UB_RING(WM, WN, TM, TN, NS)                                                                      \
@@ -587,34 +627,13 @@ void gemm(const int8_t* q, const float* sa, const int8_t* w, const float* sw, co
         q, sa, w, sw, bias, y, M, N, ld);                                                                \
     return;                                                                                              \
   }
-  const int knob = ub_tune(UB_TUNE_GEMM_TILE);
-  switch (knob) {
-    case 21: UB_RING(2, 2, 1, 1, 4)   // 64 x 64
-    case 22: UB_RING(2, 2, 1, 1, 8)
-    case 23: UB_RING(2, 2, 2, 1, 3)   // 128 x 64
-    case 24: UB_RING(2, 2, 2, 1, 6)
-    case 25: UB_RING(2, 2, 2, 2, 4)   // 128 x 128
-    case 26: UB_RING(4, 2, 2, 2, 3)   // 256 x 128
-    case 27: UB_RING(2, 4, 2, 1, 4)   // 128 x 128, 8 waves
-    case 28: UB_RING(2, 1, 1, 1, 4)   // 64 x 32
-    case 29: UB_RING(2, 1, 1, 1, 6)
-    case 30: UB_RING(1, 2, 1, 1, 6)   // 32 x 64
-    case 31: UB_RING(1, 4, 1, 1, 6)   // 32 x 128
-    case 32: UB_RING(4, 2, 1, 1, 6)   // 128 x 64, 8 waves
+  switch (tile_for(M, N)) {
+    case 0: UB_TILE(2, 4, 4, 2, 4)
+    case 1: UB_RING(2, 4, 2, 1, 4)
+    case 2: UB_TILE(2, 2, 1, 2, 6)
+    case 3: UB_RING(2, 2, 1, 1, 4)
+    default: UB_TILE(2, 1, 1, 1, 8)
   }
-  switch (knob) {
-    case 11: UB_TILE(2, 4, 4, 2, 4, 2)  // 256 x 256
-    case 12: UB_TILE(2, 4, 4, 2, 5, 2)
-    case 13: UB_TILE(2, 4, 4, 1, 6, 2)  // 256 x 128
-    case 14: UB_TILE(2, 2, 4, 2, 6, 1)  // 256 x 128, 4 waves
-    case 15: UB_TILE(2, 2, 2, 2, 4, 2)  // 128 x 128
-    case 16: UB_TILE(2, 2, 2, 2, 5, 2)
-    case 17: UB_TILE(2, 4, 2, 2, 6, 2)  // 128 x 256
-    case 18: UB_TILE(2, 2, 4, 4, 5, 1)  // 256 x 256, 4 waves
-  }
-  const long t256 = (long)ub_cdiv(M, 256) * ub_cdiv(N, 256);
-  if (t256 >= 224) UB_TILE(2, 4, 4, 2, 4, 2)
-  UB_RING(2, 2, 1, 1, 4)
 #undef UB_TILE
 #undef UB_RING
 }

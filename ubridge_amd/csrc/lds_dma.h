@@ -122,15 +122,18 @@ __device__ __forceinline__ void ub_barrier() {
 // itself walks groups of `gm` tile rows column by column, so the tiles
 // resident at one time share a few A row-panels and B column-panels
 // instead of sweeping whole rows of B.
-__device__ __forceinline__ void ub_tile_order(int tm, int tn, int gm, int& im, int& in_) {
-  const int total = tm * tn;
-  int pid = blockIdx.x;
+// ub_tile_at: tile number `pid` of the order, of which the first `dealt` are
+// regrouped (0: pid as it is).
+__device__ __forceinline__ void ub_tile_at(int pid, int dealt, int tm, int tn, int gm, int& im, int& in_) {
   constexpr int kXcd = 8;
-  if (total % kXcd == 0) pid = (pid % kXcd) * (total / kXcd) + pid / kXcd;
+  if (dealt && dealt % kXcd == 0) pid = (pid % kXcd) * (dealt / kXcd) + pid / kXcd;
   const int per_group = gm * tn;
   const int g = pid / per_group, first = g * gm;
   const int rows = min(gm, tm - first);
   const int r = pid % per_group;
   im = first + r % rows;
   in_ = r / rows;
+}
+__device__ __forceinline__ void ub_tile_order(int tm, int tn, int gm, int& im, int& in_) {
+  ub_tile_at(blockIdx.x, tm * tn, tm, tn, gm, im, in_);
 }
