@@ -35,25 +35,14 @@ __device__ __forceinline__ float get(const uint4& w, int e) {
   else return __uint_as_float((e & 1) ? p[e >> 1] & 0xffff0000u : p[e >> 1] << 16);
 }
 
-// Unit i of a row of K elements at p, zeros past its end.  The row may start
-// at any element: gfx950 loads 16 bytes from there.
+// Unit i of a row at p that has V whole ones; zeros from there on.  The row
+// may start at any element: gfx950 loads 16 bytes from there.  The K mod E
+// elements behind the whole units are one lane's each (loads of their own in
+// every unit made the kernels several times as long).
 template <int DT>
-__device__ __forceinline__ uint4 unit(const typename Elem<DT>::T* p, int i, int K) {
-  constexpr int E = Elem<DT>::E;
+__device__ __forceinline__ uint4 unit(const typename Elem<DT>::T* p, int i, int V) {
   uint4 v = make_uint4(0, 0, 0, 0);
-  const int n = K - i * E;
-  if (n >= E) {
-    __builtin_memcpy(&v, p + i * E, 16);
-  } else if (n > 0) {
-    uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int e = 0; e < E; e++)
-      if (e < n) {
-        if constexpr (DT == UB_F32) w[e] = __float_as_uint(p[i * E + e]);
-        else w[e >> 1] |= (uint32_t)p[i * E + e] << (16 * (e & 1));
-      }
-    v = make_uint4(w[0], w[1], w[2], w[3]);
-  }
+  if (i < V) __builtin_memcpy(&v, p + i * Elem<DT>::E, 16);
   return v;
 }
 
@@ -69,37 +58,42 @@ __device__ __forceinline__ float scale_of(uint32_t top) {
   return top >= 0x7f800000u ? __builtin_nanf("") : top == 0 ? 1.0f : __fdiv_rn(__uint_as_float(top), 127.0f);
 }
 
-// The codes of a unit under scale s.  The quotient is x r (r = 1 / s) corrected
-// twice by its exact residual x - q s (Markstein's division: the second
-// correction gives the correctly rounded x / s), 5 operations where the IEEE
-// divide takes 11; for s outside [2^-60, 2^60], where residuals underflow, it
-// divides (plain = true).  Adding 1.5 2^23 rounds to an integer, ties to even,
-// in the low bits.  |x / s| <= 127, but for a denormal s, whose own rounding is
-// as large as s (hence the clamp); a NaN or zero s has codes 0.
-template <int DT>
-__device__ __forceinline__ void codes(const uint4& u, float s, float r, bool plain, uint32_t (&o)[Elem<DT>::E / 4]) {
+// The code of v under scale s, in the low byte.  The quotient is v r (r = 1 / s)
+// corrected twice by its exact residual v - q s (Markstein's division: the
+// second correction gives the correctly rounded v / s), 5 operations where the
+// IEEE divide takes 11.  Adding 1.5 2^23 rounds to an integer, ties to even, in
+// the low bits.  PLAIN, for s outside [2^-60, 2^60], where residuals underflow:
+// the divide; and a clamp, since |v / s| <= 127 but for a denormal s, whose own
+// rounding is as large as s.  A NaN or zero s has codes 0.
+template <bool PLAIN>
+__device__ __forceinline__ uint32_t code(float v, float s, float r) {
+  float q;
+  if constexpr (PLAIN) {
+    q = __fdiv_rn(v, s);
+    q = q == q ? fminf(fmaxf(q, -127.f), 127.f) : 0.f;
+  } else {
+    q = v * r;
+    q = __builtin_fmaf(__builtin_fmaf(-q, s, v), r, q);
+    q = __builtin_fmaf(__builtin_fmaf(-q, s, v), r, q);
+  }
+  return __float_as_uint(q + 12582912.f);
+}
+// of a unit
+template <int DT, bool PLAIN>
+__device__ __forceinline__ void codes(const uint4& u, float s, float r, uint32_t (&o)[Elem<DT>::E / 4]) {
   constexpr int E = Elem<DT>::E;
   uint32_t c[E];
 #pragma unroll
-  for (int e = 0; e < E; e++) {
-    const float v = get<DT>(u, e);
-    float q;
-    if (plain) {
-      q = __fdiv_rn(v, s);
-      q = q == q ? fminf(fmaxf(q, -127.f), 127.f) : 0.f;
-    } else {
-      q = v * r;
-      q = __builtin_fmaf(__builtin_fmaf(-q, s, v), r, q);
-      q = __builtin_fmaf(__builtin_fmaf(-q, s, v), r, q);
-    }
-    c[e] = __float_as_uint(q + 12582912.f);
-  }
+  for (int e = 0; e < E; e++) c[e] = code<PLAIN>(get<DT>(u, e), s, r);
 #pragma unroll
   for (int h = 0; h < E / 4; h++)
     o[h] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[4 * h + 3], c[4 * h + 2], 0x0c0c0400u),
                                  __builtin_amdgcn_perm(c[4 * h + 1], c[4 * h], 0x0c0c0400u), 0x05040100u);
 }
-__device__ __forceinline__ bool plain_scale(float s) { return !(s >= 0x1p-60f && s <= 0x1p60f); }
+// (the same in every lane, as s is)
+__device__ __forceinline__ bool plain_scale(float s) {
+  return __builtin_amdgcn_readfirstlane(!(s >= 0x1p-60f && s <= 0x1p60f));
+}
 
 // One workgroup of NT threads a row; a thread keeps NV units of it in registers,
 // so the row is read once.  NV = 0: rows of any length, read twice.
@@ -111,16 +105,20 @@ __global__ void __launch_bounds__(NT) k_quant(const void* __restrict__ x, int8_t
   const int tid = threadIdx.x;
   const size_t row = blockIdx.x;
   const typename Elem<DT>::T* p = (const typename Elem<DT>::T*)x + row * K;
+  const int V = K / E;
   uint4 u[N];
   uint32_t top = 0;
+  typename Elem<DT>::T behind[1] = {0};  // element V E + tid
+  if (tid < K - V * E) behind[0] = p[V * E + tid];
   if constexpr (NV > 0) {
 #pragma unroll
-    for (int j = 0; j < NV; j++) u[j] = unit<DT>(p, tid + j * NT, K);
+    for (int j = 0; j < NV; j++) u[j] = unit<DT>(p, tid + j * NT, V);
 #pragma unroll
     for (int j = 0; j < NV; j++) top = top_of<DT>(u[j], top);
   } else {
-    for (int i = tid; i * E < K; i += NT) top = top_of<DT>(unit<DT>(p, i, K), top);
+    for (int i = tid; i < V; i += NT) top = top_of<DT>(unit<DT>(p, i, V), top);
   }
+  top = max(top, __float_as_uint(ub_load<DT>(behind, 0)) & 0x7fffffffu);
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
   if ((tid & 63) == 0) wm[tid >> 6] = top;
@@ -131,18 +129,30 @@ __global__ void __launch_bounds__(NT) k_quant(const void* __restrict__ x, int8_t
   if (tid == 0) scale[row] = s;
   const bool plain = plain_scale(s);
   const float r = plain ? 0.f : __fdiv_rn(1.0f, s);
-  auto store = [&](const uint4& v, int i) {
+  int8_t* const qr = q + row * ld;
+  auto store = [&](auto P, const uint4& v, int i) {
+    constexpr bool PLAIN = decltype(P)::value;
+    if (i == V) return;  // (below)
     uint32_t o[E / 4];
-    codes<DT>(v, s, r, plain, o);
-    if constexpr (E == 4) ((uint32_t*)(q + row * ld))[i] = o[0];
-    else ((uint2*)(q + row * ld))[i] = make_uint2(o[0], o[1]);
+    codes<DT, PLAIN>(v, s, r, o);
+    if constexpr (E == 4) ((uint32_t*)qr)[i] = o[0];
+    else ((uint2*)qr)[i] = make_uint2(o[0], o[1]);
   };
-  if constexpr (NV > 0) {
-#pragma unroll
-    for (int j = 0; j < NV; j++)
-      if ((tid + j * NT) * E < ld) store(u[j], tid + j * NT);
+  auto last = [&](auto P) {
+    if (tid < E && V * E < ld) qr[V * E + tid] = (int8_t)code<decltype(P)::value>(ub_load<DT>(behind, 0), s, r);
+  };
+  if (NV == 0 || plain) {
+    auto all = [&](auto P) {
+      for (int i = tid; i * E < ld; i += NT) store(P, unit<DT>(p, i, V), i);
+      last(P);
+    };
+    if (plain) all(std::true_type{});
+    else all(std::false_type{});
   } else {
-    for (int i = tid; i * E < ld; i += NT) store(unit<DT>(p, i, K), i);
+#pragma unroll
+    for (int j = 0; j < N; j++)
+      if ((tid + j * NT) * E < ld) store(std::false_type{}, u[j], tid + j * NT);
+    last(std::false_type{});
   }
 }
 
@@ -432,7 +442,7 @@ k_i8_ring(const int8_t* __restrict__ A, const float* __restrict__ sa, const int8
 // weight loads are on their way: a launch less, and quantizing M K values hides
 // behind the stream.  The wavefronts' sums meet
 // in LDS.
-constexpr int DW = 16;
+constexpr int DW = 16, kDecTiles = 64;  // wavefronts; tiles of a workgroup, at most
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* base, uint64_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
@@ -442,11 +452,13 @@ template <int DT, int SP>
 __global__ void __launch_bounds__(64 * DW) k_i8_dec(const void* __restrict__ x, const int8_t* __restrict__ W,
                                                     const float* __restrict__ sw, const float* __restrict__ bias,
                                                     void* __restrict__ y, int M, int K, int N, int ld) {
-  constexpr int E = Elem<DT>::E, XU = SP > 4 ? 4 : 8;
+  constexpr int E = Elem<DT>::E, XU = 8;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   int* red = (int*)lds;                       // [16 wavefronts][M][17]
   float* ssa = (float*)(red + DW * M * 17);   // [16]
-  uint8_t* a = (uint8_t*)(ssa + 16);          // [M][ld + 16]
+  float* ssw = ssa + 16;                      // [1024]: the columns of all its tiles, and their bias
+  float* sb = ssw + 16 * kDecTiles;
+  uint8_t* a = (uint8_t*)(sb + 16 * kDecTiles);  // [M][ld + 16]
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, h = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int steps = ld / 64, nc = (steps + DW * SP - 1) / (DW * SP), nt = (N + 15) / 16;
@@ -469,9 +481,16 @@ __global__ void __launch_bounds__(64 * DW) k_i8_dec(const void* __restrict__ x, 
   const int lg = M > 8 ? 0 : M > 4 ? 1 : M > 2 ? 2 : M > 1 ? 3 : 4;  // log2 of the wavefronts
   const int m = wave >> lg, u0 = ((wave & ((1 << lg) - 1)) << 6) + lane, us = 64 << lg;
   const typename Elem<DT>::T* p = (const typename Elem<DT>::T*)x + (size_t)min(m, M - 1) * K;
+  const int V = K / E;
   uint4 xu[XU];
 #pragma unroll
-  for (int j = 0; j < XU; j++) xu[j] = unit<DT>(p, u0 + j * us, K);
+  for (int j = 0; j < XU; j++) xu[j] = unit<DT>(p, u0 + j * us, V);
+  // the scales wait in LDS: asked for at the end of a tile, they would cost it
+  // their latency and, loads returning in order, that of the weights in flight
+  const int cn0 = 16 * ((int)blockIdx.x + (tid >> 4) * (int)gridDim.x) + (tid & 15);
+  const float my_sw = cn0 < N ? sw[cn0] : 0.f, my_b = bias && cn0 < N ? bias[cn0] : 0.f;
+  typename Elem<DT>::T behind[1] = {0};  // element V E + u0
+  if (u0 < K - V * E) behind[0] = p[V * E + u0];
   int t = blockIdx.x, c = 0;  // the piece being multiplied
   auto next = [&](int& t, int& c) {
     if (++c == nc) {
@@ -482,16 +501,21 @@ __global__ void __launch_bounds__(64 * DW) k_i8_dec(const void* __restrict__ x, 
   int tn = t, cn = c;
   load(b0, tn, cn);
   next(tn, cn);
-  load(b1, tn, cn);
-  next(tn, cn);
+  if constexpr (SP <= 4) {  // (no registers for the second set beside the activations' otherwise)
+    load(b1, tn, cn);
+    next(tn, cn);
+  }
   {
     uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < XU; j++) top = top_of<DT>(xu[j], top);
-    for (int i = u0 + XU * us; i * E < K; i += us) top = top_of<DT>(unit<DT>(p, i, K), top);
+    for (int i = u0 + XU * us; i < V; i += us) top = top_of<DT>(unit<DT>(p, i, V), top);
+    top = max(top, __float_as_uint(ub_load<DT>(behind, 0)) & 0x7fffffffu);
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
     if (lane == 0) red[wave] = (int)top;
+    ssw[tid] = my_sw;
+    sb[tid] = my_b;
     __syncthreads();
     for (int w = 0; w < 1 << lg; w++) top = max(top, (uint32_t)red[(m << lg) + w]);
     __syncthreads();
@@ -499,19 +523,34 @@ __global__ void __launch_bounds__(64 * DW) k_i8_dec(const void* __restrict__ x, 
     const bool plain = plain_scale(s);
     const float rs = plain ? 0.f : __fdiv_rn(1.0f, s);
     if (lane == 0 && m < M) ssa[m] = s;
-    auto store = [&](const uint4& v, int i) {
-      if (i * E >= ld || m >= M) return;
+    auto store = [&](auto P, const uint4& v, int i) {
+      if (i * E >= ld || i == V) return;  // (unit V: last)
       uint32_t o[E / 4];
-      codes<DT>(v, s, rs, plain, o);
+      codes<DT, decltype(P)::value>(v, s, rs, o);
       if constexpr (E == 4) *(uint32_t*)(a + m * pitch + 4 * i) = o[0];
       else *(uint2*)(a + m * pitch + 8 * i) = make_uint2(o[0], o[1]);
     };
+    auto rest = [&](auto P, int from) {
+      for (int i = from; i * E < ld; i += us) store(P, unit<DT>(p, i, V), i);
+      if (u0 < E && V * E < ld)
+        a[m * pitch + V * E + u0] = (uint8_t)code<decltype(P)::value>(ub_load<DT>(behind, 0), s, rs);
+    };
+    if (m >= M) {
+    } else if (plain) {
+      rest(std::true_type{}, u0);
+    } else {
 #pragma unroll
-    for (int j = 0; j < XU; j++) store(xu[j], u0 + j * us);
-    for (int i = u0 + XU * us; i * E < ld; i += us) store(unit<DT>(p, i, K), i);
+      for (int j = 0; j < XU; j++) store(std::false_type{}, xu[j], u0 + j * us);
+      rest(std::false_type{}, u0 + XU * us);
+    }
+  }
+  if constexpr (SP > 4) {
+    load(b1, tn, cn);
+    next(tn, cn);
   }
   __syncthreads();
   i32x4 acc = {0, 0, 0, 0};
+  int mine = 0;  // which of the workgroup's tiles
   const uint8_t* ar = a + min(r, M - 1) * pitch + 16 * h;  // (tokens past M: not used)
   auto work = [&](i32x4 (&b)[SP]) {
 #pragma unroll
@@ -533,11 +572,12 @@ __global__ void __launch_bounds__(64 * DW) k_i8_dec(const void* __restrict__ x, 
         int v = 0;
 #pragma unroll
         for (int w = 0; w < DW; w++) v += red[(w * M + m) * 17 + (tid & 15)];
-        if (n < N) put<DT>(y, (size_t)m * N + n, v, ssa[m], sw[n], bias ? bias[n] : 0.f);
+        if (n < N) put<DT>(y, (size_t)m * N + n, v, ssa[m], ssw[16 * mine + (tid & 15)], sb[16 * mine + (tid & 15)]);
       }
       __builtin_amdgcn_s_waitcnt(0xC07F);
       ub_barrier();
     }
+    if (c == nc - 1) mine++;
     next(t, c);
   };
   while (t < nt) {
@@ -548,7 +588,7 @@ __global__ void __launch_bounds__(64 * DW) k_i8_dec(const void* __restrict__ x, 
 }
 
 constexpr int kLds = 160 * 1024;  // of a CU
-size_t dec_lds(int M, int ld) { return sizeof(int) * DW * M * 17 + 64 + (size_t)M * (ld + 16); }
+size_t dec_lds(int M, int ld) { return sizeof(int) * (DW * M * 17 + 16 + 32 * kDecTiles) + (size_t)M * (ld + 16); }
 
 template <int DT, int SP>
 void dec(const void* x, const int8_t* w, const float* sw, const float* bias, void* y, int M, int K, int N, int ld,
@@ -641,7 +681,7 @@ void gemm(const int8_t* q, const float* sa, const int8_t* w, const float* sw, co
 template <int DT>
 int linear(const char* nm, const void* x, const int8_t* w, const float* sw, const float* bias, void* y, int M, int K,
            int N, int ld, hipStream_t s) {
-  if (M <= 16 && dec_lds(M, ld) <= kLds) {
+  if (M <= 16 && N <= 256 * 16 * kDecTiles && dec_lds(M, ld) <= kLds) {
     dec<DT>(x, w, sw, bias, y, M, K, N, ld, s);
     return UB_OK;
   }
