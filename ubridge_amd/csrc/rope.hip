@@ -16,21 +16,22 @@
 // cosine are Taylor polynomials whose first dropped terms are below 2e-9 and
 // 2e-9.  The rotation is f32 and rounds once, to the output's type.
 //
-// One workgroup turns the heads of one token (or a part of them, where the
-// tokens alone leave CUs idle).  Its threads load their first 16 bytes of q, k
-// and v, then each makes the sine and cosine of one pair into LDS, so that a
-// pair costs one evaluation a token and not one a head, and the loads are in
-// flight meanwhile.
+// A wavefront turns the heads of one token, or a part of them where there are too
+// few tokens to fill the CUs, and no wavefront waits for another.  Lanes stand
+// for 16-byte units of a head, so a lane's pairs are the same in every head: one
+// sine and cosine a pair and token, made by 64 lanes at once and dealt out
+// through LDS, then in registers for all heads.  HBM-bound: the next head's loads
+// are in flight while one is turned, in many wavefronts a SIMD.
 #include "common.h"
 
 namespace {
 
-constexpr int NT = 256;
+constexpr int NW = 4;  // wavefronts of a workgroup
 
 struct RopeDev {
   UbridgeRopeArgs a;
   int heads;    // q, k and (append) v heads of a token
-  int parts;    // workgroups a token
+  int parts;    // wavefronts a token
   int lg;       // log2 of the lanes of a head
   int* err;
 };
@@ -40,57 +41,98 @@ template <> struct Elem<UB_F32> { typedef float T; static constexpr int E = 4; }
 template <> struct Elem<UB_F16> { typedef uint16_t T; static constexpr int E = 8; };
 template <> struct Elem<UB_BF16> { typedef uint16_t T; static constexpr int E = 8; };
 
-// n <= E elements from p (element-aligned: gfx950 loads 16 bytes from there)
+// n elements from p, at most a unit (element-aligned: gfx950 loads 16 bytes
+// from there)
 template <int DT>
-__device__ __forceinline__ void ld(float (&v)[Elem<DT>::E], const typename Elem<DT>::T* p, int n) {
+__device__ __forceinline__ uint4 ld(const typename Elem<DT>::T* p, int n) {
   constexpr int E = Elem<DT>::E;
-  typename Elem<DT>::T r[E];
+  uint4 v = make_uint4(0, 0, 0, 0);
   if (n >= E) {
-    __builtin_memcpy(r, p, 16);
+    __builtin_memcpy(&v, p, 16);
   } else {
-#pragma unroll
-    for (int j = 0; j < E; j++) r[j] = j < n ? p[j] : (typename Elem<DT>::T)0;
+    uint64_t lo = 0, hi = 0;
+    constexpr int B = 8 * sizeof(typename Elem<DT>::T);
+#pragma nounroll
+    for (int e = 0; e < n; e++) {
+      uint64_t x;
+      if constexpr (DT == UB_F32) x = __float_as_uint(p[e]);
+      else x = p[e];
+      if (e < E / 2) lo |= x << (B * e);
+      else hi |= x << (B * (e - E / 2));
+    }
+    v = make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
   }
-#pragma unroll
-  for (int j = 0; j < E; j++) v[j] = ub_load<DT>(r, j);
+  return v;
+}
+template <int DT>
+__device__ __forceinline__ float get(const uint4& w, int e) {
+  const uint32_t p[4] = {w.x, w.y, w.z, w.w};
+  if constexpr (DT == UB_F32) return __uint_as_float(p[e]);
+  else if constexpr (DT == UB_F16) return ub_f16_to_f32((uint16_t)(p[e >> 1] >> (16 * (e & 1))));
+  else return __uint_as_float((e & 1) ? p[e >> 1] & 0xffff0000u : p[e >> 1] << 16);
 }
 
 template <int DT>
-__device__ __forceinline__ void st(typename Elem<DT>::T* p, const float (&v)[Elem<DT>::E], int n) {
-  constexpr int E = Elem<DT>::E;
-  typename Elem<DT>::T r[E];
-#pragma unroll
-  for (int j = 0; j < E; j++) ub_store<DT>(r, j, v[j]);
-  if (n >= E) {
-    __builtin_memcpy(p, r, 16);
+__device__ __forceinline__ uint4 pack(const float (&v)[Elem<DT>::E]) {
+  if constexpr (DT == UB_F32) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
   } else {
+    uint32_t w[4];
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-    for (int j = 0; j < E; j++)
-      if (j < n) p[j] = r[j];
+    for (int i = 0; i < 4; i++) {
+      const f32x2 x = {v[2 * i], v[2 * i + 1]};
+      if constexpr (DT == UB_BF16) {
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2));
+      } else {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, f16x2));
+      }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+template <int DT>
+__device__ __forceinline__ void st(typename Elem<DT>::T* p, const uint4& v, int n) {
+  constexpr int E = Elem<DT>::E;
+  if (n >= E) {
+    __builtin_memcpy(p, &v, 16);
+  } else {
+    uint64_t lo = (uint64_t)v.y << 32 | v.x, hi = (uint64_t)v.w << 32 | v.z;
+    constexpr int B = 8 * sizeof(typename Elem<DT>::T);
+#pragma nounroll
+    for (int e = 0; e < n; e++) {
+      if (e == E / 2) lo = hi;
+      if constexpr (DT == UB_F32) p[e] = __uint_as_float((uint32_t)lo);
+      else p[e] = (uint16_t)lo;
+      lo >>= B;
+    }
   }
 }
 
 // x / s to e4m3, saturating, NaN kept
 template <int E>
 __device__ __forceinline__ void st8(uint8_t* p, const float (&v)[E], float s, int n) {
-  float q[E];
-#pragma unroll
-  for (int j = 0; j < E; j++) {
-    const float x = __fdiv_rn(v[j], s);
-    q[j] = x != x ? x : fminf(fmaxf(x, -448.f), 448.f);
-  }
-  int w[E / 4];
+  uint32_t w[E / 4];
 #pragma unroll
   for (int h = 0; h < E / 4; h++) {
-    w[h] = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * h], q[4 * h + 1], 0, false);
-    w[h] = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * h + 2], q[4 * h + 3], w[h], true);
+    float q[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const float x = __fdiv_rn(v[4 * h + j], s);
+      q[j] = x != x ? x : fminf(fmaxf(x, -448.f), 448.f);
+    }
+    w[h] = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+    w[h] = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w[h], true);
   }
   if (n >= E) {
     __builtin_memcpy(p, w, E);
   } else {
-#pragma unroll
-    for (int j = 0; j < E; j++)
-      if (j < n) p[j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
+    uint64_t x = w[0];
+    if constexpr (E == 8) x |= (uint64_t)w[1] << 32;
+#pragma nounroll
+    for (int j = 0; j < n; j++, x >>= 8) p[j] = (uint8_t)x;
   }
 }
 
@@ -107,130 +149,143 @@ __device__ __forceinline__ float2 turn(double pos, double t, float f, float sign
   return make_float2(f * ((k == 1 || k == 2) ? -co : co), f * sign * (k >= 2 ? -si : si));
 }
 
+struct Two { uint4 a, b; };
+
 // CT: the cache's type (DT or UB_E4M3), -1 without a cache.
 template <int DT, bool INTER, int CT>
-__global__ void __launch_bounds__(NT) k_rope(const RopeDev d) {
+__global__ void __launch_bounds__(64 * NW) k_rope(const RopeDev d) {
   typedef typename Elem<DT>::T T;
-  constexpr int E = Elem<DT>::E;
+  constexpr int E = Elem<DT>::E, NP = INTER ? E / 2 : E;  // pairs of a unit
   constexpr bool APPEND = CT >= 0;
-  extern __shared__ float2 cs[];
+  extern __shared__ float2 lds[];
   const UbridgeRopeArgs& a = d.a;
-  const int tid = threadIdx.x;
-  const int t = blockIdx.x / d.parts, part = blockIdx.x - t * d.parts;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned id = blockIdx.x * NW + wave;
+  const int t = (int)(id / (unsigned)d.parts), part = (int)(id - (unsigned)t * d.parts);
+  if (t >= a.T) return;
   const int half = a.rot / 2;
-  const int lanes = 1 << d.lg, ul = tid & (lanes - 1);
-  const int hstep = (NT >> d.lg) * d.parts;
-  const int h0 = (tid >> d.lg) * d.parts + part;
+  float2* cs = lds + wave * (half > 0 ? half : 1);
+  const int lanes = 1 << d.lg, ul = lane & (lanes - 1);
+  const int step = (64 >> d.lg) * d.parts;
 
-  // where head h of the token lies, and its number of units
-  const int PU = INTER ? 0 : (half + E - 1) / E;          // units of pairs
+  const int PU = INTER ? 0 : (half + E - 1) / E;  // units of pairs, ahead of those that pass through
   const int nu_r = INTER ? (a.D + E - 1) / E : PU + (a.D - a.rot + E - 1) / E;
   const int nu_v = (a.D + E - 1) / E;
-  auto head = [&](int h) -> const T* {
-    if (h < a.Hq) return (const T*)a.q + t * a.q_st + h * a.q_sh;
-    h -= a.Hq;
-    if (h < a.Hkv) return (const T*)a.k + t * a.k_st + h * a.k_sh;
-    return (const T*)a.v + t * a.v_st + (h - a.Hkv) * a.v_sh;
-  };
-  float x0[E], x1[E];
-  // unit u of a rotated head: E pairs (x0, x1), or E elements (x0) that pass
-  // through or (interleaved) hold E / 2 pairs
-  auto load = [&](int h, int u) {
-    const T* p = head(h);
-    if (APPEND && h >= a.Hq + a.Hkv) {
-      ld<DT>(x0, p + u * E, a.D - u * E);
-    } else if (INTER) {
-      ld<DT>(x0, p + u * E, a.D - u * E);
-    } else if (u < PU) {
-      ld<DT>(x0, p + u * E, half - u * E);
-      ld<DT>(x1, p + half + u * E, half - u * E);
-    } else {
-      const int e = a.rot + (u - PU) * E;
-      ld<DT>(x0, p + e, a.D - e);
-    }
-  };
-  auto units = [&](int h) { return APPEND && h >= a.Hq + a.Hkv ? nu_v : nu_r; };
-  int h = h0, u = ul;
-  while (h < d.heads && u >= units(h)) h += hstep;  // (lanes past this head's units)
-  const bool first = h < d.heads;
-  if (first) load(h, u);
-
+  const int hr = a.Hq + a.Hkv;  // heads that turn
+  const T* const qt = (const T*)a.q + t * a.q_st;
+  const T* const kt = (const T*)a.k + t * a.k_st;
+  const T* const vt = (const T*)a.v + t * a.v_st;
   const long pos = a.rot == 0 ? 0 : a.pos64 ? ((const long*)a.positions)[t] : (long)((const int*)a.positions)[t];
-  for (int i = tid; i < half; i += NT)
-    cs[i] = turn((double)pos, a.turns[i], a.factor, a.inverse ? -1.f : 1.f);
-  long slot = 0;
-  if constexpr (APPEND) {
-    slot = a.slots[t];
-    if (slot >= (long)a.P * a.S) {  // out of the cache: reported, not stored
-      if (tid == 0 && part == 0) *d.err = UB_ERR_INDEX;
-      slot = -1;
-    }
-  }
-  __syncthreads();
-  if (!first) return;
-  const long page = APPEND && slot >= 0 ? slot / a.S : 0;
-  const int at = APPEND && slot >= 0 ? (int)(slot - page * a.S) : 0;
+  long slot = APPEND ? a.slots[t] : 0;
 
+  // unit u of head h: E pairs (x0, x1), or E elements (x0) that pass through or
+  // (interleaved) hold E / 2 pairs
+  auto load = [&](int h, int u) {
+    const T* p = h < a.Hq ? qt + h * a.q_sh : h < hr ? kt + (h - a.Hq) * a.k_sh : vt + (h - hr) * a.v_sh;
+    const bool pairs = !INTER && h < hr && u < PU;
+    const int e = pairs || INTER || h >= hr ? u * E : a.rot + (u - PU) * E;
+    Two r;
+    r.a = ld<DT>(p + e, (pairs ? half : a.D) - e);
+    r.b = make_uint4(0, 0, 0, 0);
+    if (!INTER && pairs) r.b = ld<DT>(p + half + e, half - e);
+    return r;
+  };
+  long page = 0;
+  int at = 0;
   auto put = [&](int h, int e, const float (&v)[E], int n) {
     if (h < a.Hq) {
-      st<DT>((T*)a.q_out + ((long)t * a.Hq + h) * a.D + e, v, n);
+      st<DT>((T*)a.q_out + ((long)t * a.Hq + h) * a.D + e, pack<DT>(v), n);
     } else if constexpr (!APPEND) {
-      st<DT>((T*)a.k_out + ((long)t * a.Hkv + h - a.Hq) * a.D + e, v, n);
+      st<DT>((T*)a.k_out + ((long)t * a.Hkv + h - a.Hq) * a.D + e, pack<DT>(v), n);
     } else {
       if (slot < 0) return;
-      const bool key = h < a.Hq + a.Hkv;
-      const int g = h - a.Hq - (key ? 0 : a.Hkv);
+      const bool key = h < hr;
+      const int g = h - (key ? a.Hq : hr);
       const long o = page * a.page_stride + ((long)g * a.S + at) * a.D + e;
       void* base = key ? a.k_pages : a.v_pages;
       if constexpr (CT == UB_E4M3) {
         const float* sc = key ? a.k_scale : a.v_scale;
         st8<E>((uint8_t*)base + o, v, sc ? sc[g] : 1.f, n);
       } else {
-        st<DT>((T*)base + o, v, n);
+        st<DT>((T*)base + o, pack<DT>(v), n);
       }
     }
   };
-  for (;;) {
-    if (APPEND && h >= a.Hq + a.Hkv) {
-      put(h, u * E, x0, a.D - u * E);
-    } else if (INTER) {
+
+  // this lane's heads of unit u: from h on, below end
+  int h = 0, end = 0;
+  auto range = [&](int u) {
+    h = (lane >> d.lg) * d.parts + part;
+    end = u < nu_r ? (APPEND && u < nu_v ? d.heads : hr) : u < nu_v ? d.heads : 0;
+    if (u >= nu_r && h < hr) h += (hr - h + step - 1) / step * step;  // (only v has this unit)
+  };
+  Two x = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  int u = ul;
+  range(u);
+  if (h < end) x = load(h, u);
+  for (int i = lane; i < half; i += 64)
+    cs[i] = turn((double)pos, a.turns[i], a.factor, a.inverse ? -1.f : 1.f);
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();  // (a wavefront's LDS accesses are in order)
+  if constexpr (APPEND) {
+    if (slot >= (long)a.P * a.S) {  // out of the cache: reported, not stored
+      if (lane == 0 && part == 0) *d.err = UB_ERR_INDEX;
+      slot = -1;
+    }
+    page = slot >= 0 ? slot / a.S : 0;
+    at = slot >= 0 ? (int)(slot - page * a.S) : 0;
+  }
+  const int nu = APPEND && nu_v > nu_r ? nu_v : nu_r;
+  while (u < nu) {
+    float2 w[NP];  // of this unit's pairs
+#pragma unroll
+    for (int j = 0; j < NP; j++) w[j] = u * NP + j < half ? cs[u * NP + j] : make_float2(1.f, 0.f);
+    while (h < end) {
+      const uint4 c0 = x.a, c1 = x.b;
+      const int hi = h;
+      h += step;
+      if (h < end) x = load(h, u);
       float y[E];
+      int e = u * E, n = a.D - e;
+      if (INTER && hi < hr) {
 #pragma unroll
-      for (int j = 0; j < E; j += 2) {
-        const int p = (u * E + j) / 2;
-        const float2 c = p < half ? cs[p] : make_float2(1.f, 0.f);
-        y[j] = p < half ? x0[j] * c.x - x0[j + 1] * c.y : x0[j];
-        y[j + 1] = p < half ? x0[j + 1] * c.x + x0[j] * c.y : x0[j + 1];
-      }
-      put(h, u * E, y, a.D - u * E);
-    } else if (u < PU) {
-      float y0[E], y1[E];
+        for (int j = 0; j < E; j += 2) {  // (pairs past rot turn by nothing)
+          const float x = get<DT>(c0, j), z = get<DT>(c0, j + 1);
+          const bool in = e + j < a.rot;
+          y[j] = in ? x * w[j / 2].x - z * w[j / 2].y : x;
+          y[j + 1] = in ? z * w[j / 2].x + x * w[j / 2].y : z;
+        }
+      } else if (!INTER && hi < hr && u < PU) {
+        n = half - e;
 #pragma unroll
-      for (int j = 0; j < E; j++) {
-        const float2 c = cs[min(u * E + j, half - 1)];
-        y0[j] = x0[j] * c.x - x1[j] * c.y;
-        y1[j] = x1[j] * c.x + x0[j] * c.y;
+        for (int j = 0; j < E; j++) y[j] = get<DT>(c1, j) * w[j % NP].x + get<DT>(c0, j) * w[j % NP].y;
+        put(hi, half + e, y, n);
+#pragma unroll
+        for (int j = 0; j < E; j++) y[j] = get<DT>(c0, j) * w[j % NP].x - get<DT>(c1, j) * w[j % NP].y;
+      } else {
+        if (!INTER && hi < hr) {
+          e = a.rot + (u - PU) * E;
+          n = a.D - e;
+        }
+#pragma unroll
+        for (int j = 0; j < E; j++) y[j] = get<DT>(c0, j);
       }
-      put(h, u * E, y0, half - u * E);
-      put(h, half + u * E, y1, half - u * E);
-    } else {
-      const int e = a.rot + (u - PU) * E;
-      put(h, e, x0, a.D - e);
+      put(hi, e, y, n);
     }
     u += lanes;
-    while (h < d.heads && u >= units(h)) h += hstep, u = ul;
-    if (h >= d.heads) break;
-    load(h, u);
+    range(u);
+    if (h < end) x = load(h, u);
   }
 }
 
 template <int DT, bool INTER>
 void launch(const RopeDev& d, int ct, hipStream_t s) {
-  const dim3 grid((unsigned)d.a.T * d.parts);
-  const size_t lds = sizeof(float2) * (size_t)(d.a.rot / 2 > 0 ? d.a.rot / 2 : 1);
-  if (ct < 0) k_rope<DT, INTER, -1><<<grid, NT, lds, s>>>(d);
-  else if (ct == UB_E4M3) k_rope<DT, INTER, UB_E4M3><<<grid, NT, lds, s>>>(d);
-  else k_rope<DT, INTER, DT><<<grid, NT, lds, s>>>(d);
+  const dim3 grid(ub_cdiv((long)d.a.T * d.parts, NW));
+  const size_t lds = sizeof(float2) * NW * (size_t)(d.a.rot / 2 > 0 ? d.a.rot / 2 : 1);
+  if (ct < 0) k_rope<DT, INTER, -1><<<grid, 64 * NW, lds, s>>>(d);
+  else if (ct == UB_E4M3) k_rope<DT, INTER, UB_E4M3><<<grid, 64 * NW, lds, s>>>(d);
+  else k_rope<DT, INTER, DT><<<grid, 64 * NW, lds, s>>>(d);
 }
 
 int rope(const char* nm, const UbridgeRopeArgs* p, bool append, void* stream) {
@@ -261,13 +316,13 @@ int rope(const char* nm, const UbridgeRopeArgs* p, bool append, void* stream) {
   int nu = a.interleaved ? ub_cdiv(a.D, E) : ub_cdiv(a.rot / 2, E) + ub_cdiv(a.D - a.rot, E);
   if (append && nu < ub_cdiv(a.D, E)) nu = ub_cdiv(a.D, E);
   d.lg = 0;
-  while ((1 << d.lg) < nu && d.lg < 8) d.lg++;
-  // parts: workgroups of one token while that leaves CUs idle and a part still
-  // fills its threads
-  const int rounds = ub_cdiv(d.heads, NT >> d.lg);
+  while ((1 << d.lg) < nu && d.lg < 6) d.lg++;
+  // parts: as many wavefronts a token as have a head each, while the CUs are not
+  // full (8192 tokens of 40 heads of 128: one, 32 tokens of 48: six)
+  const int rounds = ub_cdiv(d.heads, 64 >> d.lg);
   d.parts = 1;
-  while (d.parts * 2 <= rounds && (long)a.T * d.parts < 512) d.parts *= 2;
-  UB_REQUIRE((uint64_t)a.T * d.parts * NT < 1ull << 32, "%s: T=%d", nm, a.T);
+  while (d.parts < rounds && (long)a.T * d.parts < 4096) d.parts++;
+  UB_REQUIRE((uint64_t)a.T * d.parts * 64 < 1ull << 32, "%s: T=%d", nm, a.T);
   hipStream_t s = ub_stream(stream);
   const int ct = append ? a.cache_dtype : -1;
 #define UB_GO(DT)                                   \
