@@ -10,6 +10,9 @@ import torch
 from ubridge_amd import _lib, attention, int8, kvcache, rope
 
 lib = _lib.lib
+# UbridgeRopeArgs: 12 pointers, 7 strides, 12 ints, factor, padding;
+# UbridgePagedDecodeArgs: 10 pointers, 9 strides, 10 ints, scale, softcap
+ROPE_ARGS, DECODE_ARGS = struct.Struct("@12P7q12ifi"), struct.Struct("@10P9q10i2f")
 P = 256  # a pointer that is never followed
 
 
@@ -41,7 +44,7 @@ ROPE = dict(q=P, k=P, v=P, qo=P, ko=P, pos=P, turns=P, kp=P, vp=P, slots=P, ks=0
 @pytest.mark.parametrize("name", ["ubridge_rope", "ubridge_rope_append"])
 def test_rope(name):
     fn = getattr(lib, name)
-    call = lambda **kw: fn(rope._ARGS.pack(*dict(ROPE, **kw).values()), None)
+    call = lambda **kw: fn(ROPE_ARGS.pack(*dict(ROPE, **kw).values()), None)
     refused(fn(None, None), 1, b"null argument block")
     refused(call(dt=5), 1, b"dtype 5")
     refused(call(T=-1), 1, b"T=-1")
@@ -71,7 +74,7 @@ DECODE = dict(q=P, out=P, lse=0, kp=P, vp=P, tables=P, lens=P, slopes=0, ks=0, v
 
 
 def test_paged_decode():
-    call = lambda **kw: lib.ubridge_paged_decode(attention._ARGS.pack(*dict(DECODE, **kw).values()), None)
+    call = lambda **kw: lib.ubridge_paged_decode(DECODE_ARGS.pack(*dict(DECODE, **kw).values()), None)
     refused(lib.ubridge_paged_decode(None, None), 1, b"null argument block")
     refused(call(dt=0), 1, b"dtype 0")
     refused(call(ct=1), 1, b"cache type 1")

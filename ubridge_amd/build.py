@@ -3,7 +3,8 @@
 Every HIP/C++ source under ubridge_amd/csrc is compiled with hipcc in
 parallel and linked into one shared library whose exported symbols are the
 extern "C" entry points declared in include/ubridge_hip.h; then the C++ host
-driver (driver/ub_drive.cpp) is linked against it as lib/ub_drive.
+driver (driver/ub_drive.cpp) is linked against it as lib/ub_drive, and the
+host side of the attention block (binding/native.cpp) becomes _native.so.
 
     python ubridge_amd/build.py
 """
@@ -59,6 +60,7 @@ def build(verbose=False, jobs=None):
         raise RuntimeError("link failed:\n" + r.stderr)
     os.replace(tmp, LIB)
     _build_driver()
+    _build_binding(verbose)
     return LIB
 
 
@@ -78,6 +80,32 @@ def _build_driver():
     if r.returncode != 0:
         raise RuntimeError("driver build failed:\n" + r.stderr)
     os.replace(tmp, DRIVER)
+
+
+BINDING_SRC = os.path.join(HERE, "binding", "native.cpp")
+BINDING = os.path.join(HERE, "_native.so")
+
+
+def _build_binding(verbose=False):
+    """The attention block's host side (binding/native.cpp): a CPython module
+    over torch's C++ tensors and the C ABI, whose addresses it is given when it
+    is imported; host code only."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    inc = [f"-I{p}" for p in (*include_paths(), sysconfig.get_paths()["include"])]
+    tmp = BINDING + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+           "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *inc, BINDING_SRC, "-o", tmp, "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"),
+           "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("binding build failed:\n" + r.stderr)
+    if verbose and r.stderr.strip():
+        print(r.stderr, file=sys.stderr)
+    os.replace(tmp, BINDING)
 
 
 if __name__ == "__main__":

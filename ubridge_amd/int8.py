@@ -2,15 +2,10 @@
 held as int8 with one f32 scale an output channel.  The reference has no int8
 activation path; the operator mirrors its quantized matmul (device buffers in,
 device buffers out, stream last).  It has no gradient."""
-import ctypes
-
 import torch
 
-from ._lib import check, lib, register
-from .ops import _DT_CODE, _empty, _need_cuda, stream_ptr
-
-_vp, _i = ctypes.c_void_p, ctypes.c_int
-register("ubridge_int8_linear", _i, [_vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp])
+from .native import _native, call
+from .ops import _need_cuda
 
 MAX_K = 132104  # where the int32 sum of K products stays exact
 
@@ -46,27 +41,8 @@ class Linear:
         self.N, self.K, self.ld = N, K, ld
         self.w, self.w_scale = packed, w_scale.contiguous()
         self.bias = None if bias is None else bias.contiguous()
-        self._args = (self.w.data_ptr(), self.w_scale.data_ptr(),
-                      None if bias is None else self.bias.data_ptr())
 
     def forward(self, x, out=None, stream=None):
-        _need_cuda(x)
-        dt = _DT_CODE.get(x.dtype)
-        if dt is None or x.dim() == 0 or x.shape[-1] != self.K:
-            raise ValueError(f"int8.Linear takes f32, f16 or bf16 activations [..., {self.K}]")
-        flat = x.dim() == 2 and x.is_contiguous()
-        x2 = x if flat else x.reshape(-1, self.K).contiguous()
-        M = x2.shape[0]
-        shape = (*x.shape[:-1], self.N)
-        if out is None:
-            out = _empty(shape, x.dtype, x.device, stream)
-        elif not out.is_cuda or out.dtype != x.dtype or out.shape != shape or not out.is_contiguous():
-            raise ValueError(f"int8.Linear: out must be a contiguous {x.dtype} {list(shape)}")
-        w, sw, b = self._args
-        rc = lib.ubridge_int8_linear(x2.data_ptr(), dt, w, sw, b, out.data_ptr(), M, self.K, self.N,
-                                     self.ld, stream_ptr(stream))
-        if rc:
-            check(rc)
-        return out
+        return call(_native.linear, stream, x, self.w, self.w_scale, self.bias, self.K, out)
 
     __call__ = forward

@@ -7,16 +7,17 @@ import struct
 import torch
 
 from ._lib import check, lib, register
-from .attention import _CODE, paged_decode
-from .ops import _DT_CODE, _empty, _need_cuda, stream_ptr
-from .rope import _ARGS as _ROPE_ARGS
-from .rope import _heads, _positions
+from .attention import paged_decode
+from .native import _native, call
+from .ops import _empty, _need_cuda, stream_ptr
 
 _vp, _i = ctypes.c_void_p, ctypes.c_int
-register("ubridge_rope_append", _i, [_vp, _vp])
 register("ubridge_kv_free", _i, [_vp, _vp, _i, _vp])
 register("ubridge_kv_fork", _i, [_vp, _vp, _vp, _i, _vp, _vp])
 register("ubridge_kv_compact", _i, [_vp, _vp, _vp])
+
+
+_TYPES = (torch.float16, torch.bfloat16, torch.float8_e4m3fn)
 
 
 class PagedCache:
@@ -32,7 +33,7 @@ class PagedCache:
 
     def __init__(self, kv, rows, width, k_scale=None, v_scale=None, meta=None):
         _need_cuda(kv, k_scale, v_scale, meta)
-        if kv.dim() != 6 or kv.shape[1] != 2 or not kv.is_contiguous() or kv.dtype not in _CODE:
+        if kv.dim() != 6 or kv.shape[1] != 2 or not kv.is_contiguous() or kv.dtype not in _TYPES:
             raise ValueError("PagedCache takes a contiguous f16, bf16 or e4m3 [L, 2, P, H, S, D]")
         L, _, P, H, S, D = kv.shape
         if 0 in (L, H, S, D) or rows < 0 or width < 0:
@@ -67,46 +68,10 @@ class PagedCache:
         positions q and k are turned, in one launch with the store.  e4m3 pages
         take x / scale, saturating.  A slot past the cache raises the flag that
         moe.device_error() reads."""
-        _need_cuda(q, k, v, slots, positions)
-        dt, ct = _DT_CODE.get(k.dtype), _CODE[self.kv.dtype]
-        if dt is None or v.dtype != k.dtype or ct not in (dt, 3):
-            raise ValueError(f"PagedCache.append: {k.dtype} and {v.dtype} into {self.kv.dtype} pages")
-        if not 0 <= layer < self.L:
-            raise ValueError(f"PagedCache.append: layer {layer} of {self.L}")
-        if (rope is None) != (positions is None):
-            raise ValueError("PagedCache.append: rope and positions go together")
-        T, H, D = k.shape if k.dim() == 3 else (0, -1, -1)
-        if H != self.H or D != self.D or v.shape != k.shape:
-            raise ValueError(f"PagedCache.append: k and v must be [T, {self.H}, {self.D}]")
-        if slots.shape != (T,) or slots.dtype != torch.int64 or not slots.is_contiguous():
-            raise ValueError(f"PagedCache.append: slots must be contiguous int64 [{T}]")
-        kp, kt, kh = _heads("k", k, T, D)
-        vp, vt, vh = _heads("v", v, T, D)
-        qp = qt = qh = Hq = rot = pp = p64 = inter = turns = 0
-        factor, qo = 1.0, q
-        if rope is not None:
-            if q.dtype != k.dtype:
-                raise ValueError("PagedCache.append: q and k of one type")
-            if rope.rot > D:
-                raise ValueError(f"PagedCache.append: rot={rope.rot} of heads of {D}")
-            _need_cuda(rope.turns)
-            qp, qt, qh = _heads("q", q, T, D)
-            Hq = q.shape[1]
-            qo = _empty((T, Hq, D), q.dtype, q.device, stream)
-            pp, p64 = _positions(positions, T)
-            rot, inter, factor, turns = rope.rot, rope.interleaved, rope.factor, rope.turns.data_ptr()
-        page = H * self.S * D
-        base = self.kv.data_ptr() + 2 * layer * self.P * page * self.kv.element_size()
-        args = _ROPE_ARGS.pack(qp, kp, vp, qo.data_ptr() if Hq else 0, 0, pp, turns, base,
-                               base + self.P * page * self.kv.element_size(), slots.data_ptr(),
-                               0 if self.k_scale is None else self.k_scale.data_ptr(),
-                               0 if self.v_scale is None else self.v_scale.data_ptr(), qt, qh, kt,
-                               kh, vt, vh, page, T, Hq, H, D, rot, inter, 0, p64, dt, ct, self.P,
-                               self.S, factor, 0)
-        rc = lib.ubridge_rope_append(args, stream_ptr(stream))
-        if rc:
-            check(rc)
-        return qo
+        turns, rot, inter, factor = (None, 0, False, 1.0) if rope is None else (
+            rope.turns, rope.rot, rope.interleaved, rope.factor)
+        return call(_native.append, stream, self.kv, layer, self.k_scale, self.v_scale, q, k, v, slots,
+                    positions, turns, rot, inter, factor)
 
     def attend(self, layer, q, tables=None, lens=None, **kw):
         """attention.paged_decode of q [B, Hq, D] over a layer, for all rows or

@@ -3,19 +3,11 @@ layouts, part of a head, contexts stretched linearly, by a larger base, by a
 ramp over the frequencies ("yarn") or by bands of wavelengths.  The angles are
 formed in 64 bits on the device, so positions may lie as far as a context
 reaches without a table of sines; the rotation is f32."""
-import ctypes
 import math
-import struct
 
 import torch
 
-from ._lib import check, lib, register
-from .ops import _DT_CODE, _empty, _need_cuda, stream_ptr
-
-register("ubridge_rope", ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p])
-
-# UbridgeRopeArgs: 12 pointers, 7 strides, 12 ints, factor, padding
-_ARGS = struct.Struct("@12P7q12ifi")
+from .native import _native, call
 
 
 def frequencies(rot, base=10000.0, scaling=None):
@@ -72,16 +64,6 @@ def frequencies(rot, base=10000.0, scaling=None):
     return f, factor
 
 
-def _heads(name, x, T, D):
-    """x as [T, H, D] with the last dim contiguous: (ptr, token, head stride)."""
-    if x.dim() != 3 or x.shape[0] != T or x.shape[2] != D:
-        raise ValueError(f"rope: {name} must be [{T}, heads, {D}], not {list(x.shape)}")
-    st, sh, sd = x.stride()
-    if sd != 1 and D > 1:
-        raise ValueError(f"rope: the last dim of {name} must be contiguous")
-    return x.data_ptr(), st, sh
-
-
 class Rope:
     """Rotary positions on the first `rot` elements of a head (even; the rest
     pass through).  Pairs are (x[i], x[i + rot / 2]), or neighbours when
@@ -102,29 +84,8 @@ class Rope:
                                   device=device)
 
     def _run(self, q, k, positions, inverse, stream):
-        _need_cuda(q, k, positions, self.turns)
-        dt = _DT_CODE.get(q.dtype)
-        if dt is None or (k is not None and k.dtype != q.dtype):
-            raise ValueError("rope takes f32, f16 or bf16 q and k of one type")
-        T, Hq, D = q.shape if q.dim() == 3 else (0, 0, -1)
-        if self.rot > D:
-            raise ValueError(f"rope: q must be [T, heads, D] with D >= rot={self.rot}, not {list(q.shape)}")
-        qp, qt, qh = _heads("q", q, T, D)
-        kp = kt = kh = Hkv = 0
-        qo = _empty((T, Hq, D), q.dtype, q.device, stream)
-        ko = None
-        if k is not None:
-            kp, kt, kh = _heads("k", k, T, D)
-            Hkv = k.shape[1]
-            ko = _empty((T, Hkv, D), q.dtype, q.device, stream)
-        pp, p64 = _positions(positions, T)
-        args = _ARGS.pack(qp, kp, 0, qo.data_ptr(), ko.data_ptr() if ko is not None else 0, pp,
-                          self.turns.data_ptr(), 0, 0, 0, 0, 0, qt, qh, kt, kh, 0, 0, 0, T, Hq, Hkv,
-                          D, self.rot, self.interleaved, inverse, p64, dt, dt, 0, 1, self.factor, 0)
-        rc = lib.ubridge_rope(args, stream_ptr(stream))
-        if rc:
-            check(rc)
-        return [qo, ko]
+        return call(_native.rope, stream, q, k, positions, self.turns, self.rot, self.interleaved,
+                    self.factor, inverse)
 
     def forward(self, q, k, positions, stream=None):
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
@@ -151,11 +112,3 @@ class _Turn(torch.autograd.Function):
         dq, dk = (None if d is None else d if d.stride(-1) == 1 else d.contiguous() for d in (dq, dk))
         dq, dk = ctx.rope._run(dq, dk, positions, True, None)
         return dq, dk, None, None, None
-
-
-def _positions(positions, T):
-    if positions.shape != (T,) or positions.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"rope: positions must be int32 or int64 [{T}]")
-    if T > 1 and positions.stride(0) != 1:
-        raise ValueError("rope: positions must be contiguous")
-    return positions.data_ptr(), positions.dtype == torch.int64
