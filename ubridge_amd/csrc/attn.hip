@@ -45,7 +45,7 @@ constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int W = 4;         // wavefronts of a workgroup
 constexpr int kRowCost = 2;  // steps that the first loads of a row are worth
-constexpr int kShares = 2048;  // two wavefronts a SIMD
+constexpr int kShares = 2048;  // two wavefronts a SIMD (three, 3072: 64 ragged sequences 30 -> 47 us, by spills)
 
 template <int DT>
 __device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
@@ -138,6 +138,17 @@ __device__ __forceinline__ float lse_of(float m, float l) {
   return m == -kInf ? m + l : (m - (DT == UB_F16 ? 14.f : 0.f) + __log2f(l)) * kLn2;
 }
 
+// inclusive sum over the lanes, by DPP: no LDS round trip a step
+__device__ __forceinline__ int lane_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lane 15 to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 to rows 2 and 3
+  return x;
+}
+
 // DK: 32-dim pieces of a head; PG8: S is a multiple of 8, so eight tokens 8 i
 // .. 8 i + 7 share a page; HT: tiles of 16 query heads.
 template <int DT, int CT, int DK, bool PG8, int HT>
@@ -168,10 +179,9 @@ k_decode(const Dev d) {
     return s;
   };
   for (int b0 = (a.B - 1) & ~255; b0 >= 0; b0 -= 256) tot += costs(b0);
-  int x = 0, mine = 0, b0 = 0;  // (four holds the first 256)
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) tot += __shfl_xor(tot, o, 64);
-  tot = __builtin_amdgcn_readfirstlane(tot) * Hh;
+  int mine = four[0] + four[1] + four[2] + four[3], b0 = 0;  // (four holds the first 256)
+  int x = lane_scan(mine);
+  tot = (a.B <= 256 ? __builtin_amdgcn_readlane(x, 63) : __builtin_amdgcn_readlane(lane_scan(tot), 63)) * Hh;
   const int chunk = max(1, (int)(((unsigned)tot + d.shares - 1) / (unsigned)d.shares));
   const int share = blockIdx.x * W + wave;
   for (int i = share; i < a.B; i += d.shares)  // rows without tokens are nobody's share
@@ -189,18 +199,11 @@ k_decode(const Dev d) {
   }
   int cur = share * chunk;
   const int end = (int)min((int64_t)tot, (int64_t)cur + chunk);
-  for (int before = 0;; b0 += 256) {
-    if (b0) (void)costs(b0);
-    mine = (four[0] + four[1] + four[2] + four[3]) * Hh;
-    x = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(x, o, 64);
-      if (lane >= o) x += y;
-    }
-    x += before;
-    before = __builtin_amdgcn_readlane(x, 63);
-    if (cur < before) break;
+  mine *= Hh, x *= Hh;
+  for (int before; cur >= (before = __builtin_amdgcn_readlane(x, 63));) {
+    b0 += 256;
+    mine = costs(b0) * Hh;
+    x = before + lane_scan(mine);
   }
   const int owner = __builtin_ctzll(__ballot(cur < x));  // the lane whose sequences hold cur
   int at_row = cur - __builtin_amdgcn_readlane(x - mine, owner);

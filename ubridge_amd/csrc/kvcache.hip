@@ -19,7 +19,7 @@
 
 namespace {
 
-constexpr int PT = 1024;  // threads of a planning workgroup
+constexpr int PT = 1024, kNear = 4096;  // threads of a planning workgroup; pages it lists in LDS
 
 // exclusive prefix sum over the workgroup; total in `sum`
 __device__ __forceinline__ int block_scan(int v, int* lds, int& sum) {
@@ -80,10 +80,22 @@ __global__ void __launch_bounds__(PT) k_fork_plan(const int* __restrict__ refs, 
                                                   int* plan, int P, int S, int nrows, int width,
                                                   int* err) {
   __shared__ int lds[PT / 64];
+  __shared__ int near[kNear];  // the first free pages, which is mostly all of them
   const int tid = threadIdx.x;
   int* len = plan;
   int* old = plan + n;
   int* found = plan + 2 * n;
+  // asked for ahead of the rows: the counts of the first pages
+  int f[16];
+  auto counts = [&](int p) {
+    if (p + 16 <= P) {
+      __builtin_memcpy(f, refs + p, sizeof(f));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; i++) f[i] = p + i < P ? refs[p + i] : 1;
+    }
+  };
+  counts(16 * tid);
   // lengths first: a row may be a prompt here and a sample there only if empty
   for (int j = tid; j < n; j += PT) {
     const int s = src[j], d = dst[j];
@@ -101,19 +113,18 @@ __global__ void __launch_bounds__(PT) k_fork_plan(const int* __restrict__ refs, 
     const int j = j0 + tid;
     int part = 0, page = -1;
     if (j < n && len[j] >= 0) {
-      const int m = len[j];
+      const int m = len[j], d = dst[j];
+      if (m % S != 0) page = tables[(size_t)src[j] * width + m / S];
       // the row must be empty; the claim gives it to one sample
-      if (m == 0 ? lens[dst[j]] != 0 : atomicCAS(&lens[dst[j]], 0, m) != 0) {
-        len[j] = -1;
+      if (m == 0 ? lens[d] != 0 : atomicCAS(&lens[d], 0, m) != 0) {
+        len[j] = page = -1;
         *err = UB_ERR_INDEX;
       } else if (m % S != 0) {
-        page = tables[(size_t)src[j] * width + m / S];
-        if (page < 0 || page >= P) {
-          lens[dst[j]] = 0;
+        part = page >= 0 && page < P;
+        if (!part) {
+          lens[d] = 0;
           len[j] = page = -1;
           *err = UB_ERR_INDEX;
-        } else {
-          part = 1;
         }
       }
     }
@@ -127,18 +138,20 @@ __global__ void __launch_bounds__(PT) k_fork_plan(const int* __restrict__ refs, 
   }
   int have = 0;
   for (int p0 = 0; p0 < P && have < need; p0 += PT * 16) {
-    int f[16], c = 0;
     const int p = p0 + 16 * tid;
+    if (p0) counts(p);
+    int c = 0;
 #pragma unroll
-    for (int i = 0; i < 16; i++) f[i] = p + i < P && refs[p + i] == 0;
-#pragma unroll
-    for (int i = 0; i < 16; i++) c += f[i];
+    for (int i = 0; i < 16; i++) c += f[i] == 0;
     int sum;
     int k = have + block_scan(c, lds, sum);
 #pragma unroll
     for (int i = 0; i < 16; i++)
-      if (f[i]) {
-        if (k < need) found[k] = p + i;
+      if (f[i] == 0) {
+        if (k < need) {
+          if (k < kNear) near[k] = p + i;
+          else found[k] = p + i;
+        }
         k++;
       }
     have += sum;
@@ -148,7 +161,7 @@ __global__ void __launch_bounds__(PT) k_fork_plan(const int* __restrict__ refs, 
     const int k = newp[j];
     if (k < 0) continue;
     if (k < have) {
-      newp[j] = found[k];
+      newp[j] = k < kNear ? near[k] : found[k];
     } else {  // no page left: the sample stays empty
       lens[dst[j]] = 0;
       len[j] = newp[j] = -1;
@@ -158,8 +171,10 @@ __global__ void __launch_bounds__(PT) k_fork_plan(const int* __restrict__ refs, 
 }
 
 template <int B> struct Bytes;
-template <> struct Bytes<16> { typedef uint4 T; };
-template <> struct Bytes<8> { typedef uint2 T; };
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+template <> struct Bytes<16> { typedef u32x4 T; };
+template <> struct Bytes<8> { typedef u32x2 T; };
 template <> struct Bytes<4> { typedef uint32_t T; };
 template <> struct Bytes<2> { typedef uint16_t T; };
 template <> struct Bytes<1> { typedef uint8_t T; };
@@ -168,17 +183,18 @@ template <> struct Bytes<1> { typedef uint8_t T; };
 template <int B>
 __device__ __forceinline__ void copy_units(uint8_t* d, const uint8_t* s, long n) {
   typedef typename Bytes<B>::T T;
+  constexpr int Q = 8;  // in flight a thread
   T* dp = (T*)d;
   const T* sp = (const T*)s;
-  for (long i = threadIdx.x; i < n; i += 1024) {
-    T v[4];
+  long i = threadIdx.x;
+  for (; i + 256 * (Q - 1) < n; i += 256 * Q) {
+    T v[Q];
 #pragma unroll
-    for (int q = 0; q < 4; q++)
-      if (i + 256 * q < n) v[q] = sp[i + 256 * q];
+    for (int q = 0; q < Q; q++) v[q] = sp[i + 256 * q];
 #pragma unroll
-    for (int q = 0; q < 4; q++)
-      if (i + 256 * q < n) dp[i + 256 * q] = v[q];
+    for (int q = 0; q < Q; q++) dp[i + 256 * q] = v[q];
   }
+  for (; i < n; i += 256) dp[i] = sp[i];
 }
 
 // Workgroup (x, j): slice x of sample j's new page; x = 0 also writes its row.
