@@ -73,6 +73,17 @@ def test_linear_large(dev, M, K, N):
     near(lin(x.to(dev)), x, w, ws, b, dev)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N,bias", [(40, 13970, 450, True), (490, 9272, 361, False), (114, 12604, 2482, True),
+                                        (17, 20000, 33, False), (130, 5000, 129, True)])
+def test_linear_parts(dev, dtype, M, K, N, bias):
+    # long rows over few tiles: K in parts, some of unequal length
+    x, w, ws, b, lin = make(dev, M, K, N, dtype, bias)
+    y = lin(x.to(dev))
+    near(y, x, w, ws, b, dev)
+    assert torch.equal(y, lin(x.to(dev)))
+
+
 @pytest.mark.parametrize("M", [1, 16, 70])
 def test_extremes(dev, M):
     # the largest sum: every product -128 * 127, at the longest row

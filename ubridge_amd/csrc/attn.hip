@@ -151,9 +151,13 @@ __device__ __forceinline__ int lane_scan(int x) {
 
 // DK: 32-dim pieces of a head; PG8: S is a multiple of 8, so eight tokens 8 i
 // .. 8 i + 7 share a page; HT: tiles of 16 query heads.
-template <int DT, int CT, int DK, bool PG8, int HT>
-__global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(DK * HT > 4 ? 1 : 2)))
+// ROW: a workgroup per row, whose wavefronts take its steps in turn and meet in
+// LDS; otherwise a share per wavefront.
+template <int DK, int HT> constexpr int kRowWaves = DK * HT > 4 ? 4 : 8;  // (by their registers)
+template <int DT, int CT, int DK, bool PG8, int HT, bool ROW>
+__global__ void __launch_bounds__(64 * (ROW ? kRowWaves<DK, HT> : W)) __attribute__((amdgpu_waves_per_eu(DK * HT > 4 ? 1 : 2)))
 k_decode(const Dev d) {
+  constexpr int NW = ROW ? kRowWaves<DK, HT> : W, SS = ROW ? NW : 1;  // steps from one of a wavefront's to the next
   constexpr int NB = (DK + 3) / 4;      // 128-dim blocks of a head
   constexpr int NP = PG8 ? 1 : 2, NV = PG8 ? 1 : 8;  // pages a lane looks up for K and V
   constexpr int EB = Raw<CT>::B;
@@ -167,58 +171,65 @@ k_decode(const Dev d) {
 
   // ---- this wavefront's share [cur, end) of the costs of all rows: the sum
   // over the sequences (lane: four neighbours of every 256), then the place
-  int four[4], tot = 0;
-  auto costs = [&](int b0) {
-    int s = 0;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int b = b0 + 4 * lane + i;
-      four[i] = b < a.B ? cost(span(d, b)) : 0;
-      s += four[i];
-    }
-    return s;
-  };
-  for (int b0 = (a.B - 1) & ~255; b0 >= 0; b0 -= 256) tot += costs(b0);
-  int mine = four[0] + four[1] + four[2] + four[3], b0 = 0;  // (four holds the first 256)
-  int x = lane_scan(mine);
-  tot = (a.B <= 256 ? __builtin_amdgcn_readlane(x, 63) : __builtin_amdgcn_readlane(lane_scan(tot), 63)) * Hh;
-  const int chunk = max(1, (int)(((unsigned)tot + d.shares - 1) / (unsigned)d.shares));
-  const int share = blockIdx.x * W + wave;
-  for (int i = share; i < a.B; i += d.shares)  // rows without tokens are nobody's share
-    if (span(d, i).steps == 0) {
-      const uint4 z = make_uint4(0, 0, 0, 0);
-      uint16_t* p = (uint16_t*)a.out + (size_t)i * a.Hq * a.D;
-      for (int e = 8 * lane; e < a.Hq * a.D; e += 512) __builtin_memcpy(p + e, &z, 16);
-      if (a.lse)
-        for (int e = lane; e < a.Hq; e += 64) a.lse[(size_t)i * a.Hq + e] = -kInf;
-    }
+  int cur = 0, end = 1, b = 0, hh = 0, at_row = 0, chunk = 1, share = 0;
+  Span sp;
   int2 cut = make_int2(-1, 0);
-  if ((int64_t)share * chunk >= tot) {
-    if (lane == 0) d.cut[share] = cut;
-    return;
-  }
-  int cur = share * chunk;
-  const int end = (int)min((int64_t)tot, (int64_t)cur + chunk);
-  mine *= Hh, x *= Hh;
-  for (int before; cur >= (before = __builtin_amdgcn_readlane(x, 63));) {
-    b0 += 256;
-    mine = costs(b0) * Hh;
-    x = before + lane_scan(mine);
-  }
-  const int owner = __builtin_ctzll(__ballot(cur < x));  // the lane whose sequences hold cur
-  int at_row = cur - __builtin_amdgcn_readlane(x - mine, owner);
-  int b = b0 + 4 * owner;
+  if constexpr (ROW) {
+    b = (int)blockIdx.x / Hh, hh = (int)blockIdx.x - b * Hh;
+    sp = span(d, b);
+  } else {
+    int four[4], tot = 0;
+    auto costs = [&](int b0) {
+      int s = 0;
 #pragma unroll
-  for (int i = 0; i < 3; i++) {
-    const int s = __builtin_amdgcn_readlane(four[i], owner) * Hh;
-    if (b == b0 + 4 * owner + i && at_row >= s) {
-      at_row -= s;
-      b++;
+      for (int i = 0; i < 4; i++) {
+        const int b = b0 + 4 * lane + i;
+        four[i] = b < a.B ? cost(span(d, b)) : 0;
+        s += four[i];
+      }
+      return s;
+    };
+    for (int b0 = (a.B - 1) & ~255; b0 >= 0; b0 -= 256) tot += costs(b0);
+    int mine = four[0] + four[1] + four[2] + four[3], b0 = 0;  // (four holds the first 256)
+    int x = lane_scan(mine);
+    tot = (a.B <= 256 ? __builtin_amdgcn_readlane(x, 63) : __builtin_amdgcn_readlane(lane_scan(tot), 63)) * Hh;
+    chunk = max(1, (int)(((unsigned)tot + d.shares - 1) / (unsigned)d.shares));
+    share = blockIdx.x * W + wave;
+    for (int i = share; i < a.B; i += d.shares)  // rows without tokens are nobody's share
+      if (span(d, i).steps == 0) {
+        const uint4 z = make_uint4(0, 0, 0, 0);
+        uint16_t* p = (uint16_t*)a.out + (size_t)i * a.Hq * a.D;
+        for (int e = 8 * lane; e < a.Hq * a.D; e += 512) __builtin_memcpy(p + e, &z, 16);
+        if (a.lse)
+          for (int e = lane; e < a.Hq; e += 64) a.lse[(size_t)i * a.Hq + e] = -kInf;
+      }
+    if ((int64_t)share * chunk >= tot) {
+      if (lane == 0) d.cut[share] = cut;
+      return;
     }
+    cur = share * chunk;
+    end = (int)min((int64_t)tot, (int64_t)cur + chunk);
+    mine *= Hh, x *= Hh;
+    for (int before; cur >= (before = __builtin_amdgcn_readlane(x, 63));) {
+      b0 += 256;
+      mine = costs(b0) * Hh;
+      x = before + lane_scan(mine);
+    }
+    const int owner = __builtin_ctzll(__ballot(cur < x));  // the lane whose sequences hold cur
+    at_row = cur - __builtin_amdgcn_readlane(x - mine, owner);
+    b = b0 + 4 * owner;
+#pragma unroll
+    for (int i = 0; i < 3; i++) {
+      const int s = __builtin_amdgcn_readlane(four[i], owner) * Hh;
+      if (b == b0 + 4 * owner + i && at_row >= s) {
+        at_row -= s;
+        b++;
+      }
+    }
+    sp = span(d, b);
+    hh = (int)((unsigned)at_row / (unsigned)cost(sp));
+    at_row -= hh * cost(sp);  // the share starts this far into the row
   }
-  Span sp = span(d, b);
-  int hh = (int)((unsigned)at_row / (unsigned)cost(sp));
-  at_row -= hh * cost(sp);  // the share starts this far into the row
 
   const float cap = a.softcap;
   const uint8_t* const kbase = (const uint8_t*)a.k_pages;
@@ -234,8 +245,8 @@ k_decode(const Dev d) {
 
   while (cur < end) {
     // ---- one row, or the part of it that lies in the share
-    const int len = min(end - cur, cost(sp) - at_row);
-    const int st = max(at_row - kRowCost, 0), s1 = at_row + len - kRowCost;
+    const int len = ROW ? 1 : min(end - cur, cost(sp) - at_row);
+    const int st = ROW ? wave : max(at_row - kRowCost, 0), s1 = ROW ? sp.steps : at_row + len - kRowCost;
     cur += len;
     const int h = hh / d.HG, hg = hh - h * d.HG;
     const int row_of_b = hh, bb = b;
@@ -246,8 +257,14 @@ k_decode(const Dev d) {
       do sp = span(d, ++b);
       while (sp.steps == 0);
     }
-    if (s1 <= st) continue;  // (only the row's head)
+    if (!ROW && s1 <= st) continue;  // (only the row's head)
     const int q0 = hg * 16 * HT, nq = min(d.G - q0, 16 * HT);  // its query heads
+    const size_t row0 = (size_t)bb * a.Hq + h * d.G + q0;
+    if (ROW && sq.steps == 0) {
+      for (int e = (int)threadIdx.x; e < nq * a.D; e += 64 * NW) ((uint16_t*)a.out)[row0 * a.D + e] = 0;
+      if (a.lse && (int)threadIdx.x < nq) a.lse[row0 + threadIdx.x] = -kInf;
+      return;
+    }
     const int base = sq.first / 32;
     const int* tb = a.tables + bb * a.table_stride;
 
@@ -334,9 +351,9 @@ k_decode(const Dev d) {
       load_k(s);
       load_v(s);
       bad = bad_next;
-      if (s + 1 < s1) lookup(s + 1);
+      if (s + SS < s1) lookup(s + SS);
     }
-    for (; s < s1; s++) {
+    for (; s < s1; s += SS) {
       const int t0 = 32 * (base + s) + 8 * g;  // this lane's first token
       const bool edge = 32 * (base + s) < sq.first || 32 * (base + s) + 32 > sq.n;
       // scores: x[t][tau * 4 + i] of head c, token t0 + 4 tau + i
@@ -353,7 +370,7 @@ k_decode(const Dev d) {
           for (int t = 0; t < HT; t++) acc[t][i] = mfma<DT>(k, qf[t][j], acc[t][i]);
         }
       }
-      const int sn = s + 1;
+      const int sn = s + SS;
       if (sn < s1) {
         load_k(sn);
       }
@@ -438,15 +455,62 @@ k_decode(const Dev d) {
       if (sn < s1) {
         load_v(sn);
         bad = bad_next;
-        if (sn + 1 < s1) lookup(sn + 1);
+        if (sn + SS < s1) lookup(sn + SS);
       }
     }
 
+    if constexpr (ROW) {
+      // ---- the wavefronts' sums meet in LDS, in their order
+      extern __shared__ __attribute__((aligned(16))) float so[];  // [NW][nq][D + 4]
+      __shared__ float2 sml[NW][16 * HT];
+      const int pitch = a.D + 4;
+#pragma unroll
+      for (int t = 0; t < HT; t++) {
+        l[t] += __shfl_xor(l[t], 16, 64);
+        l[t] += __shfl_xor(l[t], 32, 64);
+        const int q = 16 * t + c;
+        if (q >= nq) continue;
+        if (g == 0) sml[wave][q] = make_float2(m[t], l[t]);
+        float* p = so + (wave * nq + q) * pitch;
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int dim = 128 * nb + 32 * g + 8 * i;
+            if (dim >= a.D) continue;
+#pragma unroll
+            for (int j = 0; j < 8; j += 4)
+              *(float4*)(p + dim + j) = make_float4(o[t][nb][j][i], o[t][nb][j + 1][i], o[t][nb][j + 2][i], o[t][nb][j + 3][i]);
+          }
+      }
+      __syncthreads();
+      const int V = a.D / 4;
+      for (int e = (int)threadIdx.x; e < nq * V; e += 64 * NW) {
+        const int q = e / V, v = e - q * V;
+        float M = -kInf, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) M = fmaxf(M, sml[w][q].x);
+        const float Ms = M == -kInf ? 0.f : M;
+        float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+          const float2 ml = sml[w][q];
+          const float4 x = *(const float4*)(so + (w * nq + q) * pitch + 4 * v);
+          const float f = __builtin_amdgcn_exp2f(ml.x - Ms);
+          O.x += f * x.x, O.y += f * x.y, O.z += f * x.z, O.w += f * x.w;
+          L += f * ml.y;
+        }
+        const float f = L == 0.f ? 0.f : (a.v_scale ? a.v_scale[h] : 1.f) / L;
+        const uint32_t w[2] = {pack2<DT>(O.x * f, O.y * f), pack2<DT>(O.z * f, O.w * f)};
+        __builtin_memcpy((uint16_t*)a.out + (row0 + q) * a.D + 4 * v, w, 8);
+        if (v == 0 && a.lse) a.lse[row0 + q] = lse_of<DT>(M, L);
+      }
+      return;
+    }
     // ---- a whole row is finished here; a part leaves its sums
     const bool whole = st == 0 && s1 == sq.steps;
     const int slot = 2 * share + (st == 0);
     const float vs = a.v_scale ? a.v_scale[h] : 1.f;
-    const size_t row0 = (size_t)bb * a.Hq + h * d.G + q0;
 #pragma unroll
     for (int t = 0; t < HT; t++) {
       l[t] += __shfl_xor(l[t], 16, 64);
@@ -564,10 +628,24 @@ __global__ void __launch_bounds__(512) k_join(const Dev d, int heads) {
   }
 }
 
+template <int DT, int CT, int DK, bool PG8, int HT>
+void decode(const Dev& d, hipStream_t s) {
+  if (d.shares) {
+    k_decode<DT, CT, DK, PG8, HT, false><<<d.shares / W, 64 * W, 0, s>>>(d);
+    return;
+  }
+  constexpr int NW = kRowWaves<DK, HT>;
+  static const hipError_t once =  // (beyond 64 KiB)
+      hipFuncSetAttribute((const void*)k_decode<DT, CT, DK, PG8, HT, true>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                          NW * 16 * HT * (32 * DK + 4) * (int)sizeof(float));
+  (void)once;
+  const size_t lds = sizeof(float) * NW * (d.G < 16 * HT ? d.G : 16 * HT) * (d.a.D + 4);
+  k_decode<DT, CT, DK, PG8, HT, true><<<d.a.B * d.a.Hkv * d.HG, 64 * NW, lds, s>>>(d);
+}
 template <int DT, int CT, int DK, bool PG8>
 void decode(const Dev& d, int HT, hipStream_t s) {
-  if (HT == 1) k_decode<DT, CT, DK, PG8, 1><<<d.shares / W, 64 * W, 0, s>>>(d);
-  else k_decode<DT, CT, DK, PG8, 2><<<d.shares / W, 64 * W, 0, s>>>(d);
+  if (HT == 1) decode<DT, CT, DK, PG8, 1>(d, s);
+  else decode<DT, CT, DK, PG8, 2>(d, s);
 }
 template <int DT, int CT, int DK>
 void decode(const Dev& d, int HT, hipStream_t s) {
@@ -581,7 +659,15 @@ void decode(const Dev& d, int HT, hipStream_t s) {
   else if (d.a.D <= 128) decode<DT, CT, 4>(d, HT, s);
   else if (d.a.D <= 192) decode<DT, CT, 6>(d, HT, s);
   else decode<DT, CT, 8>(d, HT, s);
-  k_join<DT><<<d.shares, 512, 0, s>>>(d, 16 * HT);
+  if (d.shares) k_join<DT><<<d.shares, 512, 0, s>>>(d, 16 * HT);
+}
+
+void go(const Dev& d, int HT, hipStream_t s) {
+  const int dt = d.a.dtype, ct = d.a.cache_dtype;
+  if (dt == UB_BF16 && ct == UB_BF16) decode<UB_BF16, UB_BF16>(d, HT, s);
+  else if (dt == UB_BF16) decode<UB_BF16, UB_E4M3>(d, HT, s);
+  else if (ct == UB_F16) decode<UB_F16, UB_F16>(d, HT, s);
+  else decode<UB_F16, UB_E4M3>(d, HT, s);
 }
 
 }  // namespace
@@ -611,22 +697,33 @@ UB_API int ubridge_paged_decode(const UbridgePagedDecodeArgs* p, void* stream) {
   const int HT = d.G > 16 ? 2 : 1, heads = 16 * HT;
   d.HG = ub_cdiv(d.G, heads);
   const int64_t rows = (int64_t)a.B * a.Hkv * d.HG;
-  const int64_t most = rows * ((int64_t)a.width * a.S / 32 + 1 + kRowCost);  // the costs of all rows
+  int64_t steps = (int64_t)a.width * a.S / 32 + 1;  // of a row, at most
+  if (a.window > 0 && steps > a.window / 32 + 2) steps = a.window / 32 + 2;
+  const int64_t most = rows * (steps + kRowCost);  // the costs of all rows
   UB_REQUIRE(most < 0x7fffffff, "%s: %ld rows of %ld tokens", nm, (long)rows, (long)a.width * a.S);
   d.s_shift = 31;
   while ((1ll << (d.s_shift - 31)) < a.S) d.s_shift++;
   d.s_mul = (1ull << d.s_shift) / a.S + 1;
+  hipStream_t s = ub_stream(stream);
+  // A workgroup a row where the CUs have one each at most and a wavefront two
+  // steps: one launch.  us of the kernels, shares + join / rows: 8 rows of 64 tokens
+  // 6.4 + 3.5 / 5.4, of 500 6.9 + 4.5 / 7.0, of 700 (three steps) 6.9 + 4.5 / 12.0;
+  // 256 rows of 64 tokens 9.6 + 3.7 / 5.6
+  const int nw = ub_cdiv(a.D, 32) * HT > 4 ? 4 : 8;
+  if (rows <= 256 && steps <= 2 * nw) {
+    d.shares = 0;
+    d.po = d.pml = nullptr;
+    d.cut = nullptr;
+    go(d, HT, s);
+    return ub_check_launch(nm);
+  }
   d.shares = most >= kShares ? kShares : ub_cdiv(most, W) * W;
   const size_t nml = sizeof(float) * 4 * heads * d.shares, no = nml / 2 * a.D;
-  hipStream_t s = ub_stream(stream);
   UbScratch ws(s, no + nml + sizeof(int2) * d.shares);
   if (!ws.get()) return ub_set_error(UB_ERR_LAUNCH, "%s: no workspace", nm);
   d.po = (float*)ws.get();
   d.pml = d.po + no / sizeof(float);
   d.cut = (int2*)((char*)ws.get() + no + nml);
-  if (a.dtype == UB_BF16 && a.cache_dtype == UB_BF16) decode<UB_BF16, UB_BF16>(d, HT, s);
-  else if (a.dtype == UB_BF16) decode<UB_BF16, UB_E4M3>(d, HT, s);
-  else if (a.cache_dtype == UB_F16) decode<UB_F16, UB_F16>(d, HT, s);
-  else decode<UB_F16, UB_E4M3>(d, HT, s);
+  go(d, HT, s);
   return ub_check_launch(nm);
 }

@@ -25,6 +25,8 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 template <int DT> struct Elem { typedef uint16_t T; static constexpr int E = 8; };  // 16-byte units
 template <> struct Elem<UB_F32> { typedef float T; static constexpr int E = 4; };
+constexpr int kSum = 100;  // "type" of the int32 sums over a part of K
+template <> struct Elem<kSum> { typedef int T; static constexpr int E = 4; };
 
 // element e of a unit
 template <int DT>
@@ -158,7 +160,8 @@ __global__ void __launch_bounds__(NT) k_quant(const void* __restrict__ x, int8_t
 
 template <int DT>
 __device__ __forceinline__ void put(void* y, size_t i, int acc, float sa, float sw, float b) {
-  ub_store<DT>(y, i, (float)acc * sw * sa + b);
+  if constexpr (DT == kSum) ((int*)y)[i] = acc;
+  else ub_store<DT>(y, i, (float)acc * sw * sa + b);
 }
 
 // ------------------------------------------------------------------ tiles
@@ -180,12 +183,12 @@ struct Epilogue {
 #pragma unroll
       for (int r = 0; r < 16; r++) {
         const int n = min(n0 + 32 * j + 8 * (r >> 2) + 4 * kh + (r & 3), N - 1);
-        s[j][r] = sw[n];
-        b[j][r] = bias ? bias[n] : 0.f;
+        s[j][r] = DT == kSum ? 0.f : sw[n];
+        b[j][r] = DT != kSum && bias ? bias[n] : 0.f;
       }
 #pragma unroll
     for (int i = 0; i < TM; i++) {
-      const float a = sa[min(m0 + 32 * i + c, M - 1)];
+      const float a = DT == kSum ? 0.f : sa[min(m0 + 32 * i + c, M - 1)];
 #pragma unroll
       for (int j = 0; j < TN; j++)
 #pragma unroll
@@ -351,12 +354,13 @@ k_i8_gemm(const int8_t* __restrict__ A, const float* __restrict__ sa, const int8
 // The same product for grids that leave a workgroup or less to a CU, where the
 // latency of a K-step's loads is what costs: a ring of NS 128-byte steps in LDS,
 // NS - 1 of them in flight, one barrier a step.  Rows of 128 bytes, unit u of row
-// r at u ^ (r & 7).
+// r at u ^ (r & 7).  Long rows over few tiles are cut in parts of K, whose int32
+// sums (DT = kSum, exact in any order) k_i8_sum adds.
 template <int DT, int WM, int WN, int TM, int TN, int NS>
 __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2, 2)))
 k_i8_ring(const int8_t* __restrict__ A, const float* __restrict__ sa, const int8_t* __restrict__ B,
           const float* __restrict__ sw, const float* __restrict__ bias, void* __restrict__ y, int M,
-          int N, int ld) {
+          int N, int ld, int part) {
   constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN, NW = WM * WN;
   constexpr int NL = (BM + BN) / 8 / NW;  // load instructions of a wavefront and step: 8 rows each
   constexpr int ST = (BM + BN) * 128;
@@ -390,14 +394,16 @@ k_i8_ring(const int8_t* __restrict__ A, const float* __restrict__ sa, const int8
 #pragma unroll
       for (int r = 0; r < 16; r++) acc[i][j][r] = 0;
   const int l32 = lane & 31, kh = lane >> 5;
-  const int nk = ld / 128;
+  // steps k0 .. k0 + nk - 1, of which part blockIdx.y has `part`
+  const int k0 = blockIdx.y * part, nk = min(part, ld / 128 - k0);
+  if constexpr (DT == kSum) y = (int*)y + (size_t)blockIdx.y * M * N;
 #pragma unroll
-  for (int k = 0; k < NS - 1; k++) issue(min(k, nk - 1), k);  // (past K: loaded again, not used)
+  for (int k = 0; k < NS - 1; k++) issue(k0 + min(k, nk - 1), k);  // (past K: loaded again, not used)
   int slot = 0;
   for (int k = 0; k < nk; k++) {
     ub_wait_vmcnt<(NS - 2) * NL>();  // step k has landed
     ub_barrier();                    // for everyone, and step k - 1 is read
-    issue(min(k + NS - 1, nk - 1), slot == 0 ? NS - 1 : slot - 1);
+    issue(k0 + min(k + NS - 1, nk - 1), slot == 0 ? NS - 1 : slot - 1);
     const uint8_t* st = lds + slot * ST;
     i32x4 af[TM][4], bf[TN][4];
 #pragma unroll
@@ -428,6 +434,20 @@ k_i8_ring(const int8_t* __restrict__ A, const float* __restrict__ sa, const int8
   typedef Epilogue<DT, TM, TN> Out;
   static_assert(NW * Out::kStage <= NS * ST, "epilogue fits");
   Out::run(acc, lds + wave * Out::kStage, sa, sw, bias, y, M, N, m0 + wm * 32 * TM, n0 + wn * 32 * TN);
+}
+
+template <int DT>
+__global__ void __launch_bounds__(256) k_i8_sum(const int* __restrict__ part, const float* __restrict__ sa,
+                                                const float* __restrict__ sw, const float* __restrict__ bias,
+                                                void* __restrict__ y, int M, int N, int parts) {
+  const unsigned i = blockIdx.x * 256u + threadIdx.x, all = (unsigned)M * (unsigned)N;
+  if (i >= all) return;
+  const unsigned m = i / (unsigned)N, n = i - m * (unsigned)N;
+  const float a = sa[m], s = sw[n], b = bias ? bias[n] : 0.f;
+  int v = 0;
+#pragma unroll 8
+  for (int p = 0; p < parts; p++) v += part[(size_t)p * all + i];
+  put<DT>(y, i, v, a, s, b);
 }
 
 // ----------------------------------------------------------- few tokens
@@ -622,30 +642,41 @@ bool quant(const void* x, int8_t* q, float* sa, int M, int K, int ld, hipStream_
   return true;
 }
 
-// The tile that takes least, by its measured time for 128 bytes of K (0.01 us) on
-// a CU that has one workgroup of it, and for each of several (larger grids leave
-// that many to a CU, side by side or in turn): 256 x 256 205 / 205, 128 x 128 68 /
-// 62, 64 x 128 57 / 50, 64 x 64 34 / 29, 64 x 32 30 / 22.  us in a graph, with the
-// quantizing launch, M x K x N: 64 x 4096 x 6144 on these 32 / - / 20 / 15 / 13.7,
-// 201 x 3520 x 9001 40 / 24 / 38 / 32 / 33, 512 x 4096 x 4096 36 / 27 / 23 / 23 /
-// 32, 1024 x 2048 x 2048 25 / 20 / 17 / 16 / 22, 1024 x 4096 x 14336 75 / 97 / ...
-int tile_for(int M, int N) {
-  static const struct { int m, n, one, each; } t[5] = {
-      {256, 256, 205, 205}, {128, 128, 68, 62}, {64, 128, 57, 50}, {64, 64, 34, 29}, {64, 32, 30, 22}};
-  int best = 0;
+// The tile and the number of K parts that take least, by the tile's measured
+// time for 128 bytes of K (0.01 us) on a CU that has one workgroup of it, and for
+// each of several (larger grids leave that many to a CU, side by side or in
+// turn): 256 x 256 205 / 205, 128 x 128 68 / 62, 64 x 128 57 / 50, 64 x 64 34 /
+// 29, 64 x 32 30 / 22; parts cost a launch and their sums' way to memory and back.
+// us in a graph, with the quantizing launch, M x K x N: 64 x 4096 x 6144 on these
+// 32 / 24 / 20 / 15 / 13.7, 201 x 3520 x 9001 40 / 24 / 38 / 32 / 33, 512 x 4096 x
+// 4096 36 / 27 / 23 / 23 / 32, 1024 x 2048 x 2048 25 / 20 / 17 / 16 / 22, 1024 x
+// 4096 x 14336 74 / 97 / 97 / - / -
+struct Plan { int tile, parts; };
+Plan plan_for(int M, int N, int nk) {
+  static const struct { int m, n, one, each; bool parts; } t[5] = {
+      {256, 256, 205, 205, false}, {128, 128, 68, 62, true}, {64, 128, 57, 50, false}, {64, 64, 34, 29, true},
+      {64, 32, 30, 22, false}};
+  Plan best = {0, 1};
   double least = 0;
   for (int i = 0; i < 5; i++) {
-    const int64_t tiles = (int64_t)ub_cdiv(M, t[i].m) * ub_cdiv(N, t[i].n), per = (tiles + 255) / 256;
-    double cost = per == 1 ? t[i].one : (double)per * t[i].each;
-    if (i == 0 && per > 1 && tiles % 256 && tiles % 256 <= 128) cost -= 0.45 * t[i].each;  // (halves)
-    if (i == 0 || cost < least) best = i, least = cost;
+    const int64_t tiles = (int64_t)ub_cdiv(M, t[i].m) * ub_cdiv(N, t[i].n);
+    for (int p = 1; p <= 32 && p <= nk; p *= 2) {
+      if (p > 1 && (!t[i].parts || tiles * p > 1024 || (int64_t)M * N >= 1 << 26)) break;
+      const int64_t per = (tiles * p + 255) / 256;
+      double cost = per == 1 ? t[i].one : (double)per * t[i].each;
+      if (i == 0 && per > 1 && tiles % 256 && tiles % 256 <= 128) cost -= 0.45 * t[i].each;  // (halves)
+      cost *= ub_cdiv(nk, p);
+      if (p > 1) cost += 400 + (double)M * N * 8 * p / 52e3;
+      if ((i == 0 && p == 1) || cost < least) best = {i, p}, least = cost;
+    }
   }
   return best;
 }
 
 template <int DT>
-void gemm(const int8_t* q, const float* sa, const int8_t* w, const float* sw, const float* bias, void* y, int M, int N,
-          int ld, hipStream_t s) {
+void gemm(Plan plan, const int8_t* q, const float* sa, const int8_t* w, const float* sw, const float* bias, void* y, int M,
+          int N, int ld, hipStream_t s) {
+  const int part = ub_cdiv(ld / 128, plan.parts);
 #define UB_TILE(WM, WN, TM, TN, NS)                                                                      \
   {                                                                                                      \
     constexpr int lds = NS * 64 * 32 * (WM * TM + WN * TN);                                              \
@@ -653,7 +684,7 @@ void gemm(const int8_t* q, const float* sa, const int8_t* w, const float* sw, co
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, lds); \
     (void)once;                                                                                          \
     const int tiles = ub_cdiv(M, 32 * WM * TM) * ub_cdiv(N, 32 * WN * TN), rest = tiles % 256;           \
-    const int full = TM > 1 && tiles > 256 && rest <= 128 ? tiles - rest : tiles;                                  \
+    const int full = TM > 1 && tiles > 256 && rest <= 128 ? tiles - rest : tiles;                        \
     k_i8_gemm<DT, WM, WN, TM, TN, NS><<<2 * tiles - full, 64 * WM * WN, lds, s>>>(q, sa, w, sw, bias, y, M, N, ld, full); \
     return;                                                                                              \
   }
@@ -663,16 +694,16 @@ void gemm(const int8_t* q, const float* sa, const int8_t* w, const float* sw, co
     static const hipError_t once = hipFuncSetAttribute((const void*)k_i8_ring<DT, WM, WN, TM, TN, NS>,   \
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, lds); \
     (void)once;                                                                                          \
-    k_i8_ring<DT, WM, WN, TM, TN, NS><<<ub_cdiv(M, 32 * WM * TM) * ub_cdiv(N, 32 * WN * TN), 64 * WM * WN, lds, s>>>( \
-        q, sa, w, sw, bias, y, M, N, ld);                                                                \
+    k_i8_ring<DT, WM, WN, TM, TN, NS><<<dim3(ub_cdiv(M, 32 * WM * TM) * ub_cdiv(N, 32 * WN * TN), ub_cdiv(ld / 128, part)), \
+                                        64 * WM * WN, lds, s>>>(q, sa, w, sw, bias, y, M, N, ld, part);  \
     return;                                                                                              \
   }
-  switch (tile_for(M, N)) {
-    case 0: UB_TILE(2, 4, 4, 2, 4)
-    case 1: UB_RING(2, 4, 2, 1, 4)
-    case 2: UB_TILE(2, 2, 1, 2, 6)
-    case 3: UB_RING(2, 2, 1, 1, 4)
-    default: UB_TILE(2, 1, 1, 1, 8)
+  if (plan.tile == 1) UB_RING(2, 4, 2, 1, 4)
+  if (plan.tile == 3) UB_RING(2, 2, 1, 1, 4)
+  if constexpr (DT != kSum) {
+    if (plan.tile == 0) UB_TILE(2, 4, 4, 2, 4)
+    if (plan.tile == 2) UB_TILE(2, 2, 1, 2, 6)
+    UB_TILE(2, 1, 1, 1, 8)
   }
 #undef UB_TILE
 #undef UB_RING
@@ -685,13 +716,22 @@ int linear(const char* nm, const void* x, const int8_t* w, const float* sw, cons
     dec<DT>(x, w, sw, bias, y, M, K, N, ld, s);
     return UB_OK;
   }
-  UbScratch ws(s, (size_t)M * ld + sizeof(float) * (size_t)M);
+  const Plan plan = plan_for(M, N, ld / 128);
+  const int parts = ub_cdiv(ld / 128, ub_cdiv(ld / 128, plan.parts));  // (none empty)
+  const size_t sums = parts > 1 ? sizeof(int) * parts * (size_t)M * N : 0;
+  UbScratch ws(s, (size_t)M * ld + sizeof(float) * (size_t)M + sums);
   int8_t* q = (int8_t*)ws.get();
   if (!q) return ub_set_error(UB_ERR_LAUNCH, "%s: no workspace", nm);
   float* sa = (float*)(q + (size_t)M * ld);
   if (!((M >= 512 || ld <= 2048) && quant<DT, 256>(x, q, sa, M, K, ld, s)) && !quant<DT, 1024>(x, q, sa, M, K, ld, s))
     k_quant<DT, 1024, 0><<<M, 1024, 0, s>>>(x, q, sa, K, ld);
-  gemm<DT>(q, sa, w, sw, bias, y, M, N, ld, s);
+  if (parts > 1) {
+    int* part = (int*)(sa + M);
+    gemm<kSum>(plan, q, sa, w, sw, bias, part, M, N, ld, s);
+    k_i8_sum<DT><<<ub_cdiv((long)M * N, 256), 256, 0, s>>>(part, sa, sw, bias, y, M, N, parts);
+  } else {
+    gemm<DT>(plan, q, sa, w, sw, bias, y, M, N, ld, s);
+  }
   return UB_OK;
 }
 
