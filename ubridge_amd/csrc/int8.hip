@@ -174,7 +174,7 @@ struct Epilogue {
   typedef typename Elem<DT>::T T;
   static constexpr int kPitch = 32 * TN * sizeof(T) + 16, kStage = 32 * kPitch;
   static __device__ __forceinline__ void run(const i32x16 (&acc)[TM][TN], uint8_t* st, const float* sa, const float* sw,
-                                             const float* bias, void* y, int M, int N, int m0, int n0) {
+                                             const float* bias, void* y, int M, int N, int pitch, int m0, int n0) {
     constexpr int E = Elem<DT>::E, LR = 32 * TN / E, RI = 64 / LR;  // lanes a row, rows an instruction
     const int lane = threadIdx.x & 63, c = lane & 31, kh = lane >> 5;
     float s[TN][16], b[TN][16];
@@ -204,7 +204,7 @@ struct Epilogue {
         const uint4 v = *(const uint4*)(st + row * kPitch + col * sizeof(T));
         const int m = m0 + 32 * i + row, n = n0 + col;
         if (m < M && row < 32) {
-          T* p = (T*)y + (size_t)m * N + n;
+          T* p = (T*)y + (size_t)m * pitch + n;
           if (n + E <= N) {
             __builtin_memcpy(p, &v, 16);
           } else {
@@ -219,6 +219,13 @@ struct Epilogue {
     }
   }
 };
+
+// Workgroup i runs on XCD i % 8: its place in an order of `total` of which every
+// XCD, each with its own L2, takes one contiguous run.
+__device__ __forceinline__ int xcd_run(int i, int total) {
+  const int x = i % 8;
+  return x * (total / 8) + min(x, total % 8) + i / 8;
+}
 
 // WM x WN wavefronts of 32 TM x 32 TN outputs each, v_mfma_i32_32x32x32_i8.  The
 // operands reach LDS by direct loads in a ring of NS 64-byte K-steps, each row of
@@ -324,10 +331,10 @@ __device__ __forceinline__ void i8_tile(const int8_t* A, const float* sa, const 
   __builtin_amdgcn_s_waitcnt(0xC07F);
   ub_wait_vmcnt<0>();
   ub_barrier();
-  Out::run(acc, lds + wave * Out::kStage, sa, sw, bias, y, M, N, m0 + wm * 32 * TM, n0 + wn * 32 * TN);
+  Out::run(acc, lds + wave * Out::kStage, sa, sw, bias, y, M, N, N, m0 + wm * 32 * TM, n0 + wn * 32 * TN);
 }
 
-// The tiles in ub_tile_order; from tile `full` on (a multiple of the CUs) a tile is
+// The tiles in ub_tile_at's order, dealt to the XCDs in runs; from tile `full` on (a multiple of the CUs) a tile is
 // two workgroups, its upper and its lower half: the last round, where at most
 // half the CUs had a tile, then takes about half as long.  full = all tiles
 // otherwise, as for tiles of one product's height (TM = 1).
@@ -342,7 +349,7 @@ k_i8_gemm(const int8_t* __restrict__ A, const float* __restrict__ sa, const int8
   const int b = (int)blockIdx.x;
   int tile_m, tile_n;
   if (TM == 1 || b < full) {
-    ub_tile_at(b, full, tm, tn, 8, tile_m, tile_n);
+    ub_tile_at(xcd_run(b, full), 0, tm, tn, 8, tile_m, tile_n);
     i8_tile<DT, WM, WN, TM, TN, NS>(A, sa, B, sw, bias, y, M, N, ld, tile_m * BM, tile_n * BN, lds);
   } else if constexpr (TM > 1) {
     ub_tile_at(full + ((b - full) >> 1), 0, tm, tn, 8, tile_m, tile_n);
@@ -354,7 +361,7 @@ k_i8_gemm(const int8_t* __restrict__ A, const float* __restrict__ sa, const int8
 // The same product for grids that leave a workgroup or less to a CU, where the
 // latency of a K-step's loads is what costs: a ring of NS 128-byte steps in LDS,
 // NS - 1 of them in flight, one barrier a step.  Rows of 128 bytes, unit u of row
-// r at u ^ (r & 7).  Long rows over few tiles are cut in parts of K, whose int32
+// r at u ^ ((r >> 1) & 7).  Long rows over few tiles are cut in parts of K, whose int32
 // sums (DT = kSum, exact in any order) k_i8_sum adds.
 template <int DT, int WM, int WN, int TM, int TN, int NS>
 __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2, 2)))
@@ -370,16 +377,22 @@ k_i8_ring(const int8_t* __restrict__ A, const float* __restrict__ sa, const int8
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   int tile_m, tile_n;
-  ub_tile_order((M + BM - 1) / BM, (N + BN - 1) / BN, 8, tile_m, tile_n);
-  const int n0 = tile_n * BN, m0 = tile_m * BM;
-  const ub_u32x4 ra = ub_desc(A + (size_t)m0 * ld, (uint64_t)min(BM, M - m0) * ld);
-  const ub_u32x4 rb = ub_desc(B + (size_t)n0 * ld, (uint64_t)min(BN, N - n0) * ld);
+  const int tm = (M + BM - 1) / BM, tn = (N + BN - 1) / BN;
+  const int id = xcd_run((int)blockIdx.x, (int)gridDim.x), kp = id / (tm * tn);  // part kp of K
+  ub_tile_at(id - kp * tm * tn, 0, tm, tn, 8, tile_m, tile_n);
+  // rows and columns even over the tiles: what a tile does not need, it does not
+  // load (rows past the end lie past the buffers: zeros)
+  const int rows = (M + tm - 1) / tm, cols = min(BN, ((N + tn - 1) / tn + 15) & ~15);
+  const int n0 = tile_n * cols, m0 = tile_m * rows, n1 = min(N, n0 + cols), m1 = min(M, m0 + rows);
+  if (m0 >= m1 || n0 >= n1) return;  // (the same in every thread)
+  const ub_u32x4 ra = ub_desc(A + (size_t)m0 * ld, (uint64_t)(m1 - m0) * ld);
+  const ub_u32x4 rb = ub_desc(B + (size_t)n0 * ld, (uint64_t)(n1 - n0) * ld);
   const uint32_t base = ub_lds_addr(lds);
   uint32_t v[NL];
 #pragma unroll
   for (int i = 0; i < NL; i++) {
     const int row = (i * NW + wave) * 8 + (lane >> 3);  // of A, then of B
-    v[i] = (uint32_t)(row < BM ? row : row - BM) * (uint32_t)ld + 16 * ((lane & 7) ^ (row & 7));
+    v[i] = (uint32_t)(row < BM ? row : row - BM) * (uint32_t)ld + 16 * ((lane & 7) ^ ((row >> 1) & 7));
   }
   auto issue = [&](int k, int slot) {
 #pragma unroll
@@ -394,9 +407,8 @@ k_i8_ring(const int8_t* __restrict__ A, const float* __restrict__ sa, const int8
 #pragma unroll
       for (int r = 0; r < 16; r++) acc[i][j][r] = 0;
   const int l32 = lane & 31, kh = lane >> 5;
-  // steps k0 .. k0 + nk - 1, of which part blockIdx.y has `part`
-  const int k0 = blockIdx.y * part, nk = min(part, ld / 128 - k0);
-  if constexpr (DT == kSum) y = (int*)y + (size_t)blockIdx.y * M * N;
+  const int k0 = kp * part, nk = min(part, ld / 128 - k0);
+  if constexpr (DT == kSum) y = (int*)y + (size_t)kp * M * N;
 #pragma unroll
   for (int k = 0; k < NS - 1; k++) issue(k0 + min(k, nk - 1), k);  // (past K: loaded again, not used)
   int slot = 0;
@@ -411,12 +423,12 @@ k_i8_ring(const int8_t* __restrict__ A, const float* __restrict__ sa, const int8
 #pragma unroll
       for (int i = 0; i < TM; i++) {
         const int row = wm * 32 * TM + 32 * i + l32;
-        af[i][q] = *(const i32x4*)(st + row * 128 + 16 * ((2 * q + kh) ^ (row & 7)));
+        af[i][q] = *(const i32x4*)(st + row * 128 + 16 * ((2 * q + kh) ^ ((row >> 1) & 7)));
       }
 #pragma unroll
       for (int j = 0; j < TN; j++) {
         const int row = BM + wn * 32 * TN + 32 * j + l32;
-        bf[j][q] = *(const i32x4*)(st + row * 128 + 16 * ((2 * q + kh) ^ (row & 7)));
+        bf[j][q] = *(const i32x4*)(st + row * 128 + 16 * ((2 * q + kh) ^ ((row >> 1) & 7)));
       }
     }
 #pragma unroll
@@ -433,7 +445,7 @@ k_i8_ring(const int8_t* __restrict__ A, const float* __restrict__ sa, const int8
   ub_barrier();
   typedef Epilogue<DT, TM, TN> Out;
   static_assert(NW * Out::kStage <= NS * ST, "epilogue fits");
-  Out::run(acc, lds + wave * Out::kStage, sa, sw, bias, y, M, N, m0 + wm * 32 * TM, n0 + wn * 32 * TN);
+  Out::run(acc, lds + wave * Out::kStage, sa, sw, bias, y, m1, n1, N, m0 + wm * 32 * TM, n0 + wn * 32 * TN);
 }
 
 template <int DT>
@@ -645,16 +657,16 @@ bool quant(const void* x, int8_t* q, float* sa, int M, int K, int ld, hipStream_
 // The tile and the number of K parts that take least, by the tile's measured
 // time for 128 bytes of K (0.01 us) on a CU that has one workgroup of it, and for
 // each of several (larger grids leave that many to a CU, side by side or in
-// turn): 256 x 256 205 / 205, 128 x 128 68 / 62, 64 x 128 57 / 50, 64 x 64 34 /
-// 29, 64 x 32 30 / 22; parts cost a launch and their sums' way to memory and back.
-// us in a graph, with the quantizing launch, M x K x N: 64 x 4096 x 6144 on these
-// 32 / 24 / 20 / 15 / 13.7, 201 x 3520 x 9001 40 / 24 / 38 / 32 / 33, 512 x 4096 x
-// 4096 36 / 27 / 23 / 23 / 32, 1024 x 2048 x 2048 25 / 20 / 17 / 16 / 22, 1024 x
-// 4096 x 14336 74 / 97 / 97 / - / -
+// turn); parts cost a launch and their sums' way to memory and back.  us in a
+// graph, with the quantizing launch, M x K x N on 256 x 256 / 128 x 128 / 64 x 128
+// / 64 x 64 / 64 x 32: 64 x 4096 x 6144 32 / 23 / 19 / 15 / 13.7, 201 x 3520 x 9001
+// 40 / 23 / 33 / 27 / 34, 512 x 4096 x 4096 36 / 26 / 22.3 / 22.3 / 30, 1024 x 2048 x
+// 2048 25 / 18 / 16 / 15.5 / 21, 1024 x 4096 x 14336 74 / 97 / 97 / - / -; in parts,
+// 40 x 13970 x 450 31 -> 13, 490 x 9272 x 361 32 -> 19.
 struct Plan { int tile, parts; };
 Plan plan_for(int M, int N, int nk) {
   static const struct { int m, n, one, each; bool parts; } t[5] = {
-      {256, 256, 205, 205, false}, {128, 128, 68, 62, true}, {64, 128, 57, 50, false}, {64, 64, 34, 29, true},
+      {256, 256, 205, 205, false}, {128, 128, 64, 60, true}, {64, 128, 57, 50, false}, {64, 64, 32, 27, true},
       {64, 32, 30, 22, false}};
   Plan best = {0, 1};
   double least = 0;
@@ -694,7 +706,7 @@ void gemm(Plan plan, const int8_t* q, const float* sa, const int8_t* w, const fl
     static const hipError_t once = hipFuncSetAttribute((const void*)k_i8_ring<DT, WM, WN, TM, TN, NS>,   \
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, lds); \
     (void)once;                                                                                          \
-    k_i8_ring<DT, WM, WN, TM, TN, NS><<<dim3(ub_cdiv(M, 32 * WM * TM) * ub_cdiv(N, 32 * WN * TN), ub_cdiv(ld / 128, part)), \
+    k_i8_ring<DT, WM, WN, TM, TN, NS><<<ub_cdiv(M, 32 * WM * TM) * ub_cdiv(N, 32 * WN * TN) * ub_cdiv(ld / 128, part), \
                                         64 * WM * WN, lds, s>>>(q, sa, w, sw, bias, y, M, N, ld, part);  \
     return;                                                                                              \
   }

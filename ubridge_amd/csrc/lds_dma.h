@@ -122,8 +122,8 @@ __device__ __forceinline__ void ub_barrier() {
 // itself walks groups of `gm` tile rows column by column, so the tiles
 // resident at one time share a few A row-panels and B column-panels
 // instead of sweeping whole rows of B.
-// ub_tile_at: tile number `pid` of the order, of which the first `dealt` are
-// regrouped (0: pid as it is).
+// ub_tile_at: tile number `pid` of that order, after the regrouping of `dealt`
+// tiles (0: none, the caller's own).
 __device__ __forceinline__ void ub_tile_at(int pid, int dealt, int tm, int tn, int gm, int& im, int& in_) {
   constexpr int kXcd = 8;
   if (dealt && dealt % kXcd == 0) pid = (pid % kXcd) * (dealt / kXcd) + pid / kXcd;
