@@ -41,6 +41,12 @@ template <> struct Elem<UB_F32> { typedef float T; static constexpr int E = 4; }
 template <> struct Elem<UB_F16> { typedef uint16_t T; static constexpr int E = 8; };
 template <> struct Elem<UB_BF16> { typedef uint16_t T; static constexpr int E = 8; };
 
+// Unit u of a run of `len` elements: its first element.  The last unit of a run
+// that is not whole units ends with the run and overlaps the one before (the
+// same values twice), unless the run is shorter than a unit.
+template <int E>
+__device__ __forceinline__ int place(int u, int len) { return max(0, min(u * E, len - E)); }
+
 // n elements from p, at most a unit (element-aligned: gfx950 loads 16 bytes
 // from there)
 template <int DT>
@@ -50,15 +56,19 @@ __device__ __forceinline__ uint4 ld(const typename Elem<DT>::T* p, int n) {
   if (n >= E) {
     __builtin_memcpy(&v, p, 16);
   } else {
+    typename Elem<DT>::T x[E];  // (all in flight at once)
+#pragma unroll
+    for (int e = 0; e < E; e++) x[e] = p[min(e, n - 1)];
     uint64_t lo = 0, hi = 0;
     constexpr int B = 8 * sizeof(typename Elem<DT>::T);
-#pragma nounroll
-    for (int e = 0; e < n; e++) {
-      uint64_t x;
-      if constexpr (DT == UB_F32) x = __float_as_uint(p[e]);
-      else x = p[e];
-      if (e < E / 2) lo |= x << (B * e);
-      else hi |= x << (B * (e - E / 2));
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      uint64_t b;
+      if constexpr (DT == UB_F32) b = __float_as_uint(x[e]);
+      else b = x[e];
+      if (e >= n) b = 0;
+      if (e < E / 2) lo |= b << (B * e);
+      else hi |= b << (B * (e - E / 2));
     }
     v = make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
   }
@@ -179,16 +189,32 @@ __global__ void __launch_bounds__(64 * NW) k_rope(const RopeDev d) {
   const long pos = a.rot == 0 ? 0 : a.pos64 ? ((const long*)a.positions)[t] : (long)((const int*)a.positions)[t];
   long slot = APPEND ? a.slots[t] : 0;
 
-  // unit u of head h: E pairs (x0, x1), or E elements (x0) that pass through or
+  // unit u of head h: E pairs (a, b), or E elements (a) that pass through or
   // (interleaved) hold E / 2 pairs
+  struct Where { int e, n; bool pairs; };
+  auto where = [&](int h, int u) {
+    Where w;
+    w.pairs = !INTER && h < hr && u < PU;
+    if (w.pairs) {
+      w.e = place<E>(u, half);
+      w.n = half - w.e;
+    } else if (INTER && (a.D & 1) && h < hr) {  // (whole pairs a unit)
+      w.e = u * E;
+      w.n = a.D - w.e;
+    } else {
+      const int from = INTER || h >= hr ? 0 : a.rot;
+      w.e = from + place<E>(from ? u - PU : u, a.D - from);
+      w.n = a.D - w.e;
+    }
+    return w;
+  };
   auto load = [&](int h, int u) {
     const T* p = h < a.Hq ? qt + h * a.q_sh : h < hr ? kt + (h - a.Hq) * a.k_sh : vt + (h - hr) * a.v_sh;
-    const bool pairs = !INTER && h < hr && u < PU;
-    const int e = pairs || INTER || h >= hr ? u * E : a.rot + (u - PU) * E;
+    const Where w = where(h, u);
     Two r;
-    r.a = ld<DT>(p + e, (pairs ? half : a.D) - e);
+    r.a = ld<DT>(p + w.e, w.n);
     r.b = make_uint4(0, 0, 0, 0);
-    if (!INTER && pairs) r.b = ld<DT>(p + half + e, half - e);
+    if (!INTER && w.pairs) r.b = ld<DT>(p + half + w.e, w.n);
     return r;
   };
   long page = 0;
@@ -238,40 +264,39 @@ __global__ void __launch_bounds__(64 * NW) k_rope(const RopeDev d) {
   }
   const int nu = APPEND && nu_v > nu_r ? nu_v : nu_r;
   while (u < nu) {
-    float2 w[NP];  // of this unit's pairs
+    const Where at_q = where(0, u);  // (the same in every head that turns)
+    float2 w[NP];                    // of this unit's pairs
 #pragma unroll
-    for (int j = 0; j < NP; j++) w[j] = u * NP + j < half ? cs[u * NP + j] : make_float2(1.f, 0.f);
+    for (int j = 0; j < NP; j++) {
+      const int i = (INTER ? at_q.e / 2 : at_q.e) + j;
+      w[j] = i < half ? cs[i] : make_float2(1.f, 0.f);
+    }
     while (h < end) {
       const uint4 c0 = x.a, c1 = x.b;
       const int hi = h;
       h += step;
       if (h < end) x = load(h, u);
       float y[E];
-      int e = u * E, n = a.D - e;
+      const Where v = hi < hr ? at_q : where(hi, u);
       if (INTER && hi < hr) {
 #pragma unroll
         for (int j = 0; j < E; j += 2) {  // (pairs past rot turn by nothing)
           const float x = get<DT>(c0, j), z = get<DT>(c0, j + 1);
-          const bool in = e + j < a.rot;
+          const bool in = v.e + j < a.rot;
           y[j] = in ? x * w[j / 2].x - z * w[j / 2].y : x;
           y[j + 1] = in ? z * w[j / 2].x + x * w[j / 2].y : z;
         }
-      } else if (!INTER && hi < hr && u < PU) {
-        n = half - e;
+      } else if (!INTER && v.pairs) {
 #pragma unroll
         for (int j = 0; j < E; j++) y[j] = get<DT>(c1, j) * w[j % NP].x + get<DT>(c0, j) * w[j % NP].y;
-        put(hi, half + e, y, n);
+        put(hi, half + v.e, y, v.n);
 #pragma unroll
         for (int j = 0; j < E; j++) y[j] = get<DT>(c0, j) * w[j % NP].x - get<DT>(c1, j) * w[j % NP].y;
       } else {
-        if (!INTER && hi < hr) {
-          e = a.rot + (u - PU) * E;
-          n = a.D - e;
-        }
 #pragma unroll
         for (int j = 0; j < E; j++) y[j] = get<DT>(c0, j);
       }
-      put(hi, e, y, n);
+      put(hi, v.e, y, v.n);
     }
     u += lanes;
     range(u);
