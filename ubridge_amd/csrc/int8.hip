@@ -759,7 +759,7 @@ UB_API int ubridge_int8_linear(const void* x, int dtype, const int8_t* w, const 
   if ((size_t)M * N == 0) return UB_OK;
   UB_REQUIRE(x && w && sw && y, "%s: null pointer", nm);
   UB_REQUIRE(((uintptr_t)w & 15) == 0, "%s: weight not 16-byte aligned", nm);
-  UB_REQUIRE(M < 1 << 22, "%s: M=%d", nm, M);  // (a launch has fewer than 2^32 threads)
+  UB_REQUIRE(M < 1 << 22 && (int64_t)M * N < 1ll << 38, "%s: M=%d N=%d", nm, M, N);  // (2^32 threads a launch)
   hipStream_t s = ub_stream(stream);
   const int e = dtype == UB_F32   ? linear<UB_F32>(nm, x, w, sw, bias, y, M, K, N, ld, s)
                 : dtype == UB_F16 ? linear<UB_F16>(nm, x, w, sw, bias, y, M, K, N, ld, s)
