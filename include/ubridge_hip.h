@@ -10,7 +10,8 @@
  *     (at most 256 MB) of ubridge_qmatmul at prefill sizes and of the
  *     quantized matmul_* / ubridge_w4a16_gemm beyond 1024 tokens (uint8
  *     4-bit: from 640), and the f32 partials (at most 8 x M x N x 4 bytes)
- *     of the pipelined GEMMs when they split K over workgroups.  That
+ *     of the pipelined GEMMs when they split K over workgroups, and what the
+ *     attention block's entries (below) say of theirs.  That
  *     scratch comes from the allocator the caller registers with
  *     ubridge_set_workspace_allocator (taken and handed back on the call's
  *     stream, as the reference's topsaten workspaces are), else from a

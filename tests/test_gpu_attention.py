@@ -138,6 +138,25 @@ def test_masks_and_biases(dev, cap, window, slopes, scaled, D, S, cache):
     check(out, q, kv, tables, n, lse, scale=0.3, softcap=cap, window=window, slopes=sl, k_scale=ks, v_scale=vs)
 
 
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+def test_lse_of_few_tokens(dev, t):
+    # one token: lse is its score, exact where the products are; equal tokens: the
+    # logarithm of their number beside it, to an ulp or two of the sum
+    q, kv, tables, n = make(dev, [1, 4, 64, 1000], 4, 2, 64, 16, t)
+    q = torch.randint(-4, 5, q.shape, generator=torch.Generator().manual_seed(1)).to(q.dtype).to(dev)
+    kv[0] = 0.5
+    x = q.float().sum(-1) * 0.5 * 0.125
+    lse = attention.paged_decode(q, kv[0], kv[1], tables, n, scale=0.125, return_lse=True)[1]
+    assert torch.equal(lse[0], x[0])
+    want = x.double() + torch.log(n.double())[:, None]
+    assert bool(((lse.double() - want).abs() <= 2.0**-23 * (want.abs() + 8)).all())
+    # capped: c tanh(x / c), to some ulp of the value
+    x = x * 3
+    lse = attention.paged_decode(q, kv[0], kv[1], tables, n, scale=0.375, softcap=5.0, return_lse=True)[1]
+    want = 5 * torch.tanh(x[0].double() / 5)
+    assert bool(((lse[0].double() - want).abs() <= 2.0**-21 * want.abs()).all())
+
+
 def test_large_scores(dev):
     # scores far beyond exp's range, growing and falling along the sequence
     lens = [300, 2000]

@@ -100,3 +100,37 @@ def test_decode_with_samples(dev):
         p.k[0], p.v[0] = p.k[2], p.v[2]
     both([0, 1, 2, 5], 5)
     moe.device_error()
+
+
+def test_caller_allocator(dev):
+    # scratch from the caller's allocator: handed back after each call, the same bits
+    from ubridge_amd import attention, int8, ops
+    g = torch.Generator().manual_seed(1)
+    kv = torch.randn(1, 2, 300, 2, 8, 32, generator=g).bfloat16().to(dev)
+    tables = torch.randperm(300, generator=g).int().view(2, 150).to(dev)
+    lens = torch.tensor([1200, 777], dtype=torch.int32, device=dev)
+    q = torch.randn(2, 8, 32, generator=g).bfloat16().to(dev)
+    w = torch.randint(-127, 128, (96, 5000), generator=g, dtype=torch.int8)
+    lin = int8.Linear(w.to(dev), torch.ones(96, device=dev))
+    x = torch.randn(33, 5000, generator=g).to(dev)
+
+    def run():
+        c = kvcache.PagedCache(kv.clone(), rows=3, width=4)
+        c.meta[:5] = 1
+        c.lens[0], c.tables[0, :2] = 11, torch.tensor([0, 3], dtype=torch.int32)
+        rows = torch.tensor([0, 1], dtype=torch.int32, device=dev)
+        new = c.fork(rows[:1], rows[1:])
+        n = c.compact()
+        return [attention.paged_decode(q, kv[0, 0], kv[0, 1], tables, lens), lin(x), new, n, c.meta,
+                c.kv.view(torch.int16)]
+
+    want = run()
+    alloc = ops.TorchWorkspaceAllocator()
+    ops.set_workspace_allocator(alloc)
+    try:
+        got = run()
+        torch.cuda.synchronize()
+    finally:
+        ops.set_workspace_allocator(None)
+    assert alloc.calls >= 4 and not alloc.live and ops.workspace_stats()[2] == 0
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -22,9 +22,19 @@
 //    lane.  A lane reads its eight values rows of V 16 bytes each (8 dims) and
 //    swaps tokens against dims with one byte permute a dword.
 //  * The steps of all (sequence, kv head) rows, whose number only the device
-//    knows, are laid end to end and cut into equal shares, one a workgroup.  A row
-//    inside one share is finished there; a row that is cut leaves f32 partial
-//    sums, which k_join adds in the order of the shares.
+//    knows, are laid end to end and cut into equal shares, one a wavefront (a
+//    row counts two steps more than it has, for the latency of its first loads,
+//    so that short rows are not heaped on one share).  A row inside one share
+//    is finished there; a row that is cut leaves f32 partial sums, which k_join
+//    adds in the order of the shares.  Where a workgroup a row is enough, there
+//    are no shares and one launch (ROW).
+//
+// us of the kernels: 4 sequences of 100003 tokens, 8 kv heads of 128 in bf16 (1.64
+// GB) 280 + 11 (5.8 TB/s); 64 sequences of up to 4096 (118 MB) 27 + 5.6; 24 of up
+// to 6000 under a window of 2048, 16 e4m3 heads of 80 (43 MB) 13.8 + 5.2, where
+// half the time is latency and the softmax of one head in sixteen columns; one of
+// 700 tokens 7.0 + 4.6, all latency: the search for the share, the page, the row,
+// then the join's own three reads.
 //
 // Numerics.  Scores, the running maximum and sum, and the output's sum are f32.
 // The weights exp(x - m) enter the second product as the sum of two 16-bit
@@ -42,7 +52,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float kInf = __builtin_inff();
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f;
 constexpr int W = 4;         // wavefronts of a workgroup
 constexpr int kRowCost = 2;  // steps that the first loads of a row are worth
 constexpr int kShares = 2048;  // two wavefronts a SIMD (three, 3072: 64 ragged sequences 30 -> 47 us, by spills)
@@ -109,7 +119,7 @@ struct Dev {
   uint64_t s_mul;  // t / S = t s_mul >> s_shift for 0 <= t < 2^31
   int s_shift;
   float* po;       // [2 shares][heads of a group][D] partial sums, relative to the maximum
-  float* pml;      // [2 shares][heads of a group][2] maximum (log2) and sum
+  float* pml;      // [2 shares][heads of a group][2] maximum and sum
   int2* cut;       // [shares] the row that starts in a share and ends past it (-1: none), and its shares
   int* err;
 };
@@ -132,10 +142,23 @@ __device__ __forceinline__ Span span(const Dev& d, int b) {
 // what a row costs, in steps: its own and the latency of its first loads
 __device__ __forceinline__ int cost(const Span& s) { return s.steps ? s.steps + kRowCost : 0; }
 
-// m (log2) and l of a row -> log of the sum
+// e^x 2^off: of differences to a maximum, which f32 holds exactly where they are
+// small (scores kept in powers of two would carry the error of their own factor)
+__device__ __forceinline__ float exp_of(float x, float off = 0.f) {
+  return __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2e, off));
+}
+// tanh z = (1 - t) / (1 + t), t = e^(-2 |z|); below a quarter, where 1 - t would
+// keep t's rounding, the series, whose next term is below 1e-8 of it
+__device__ __forceinline__ float tanh_of(float z) {
+  const float t = exp_of(-2.f * fabsf(z)), u = z * z;
+  const float far = copysignf((1.f - t) * __builtin_amdgcn_rcpf(1.f + t), z);
+  const float near = z * (1.f + u * (-1.f / 3 + u * (2.f / 15 + u * (-17.f / 315 + u * (62.f / 2835)))));
+  return fabsf(z) < 0.25f ? near : far;
+}
+// maximum and sum of a row -> log of the sum
 template <int DT>
 __device__ __forceinline__ float lse_of(float m, float l) {
-  return m == -kInf ? m + l : (m - (DT == UB_F16 ? 14.f : 0.f) + __log2f(l)) * kLn2;
+  return m == -kInf ? m + l : m + logf(DT == UB_F16 ? l * 0x1p-14f : l);
 }
 
 // inclusive sum over the lanes, by DPP: no LDS round trip a step
@@ -280,10 +303,10 @@ k_decode(const Dev d) {
         qf[t][j] = make_uint4(0, 0, 0, 0);
         if (live && kin[j]) __builtin_memcpy(&qf[t][j], p + 32 * j + 8 * g, 16);
       }
-      slope[t] = live && a.slopes ? a.slopes[hq] * kLog2e : 0.f;
+      slope[t] = live && a.slopes ? a.slopes[hq] : 0.f;
     }
     const float ks = a.scale * (a.k_scale ? a.k_scale[h] : 1.f);
-    const float kx = cap > 0.f ? 2.f * kLog2e * ks / cap : ks * kLog2e;  // on q . k
+    const float kx = cap > 0.f ? ks / cap : ks;  // on q . k
 
     f32x4 o[HT][NB][8];
     float m[HT], l[HT];
@@ -382,8 +405,7 @@ k_decode(const Dev d) {
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           float v = acc[t][e >> 2][e & 3] * kx;
-          if (cap > 0.f)  // tanh z = 1 - 2 / (exp(2 z) + 1)
-            v = cap * kLog2e * (1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(v) + 1.f));
+          if (cap > 0.f) v = cap * tanh_of(v);
           v += slope[t] * (float)(t0 + e - (sq.n - 1));
           if (bad >> e & 1) v = __builtin_nanf("");
           if (edge && (t0 + e < sq.first || t0 + e >= sq.n)) v = -kInf;
@@ -393,12 +415,12 @@ k_decode(const Dev d) {
         mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
         const float mn = fmaxf(m[t], mx), ms = mn == -kInf ? 0.f : mn;  // (a NaN score: its weight is NaN)
-        const float al = __builtin_amdgcn_exp2f(m[t] - ms);
+        const float al = exp_of(m[t] - ms);
         m[t] = mn;
         float p[8], sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          p[e] = __builtin_amdgcn_exp2f(x[e] - ms + kOff);
+          p[e] = exp_of(x[e] - ms, kOff);
           sum += p[e];
         }
         l[t] = l[t] * al + sum;
@@ -496,7 +518,7 @@ k_decode(const Dev d) {
         for (int w = 0; w < NW; w++) {
           const float2 ml = sml[w][q];
           const float4 x = *(const float4*)(so + (w * nq + q) * pitch + 4 * v);
-          const float f = __builtin_amdgcn_exp2f(ml.x - Ms);
+          const float f = exp_of(ml.x - Ms);
           O.x += f * x.x, O.y += f * x.y, O.z += f * x.z, O.w += f * x.w;
           L += f * ml.y;
         }
@@ -588,13 +610,13 @@ __global__ void __launch_bounds__(512) k_join(const Dev d, int heads) {
         float mn = M;
 #pragma unroll
         for (int i = 0; i < 4; i++) mn = fmaxf(mn, ml[i].x);
-        const float ms = mn == -kInf ? 0.f : mn, al = __builtin_amdgcn_exp2f(M - ms);
+        const float ms = mn == -kInf ? 0.f : mn, al = exp_of(M - ms);
         M = mn;
         O.x *= al, O.y *= al, O.z *= al, O.w *= al, L *= al;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           if (p0 + i * U >= cut.y) continue;
-          const float w = __builtin_amdgcn_exp2f(ml[i].x - ms);
+          const float w = exp_of(ml[i].x - ms);
           O.x += w * x[i].x, O.y += w * x[i].y, O.z += w * x[i].z, O.w += w * x[i].w;
           L += w * ml[i].y;
         }
@@ -606,13 +628,13 @@ __global__ void __launch_bounds__(512) k_join(const Dev d, int heads) {
       if (u == 0) {
         float mn = M;
         for (int i = 1; i < U; i++) mn = fmaxf(mn, sml[threadIdx.x + i * cols].x);
-        const float ms = mn == -kInf ? 0.f : mn, al = __builtin_amdgcn_exp2f(M - ms);
+        const float ms = mn == -kInf ? 0.f : mn, al = exp_of(M - ms);
         M = mn;
         O.x *= al, O.y *= al, O.z *= al, O.w *= al, L *= al;
         for (int i = 1; i < U; i++) {
           const float2 ml = sml[threadIdx.x + i * cols];
           const float4 x = so[threadIdx.x + i * cols];
-          const float w = __builtin_amdgcn_exp2f(ml.x - ms);
+          const float w = exp_of(ml.x - ms);
           O.x += w * x.x, O.y += w * x.y, O.z += w * x.z, O.w += w * x.w;
           L += w * ml.y;
         }
