@@ -23,6 +23,9 @@ struct {
   decltype(&ubridge_rope) rope;
   decltype(&ubridge_rope_append) append;
   decltype(&ubridge_int8_linear) linear;
+  decltype(&ubridge_kv_free) free;
+  decltype(&ubridge_kv_fork) fork;
+  decltype(&ubridge_kv_compact) compact;
 } fn;
 
 #define REFUSE(...)                             \
@@ -88,12 +91,15 @@ struct Args {
   }
 
 PyObject* py_bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  COUNT(4)
+  COUNT(7)
   const Args A{args};
   fn.decode = (decltype(fn.decode))A.p(0);
   fn.rope = (decltype(fn.rope))A.p(1);
   fn.append = (decltype(fn.append))A.p(2);
   fn.linear = (decltype(fn.linear))A.p(3);
+  fn.free = (decltype(fn.free))A.p(4);
+  fn.fork = (decltype(fn.fork))A.p(5);
+  fn.compact = (decltype(fn.compact))A.p(6);
   if (PyErr_Occurred()) return nullptr;
   Py_RETURN_NONE;
 }
@@ -308,12 +314,81 @@ PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// The pool as kvcache.py packed it (UbridgeKvPool), or null: refused.
+const UbridgeKvPool* pool(PyObject* o) {
+  if (!PyBytes_Check(o) || PyBytes_GET_SIZE(o) != (Py_ssize_t)sizeof(UbridgeKvPool)) {
+    PyErr_SetString(PyExc_TypeError, "a packed pool expected");
+    return nullptr;
+  }
+  return (const UbridgeKvPool*)PyBytes_AS_STRING(o);
+}
+bool row_list(const char* name, const at::Tensor& t) {
+  if (t.dim() == 1 && t.scalar_type() == at::kInt && dense(t) && fits(t.size(0))) return true;
+  PyErr_Format(PyExc_ValueError, "PagedCache: %s must be contiguous int32 [n]", name);
+  return false;
+}
+
+// rows, pool, stream
+PyObject* py_free(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  COUNT(3)
+  HANDLE_TH_ERRORS
+  const Args A{args};
+  Ten rows;
+  const UbridgeKvPool* p = pool(args[1]);
+  if (!p || !device_tensor(args[0], rows) || !row_list("rows", *rows)) return nullptr;
+  void* stream = A.p(2);
+  if (PyErr_Occurred()) return nullptr;
+  if (const int rc = fn.free(p, ptr<int32_t>(rows), (int)rows->size(0), stream)) return PyLong_FromLong(rc);
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// src, dst, pool, stream
+PyObject* py_fork(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  COUNT(4)
+  HANDLE_TH_ERRORS
+  const Args A{args};
+  Ten src, dst;
+  const UbridgeKvPool* p = pool(args[2]);
+  if (!p || !device_tensor(args[0], src) || !device_tensor(args[1], dst) || !row_list("src", *src) || !row_list("dst", *dst))
+    return nullptr;
+  const int64_t n = src->size(0);
+  if (dst->size(0) != n || n > 65535)
+    REFUSE("PagedCache.fork: %ld prompts, %ld samples (as many, at most 65535)", n, dst->size(0));
+  at::Tensor pages = result({n}, *src);
+  void* stream = A.p(3);
+  if (PyErr_Occurred()) return nullptr;
+  if (const int rc = fn.fork(p, ptr<int32_t>(src), ptr<int32_t>(dst), (int)n, (int32_t*)pages.data_ptr(), stream))
+    return PyLong_FromLong(rc);
+  return THPVariable_Wrap(std::move(pages));
+  END_HANDLE_TH_ERRORS
+}
+
+// meta, pool, stream
+PyObject* py_compact(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  COUNT(3)
+  HANDLE_TH_ERRORS
+  const Args A{args};
+  Ten meta;
+  const UbridgeKvPool* p = pool(args[1]);
+  if (!p || !device_tensor(args[0], meta)) return nullptr;
+  at::Tensor n = result({}, *meta);
+  void* stream = A.p(2);
+  if (PyErr_Occurred()) return nullptr;
+  if (const int rc = fn.compact(p, (int32_t*)n.data_ptr(), stream)) return PyLong_FromLong(rc);
+  return THPVariable_Wrap(std::move(n));
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"bind", (PyCFunction)(void (*)())py_bind, METH_FASTCALL, "the C entry points, as addresses"},
     {"paged_decode", (PyCFunction)(void (*)())py_decode, METH_FASTCALL, nullptr},
     {"rope", (PyCFunction)(void (*)())py_rope, METH_FASTCALL, nullptr},
     {"append", (PyCFunction)(void (*)())py_append, METH_FASTCALL, nullptr},
     {"linear", (PyCFunction)(void (*)())py_linear, METH_FASTCALL, nullptr},
+    {"free", (PyCFunction)(void (*)())py_free, METH_FASTCALL, nullptr},
+    {"fork", (PyCFunction)(void (*)())py_fork, METH_FASTCALL, nullptr},
+    {"compact", (PyCFunction)(void (*)())py_compact, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods};
 

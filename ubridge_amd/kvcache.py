@@ -1,20 +1,13 @@
 """A paged key-value cache whose state stays on the device: storing new tokens
 (with their rotation), freeing, forking and compacting without a host copy of
 page tables, so that the calls can be enqueued, or captured, ahead."""
-import ctypes
 import struct
 
 import torch
 
-from ._lib import check, lib, register
 from .attention import paged_decode
 from .native import _native, call
-from .ops import _empty, _need_cuda, stream_ptr
-
-_vp, _i = ctypes.c_void_p, ctypes.c_int
-register("ubridge_kv_free", _i, [_vp, _vp, _i, _vp])
-register("ubridge_kv_fork", _i, [_vp, _vp, _vp, _i, _vp, _vp])
-register("ubridge_kv_compact", _i, [_vp, _vp, _vp])
+from .ops import _need_cuda
 
 
 _TYPES = (torch.float16, torch.bfloat16, torch.float8_e4m3fn)
@@ -81,18 +74,9 @@ class PagedCache:
                             self.lens if lens is None else lens, k_scale=self.k_scale,
                             v_scale=self.v_scale, **kw)
 
-    def _rows(self, name, t):
-        _need_cuda(t)
-        if t.dim() != 1 or t.dtype != torch.int32 or not t.is_contiguous():
-            raise ValueError(f"PagedCache: {name} must be contiguous int32 [n]")
-        return t.data_ptr(), t.shape[0]
-
     def free(self, rows, stream=None):
         """The rows named (int32 [n]) lose their pages and become empty."""
-        p, n = self._rows("rows", rows)
-        rc = lib.ubridge_kv_free(self._pool, p, n, stream_ptr(stream))
-        if rc:
-            check(rc)
+        call(_native.free, stream, rows, self._pool)
 
     def fork(self, src, dst, stream=None):
         """Empty rows dst (int32 [n], all different) become samples of rows src:
@@ -100,21 +84,9 @@ class PagedCache:
         free page.  Returns int32 [n], the new page or -1.  A row that is not
         empty or not there, or for which no page is left, keeps its state, gives
         -1 and raises the flag that moe.device_error() reads."""
-        sp, n = self._rows("src", src)
-        dp, m = self._rows("dst", dst)
-        if m != n or n > 65535:
-            raise ValueError(f"PagedCache.fork: {n} prompts, {m} samples (as many, at most 65535)")
-        new = _empty((n,), torch.int32, self.kv.device, stream)
-        rc = lib.ubridge_kv_fork(self._pool, sp, dp, n, new.data_ptr(), stream_ptr(stream))
-        if rc:
-            check(rc)
-        return new
+        return call(_native.fork, stream, src, dst, self._pool)
 
     def compact(self, stream=None):
         """Move the used pages to the low end of the pool; tables and refs follow.
         Returns their number, an int32 tensor."""
-        n = _empty((), torch.int32, self.kv.device, stream)
-        rc = lib.ubridge_kv_compact(self._pool, n.data_ptr(), stream_ptr(stream))
-        if rc:
-            check(rc)
-        return n
+        return call(_native.compact, stream, self.meta, self._pool)

@@ -16,7 +16,10 @@ except ImportError as e:
 _vp, _i = ctypes.c_void_p, ctypes.c_int
 _ENTRIES = (register("ubridge_paged_decode", _i, [_vp, _vp]), register("ubridge_rope", _i, [_vp, _vp]),
             register("ubridge_rope_append", _i, [_vp, _vp]),
-            register("ubridge_int8_linear", _i, [_vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]))
+            register("ubridge_int8_linear", _i, [_vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+            register("ubridge_kv_free", _i, [_vp, _vp, _i, _vp]),
+            register("ubridge_kv_fork", _i, [_vp, _vp, _vp, _i, _vp, _vp]),
+            register("ubridge_kv_compact", _i, [_vp, _vp, _vp]))
 _native.bind(*(ctypes.cast(f, _vp).value for f in _ENTRIES))
 
 _raw_stream = torch._C._cuda_getCurrentRawStream

@@ -51,15 +51,6 @@ def _need_cuda(*ts):
             raise ValueError("ubridge_amd ops take device tensors")
 
 
-def _empty(shape, dtype, device, stream=None):
-    """A result of a call on `stream`: its memory belongs to that stream, so it
-    is not handed out again while the call may still write it."""
-    if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
-
-
 def quant_bytes(qtype, numel):
     """Bytes of a SoA-packed tensor with numel elements."""
     return numel // BLOCK[qtype] * BLOCK_BYTES[qtype]
