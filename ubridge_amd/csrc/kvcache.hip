@@ -14,7 +14,7 @@
 //          free page below n; tables and counts follow
 //
 // free and the planning of fork and compact touch a few hundred KiB and are
-// bound by latency (us: free 3, fork's plan 5.5, compact's 4.9); the page copies
+// bound by latency (us: free 3, fork's plan 5.5, compact's 3.5); the page copies
 // are bound by HBM, with eight 16-byte loads in flight a thread: 507 pages of 512
 // KiB (530 MB in and out) 109 us, 4.9 TB/s (four in flight 119).  Non-temporal
 // access was 4% faster there and 40% slower on fork, whose pages stay in the
@@ -234,66 +234,98 @@ __global__ void __launch_bounds__(256) k_fork(uint8_t* kv, int* refs, int* table
 }
 
 // One workgroup: the moves.  plan: [1] their number, [P / 2] from, [P / 2] to;
-// map [P]: where a page of the old numbering lies now.
-__global__ void __launch_bounds__(PT) k_compact_plan(int* refs, int P, int* plan, int* map,
+// map [P]: where a page of the old numbering lies now, or -2 - k for move k.
+// Q: pages of a thread, in a tile of PT Q.
+template <int Q>
+__global__ void __launch_bounds__(PT) k_compact_plan(const int* refs, int P, int* plan, int* map,
                                                      int* n_out) {
   __shared__ int lds[PT / 64];
-  __shared__ int below;  // used pages below n
+  __shared__ int below_n;
   const int tid = threadIdx.x;
-  const int per = (P + PT - 1) / PT;
-  const int p0 = min(P, tid * per), p1 = min(P, p0 + per);
-  int c = 0;
-  for (int p = p0; p < p1; p++) c += refs[p] != 0;
-  int n;
-  const int u0 = block_scan(c, lds, n);
-  int u = u0;
-  for (int p = p0; p < p1; p++) {
-    if (p == n) below = u;
-    u += refs[p] != 0;
+  int f[Q];
+  auto counts = [&](int p) {
+    if (p + Q <= P) {
+      __builtin_memcpy(f, refs + p, sizeof(f));
+    } else {
+#pragma unroll
+      for (int i = 0; i < Q; i++) f[i] = p + i < P ? refs[p + i] : 0;
+    }
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < Q; i++) c += f[i] != 0;
+    return c;
+  };
+  int n = 0, sum = 0, u = 0;
+  for (int p0 = 0; p0 < P; p0 += PT * Q) {
+    u = block_scan(counts(p0 + Q * tid), lds, sum);
+    n += sum;
   }
-  if (tid == 0 && n == P) below = n;
-  __syncthreads();
-  const int moves = n - below;
   int* from = plan + 1;
   int* to = from + P / 2;
-  u = u0;
-  for (int p = p0; p < p1; p++) {
-    const bool used = refs[p] != 0;
-    map[p] = p;
-    if (used && p >= n) from[u - below] = p;
-    if (!used && p < n) to[p - u] = p;
-    u += used;
-  }
-  __syncthreads();
-  for (int k = tid; k < moves; k += PT) {
-    const int f = from[k], t = to[k];
-    map[f] = t;
-    refs[t] = refs[f];
-    refs[f] = 0;
+  int below = n;  // used pages below page n (all of them, if none lies from n on)
+  for (int p0 = 0, before = 0; p0 < P; p0 += PT * Q, before += sum) {
+    const int p = p0 + Q * tid;
+    if (P > PT * Q) u = before + block_scan(counts(p), lds, sum);  // (else as it is)
+    if (n >= p && n < p + Q && n < P) {
+      int b = u;
+#pragma unroll
+      for (int i = 0; i < Q; i++)
+        if (p + i < n) b += f[i] != 0;
+      below_n = b;
+    }
+    __syncthreads();
+    if (n >= p0 && n < p0 + PT * Q && n < P) below = below_n;
+    int mv[Q];
+#pragma unroll
+    for (int i = 0; i < Q; i++) {
+      mv[i] = p + i;
+      if (p + i >= P) continue;
+      const bool used = f[i] != 0;
+      if (used && p + i >= n) mv[i] = below - u - 2;
+      if (used && p + i >= n) from[u - below] = p + i;
+      if (!used && p + i < n) to[p + i - u] = p + i;
+      u += used;
+    }
+    if (p + Q <= P) {
+      __builtin_memcpy(map + p, mv, sizeof(mv));
+    } else {
+#pragma unroll
+      for (int i = 0; i < Q; i++)
+        if (p + i < P) map[p + i] = mv[i];
+    }
   }
   if (tid == 0) {
-    plan[0] = moves;
+    plan[0] = n - below;
     *n_out = n;
   }
 }
 
-// A grid that walks the (move, layer, key / value, slice) units, then the
-// tables.  Sources are pages from n on, destinations pages below n.
+// A grid that walks the tables and counts, then the (move, layer, key / value,
+// slice) units.  Sources are pages from n on, destinations pages below n.
 template <int B>
-__global__ void __launch_bounds__(256) k_compact(uint8_t* kv, int* tables,
+__global__ void __launch_bounds__(256) k_compact(uint8_t* kv, int* refs, int* tables,
                                                  const int* __restrict__ plan,
                                                  const int* __restrict__ map, int L2, int P,
                                                  long entries, long page_bytes, int slices,
                                                  int* err) {
-  for (long i = blockIdx.x * 256l + threadIdx.x; i < entries; i += gridDim.x * 256l) {
-    const int p = tables[i];
-    if (p < 0) continue;
-    if (p < P) tables[i] = map[p];
-    else *err = UB_ERR_INDEX;
-  }
   const int moves = plan[0];
   const int* from = plan + 1;
   const int* to = from + P / 2;
+  const long first = blockIdx.x * 256l + threadIdx.x, step = gridDim.x * 256l;
+  for (long i = first; i < entries; i += step) {
+    const int p = tables[i];
+    if (p < 0) continue;
+    if (p < P) {
+      const int m = map[p];
+      tables[i] = m >= 0 ? m : to[-2 - m];
+    } else {
+      *err = UB_ERR_INDEX;
+    }
+  }
+  for (long k = first; k < moves; k += step) {
+    refs[to[k]] = refs[from[k]];
+    refs[from[k]] = 0;
+  }
   const long units = page_bytes / B, per = (units + slices - 1) / slices;
   const long total = (long)moves * L2 * slices;
   for (long w = blockIdx.x; w < total; w += gridDim.x) {
@@ -379,11 +411,13 @@ UB_API int ubridge_kv_compact(const UbridgeKvPool* p, int32_t* n_used, void* str
   int* plan = (int*)ws.get();
   if (!plan) return ub_set_error(UB_ERR_LAUNCH, "%s: no workspace", nm);
   int* map = plan + 2 * (p->P / 2) + 1;
-  k_compact_plan<<<1, PT, 0, s>>>(p->refs, p->P, plan, map, n_used);
+  // four pages a thread up to 4096: 2048 pages take 3.6 us, 6.6 with sixteen
+  if (p->P <= 4 * PT) k_compact_plan<4><<<1, PT, 0, s>>>(p->refs, p->P, plan, map, n_used);
+  else k_compact_plan<16><<<1, PT, 0, s>>>(p->refs, p->P, plan, map, n_used);
   const int b = unit_bytes(p->kv, p->page_bytes);
   const int slices = (int)(p->page_bytes / 32768 > 0 ? p->page_bytes / 32768 : 1);
 #define UB_GO(B)                                                                             \
-  k_compact<B><<<2048, 256, 0, s>>>((uint8_t*)p->kv, p->tables, plan, map, 2 * p->L, p->P,   \
+  k_compact<B><<<2048, 256, 0, s>>>((uint8_t*)p->kv, p->refs, p->tables, plan, map, 2 * p->L, p->P,   \
                                     (long)p->rows * p->width, p->page_bytes, slices, err)
   if (b == 16) UB_GO(16);
   else if (b == 8) UB_GO(8);
