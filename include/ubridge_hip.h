@@ -426,7 +426,8 @@ int ubridge_int8_linear(const void* x, int dtype, const int8_t* w, const float* 
  * q_out and k_out: pair i (x[i], x[i + rot / 2]), or (x[2 i], x[2 i + 1]) when
  * interleaved, turns by 2 pi positions[t] turns[i] (turns f64 [rot / 2],
  * positions int32, or int64 with pos64) and is scaled by factor; elements from
- * rot on pass through.  inverse: by minus the angle, the gradient.
+ * rot on pass through.  inverse: by minus the angle, the gradient.  Results
+ * overlap no input.
  * ubridge_rope_append: q to q_out; the turned k and v [T, Hkv, D] to slot
  * slots[t] (page slot / S, place slot % S; negative: nowhere) of k_pages and
  * v_pages [P, Hkv, S, D], page_stride elements apart, k_out unused.  Slots of

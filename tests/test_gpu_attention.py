@@ -102,6 +102,28 @@ def test_lengths(dev, t, cache, Hq, Hkv, D, S):
     moe.device_error()
 
 
+@pytest.mark.parametrize("t,cache", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "e4m3"), ("f16", "e4m3")])
+@pytest.mark.parametrize("Hq,Hkv,D,S", [(4, 1, 128, 16), (3, 3, 40, 1), (17, 1, 64, 8), (14, 2, 80, 24), (70, 1, 96, 64),
+                                        (8, 8, 192, 16), (33, 1, 256, 5), (40, 2, 128, 12), (2, 1, 8, 3)])
+def test_short(dev, t, cache, Hq, Hkv, D, S):
+    # few rows and few steps: a workgroup a row, its wavefronts with and without steps
+    for lens in ([0, 1, 31, 32, 33, 100, 200], [120], [0]):
+        q, kv, tables, n = make(dev, lens, Hq, Hkv, D, S, t, cache)
+        out, lse = attention.paged_decode(q, kv[0], kv[1], tables, n, return_lse=True)
+        check(out, q, kv, tables, n, lse)
+        out, lse = attention.paged_decode(q, kv[0], kv[1], tables, n, window=33, softcap=4.0, return_lse=True)
+        check(out, q, kv, tables, n, lse, window=33, softcap=4.0)
+    moe.device_error()
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(70, 1, 64), (130, 2, 128), (33, 1, 256)])
+def test_many_heads(dev, Hq, Hkv, D):
+    # more query heads to a kv head than one pass takes
+    q, kv, tables, n = make(dev, [3000, 5, 0, 777], Hq, Hkv, D, 16, "bf16")
+    out, lse = attention.paged_decode(q, kv[0], kv[1], tables, n, return_lse=True)
+    check(out, q, kv, tables, n, lse)
+
+
 @pytest.mark.parametrize("lens,Hq,Hkv,D,S", [([5000], 8, 2, 128, 16), ([20011, 3], 4, 4, 64, 64),
                                              ([1, 0, 9000, 4097], 16, 1, 128, 24), ([3001] * 5, 24, 3, 256, 8)])
 @pytest.mark.parametrize("t,cache", [("bf16", "bf16"), ("f16", "e4m3")])

@@ -56,7 +56,8 @@ def heads(g, T, Hq, Hkv, D, dtype, dev, pad=0):
 @pytest.mark.parametrize("T,Hq,Hkv,D,rot,pad", [
     (1, 1, 1, 2, 2, 0), (1, 8, 2, 64, 64, 0), (7, 3, 1, 40, 26, 3), (33, 4, 4, 80, 80, 1),
     (5, 6, 2, 96, 0, 0), (300, 2, 1, 128, 96, 0), (3, 16, 16, 256, 254, 5), (9, 1, 1, 7, 4, 0),
-    (2, 40, 8, 192, 192, 8), (1100, 1, 1, 64, 2, 0)])
+    (2, 40, 8, 192, 192, 8), (1100, 1, 1, 64, 2, 0), (2, 3, 1, 1000, 600, 0), (3, 2, 2, 1001, 1000, 1),
+    (1, 1, 1, 4096, 4096, 0), (4, 5, 3, 130, 18, 0), (6, 2, 1, 70, 66, 2)])
 def test_turn(dev, dtype, inter, T, Hq, Hkv, D, rot, pad):
     g = torch.Generator().manual_seed(T + D + rot)
     q, k, _ = heads(g, T, Hq, Hkv, D, dtype, dev, pad)
