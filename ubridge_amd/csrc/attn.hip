@@ -55,7 +55,7 @@ constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int W = 4;         // wavefronts of a workgroup
 constexpr int kRowCost = 2;  // steps that the first loads of a row are worth
-constexpr int kShares = 2048;  // two wavefronts a SIMD (three, 3072: 64 ragged sequences 30 -> 47 us, by spills)
+constexpr int kShares = 2048;  // two wavefronts a SIMD (three: 64 ragged sequences 30 -> 47 us, by spills)
 
 template <int DT>
 __device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
