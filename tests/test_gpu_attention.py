@@ -313,3 +313,16 @@ def test_refusals(dev):
             attention.paged_decode(**dict(ok, **bad))
     e = attention.paged_decode(q[:0], kv[0], kv[1], tables[:0], n[:0], return_lse=True)
     assert e[0].shape == (0, 4, 64) and e[1].shape == (0, 4)
+
+
+def test_result_over_an_input_is_refused(dev):
+    q, kv, tables, n = make(dev, [40, 33], 4, 2, 64, 16, "bf16")
+    pool = torch.zeros(2 * q.numel(), dtype=q.dtype, device=dev)
+    a, b = pool[:q.numel()].view_as(q), pool[q.numel():].view_as(q)
+    a.copy_(q)
+    for out in (a, pool[8:8 + q.numel()].view_as(q), kv.view(-1)[:q.numel()].view_as(q)):
+        with pytest.raises(ValueError, match="overlaps"):
+            attention.paged_decode(a, kv[0], kv[1], tables, n, out=out)
+    want = attention.paged_decode(q, kv[0], kv[1], tables, n)
+    assert attention.paged_decode(a, kv[0], kv[1], tables, n, out=b) is not None
+    assert torch.equal(b, want)  # the neighbour in the same storage is fine

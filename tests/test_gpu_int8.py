@@ -176,3 +176,24 @@ def test_refusals(dev):
                 torch.zeros(16, 4, device=dev).t()):
         with pytest.raises(ValueError):
             lin(x, out=out)
+
+
+def test_result_over_its_input_is_refused(dev):
+    lin = int8.Linear(torch.ones(32, 32, dtype=torch.int8, device=dev), torch.ones(32, device=dev))
+    pool = torch.ones(12, 32, device=dev)
+    for out in (pool[:4], pool[3:7]):
+        with pytest.raises(ValueError, match="overlaps"):
+            lin(pool[:4], out=out)
+    want = lin(pool[:4])
+    lin(pool[:4], out=pool[4:8])
+    assert torch.equal(pool[4:8], want)
+
+
+def test_replaced_weights_are_checked(dev):
+    x = torch.ones(4, 32, device=dev)
+    for name, t in (("w", torch.ones(32, 16, dtype=torch.int8, device=dev)), ("w", torch.ones(32, 128, device=dev)),
+                    ("w_scale", torch.ones(31, device=dev)), ("bias", torch.ones(32, device=dev).half())):
+        lin = int8.Linear(torch.ones(32, 32, dtype=torch.int8, device=dev), torch.ones(32, device=dev))
+        setattr(lin, name, t)
+        with pytest.raises(ValueError):
+            lin(x)

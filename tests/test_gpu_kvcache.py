@@ -251,3 +251,27 @@ def test_refusals(dev):
                  lambda: c.fork(t.view(1, 2), t), lambda: c.free(torch.zeros(4, dtype=torch.int32, device=dev)[::2])):
         with pytest.raises(ValueError):
             call()
+
+
+def test_state_is_written_in_place(dev):
+    kv = torch.zeros(1, 2, 4, 2, 4, 8, device=dev, dtype=torch.bfloat16)
+    c = kvcache.PagedCache(kv, 2, 2)
+    for name in ("kv", "meta", "refs", "lens", "tables"):
+        with pytest.raises(AttributeError):
+            setattr(c, name, getattr(c, name).clone())
+    c.lens += 1
+    assert c.lens.tolist() == [1, 1] and c.meta[4:6].tolist() == [1, 1]
+    x = torch.ones(1, 2, 8, device=dev, dtype=torch.bfloat16)
+    slots = torch.zeros(1, dtype=torch.int64, device=dev)
+    c.k_scale = torch.ones(1, device=dev)  # of two heads
+    with pytest.raises(ValueError):
+        c.append(0, None, x, x, slots)
+    c.k_scale = None
+    r = rope.Rope(8, device=dev)
+    for turns in (r.turns[:3], r.turns.float()):
+        bad = rope.Rope(8, device=dev)
+        bad.turns = turns
+        with pytest.raises(ValueError):
+            c.append(0, x, x, x, slots, slots, bad)
+        with pytest.raises(ValueError):
+            bad(x, x, slots)

@@ -17,8 +17,8 @@ def paged_decode(q, k_pages, v_pages, tables, lens, scale=None, softcap=0.0, win
     scale (default D ** -0.5) multiplies q . k; softcap c > 0 turns a score x
     into c tanh(x / c); slopes f32 [Hq] then add slope * (t - newest); window >
     0 keeps the newest `window` tokens; k_scale, v_scale f32 [Hkv] are what a
-    stored value stands for.  Returns [B, Hq, D] of q's type, zeros for an
-    empty sequence; with return_lse also the logarithm of the softmax's sum,
+    stored value stands for.  Returns [B, Hq, D] of q's type (in `out`, which
+    overlaps no input, if it is given), zeros for an empty sequence; with return_lse also the logarithm of the softmax's sum,
     f32 [B, Hq], -inf for an empty sequence.  It has no gradient.
     """
     return call(_native.paged_decode, stream, q, k_pages, v_pages, tables, lens, scale, softcap, window,

@@ -75,6 +75,16 @@ at::Tensor result(at::IntArrayRef sizes, const at::Tensor& like) { return at::em
 at::Tensor result(at::IntArrayRef sizes, const at::Tensor& like, at::ScalarType t) {
   return at::empty(sizes, like.options().requires_grad(false).dtype(t));
 }
+// whether the memory of two tensors meets (strides are never negative)
+bool meet(const at::Tensor& x, const at::Tensor& y) {
+  if (x.numel() == 0 || y.numel() == 0) return false;
+  auto end = [](const at::Tensor& t) {
+    int64_t n = 1;
+    for (int64_t i = 0; i < t.dim(); i++) n += (t.size(i) - 1) * t.stride(i);
+    return (const char*)t.data_ptr() + n * t.element_size();
+  };
+  return (const char*)x.data_ptr() < end(y) && (const char*)y.data_ptr() < end(x);
+}
 bool fits(int64_t x) { return x >= 0 && x <= 0x7fffffff; }
 
 // args: count and place checks
@@ -142,6 +152,7 @@ PyObject* py_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!vec(ks, Hkv) || !vec(vs, Hkv)) REFUSE("paged_decode: k_scale and v_scale must be contiguous float32 [%ld]", Hkv);
   if (out && (out->sizes() != q->sizes() || out->scalar_type() != q->scalar_type() || !dense(*out)))
     REFUSE("paged_decode: out must be contiguous, of q's type and shape");
+  if (out && (meet(*out, *q) || meet(*out, *k) || meet(*out, *v))) REFUSE("paged_decode: out overlaps an input");
   const bool with_lse = PyObject_IsTrue(args[12]);
   at::Tensor o = out ? *out : result({B, Hq, D}, *q), l;
   if (with_lse) l = result({B, Hq}, *q, at::kFloat);
@@ -165,6 +176,12 @@ PyObject* py_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// a Rope's turns per position, f64 [rot / 2]
+bool turn_list(Ten t, int rot) {
+  if (rot >= 0 && t->scalar_type() == at::kDouble && t->dim() == 1 && t->size(0) == rot / 2 && dense(*t)) return true;
+  PyErr_Format(PyExc_ValueError, "rope: turns must be contiguous float64 [%d]", rot / 2);
+  return false;
+}
 // x [T, H, D] with its last dim contiguous
 bool heads(const char* name, const at::Tensor& x, int64_t T, int64_t D) {
   if (x.dim() != 3 || x.size(0) != T || x.size(2) != D) {
@@ -203,7 +220,8 @@ PyObject* py_rope(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   p.rot = (int)A.n(4);
   if (q->dim() != 3 || p.rot > q->size(2)) REFUSE("rope: q must be [T, heads, D] with D >= rot=%d", p.rot);
   const int64_t T = q->size(0), Hq = q->size(1), D = q->size(2), Hkv = k ? k->size(k->dim() == 3 ? 1 : 0) : 0;
-  if (!heads("q", *q, T, D) || (k && !heads("k", *k, T, D)) || !position_list(pos, T, p)) return nullptr;
+  if (!heads("q", *q, T, D) || (k && !heads("k", *k, T, D)) || !position_list(pos, T, p) || !turn_list(turns, p.rot))
+    return nullptr;
   if (!fits(T) || !fits(Hq) || !fits(Hkv) || !fits(D)) REFUSE("rope: sizes of 32 bits");
   at::Tensor qo = result({T, Hq, D}, *q), ko;
   p.q = q->data_ptr(), p.q_out = qo.data_ptr(), p.turns = ptr<double>(turns);
@@ -237,6 +255,8 @@ PyObject* py_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       !device_tensor(args[7], slots) || !device_tensor(args[8], pos, true) || !device_tensor(args[9], turns, true))
     return nullptr;
   const long layer = A.n(1);
+  if (kv->dim() != 6 || kv->size(1) != 2 || !dense(*kv) || !vec(ks, kv->size(3)) || !vec(vs, kv->size(3)))
+    REFUSE("PagedCache.append: kv [L, 2, P, H, S, D], scales float32 [H], all contiguous");
   const int64_t L = kv->size(0), P = kv->size(2), H = kv->size(3), S = kv->size(4), D = kv->size(5);
   const int dt = code(*k), ct = code(*kv);
   if (dt < 0 || dt > 2 || v->scalar_type() != k->scalar_type() || (ct != dt && ct != 3))
@@ -257,7 +277,7 @@ PyObject* py_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     p.rot = (int)A.n(10);
     if (q->scalar_type() != k->scalar_type()) REFUSE("PagedCache.append: q and k of one type");
     if (p.rot > D) REFUSE("PagedCache.append: rot=%d of heads of %ld", p.rot, D);
-    if (!heads("q", *q, T, D) || !position_list(pos, T, p)) return nullptr;
+    if (!heads("q", *q, T, D) || !position_list(pos, T, p) || !turn_list(turns, p.rot)) return nullptr;
     if (!fits(q->size(1))) REFUSE("PagedCache.append: sizes of 32 bits");
     p.Hq = q->size(1);
     qo = result({T, q->size(1), D}, *q);
@@ -289,6 +309,9 @@ PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       !device_tensor(args[3], b, true))
     return nullptr;
   const long K = A.n(4);
+  if (w->scalar_type() != at::kChar || w->dim() != 2 || !dense(*w) || K <= 0 || w->size(1) < K || !vec(sw, w->size(0)) ||
+      !vec(b, w->size(0)))
+    REFUSE("int8.Linear: weight int8 [N, >= %ld], w_scale and bias float32 [N], all contiguous", K);
   const int dt = code(*x);
   if (dt < 0 || dt > 2 || x->dim() == 0 || x->size(-1) != K)
     REFUSE("int8.Linear takes f32, f16 or bf16 activations [..., %ld]", K);
@@ -300,6 +323,7 @@ PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   out = args[5] == Py_None ? nullptr : &THPVariable_Unpack(args[5]);
   if (out && (!out->is_cuda() || out->scalar_type() != x->scalar_type() || out->sizes() != at::IntArrayRef(sizes) || !dense(*out)))
     REFUSE("int8.Linear: out must be contiguous, of x's type, [..., %ld]", N);
+  if (out && meet(*out, *x)) REFUSE("int8.Linear: out overlaps x");
   at::Tensor y = out ? *out : result(sizes, *x), xc;
   const void* xp = x->data_ptr();
   if (!dense(*x)) {

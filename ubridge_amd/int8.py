@@ -16,7 +16,7 @@ class Linear:
     w int8 [N, K], w_scale f32 [N], bias f32 [N] or None.  x is f32, f16 or
     bf16 [..., K] and y has its type.  A row's scale is amax / 127 (1 for a row
     of zeros), its codes round to even; a row that holds an infinity or a NaN
-    gives NaN.  K is padded once to a multiple of 128, so the weight is copied
+    gives NaN.  `out`, if given, does not overlap x.  K is padded once to a multiple of 128, so the weight is copied
     unless K is one already.
     """
 

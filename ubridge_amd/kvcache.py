@@ -1,6 +1,7 @@
 """A paged key-value cache whose state stays on the device: storing new tokens
 (with their rotation), freeing, forking and compacting without a host copy of
 page tables, so that the calls can be enqueued, or captured, ahead."""
+import operator
 import struct
 
 import torch
@@ -13,6 +14,15 @@ from .ops import _need_cuda
 _TYPES = (torch.float16, torch.bfloat16, torch.float8_e4m3fn)
 
 
+def _in_place(name):
+    """A tensor of a cache, whose address is packed once: it may be written (x += 1
+    assigns the same tensor again), not replaced."""
+    def replace(self, t):
+        if t is not getattr(self, "_" + name):
+            raise AttributeError(f"PagedCache.{name} is written in place, not replaced")
+    return property(operator.attrgetter("_" + name), replace)
+
+
 class PagedCache:
     """kv [L, 2, P, H, S, D]: keys and values of L layers in P pages of S tokens
     (f16, bf16 or e4m3; k_scale, v_scale f32 [H] are what a stored e4m3 value
@@ -21,7 +31,7 @@ class PagedCache:
     The state is one int32 buffer `meta` [P + rows + rows * width]: refs [P],
     how many rows hold a page; lens [rows], tokens; tables [rows, width], pages
     in order, -1 for none.  The three are views a program may read and write
-    (it gives a growing row its pages); without `meta` the pool starts empty.
+    in place (it gives a growing row its pages); without `meta` the pool starts empty.
     """
 
     def __init__(self, kv, rows, width, k_scale=None, v_scale=None, meta=None):
@@ -42,14 +52,16 @@ class PagedCache:
             meta[P + rows:] = -1
         elif meta.shape != (n,) or meta.dtype != torch.int32 or not meta.is_contiguous():
             raise ValueError(f"PagedCache: meta must be contiguous int32 [{n}]")
-        self.kv, self.meta, self.k_scale, self.v_scale = kv, meta, k_scale, v_scale
+        self._kv, self._meta, self.k_scale, self.v_scale = kv, meta, k_scale, v_scale
         self.L, self.P, self.H, self.S, self.D, self.rows, self.width = L, P, H, S, D, rows, width
-        self.refs, self.lens = meta[:P], meta[P:P + rows]
-        self.tables = meta[P + rows:].view(rows, width)
+        self._refs, self._lens = meta[:P], meta[P:P + rows]
+        self._tables = meta[P + rows:].view(rows, width)
         page = H * S * D * kv.element_size()
         p = meta.data_ptr()
         self._pool = struct.pack("@4Pq6i", kv.data_ptr(), p, p + 4 * P, p + 4 * (P + rows), page, L,
                                  P, S, rows, width, 0)
+
+    kv, meta, refs, lens, tables = map(_in_place, ("kv", "meta", "refs", "lens", "tables"))
 
     def layer(self, i):
         """(k_pages, v_pages) of a layer, [P, H, S, D] each."""
