@@ -416,8 +416,9 @@ int ubridge_device_error(void* stream);
  * zeros; codes rounded to even; a row with an infinity or a NaN gives NaN), w
  * int8 [N, ld], 16-byte aligned, rows padded with zeros to ld, a multiple of
  * 128; sw, bias f32 [N] (bias may be NULL); dtype 0 f32, 1 f16, 2 bf16.  K <=
- * 132104, where the int32 sum stays exact.  Scratch beyond 16 tokens: M (ld +
- * 4) bytes, and 4 M N bytes a part where long rows are cut (at most 32). */
+ * 132104, where the int32 sum stays exact.  Scratch beyond 16 tokens or M ld =
+ * 65536: M (ld + 4) bytes, and 4 M N bytes a part where long rows are cut (at
+ * most 32). */
 int ubridge_int8_linear(const void* x, int dtype, const int8_t* w, const float* sw,
                         const float* bias, void* y, int M, int K, int N, int ld, void* stream);
 

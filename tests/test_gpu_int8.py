@@ -197,3 +197,11 @@ def test_replaced_weights_are_checked(dev):
         setattr(lin, name, t)
         with pytest.raises(ValueError):
             lin(x)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N", [(8, 8192, 40), (9, 8192, 40), (16, 4096, 100), (16, 4097, 100), (5, 13107, 33),
+                                   (6, 13107, 33), (1, 65536, 17), (1, 65537, 17), (2, 32768, 50), (1, 132104, 5)])
+def test_few_tokens_of_long_rows(dev, dtype, M, K, N):
+    x, w, ws, b, lin = make(dev, M, K, N, dtype, True)
+    near(lin(x.to(dev)), x, w, ws, b, dev)

@@ -11,8 +11,8 @@
 //
 // Rows of a and w are padded with zeros to ld bytes, a multiple of 128.
 //
-// Up to 16 tokens the product is a stream of the weight and one kernel does it
-// all (k_i8_dec); beyond, k_quant makes the codes and k_i8_gemm (or k_i8_ring, by
+// Up to 16 tokens (of 64 KiB in all) the product is a stream of the weight and one
+// kernel does it all (k_i8_dec); beyond, k_quant makes the codes and k_i8_gemm (or k_i8_ring, by
 // plan_for) multiplies them.  us: 8 x 4096 x 6144 (M x K x N) 10.8, of which the
 // weight's 25 MB are 5 and the rest is the launch, the activations' codes ahead of
 // the first product and the sum over the wavefronts; 8 x 4096 x 28672 26 (4.5 TB/s);
@@ -626,6 +626,11 @@ __global__ void __launch_bounds__(64 * DW) k_i8_dec(const void* __restrict__ x, 
   }
 }
 
+// Every workgroup makes all the codes: past 64 KiB of them that costs more than the
+// launch it saves.  us (M x K x N), k_i8_dec / the tiles: 16 x 4096 x 4096 10.4 / 11.4,
+// 8 x 8192 x 8192 18.4 / 20.2, 4 x 14336 x 4096 17.2 / 18.4, then 12 x 8192 x 8192 23.9 /
+// 20.4, 6 x 14336 x 4096 21.8 / 18.5, 4 x 28672 x 8192 54.8 / 49.1
+constexpr int kDecCodes = 64 * 1024;
 constexpr int kLds = 160 * 1024;  // of a CU
 size_t dec_lds(int M, int ld) { return sizeof(int) * (DW * M * 17 + 16 + 32 * kDecTiles) + (size_t)M * (ld + 16); }
 
@@ -731,7 +736,7 @@ void gemm(Plan plan, const int8_t* q, const float* sa, const int8_t* w, const fl
 template <int DT>
 int linear(const char* nm, const void* x, const int8_t* w, const float* sw, const float* bias, void* y, int M, int K,
            int N, int ld, hipStream_t s) {
-  if (M <= 16 && N <= 256 * 16 * kDecTiles && dec_lds(M, ld) <= kLds) {
+  if (M <= 16 && M * ld <= kDecCodes && N <= 256 * 16 * kDecTiles) {
     dec<DT>(x, w, sw, bias, y, M, K, N, ld, s);
     return UB_OK;
   }
