@@ -326,3 +326,16 @@ def test_result_over_an_input_is_refused(dev):
     want = attention.paged_decode(q, kv[0], kv[1], tables, n)
     assert attention.paged_decode(a, kv[0], kv[1], tables, n, out=b) is not None
     assert torch.equal(b, want)  # the neighbour in the same storage is fine
+
+
+@pytest.mark.parametrize("lens,Hq,Hkv,D,S", [
+    ([4100], 4, 1, 128, 16), ([3000, 0, 77, 2500], 40, 1, 128, 16), ([2000, 1500], 72, 2, 64, 8),
+    ([1700, 0, 0, 900], 13, 1, 256, 16), ([900, 33], 48, 2, 256, 5), ([2600], 128, 1, 8, 16),
+    ([700] * 3 + [0] + [40] * 60, 32, 8, 64, 16), ([300] * 63 + [0, 1], 16, 8, 40, 16)])
+def test_rows_in_parts(dev, lens, Hq, Hkv, D, S):
+    # one row to 520, each in many shares or few, their heads joined by one workgroup or several
+    q, kv, tables, n = make(dev, lens, Hq, Hkv, D, S)
+    out, lse = attention.paged_decode(q, kv[0], kv[1], tables, n, return_lse=True)
+    check(out, q, kv, tables, n, lse)
+    assert torch.equal(out, attention.paged_decode(q, kv[0], kv[1], tables, n))
+    moe.device_error()

@@ -34,7 +34,7 @@
 // to 6000 under a window of 2048, 16 e4m3 heads of 80 (43 MB) 13.8 + 5.2, where
 // half the time is latency and the softmax of one head in sixteen columns; one of
 // 700 tokens 7.0 + 4.6, all latency: the search for the share, the page, the row,
-// then the join's own three reads.
+// then the join's own reads.
 //
 // Numerics.  Scores, the running maximum and sum, and the output's sum are f32.
 // The weights exp(x - m) enter the second product as the sum of two 16-bit
@@ -55,6 +55,11 @@ constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int W = 4;         // wavefronts of a workgroup
 constexpr int kRowCost = 2;  // steps that the first loads of a row are worth
+// Workgroups of k_join up to which the heads of a row are dealt out to several
+// (its ROWS).  us of the whole call, one workgroup a row / dealt: 1 x 4096 tokens, 8 kv
+// heads of 128 20.0 / 16.5, 1 x 131072 118 / 108, 32 x 4096 with 32 query heads on one
+// kv head 56 / 43; up to 1024 workgroups 256 rows took 2 us longer, at 512 as long
+constexpr int kJoins = 512;
 constexpr int kShares = 2048;  // two wavefronts a SIMD (three: 64 ragged sequences 30 -> 47 us, by spills)
 
 template <int DT>
@@ -574,36 +579,59 @@ k_decode(const Dev d) {
   if (lane == 0) d.cut[share] = cut;
 }
 
-// Workgroup i: the row that starts in share i and is cut, if there is one.
-// Thread (u, column) adds four dims of one head over every U-th of the row's
+// Workgroup (i, j): `part` heads of row i (ROWS, at most 512: where it lies follows
+// from the costs), else of the row that starts in share i; nothing if that row
+// is not cut.  Thread (u, column) adds four dims of one head over every U-th of the row's
 // shares, four of them in flight, under a running maximum; the U sums meet in
 // LDS, in order.
-template <int DT>
-__global__ void __launch_bounds__(512) k_join(const Dev d, int heads) {
+template <int DT, bool ROWS>
+__global__ void __launch_bounds__(512) k_join(const Dev d, int heads, int part) {
   __shared__ float4 so[512];
   __shared__ float2 sml[512];
   const UbridgePagedDecodeArgs& a = d.a;
-  const int2 cut = d.cut[blockIdx.x];
-  if (cut.x < 0) return;
-  const int Hh = a.Hkv * d.HG, b = cut.x / Hh, hh = cut.x - b * Hh;
+  const int Hh = a.Hkv * d.HG;
+  int row, first, parts;  // its first share and their number
+  if constexpr (ROWS) {
+    __shared__ int2 sums[8];  // of a wavefront's costs: all, those of sequences ahead of the row's
+    row = blockIdx.x;
+    const int b = row / Hh, own = cost(span(d, b)), i = threadIdx.x;
+    const int c = i < a.B ? cost(span(d, i)) : 0;
+    const int x = lane_scan(c), y = lane_scan(i < b ? c : 0);
+    if ((i & 63) == 63) sums[i >> 6] = make_int2(x, y);
+    __syncthreads();
+    int tot = 0, at = 0;
+#pragma unroll
+    for (int w = 0; w < 8; w++) tot += sums[w].x, at += sums[w].y;
+    const int chunk = max(1, (int)(((unsigned)(tot * Hh) + d.shares - 1) / (unsigned)d.shares));
+    at = at * Hh + (row - b * Hh) * own;
+    first = (unsigned)(at + kRowCost) / (unsigned)chunk;  // of its first step
+    parts = own ? (int)((unsigned)(at + own - 1) / (unsigned)chunk) - first + 1 : 0;
+    if (parts <= 1) return;
+  } else {
+    const int2 cut = d.cut[blockIdx.x];
+    if (cut.x < 0) return;
+    row = cut.x, first = blockIdx.x, parts = cut.y;
+  }
+  const int b = row / Hh, hh = row - b * Hh;
   const int h = hh / d.HG, q0 = (hh - h * d.HG) * heads;
-  const int V = a.D / 4, cols = min(d.G - q0, heads) * V;
+  const int qa = (int)blockIdx.y * part, V = a.D / 4, cols = min(min(d.G - q0, heads) - qa, part) * V;
+  if (cols <= 0) return;
   const int U = cols < 512 ? 512 / cols : 1;
   const float vs = a.v_scale ? a.v_scale[h] : 1.f;
   for (int c0 = 0; c0 < cols; c0 += 512) {
     const int u = (int)threadIdx.x / cols, col = c0 + (int)threadIdx.x - u * cols;
-    const int q = col / V, v = col - q * V;
+    const int q = qa + col / V, v = col % V;
     const bool live = u < U && col < cols;
     float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
     float M = -kInf, L = 0.f;
     if (live)
-      for (int p0 = u; p0 < cut.y; p0 += 4 * U) {
+      for (int p0 = u; p0 < parts; p0 += 4 * U) {
         float2 ml[4];
         float4 x[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          const int p = min(p0 + i * U, cut.y - 1);
-          const size_t slot = (size_t)(2 * ((int)blockIdx.x + p) + (p == 0)) * heads + q;
+          const int p = min(p0 + i * U, parts - 1);
+          const size_t slot = (size_t)(2 * (first + p) + (p == 0)) * heads + q;
           ml[i] = *(const float2*)(d.pml + 2 * slot);
           x[i] = *(const float4*)(d.po + slot * a.D + 4 * v);
         }
@@ -615,7 +643,7 @@ __global__ void __launch_bounds__(512) k_join(const Dev d, int heads) {
         O.x *= al, O.y *= al, O.z *= al, O.w *= al, L *= al;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          if (p0 + i * U >= cut.y) continue;
+          if (p0 + i * U >= parts) continue;
           const float w = exp_of(ml[i].x - ms);
           O.x += w * x[i].x, O.y += w * x[i].y, O.z += w * x[i].z, O.w += w * x[i].w;
           L += w * ml[i].y;
@@ -641,11 +669,11 @@ __global__ void __launch_bounds__(512) k_join(const Dev d, int heads) {
       }
     }
     if (live && u == 0) {
-      const size_t row = (size_t)b * a.Hq + h * d.G + q0 + q;
+      const size_t to = (size_t)b * a.Hq + h * d.G + q0 + q;
       const float f = L == 0.f ? 0.f : vs / L;
       const uint32_t w[2] = {pack2<DT>(O.x * f, O.y * f), pack2<DT>(O.z * f, O.w * f)};
-      __builtin_memcpy((uint16_t*)a.out + row * a.D + 4 * v, w, 8);
-      if (v == 0 && a.lse) a.lse[row] = lse_of<DT>(M, L);
+      __builtin_memcpy((uint16_t*)a.out + to * a.D + 4 * v, w, 8);
+      if (v == 0 && a.lse) a.lse[to] = lse_of<DT>(M, L);
     }
   }
 }
@@ -681,7 +709,15 @@ void decode(const Dev& d, int HT, hipStream_t s) {
   else if (d.a.D <= 128) decode<DT, CT, 4>(d, HT, s);
   else if (d.a.D <= 192) decode<DT, CT, 6>(d, HT, s);
   else decode<DT, CT, 8>(d, HT, s);
-  if (d.shares) k_join<DT><<<d.shares, 512, 0, s>>>(d, 16 * HT);
+  if (!d.shares) return;
+  const int rows = d.a.B * d.a.Hkv * d.HG, heads = d.G < 16 * HT ? d.G : 16 * HT;
+  if (rows > kJoins) {
+    k_join<DT, false><<<d.shares, 512, 0, s>>>(d, 16 * HT, heads);
+    return;
+  }
+  int part = 1;
+  while (rows * ub_cdiv(heads, part) > kJoins && part < heads) part *= 2;
+  k_join<DT, true><<<dim3(rows, ub_cdiv(heads, part)), 512, 0, s>>>(d, 16 * HT, part);
 }
 
 void go(const Dev& d, int HT, hipStream_t s) {
@@ -739,7 +775,11 @@ UB_API int ubridge_paged_decode(const UbridgePagedDecodeArgs* p, void* stream) {
     go(d, HT, s);
     return ub_check_launch(nm);
   }
-  d.shares = most >= kShares ? kShares : ub_cdiv(most, W) * W;
+  // one wavefront a SIMD where the registers allow no more: half the partial sums.  us
+  // with 2048 / 1024 shares: 32 x 4096 tokens, 32 query heads on one kv head of 128
+  // 43 / 30, 8 x 4 heads of 256 201 / 196, in e4m3 120 / 110
+  const int shares = nw == 4 ? kShares / 2 : kShares;
+  d.shares = most >= shares ? shares : ub_cdiv(most, W) * W;
   const size_t nml = sizeof(float) * 4 * heads * d.shares, no = nml / 2 * a.D;
   UbScratch ws(s, no + nml + sizeof(int2) * d.shares);
   if (!ws.get()) return ub_set_error(UB_ERR_LAUNCH, "%s: no workspace", nm);
