@@ -339,3 +339,54 @@ def test_rows_in_parts(dev, lens, Hq, Hkv, D, S):
     check(out, q, kv, tables, n, lse)
     assert torch.equal(out, attention.paged_decode(q, kv[0], kv[1], tables, n))
     moe.device_error()
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("lens", [[1, 2, 33, 70, 200], [1, 2, 40, 3000, 5000]], ids=["rows", "shares"])
+@pytest.mark.parametrize("place", ["greatest", "least", "last"])
+def test_infinite_values(dev, t, lens, place):
+    # an infinite value gives its infinity under any weight (their two parts of
+    # either size, the greatest's second one zero, a single token's too), two of
+    # opposite signs NaN, and the other dims keep their bits
+    q, kv, tables, n = make(dev, lens, 32, 2, 64, 16, t)
+    clean, lse = attention.paged_decode(q, kv[0], kv[1], tables, n, return_lse=True)
+    check(clean, q, kv, tables, n, lse)
+    bad = kv.clone()
+    want = clean.clone()
+    for b, m in enumerate(lens):
+        for h in range(2):
+            pages = tables[b, :-(-m // 16)].long()
+            x = kv[0, pages, h].double().reshape(-1, 64)[:m] @ q[b, 16 * h].double()
+            at = {"greatest": int(x.argmax()), "least": int(x.argmin()), "last": m - 1}[place]
+            heads = slice(16 * h, 16 * h + 16)
+
+            def plant(at, dims, val):
+                bad[1, tables[b, at // 16].long(), h, at % 16, dims] = val
+            plant(at, slice(0, 16), math.inf)
+            plant(at, slice(16, 32), -math.inf)
+            want[b, heads, :16], want[b, heads, 16:32] = math.inf, -math.inf
+            if m > 1:
+                plant(at, slice(32, 40), math.inf)
+                plant((at + m // 2) % m, slice(32, 40), -math.inf)
+                want[b, heads, 32:40] = math.nan
+    got, lse2 = attention.paged_decode(q, bad[0], bad[1], tables, n, return_lse=True)
+    assert torch.equal(lse, lse2)
+    assert torch.equal(got.nan_to_num(7.0, 8.0, 9.0), want.nan_to_num(7.0, 8.0, 9.0))
+    assert torch.equal(got.isnan(), want.isnan())
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("n", [30, 70, 6000])
+@pytest.mark.parametrize("newest", [False, True])
+def test_infinite_value_of_small_weight(dev, t, n, newest):
+    # e^-60 of the greatest weight, in one step or over many: far below f16's
+    # range, above f32's least
+    q, kv, tables, lens = make(dev, [n], 4, 1, 64, 16, t)
+    kv[0] *= 0.125
+    at = n - 1 if newest else 0
+    kv[1, tables[0, at // 16].long(), 0, at % 16, :8] = math.inf
+    kv[1, tables[0, at // 16].long(), 0, at % 16, 8:16] = -math.inf
+    slopes = torch.full((4,), (-60.0 if newest else 60.0) / (n - 1), device=dev)
+    out = attention.paged_decode(q, kv[0], kv[1], tables, lens, slopes=slopes)
+    assert bool((out[..., :8] == math.inf).all() and (out[..., 8:16] == -math.inf).all())
+    assert bool(torch.isfinite(out[..., 16:]).all())

@@ -38,10 +38,13 @@
 //
 // Numerics.  Scores, the running maximum and sum, and the output's sum are f32.
 // The weights exp(x - m) enter the second product as the sum of two 16-bit
-// numbers (16 bits for bf16, 22 for f16; f16 weights are scaled by 2^14 so that
-// those far below the maximum keep them): one number would cost as much as the
-// output's own rounding, and the products are not what bounds the kernel.
-// e4m3 values are exact in both types.
+// numbers (off by at most 2^-16 of the weight for bf16, 2^-22 for f16; f16 weights
+// are scaled by 2^14 so that those far below the maximum keep them): one number
+// would cost as much as the output's own rounding, and the products are not what
+// bounds the kernel.  The first is cut toward zero, and neither part of a weight
+// above zero is zero: an infinite value then gives infinities of one sign, where
+// parts of two signs, or a zero one, made it NaN (rounding the first to nearest
+// would be worth one more bit).  e4m3 values are exact in both types.
 #include "common.h"
 
 namespace {
@@ -83,6 +86,12 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
   }
+}
+// the same, toward zero
+template <int DT>
+__device__ __forceinline__ uint32_t cut2(float lo, float hi) {
+  if constexpr (DT == UB_BF16) return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(lo, hi));
 }
 template <int DT>
 __device__ __forceinline__ float half_of(uint32_t w, int hi) {
@@ -191,6 +200,7 @@ k_decode(const Dev d) {
   constexpr int EB = Raw<CT>::B;
   constexpr int kLeastD = DK == 2 ? 8 : DK == 3 ? 72 : DK == 4 ? 104 : DK == 6 ? 136 : 200;  // that takes this DK
   constexpr float kOff = DT == UB_F16 ? 14.f : 0.f;
+  constexpr float kLeast = DT == UB_F16 ? 0x1p-24f : 0x1p-126f;  // of a weight's parts
   typedef typename Raw<CT>::T R;
   const UbridgePagedDecodeArgs& a = d.a;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
@@ -427,14 +437,17 @@ k_decode(const Dev d) {
         for (int e = 0; e < 8; e++) {
           p[e] = exp_of(x[e] - ms, kOff);
           sum += p[e];
+          p[e] = p[e] > 0.f ? fmaxf(p[e], kLeast) : 0.f;  // (a NaN is in the sum)
         }
         l[t] = l[t] * al + sum;
         uint32_t* hi = (uint32_t*)&ph[t];
         uint32_t* lo = (uint32_t*)&pl[t];
 #pragma unroll
         for (int q = 0; q < 4; q++) {
-          hi[q] = pack2<DT>(p[2 * q], p[2 * q + 1]);
-          lo[q] = pack2<DT>(p[2 * q] - half_of<DT>(hi[q], 0), p[2 * q + 1] - half_of<DT>(hi[q], 1));
+          const float a = p[2 * q], b = p[2 * q + 1];
+          hi[q] = cut2<DT>(a, b);
+          lo[q] = pack2<DT>(fmaxf(a - half_of<DT>(hi[q], 0), fminf(a, kLeast)),
+                            fmaxf(b - half_of<DT>(hi[q], 1), fminf(b, kLeast)));
         }
         if (__any(al != 1.f)) {
 #pragma unroll
