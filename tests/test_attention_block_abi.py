@@ -1,7 +1,9 @@
 """CPU checks of the attention block's C entries: each refuses what it cannot
 take before it touches a device, and the argument blocks have the layout that
 the header gives them."""
+import copy
 import math
+import pickle
 import struct
 
 import pytest
@@ -146,3 +148,27 @@ def test_frequencies():
                 dict(kind="yarn", factor=2.0), dict(kind="ntk", factor=2.0, original=5)):
         with pytest.raises(ValueError):
             rope.frequencies(64, 10000.0, bad)
+
+
+@pytest.mark.parametrize("how", ["deepcopy", "pickle"])
+def test_a_copied_cache_works_on_its_own_memory(monkeypatch, how):
+    # what its page operations hand over: the copy's tensors, no address of the original's
+    monkeypatch.setattr(kvcache, "_need_cuda", lambda *t: None)
+    handed = []
+    monkeypatch.setattr(kvcache, "call", lambda fn, stream, *args: handed.extend(args))
+    c = kvcache.PagedCache(torch.zeros(1, 2, 4, 1, 4, 8).half(), 3, 2)
+    other = copy.deepcopy(c) if how == "deepcopy" else pickle.loads(pickle.dumps(c))
+    theirs = {c.kv.data_ptr(), c.meta.data_ptr(), c.lens.data_ptr(), c.tables.data_ptr()}
+    rows = torch.zeros(1, dtype=torch.int32)
+    for run in (lambda: other.free(rows), lambda: other.fork(rows, rows), other.compact):
+        del handed[:]
+        run()
+        at = {t.data_ptr() for t in handed if isinstance(t, torch.Tensor)}
+        for b in handed:
+            if isinstance(b, bytes):
+                at.update(struct.unpack(f"@{len(b) // 8}P", b[:len(b) // 8 * 8]))
+        assert not at & theirs and {other.kv.data_ptr(), other.meta.data_ptr()} <= at
+    other.refs[1], other.lens[2], other.tables[2, 1] = 5, 6, 7
+    assert other.meta.tolist() == [0, 5, 0, 0, 0, 0, 6] + [-1] * 5 + [7]
+    assert c.meta.tolist() == [0] * 7 + [-1] * 6
+    assert (c.P, c.rows, c.width) == (other.P, other.rows, other.width)

@@ -1,5 +1,8 @@
 """Freeing, forking and compacting a paged cache against the same steps on
 lists.  All of it is copies and counts: equality throughout."""
+import copy
+import pickle
+
 import numpy as np
 import pytest
 import torch
@@ -275,3 +278,19 @@ def test_state_is_written_in_place(dev):
             c.append(0, x, x, x, slots, slots, bad)
         with pytest.raises(ValueError):
             bad(x, x, slots)
+
+
+@pytest.mark.parametrize("how", [copy.deepcopy, lambda c: pickle.loads(pickle.dumps(c))], ids=["deepcopy", "pickle"])
+def test_copies_are_caches_of_their_own(dev, how):
+    c, m, kv = pool(dev, 2, 200, 2, 8, 32, 40, 8, torch.bfloat16, 5)
+    live = [b for b in range(40) if m.lens[b]]
+    meta0, kv0 = c.meta.clone(), c.kv.clone()
+    other = how(c)
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+    other.free(t(live[:3]))
+    m.free(live[:3])
+    assert other.fork(t(live[4:7]), t(live[:3])).tolist() == m.fork(live[4:7], live[:3], kv)
+    assert int(other.compact()) == m.compact(kv)
+    same(other, m, kv)
+    assert torch.equal(other.tables.flatten(), other.meta[240:])
+    assert torch.equal(c.meta, meta0) and torch.equal(raw(c.kv), raw(kv0))

@@ -338,13 +338,23 @@ PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// The pool as kvcache.py packed it (UbridgeKvPool), or null: refused.
-const UbridgeKvPool* pool(PyObject* o) {
-  if (!PyBytes_Check(o) || PyBytes_GET_SIZE(o) != (Py_ssize_t)sizeof(UbridgeKvPool)) {
-    PyErr_SetString(PyExc_TypeError, "a packed pool expected");
-    return nullptr;
+// The pool of a cache, whose two tensors are kv [L, 2, P, H, S, D] and meta [refs P
+// | lens rows | tables rows x width]; false: refused.  (From the tensors at every
+// call: addresses kept from another would outlive a copy of the cache.)
+bool pool(PyObject* okv, PyObject* ometa, int64_t rows, int64_t width, UbridgeKvPool& p) {
+  Ten kv, meta;
+  if (!device_tensor(okv, kv) || !device_tensor(ometa, meta)) return false;
+  if (kv->dim() != 6 || kv->size(1) != 2 || !dense(*kv) || !fits(rows) || !fits(width) || !fits(kv->size(0)) ||
+      !fits(kv->size(2)) || !fits(kv->size(4)) || meta->scalar_type() != at::kInt || meta->dim() != 1 ||
+      meta->size(0) != kv->size(2) + rows + rows * width || !dense(*meta)) {
+    PyErr_SetString(PyExc_ValueError, "PagedCache: kv [L, 2, P, H, S, D] and meta int32 [P + rows + rows * width], contiguous");
+    return false;
   }
-  return (const UbridgeKvPool*)PyBytes_AS_STRING(o);
+  p = {};
+  p.L = kv->size(0), p.P = kv->size(2), p.S = kv->size(4), p.rows = rows, p.width = width;
+  p.kv = kv->data_ptr(), p.page_bytes = kv->size(3) * kv->size(4) * kv->size(5) * kv->element_size();
+  p.refs = (int32_t*)meta->data_ptr(), p.lens = p.refs + p.P, p.tables = p.lens + rows;
+  return true;
 }
 bool row_list(const char* name, const at::Tensor& t) {
   if (t.dim() == 1 && t.scalar_type() == at::kInt && dense(t) && fits(t.size(0))) return true;
@@ -352,54 +362,55 @@ bool row_list(const char* name, const at::Tensor& t) {
   return false;
 }
 
-// rows, pool, stream
+// kv, meta, the pool's rows, width, rows to free, stream
 PyObject* py_free(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  COUNT(3)
+  COUNT(6)
   HANDLE_TH_ERRORS
   const Args A{args};
   Ten rows;
-  const UbridgeKvPool* p = pool(args[1]);
-  if (!p || !device_tensor(args[0], rows) || !row_list("rows", *rows)) return nullptr;
-  void* stream = A.p(2);
+  UbridgeKvPool p;
+  if (!pool(args[0], args[1], A.n(2), A.n(3), p) || !device_tensor(args[4], rows) || !row_list("rows", *rows))
+    return nullptr;
+  void* stream = A.p(5);
   if (PyErr_Occurred()) return nullptr;
-  if (const int rc = fn.free(p, ptr<int32_t>(rows), (int)rows->size(0), stream)) return PyLong_FromLong(rc);
+  if (const int rc = fn.free(&p, ptr<int32_t>(rows), (int)rows->size(0), stream)) return PyLong_FromLong(rc);
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
 
-// src, dst, pool, stream
+// kv, meta, rows, width, src, dst, stream
 PyObject* py_fork(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  COUNT(4)
+  COUNT(7)
   HANDLE_TH_ERRORS
   const Args A{args};
   Ten src, dst;
-  const UbridgeKvPool* p = pool(args[2]);
-  if (!p || !device_tensor(args[0], src) || !device_tensor(args[1], dst) || !row_list("src", *src) || !row_list("dst", *dst))
+  UbridgeKvPool p;
+  if (!pool(args[0], args[1], A.n(2), A.n(3), p) || !device_tensor(args[4], src) || !device_tensor(args[5], dst) ||
+      !row_list("src", *src) || !row_list("dst", *dst))
     return nullptr;
   const int64_t n = src->size(0);
   if (dst->size(0) != n || n > 65535)
     REFUSE("PagedCache.fork: %ld prompts, %ld samples (as many, at most 65535)", n, dst->size(0));
   at::Tensor pages = result({n}, *src);
-  void* stream = A.p(3);
+  void* stream = A.p(6);
   if (PyErr_Occurred()) return nullptr;
-  if (const int rc = fn.fork(p, ptr<int32_t>(src), ptr<int32_t>(dst), (int)n, (int32_t*)pages.data_ptr(), stream))
+  if (const int rc = fn.fork(&p, ptr<int32_t>(src), ptr<int32_t>(dst), (int)n, (int32_t*)pages.data_ptr(), stream))
     return PyLong_FromLong(rc);
   return THPVariable_Wrap(std::move(pages));
   END_HANDLE_TH_ERRORS
 }
 
-// meta, pool, stream
+// kv, meta, rows, width, stream
 PyObject* py_compact(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  COUNT(3)
+  COUNT(5)
   HANDLE_TH_ERRORS
   const Args A{args};
-  Ten meta;
-  const UbridgeKvPool* p = pool(args[1]);
-  if (!p || !device_tensor(args[0], meta)) return nullptr;
-  at::Tensor n = result({}, *meta);
-  void* stream = A.p(2);
+  UbridgeKvPool p;
+  if (!pool(args[0], args[1], A.n(2), A.n(3), p)) return nullptr;
+  at::Tensor n = result({}, THPVariable_Unpack(args[1]));
+  void* stream = A.p(4);
   if (PyErr_Occurred()) return nullptr;
-  if (const int rc = fn.compact(p, (int32_t*)n.data_ptr(), stream)) return PyLong_FromLong(rc);
+  if (const int rc = fn.compact(&p, (int32_t*)n.data_ptr(), stream)) return PyLong_FromLong(rc);
   return THPVariable_Wrap(std::move(n));
   END_HANDLE_TH_ERRORS
 }

@@ -2,7 +2,6 @@
 (with their rotation), freeing, forking and compacting without a host copy of
 page tables, so that the calls can be enqueued, or captured, ahead."""
 import operator
-import struct
 
 import torch
 
@@ -15,8 +14,8 @@ _TYPES = (torch.float16, torch.bfloat16, torch.float8_e4m3fn)
 
 
 def _in_place(name):
-    """A tensor of a cache, whose address is packed once: it may be written (x += 1
-    assigns the same tensor again), not replaced."""
+    """A tensor of a cache, one of several views of the same memory: it may be
+    written (x += 1 assigns the same tensor again), not replaced."""
     def replace(self, t):
         if t is not getattr(self, "_" + name):
             raise AttributeError(f"PagedCache.{name} is written in place, not replaced")
@@ -54,12 +53,20 @@ class PagedCache:
             raise ValueError(f"PagedCache: meta must be contiguous int32 [{n}]")
         self._kv, self._meta, self.k_scale, self.v_scale = kv, meta, k_scale, v_scale
         self.L, self.P, self.H, self.S, self.D, self.rows, self.width = L, P, H, S, D, rows, width
+        self._views()
+
+    def _views(self):
+        P, rows, meta = self.P, self.rows, self._meta
         self._refs, self._lens = meta[:P], meta[P:P + rows]
-        self._tables = meta[P + rows:].view(rows, width)
-        page = H * S * D * kv.element_size()
-        p = meta.data_ptr()
-        self._pool = struct.pack("@4Pq6i", kv.data_ptr(), p, p + 4 * P, p + 4 * (P + rows), page, L,
-                                 P, S, rows, width, 0)
+        self._tables = meta[P + rows:].view(rows, self.width)
+
+    # a copy (deepcopy, pickle) is a cache of its own: its views are of its own state
+    def __getstate__(self):
+        return {k: v for k, v in vars(self).items() if k not in ("_refs", "_lens", "_tables")}
+
+    def __setstate__(self, state):
+        vars(self).update(state)
+        self._views()
 
     kv, meta, refs, lens, tables = map(_in_place, ("kv", "meta", "refs", "lens", "tables"))
 
@@ -88,7 +95,7 @@ class PagedCache:
 
     def free(self, rows, stream=None):
         """The rows named (int32 [n]) lose their pages and become empty."""
-        call(_native.free, stream, rows, self._pool)
+        call(_native.free, stream, self.kv, self.meta, self.rows, self.width, rows)
 
     def fork(self, src, dst, stream=None):
         """Empty rows dst (int32 [n], all different) become samples of rows src:
@@ -96,9 +103,9 @@ class PagedCache:
         free page.  Returns int32 [n], the new page or -1.  A row that is not
         empty or not there, or for which no page is left, keeps its state, gives
         -1 and raises the flag that moe.device_error() reads."""
-        return call(_native.fork, stream, src, dst, self._pool)
+        return call(_native.fork, stream, self.kv, self.meta, self.rows, self.width, src, dst)
 
     def compact(self, stream=None):
         """Move the used pages to the low end of the pool; tables and refs follow.
         Returns their number, an int32 tensor."""
-        return call(_native.compact, stream, self.meta, self._pool)
+        return call(_native.compact, stream, self.kv, self.meta, self.rows, self.width)
