@@ -484,8 +484,9 @@ int ubridge_paged_decode(const UbridgePagedDecodeArgs* args, void* stream);
  * fork: row dst[i], empty, becomes a sample of row src[i]: whole pages are
  * shared, a part-filled last page is copied to the lowest free page, in the
  * order of i; new_pages[i] receives it, else -1.  Rows dst differ; a row that is
- * not empty, out of range or for which no page is left is not changed, gives -1
- * and raises the flag of ubridge_device_error.  n <= 65535.  Scratch: 12 n bytes.
+ * not empty, out of range or for which no page is left, or whose prompt's table
+ * names a page that is not there, is not changed, gives -1 and raises the flag of
+ * ubridge_device_error.  n <= 65535.  Scratch: 12 n bytes.
  * compact: with u pages in use, the k-th used page from u on moves to the k-th
  * free page below u, tables and refs with it; n_used[0] = u.  Scratch: 8 P + 8
  * bytes. */

@@ -294,3 +294,51 @@ def test_copies_are_caches_of_their_own(dev, how):
     same(other, m, kv)
     assert torch.equal(other.tables.flatten(), other.meta[240:])
     assert torch.equal(c.meta, meta0) and torch.equal(raw(c.kv), raw(kv0))
+
+
+@pytest.mark.parametrize("rows,width", [(20, 4), (20, 5000)])
+def test_fork_of_a_prompt_with_a_bad_page(dev, rows, width):
+    # a page that is not there, the last or a whole one before it: the sample is
+    # refused, its row and the counts stay, the next sample gets the lowest free page
+    P, S = 40, 4
+    m = Lists(P, S, rows, width)
+    for b, n in enumerate((9, 9, 9, 8, 9)):
+        m.rows[b], m.lens[b] = [6 * b + 1 + i for i in range(-(-n // S))], n
+        for p in m.rows[b]:
+            m.refs[p] = 1
+    kv = torch.randint(0, 1000, (2, 2, P, 1, S, 8), dtype=torch.int16).view(torch.float16)
+    c = kvcache.PagedCache(kv.to(dev), rows, width, meta=m.meta().to(dev))
+    t = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)
+    bad = {(0, 0): -1, (1, 1): P, (2, 3): 1 << 29, (3, 1): -7, (4, 2): 1 << 30}  # (row 2's lies past its pages)
+    for at, page in bad.items():
+        c.tables[at] = page
+    moe.device_error()
+    got = c.fork(t(0, 2, 1, 2, 3, 4, 2), t(9, 10, 11, 12, 13, 14, 15)).tolist()
+    new = m.fork([2, 2, 2], [10, 12, 15], kv)
+    assert got == [-1, new[0], -1, new[1], -1, -1, new[2]]
+    flagged()
+    want = kvcache.PagedCache(kv.to(dev), rows, width, meta=m.meta().to(dev))
+    for at, page in bad.items():
+        want.tables[at] = page
+    assert torch.equal(c.meta, want.meta) and torch.equal(raw(c.kv), raw(kv))
+
+
+def test_fork_of_long_tables(dev):
+    # some 300 samples of rows of up to 64 pages, one of no tokens among their prompts
+    r = np.random.RandomState(3)
+    P, S, rows, width = 5000, 4, 300, 64
+    m = Lists(P, S, rows, width)
+    order = [int(p) for p in r.permutation(P)]
+    for b in range(8):
+        n = int(r.randint(1, width * S + 1))
+        m.rows[b], m.lens[b] = [order.pop() for _ in range(-(-n // S))], n
+        for p in m.rows[b]:
+            m.refs[p] = 1
+    kv = torch.randint(0, 1000, (1, 2, P, 1, S, 8), dtype=torch.int16).view(torch.float16)
+    c = kvcache.PagedCache(kv.to(dev), rows, width, meta=m.meta().to(dev))
+    src, dst = [j % 9 for j in range(291)], [8 + j for j in range(291)]
+    src = [8 + 291 if s == 8 else s for s in src]  # (an empty prompt)
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+    assert c.fork(t(src), t(dst)).tolist() == m.fork(src, dst, kv)
+    same(c, m, kv)
+    moe.device_error()

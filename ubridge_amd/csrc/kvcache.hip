@@ -74,15 +74,36 @@ __global__ void __launch_bounds__(256) k_free(int* __restrict__ refs, int* __res
   if (threadIdx.x == 0) lens[r] = 0;
 }
 
+// Workgroup j: len[j], tokens of sample j, and old[j], the page to copy for it (-1:
+// none).  A sample of a row that is not there, or of a table with a page in use that
+// is not there, is refused: -1 tokens.  (A launch of its own, about 2 us: the
+// planning workgroup took as long for 4096 entries and 8 us for 16384.)
+__global__ void __launch_bounds__(256) k_fork_check(const int* __restrict__ lens,
+                                                    const int* __restrict__ tables,
+                                                    const int* __restrict__ src,
+                                                    const int* __restrict__ dst, int* len, int* old,
+                                                    int P, int S, int nrows, int width, int* err) {
+  const int j = blockIdx.x, s = src[j], d = dst[j];
+  const int m = s >= 0 && s < nrows && d >= 0 && d < nrows ? lens[s] : -1;
+  int bad = m < 0 || m > (long)width * S;
+  if (!bad)
+    for (int i = threadIdx.x; i < width; i += 256) {
+      const int p = tables[(size_t)s * width + i];
+      if (m > 0 && i <= (m - 1) / S) bad |= p < 0 || p >= P;
+    }
+  bad = __syncthreads_or(bad);
+  if (threadIdx.x != 0) return;
+  len[j] = bad ? -1 : m;
+  old[j] = bad || m % S == 0 ? -1 : tables[(size_t)s * width + m / S];
+  if (bad) *err = UB_ERR_INDEX;
+}
+
 // One workgroup: who gets which new page.  plan: [n] tokens of the sample (-1:
 // refused), [n] page to copy, [n] free pages found.  newp [n]: the sample's
 // own page, -1 where it has none.
 __global__ void __launch_bounds__(PT) k_fork_plan(const int* __restrict__ refs, int* lens,
-                                                  const int* __restrict__ tables,
-                                                  const int* __restrict__ src,
                                                   const int* __restrict__ dst, int n, int* newp,
-                                                  int* plan, int P, int S, int nrows, int width,
-                                                  int* err) {
+                                                  int* plan, int P, int* err) {
   __shared__ int lds[PT / 64];
   __shared__ int near[kNear];  // the first free pages, which is mostly all of them
   const int tid = threadIdx.x;
@@ -100,44 +121,23 @@ __global__ void __launch_bounds__(PT) k_fork_plan(const int* __restrict__ refs, 
     }
   };
   counts(16 * tid);
-  // lengths first: a row may be a prompt here and a sample there only if empty
-  for (int j = tid; j < n; j += PT) {
-    const int s = src[j], d = dst[j];
-    int m = -1;
-    if (s >= 0 && s < nrows && d >= 0 && d < nrows) m = lens[s];
-    if (m < 0 || m > (long)width * S) {
-      m = -1;
-      *err = UB_ERR_INDEX;
-    }
-    len[j] = m;
-  }
-  __syncthreads();
   int need = 0;
   for (int j0 = 0; j0 < n; j0 += PT) {
     const int j = j0 + tid;
-    int part = 0, page = -1;
+    int part = 0;
     if (j < n && len[j] >= 0) {
       const int m = len[j], d = dst[j];
-      if (m % S != 0) page = tables[(size_t)src[j] * width + m / S];
       // the row must be empty; the claim gives it to one sample
       if (m == 0 ? lens[d] != 0 : atomicCAS(&lens[d], 0, m) != 0) {
-        len[j] = page = -1;
+        len[j] = -1;
         *err = UB_ERR_INDEX;
-      } else if (m % S != 0) {
-        part = page >= 0 && page < P;
-        if (!part) {
-          lens[d] = 0;
-          len[j] = page = -1;
-          *err = UB_ERR_INDEX;
-        }
+      } else {
+        part = old[j] >= 0;
       }
     }
     int sum;
     const int k = block_scan(part, lds, sum);
-    if (j < n) {
-      old[j] = page;
-      newp[j] = part ? need + k : -1;  // the rank, until the pages are known
-    }
+    if (j < n) newp[j] = part ? need + k : -1;  // the rank, until the pages are known
     need += sum;
   }
   int have = 0;
@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(256) k_fork(uint8_t* kv, int* refs, int* table
                                               const int* __restrict__ dst,
                                               const int* __restrict__ newp,
                                               const int* __restrict__ plan, int n, int P, int S,
-                                              int width, long page_bytes, int slices, int* err) {
+                                              int width, long page_bytes, int slices) {
   const int j = blockIdx.y, m = plan[j];
   if (m <= 0) return;
   const int np = newp[j];
@@ -219,8 +219,7 @@ __global__ void __launch_bounds__(256) k_fork(uint8_t* kv, int* refs, int* table
     for (int i = threadIdx.x; i < pages; i += 256) {
       const int p = np >= 0 && i == pages - 1 ? np : from[i];
       to[i] = p;
-      if (p >= 0 && p < P) atomicAdd(&refs[p], 1);
-      else *err = UB_ERR_INDEX;
+      atomicAdd(&refs[p], 1);
     }
   }
   if (np < 0) return;
@@ -383,14 +382,14 @@ UB_API int ubridge_kv_fork(const UbridgeKvPool* p, const int32_t* src, const int
   UbScratch ws(s, sizeof(int) * 3 * (size_t)n);
   int* plan = (int*)ws.get();
   if (!plan) return ub_set_error(UB_ERR_LAUNCH, "%s: no workspace", nm);
-  k_fork_plan<<<1, PT, 0, s>>>(p->refs, p->lens, p->tables, src, dst, n, new_pages, plan, p->P,
-                               p->S, p->rows, p->width, err);
+  k_fork_check<<<n, 256, 0, s>>>(p->lens, p->tables, src, dst, plan, plan + n, p->P, p->S, p->rows, p->width, err);
+  k_fork_plan<<<1, PT, 0, s>>>(p->refs, p->lens, dst, n, new_pages, plan, p->P, err);
   const int b = unit_bytes(p->kv, p->page_bytes);
   const int slices = (int)(p->page_bytes / 32768 > 0 ? p->page_bytes / 32768 : 1);
   const dim3 grid(2 * p->L * slices, n);
 #define UB_GO(B)                                                                                 \
   k_fork<B><<<grid, 256, 0, s>>>((uint8_t*)p->kv, p->refs, p->tables, src, dst, new_pages, plan, \
-                                 n, p->P, p->S, p->width, p->page_bytes, slices, err)
+                                 n, p->P, p->S, p->width, p->page_bytes, slices)
   if (b == 16) UB_GO(16);
   else if (b == 8) UB_GO(8);
   else if (b == 4) UB_GO(4);

@@ -101,8 +101,9 @@ class PagedCache:
         """Empty rows dst (int32 [n], all different) become samples of rows src:
         whole pages are shared, a part-filled last page is copied to the lowest
         free page.  Returns int32 [n], the new page or -1.  A row that is not
-        empty or not there, or for which no page is left, keeps its state, gives
-        -1 and raises the flag that moe.device_error() reads."""
+        empty or not there, for which no page is left, or whose prompt has a
+        page that is not there, keeps its state, gives -1 and raises the flag
+        that moe.device_error() reads."""
         return call(_native.fork, stream, self.kv, self.meta, self.rows, self.width, src, dst)
 
     def compact(self, stream=None):
