@@ -481,7 +481,7 @@ int ubridge_paged_decode(const UbridgePagedDecodeArgs* args, void* stream);
  * int32 [P] and listed by tables int32 [rows, width] (-1: none) with lens int32
  * [rows] tokens, S to a page.  All state stays on the device.
  * free: the rows named lose their pages and become empty.
- * fork: row dst[i], empty, becomes a sample of row src[i]: whole pages are
+ * fork: row dst[i], empty (no tokens, no pages), becomes a sample of row src[i]: whole pages are
  * shared, a part-filled last page is copied to the lowest free page, in the
  * order of i; new_pages[i] receives it, else -1.  Rows dst differ; a row that is
  * not empty, out of range or for which no page is left, or whose prompt's table

@@ -342,3 +342,40 @@ def test_fork_of_long_tables(dev):
     assert c.fork(t(src), t(dst)).tolist() == m.fork(src, dst, kv)
     same(c, m, kv)
     moe.device_error()
+
+
+def test_fork_into_a_row_that_holds_a_page(dev):
+    # a row without tokens that was given its pages ahead is not empty: it keeps
+    # them, and no page is lost to the pool
+    P, S, rows, width = 12, 4, 6, 70
+    m = Lists(P, S, rows, width)
+    m.rows[0], m.lens[0] = [2, 5], 6
+    m.rows[1], m.rows[2] = [7], [8, 9]  # (no tokens)
+    for p in (2, 5, 7, 8, 9):
+        m.refs[p] = 1
+    kv = torch.randn(1, 2, P, 1, S, 8).half()
+    c = kvcache.PagedCache(kv.to(dev), rows, width, meta=m.meta().to(dev))
+    c.tables[2, :2] = torch.tensor([-1, 8], device=dev)  # one page, not the first
+    m.refs[9], m.rows[2] = 0, []
+    c.refs[9] = 0
+    moe.device_error()
+    t = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)
+
+    def state():
+        meta = m.meta()
+        meta[P + rows + 2 * width + 1] = 8 if m.refs[8] else -1
+        return meta
+    assert c.fork(t(0, 0, 0), t(1, 2, 3)).tolist() == [-1, -1] + m.fork([0], [3], kv)
+    assert torch.equal(c.meta.cpu(), state()) and torch.equal(raw(c.kv), raw(kv))
+    flagged()
+    # a prompt of no tokens leaves such a row as it is
+    assert c.fork(t(4), t(1)).tolist() == [-1]
+    assert torch.equal(c.meta.cpu(), state())
+    moe.device_error()
+    # freed, it is empty
+    c.free(t(1, 2))
+    m.free([1])
+    m.refs[8] = 0
+    assert c.fork(t(0, 3), t(2, 1)).tolist() == m.fork([0, 3], [2, 1], kv)
+    same(c, m, kv)
+    moe.device_error()

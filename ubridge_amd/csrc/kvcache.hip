@@ -75,8 +75,8 @@ __global__ void __launch_bounds__(256) k_free(int* __restrict__ refs, int* __res
 }
 
 // Workgroup j: len[j], tokens of sample j, and old[j], the page to copy for it (-1:
-// none).  A sample of a row that is not there, or of a table with a page in use that
-// is not there, is refused: -1 tokens.  (A launch of its own, about 2 us: the
+// none).  A sample of a row that is not there, of a table with a page in use that is
+// not there, or in a row that holds a page is refused: -1 tokens.  (A launch of its own, about 2 us: the
 // planning workgroup took as long for 4096 entries and 8 us for 16384.)
 __global__ void __launch_bounds__(256) k_fork_check(const int* __restrict__ lens,
                                                     const int* __restrict__ tables,
@@ -88,8 +88,8 @@ __global__ void __launch_bounds__(256) k_fork_check(const int* __restrict__ lens
   int bad = m < 0 || m > (long)width * S;
   if (!bad)
     for (int i = threadIdx.x; i < width; i += 256) {
-      const int p = tables[(size_t)s * width + i];
-      if (m > 0 && i <= (m - 1) / S) bad |= p < 0 || p >= P;
+      const int p = tables[(size_t)s * width + i], own = tables[(size_t)d * width + i];
+      if (m > 0) bad |= own >= 0 || (i <= (m - 1) / S && (p < 0 || p >= P));
     }
   bad = __syncthreads_or(bad);
   if (threadIdx.x != 0) return;
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(PT) k_fork_plan(const int* __restrict__ refs, 
     int part = 0;
     if (j < n && len[j] >= 0) {
       const int m = len[j], d = dst[j];
-      // the row must be empty; the claim gives it to one sample
+      // the row must have no tokens; the claim gives it to one sample
       if (m == 0 ? lens[d] != 0 : atomicCAS(&lens[d], 0, m) != 0) {
         len[j] = -1;
         *err = UB_ERR_INDEX;

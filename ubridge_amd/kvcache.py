@@ -98,8 +98,8 @@ class PagedCache:
         call(_native.free, stream, self.kv, self.meta, self.rows, self.width, rows)
 
     def fork(self, src, dst, stream=None):
-        """Empty rows dst (int32 [n], all different) become samples of rows src:
-        whole pages are shared, a part-filled last page is copied to the lowest
+        """Empty rows dst (int32 [n], all different, without tokens or pages)
+        become samples of rows src: whole pages are shared, a part-filled last page is copied to the lowest
         free page.  Returns int32 [n], the new page or -1.  A row that is not
         empty or not there, for which no page is left, or whose prompt has a
         page that is not there, keeps its state, gives -1 and raises the flag
