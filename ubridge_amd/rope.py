@@ -6,6 +6,7 @@ reaches without a table of sines; the rotation is f32."""
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from .native import _native, call
 
@@ -71,8 +72,9 @@ class Rope:
 
     rope(q, k, positions) -> [q', k'] for q [T, Hq, D], k [T, Hkv, D] (f32, f16
     or bf16, any token and head strides) and positions int32 or int64 [T].  k
-    may be None.  It is differentiable; backward(dq, dk, positions) is the
-    gradient by itself, the inverse turn.
+    may be None.  backward(dq, dk, positions) is the gradient by itself, the
+    inverse turn.  Both are differentiable, any number of times and in forward
+    mode: they are linear in q and k.
     """
 
     def __init__(self, rot, base=10000.0, interleaved=False, scaling=None, device="cuda"):
@@ -87,28 +89,56 @@ class Rope:
         return call(_native.rope, stream, q, k, positions, self.turns, self.rot, self.interleaved,
                     self.factor, inverse)
 
+    def _turn(self, q, k, positions, inverse, stream):
+        if _level() >= 0 or torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+            return list(_Turn.apply(q, k, positions, self, inverse, stream))
+        return self._run(q, k, positions, inverse, stream)
+
     def forward(self, q, k, positions, stream=None):
-        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-            return list(_Turn.apply(q, k, positions, self, stream))
-        return self._run(q, k, positions, False, stream)
+        return self._turn(q, k, positions, False, stream)
 
     __call__ = forward
 
     def backward(self, dq, dk, positions, stream=None):
         """The gradients of q and k from those of the turned ones."""
-        return self._run(dq, dk, positions, True, stream)
+        return self._turn(dq, dk, positions, True, stream)
+
+
+def _level():
+    return forward_ad._current_level  # (-1: not in forward mode)
+
+
+def _stored(d):
+    """A gradient or tangent that the kernel can read: expanded ones, and zeros
+    that have no memory, written out."""
+    if d is None or d.stride(-1) == 1 and not d._is_zerotensor():
+        return d
+    return torch.zeros(d.shape, dtype=d.dtype, device=d.device) if d._is_zerotensor() else d.contiguous()
 
 
 class _Turn(torch.autograd.Function):
+    """The turn, or the inverse one: each is the other's gradient, and its own
+    derivative along q and k."""
+
     @staticmethod
-    def forward(ctx, q, k, positions, rope, stream):
+    def forward(q, k, positions, rope, inverse, stream):
+        return tuple(rope._run(q, k, positions, inverse, stream))
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        _, k, positions, ctx.rope, ctx.inverse, _ = inputs
         ctx.save_for_backward(positions)
-        ctx.rope = rope
-        return tuple(rope._run(q, k, positions, False, stream))
+        ctx.save_for_forward(positions)
+        ctx.keys = k is not None
 
     @staticmethod
     def backward(ctx, dq, dk):
         (positions,) = ctx.saved_tensors
-        dq, dk = (None if d is None else d if d.stride(-1) == 1 else d.contiguous() for d in (dq, dk))
-        dq, dk = ctx.rope._run(dq, dk, positions, True, None)
-        return dq, dk, None, None, None
+        dq, dk = ctx.rope._turn(_stored(dq), _stored(dk), positions, not ctx.inverse, None)
+        return dq, dk, None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, q, k, *_):
+        (positions,) = ctx.saved_tensors
+        k = _stored(k) if ctx.keys else None
+        return tuple(ctx.rope._turn(_stored(q), k, positions, ctx.inverse, None))
