@@ -172,3 +172,8 @@ def test_a_copied_cache_works_on_its_own_memory(monkeypatch, how):
     assert other.meta.tolist() == [0, 5, 0, 0, 0, 0, 6] + [-1] * 5 + [7]
     assert c.meta.tolist() == [0] * 7 + [-1] * 6
     assert (c.P, c.rows, c.width) == (other.P, other.rows, other.width)
+
+
+def test_operators_without_a_gradient_say_so():
+    for what in (attention.paged_decode, kvcache.PagedCache.append, kvcache.PagedCache.attend, int8):
+        assert "no gradient" in " ".join(what.__doc__.split()), what

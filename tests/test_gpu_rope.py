@@ -222,3 +222,13 @@ def test_append_refusals(dev):
             c.append(**args)
     assert c.append(0, k[:0], k[:0], k[:0], s[:0], positions=s[:0], rope=r).shape == (0, 2, 16)
     assert not bool(kv.any())
+
+
+def test_append_has_no_gradient(dev):
+    kv = torch.zeros(1, 2, 4, 1, 8, 16, device=dev, dtype=torch.bfloat16)
+    c = kvcache.PagedCache(kv, rows=1, width=4)
+    q, k, v = (torch.ones(2, 1, 16, device=dev, dtype=torch.bfloat16, requires_grad=True) for _ in "qkv")
+    slots = torch.arange(2, device=dev)
+    assert not c.append(0, q, k, v, slots, slots, rope.Rope(16)).requires_grad
+    assert not c.kv.requires_grad
+    assert c.append(0, q, k, v, slots) is q  # without a rotation q is not touched

@@ -79,7 +79,9 @@ class PagedCache:
         negative: nowhere; no slot twice) and return q.  With a Rope and
         positions q and k are turned, in one launch with the store.  e4m3 pages
         take x / scale, saturating.  A slot past the cache raises the flag that
-        moe.device_error() reads."""
+        moe.device_error() reads.  It has no gradient: what is stored, and a turned
+        q, is cut from the graph of k, v and q (rope.Rope by itself is
+        differentiable)."""
         turns, rot, inter, factor = (None, 0, False, 1.0) if rope is None else (
             rope.turns, rope.rot, rope.interleaved, rope.factor)
         return call(_native.append, stream, self.kv, layer, self.k_scale, self.v_scale, q, k, v, slots,
@@ -87,7 +89,7 @@ class PagedCache:
 
     def attend(self, layer, q, tables=None, lens=None, **kw):
         """attention.paged_decode of q [B, Hq, D] over a layer, for all rows or
-        for the rows whose tables and lens are given."""
+        for the rows whose tables and lens are given.  It has no gradient."""
         k, v = self.layer(layer)
         return paged_decode(q, k, v, self.tables if tables is None else tables,
                             self.lens if lens is None else lens, k_scale=self.k_scale,
