@@ -698,10 +698,8 @@ void decode(const Dev& d, hipStream_t s) {
     return;
   }
   constexpr int NW = kRowWaves<DK, HT>;
-  static const hipError_t once =  // (beyond 64 KiB)
-      hipFuncSetAttribute((const void*)k_decode<DT, CT, DK, PG8, HT, true>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                          NW * 16 * HT * (32 * DK + 4) * (int)sizeof(float));
-  (void)once;
+  static UbLdsLimit limit;
+  limit.raise((const void*)k_decode<DT, CT, DK, PG8, HT, true>, NW * 16 * HT * (32 * DK + 4) * (int)sizeof(float));
   const size_t lds = sizeof(float) * NW * (d.G < 16 * HT ? d.G : 16 * HT) * (d.a.D + 4);
   k_decode<DT, CT, DK, PG8, HT, true><<<d.a.B * d.a.Hkv * d.HG, 64 * NW, lds, s>>>(d);
 }

@@ -5,6 +5,7 @@
 #include <hip/hip_fp16.h>
 #include <stdint.h>
 #include <stddef.h>
+#include <atomic>
 #include "../../include/ubridge_hip.h"  // definitions below must match the public ABI
 
 #define UB_API extern "C" __attribute__((visibility("default")))
@@ -82,6 +83,24 @@ class UbRelaxCapture {
 
  private:
   hipStreamCaptureMode m_ = hipStreamCaptureModeRelaxed;
+};
+
+// Raises kernel f's limit of dynamic LDS to `bytes`, once on each device (a call of
+// every launch's own costs the runtime's lookup of the kernel).  A static object a
+// kernel; beyond 64 devices, at every launch.
+class UbLdsLimit {
+ public:
+  void raise(const void* f, int bytes) {
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return;  // (the launch reports it)
+    const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+    if (done_.load(std::memory_order_acquire) & bit) return;
+    if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess)
+      done_.fetch_or(bit, std::memory_order_release);
+  }
+
+ private:
+  std::atomic<uint64_t> done_{0};
 };
 
 #define UB_REQUIRE(cond, ...)                                   \

@@ -637,9 +637,8 @@ size_t dec_lds(int M, int ld) { return sizeof(int) * (DW * M * 17 + 16 + 32 * kD
 template <int DT, int SP>
 void dec(const void* x, const int8_t* w, const float* sw, const float* bias, void* y, int M, int K, int N, int ld,
          hipStream_t s) {
-  static const hipError_t once =  // (beyond 64 KiB)
-      hipFuncSetAttribute((const void*)k_i8_dec<DT, SP>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-  (void)once;
+  static UbLdsLimit limit;
+  limit.raise((const void*)k_i8_dec<DT, SP>, kLds);
   const int nt = ub_cdiv(N, 16);
   k_i8_dec<DT, SP><<<nt < 256 ? nt : 256, 64 * DW, dec_lds(M, ld), s>>>(x, w, sw, bias, y, M, K, N, ld);
 }
@@ -704,9 +703,8 @@ void gemm(Plan plan, const int8_t* q, const float* sa, const int8_t* w, const fl
 #define UB_TILE(WM, WN, TM, TN, NS)                                                                      \
   {                                                                                                      \
     constexpr int lds = NS * 64 * 32 * (WM * TM + WN * TN);                                              \
-    static const hipError_t once = hipFuncSetAttribute((const void*)k_i8_gemm<DT, WM, WN, TM, TN, NS>,   \
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds); \
-    (void)once;                                                                                          \
+    static UbLdsLimit limit;                                                                             \
+    limit.raise((const void*)k_i8_gemm<DT, WM, WN, TM, TN, NS>, lds);                                    \
     const int tiles = ub_cdiv(M, 32 * WM * TM) * ub_cdiv(N, 32 * WN * TN), rest = tiles % 256;           \
     const int full = TM > 1 && tiles > 256 && rest <= 128 ? tiles - rest : tiles;                        \
     k_i8_gemm<DT, WM, WN, TM, TN, NS><<<2 * tiles - full, 64 * WM * WN, lds, s>>>(q, sa, w, sw, bias, y, M, N, ld, full); \
@@ -715,9 +713,8 @@ void gemm(Plan plan, const int8_t* q, const float* sa, const int8_t* w, const fl
 #define UB_RING(WM, WN, TM, TN, NS)                                                                      \
   {                                                                                                      \
     constexpr int lds = NS * 128 * 32 * (WM * TM + WN * TN);                                             \
-    static const hipError_t once = hipFuncSetAttribute((const void*)k_i8_ring<DT, WM, WN, TM, TN, NS>,   \
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds); \
-    (void)once;                                                                                          \
+    static UbLdsLimit limit;                                                                             \
+    limit.raise((const void*)k_i8_ring<DT, WM, WN, TM, TN, NS>, lds);                                    \
     k_i8_ring<DT, WM, WN, TM, TN, NS><<<ub_cdiv(M, 32 * WM * TM) * ub_cdiv(N, 32 * WN * TN) * ub_cdiv(ld / 128, part), \
                                         64 * WM * WN, lds, s>>>(q, sa, w, sw, bias, y, M, N, ld, part);  \
     return;                                                                                              \
