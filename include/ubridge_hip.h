@@ -457,9 +457,9 @@ int ubridge_rope_append(const UbridgeRopeArgs* args, void* stream);
  * [P, Hkv, S, D] of q's type or e4m3 (cache_dtype 3), strides in elements of sp
  * per page, sh per head and ss per slot; tables int32 [B, width], table_stride
  * apart, lens int32 [B].  Query head i reads kv head i / (Hq / Hkv).  scale is
- * the factor on q . k, softcap c > 0 makes a score c tanh(x / c), slopes f32
- * [Hq] add slope (t - (len - 1)), window > 0 keeps the last window tokens,
- * k_scale / v_scale f32 [Hkv] multiply the stored values (each may be NULL).
+ * the factor on q . k, softcap c > 0 (finite, not denormal) makes a score c tanh(x /
+ * c), slopes f32 [Hq] add slope (t - (len - 1)), window > 0 keeps the last window
+ * tokens, k_scale / v_scale f32 [Hkv] multiply the stored values (each may be NULL).
  * D is a multiple of 8 up to 256.  A sequence of length 0 gives zeros and lse
  * -inf.  A length past width S is cut, a page outside [0, P) gives NaN; both
  * raise the flag of ubridge_device_error.  Scratch: where a sequence is split,

@@ -177,3 +177,10 @@ def test_a_copied_cache_works_on_its_own_memory(monkeypatch, how):
 def test_operators_without_a_gradient_say_so():
     for what in (attention.paged_decode, kvcache.PagedCache.append, kvcache.PagedCache.attend, int8):
         assert "no gradient" in " ".join(what.__doc__.split()), what
+
+
+def test_paged_decode_refuses_an_infinite_cap():
+    # c tanh(x / c) has no value there (it came out as NaN everywhere); 0 is no cap
+    call = lambda **kw: lib.ubridge_paged_decode(DECODE_ARGS.pack(*dict(DECODE, **kw).values()), None)
+    refused(call(cap=float("inf")), 1, b"softcap")
+    refused(call(cap=1e-39), 1, b"softcap")

@@ -390,3 +390,14 @@ def test_infinite_value_of_small_weight(dev, t, n, newest):
     out = attention.paged_decode(q, kv[0], kv[1], tables, lens, slopes=slopes)
     assert bool((out[..., :8] == math.inf).all() and (out[..., 8:16] == -math.inf).all())
     assert bool(torch.isfinite(out[..., 16:]).all())
+
+
+def test_caps_at_the_ends_of_the_range(dev):
+    q, kv, tables, n = make(dev, [40, 33], 4, 2, 64, 16, "bf16")
+    run = lambda cap: attention.paged_decode(q, kv[0], kv[1], tables, n, softcap=cap, return_lse=True)
+    for cap in (math.inf, 1e300, 1e-39, 1e-60):
+        with pytest.raises(ValueError, match="softcap"):
+            run(cap)
+    for cap in (1e-30, 1e-3, 1e6, 1e30):
+        out, lse = run(cap)
+        check(out, q, kv, tables, n, lse, softcap=cap if cap < 1e6 else 0.0)

@@ -10,6 +10,8 @@
 // attention.py, rope.py, kvcache.py and int8.py hand over (bind) from the library
 // they have loaded.
 #include <Python.h>
+#include <cfloat>
+#include <cmath>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -147,7 +149,9 @@ PyObject* py_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const double cap = A.f(6), scale = args[5] == Py_None ? 1.0 / std::sqrt((double)D) : A.f(5);
   const long window = A.n(7);
   if (PyErr_Occurred()) return nullptr;
-  if (window < 0 || !(cap >= 0)) REFUSE("paged_decode: window=%ld, softcap (at least 0)", window);
+  const float fcap = (float)cap;
+  if (window < 0 || !(cap == 0 || (fcap >= FLT_MIN && fcap <= FLT_MAX)))
+    REFUSE("paged_decode: window=%ld (at least 0), softcap (0, or a float32 above it)", window);
   if (!vec(slopes, Hq)) REFUSE("paged_decode: slopes must be contiguous float32 [%ld]", Hq);
   if (!vec(ks, Hkv) || !vec(vs, Hkv)) REFUSE("paged_decode: k_scale and v_scale must be contiguous float32 [%ld]", Hkv);
   if (out && (out->sizes() != q->sizes() || out->scalar_type() != q->scalar_type() || !dense(*out)))
@@ -167,7 +171,7 @@ PyObject* py_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   p.table_stride = tables->stride(0);
   p.B = B, p.Hq = Hq, p.Hkv = Hkv, p.D = D, p.S = S, p.P = P, p.width = width;
   p.window = window > 0x7fffffff ? 0x7fffffff : (int)window;
-  p.dtype = dt, p.cache_dtype = ct, p.scale = (float)scale, p.softcap = (float)cap;
+  p.dtype = dt, p.cache_dtype = ct, p.scale = (float)scale, p.softcap = fcap;
   void* stream = A.p(13);
   if (PyErr_Occurred()) return nullptr;
   if (const int rc = fn.decode(&p, stream)) return PyLong_FromLong(rc);

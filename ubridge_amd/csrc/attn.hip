@@ -753,7 +753,8 @@ UB_API int ubridge_paged_decode(const UbridgePagedDecodeArgs* p, void* stream) {
   UB_REQUIRE(a.D > 0 && a.D % 8 == 0 && a.D <= 256, "%s: D=%d (a multiple of 8, at most 256)", nm, a.D);
   UB_REQUIRE(a.S > 0 && a.P >= 0 && a.width >= 0 && (int64_t)a.width * a.S <= 0x7fffffc0,
              "%s: S=%d P=%d width=%d", nm, a.S, a.P, a.width);
-  UB_REQUIRE(a.window >= 0 && a.softcap >= 0.f, "%s: window=%d softcap=%g", nm, a.window, a.softcap);
+  UB_REQUIRE(a.window >= 0 && (a.softcap == 0.f || (a.softcap >= 0x1p-126f && a.softcap < kInf)),
+             "%s: window=%d softcap=%g (0, or normal and finite)", nm, a.window, a.softcap);
   if (a.B == 0 || a.Hq == 0) return UB_OK;
   UB_REQUIRE(a.q && a.out && a.lens && (a.tables || a.width == 0), "%s: null pointer", nm);
   UB_REQUIRE(a.P == 0 || (a.k_pages && a.v_pages), "%s: null pages", nm);
