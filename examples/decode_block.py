@@ -39,17 +39,24 @@ class Block:
 
 def grow(cache, rows):
     """A place for one more token of each row (all different): (positions,
-    slots).  A row whose pages are full gets the lowest free one."""
+    slots).  A row whose pages are full gets the lowest free one.  Where none is
+    left, or the row has its width of pages, the slot is negative (the token is
+    stored nowhere) and attention reports the row."""
     r = rows.long()
     at = cache.lens[r].long()
+    full = at >= cache.width * cache.S
     i = (at // cache.S).clamp(max=cache.width - 1)
-    need = at % cache.S == 0
-    free = torch.argsort((cache.refs != 0).int(), stable=True)
-    page = torch.where(need, free[(torch.cumsum(need, 0) - 1).clamp(min=0)].int(), cache.tables[r, i])
+    need = (at % cache.S == 0) & ~full
+    used = cache.refs != 0
+    rank = torch.cumsum(need, 0) - 1
+    got = need & (rank < (~used).sum())
+    free = torch.argsort(used.int(), stable=True)[rank.clamp(0, len(used) - 1)].int()
+    held = cache.tables[r, i]
+    page = torch.where(need, torch.where(got, free, -1), held)
     cache.tables[r, i] = page
-    cache.refs.index_add_(0, page.long(), need.int())
+    cache.refs.index_add_(0, page.clamp(min=0).long(), got.int())
     cache.lens[r] += 1
-    return at, page.long() * cache.S + at % cache.S
+    return at, torch.where(full | (page < 0), -1, page.long() * cache.S + at % cache.S)
 
 
 def step(blocks, x, cache, turn, rows):
