@@ -30,11 +30,11 @@
 //    are no shares and one launch (ROW).
 //
 // us of the kernels: 4 sequences of 100003 tokens, 8 kv heads of 128 in bf16 (1.64
-// GB) 273 + 8 (6.0 TB/s); 64 sequences of up to 4096 (118 MB) 26 + 5.9; 24 of up
-// to 6000 under a window of 2048, 16 e4m3 heads of 80 (43 MB) 14 + 5.4, where
-// half the time is latency and the softmax of one head in sixteen columns; one of
-// 700 tokens 6.8 + 5.3, all latency: the search for the share, the page, the row,
-// then the join's own reads.
+// GB) 283 + 8 (5.8 TB/s); 64 sequences of up to 4096 (118 MB) 26 + 5.8, where a row's
+// first loads wait for the last one's sums; 24 of up to 6000 under a window of 2048,
+// 16 e4m3 heads of 80 (43 MB) 14 + 5.3, where half the time is latency and the
+// softmax of one head in sixteen columns; one of 700 tokens 6.9 + 4.8, all latency:
+// the search for the share, the page, the row, then the join's own reads.
 //
 // Numerics.  Scores, the running maximum and sum, and the output's sum are f32.
 // The weights exp(x - m) enter the second product as the sum of two 16-bit

@@ -13,13 +13,13 @@
 //
 // Up to 16 tokens (of 64 KiB in all) the product is a stream of the weight and one
 // kernel does it all (k_i8_dec); beyond, k_quant makes the codes and k_i8_gemm (or k_i8_ring, by
-// plan_for) multiplies them.  us: 8 x 4096 x 6144 (M x K x N) 10.8, of which the
-// weight's 25 MB are 5 and the rest is the launch, the activations' codes ahead of
+// plan_for) multiplies them.  us: 8 x 4096 x 6144 (M x K x N) 10.7, of which the
+// weight's 25 MB are 4 and the rest is the launch, the activations' codes ahead of
 // the first product and the sum over the wavefronts; 8 x 4096 x 28672 26 (4.5 TB/s);
-// 201 x 3520 x 9001 4 + 18, bound by a tile's K-steps (0.55 us each, of which 0.2
-// are products); 4096 x 4096 x 14336 10 + 250 (1.9 POP/s, 2.1 on 4096 x 8192 x 8192,
-// where the library's own int8 product of 8192^3 reaches 2.1): bound by power --
-// the same products of zeros run at 3.0.
+// 201 x 3520 x 9001 4 + 19, bound by a tile's K-steps (0.55 us each, of which 0.2
+// are products); 4096 x 4096 x 14336 10 + 243 (2.0 POP/s, 2.3 on 4096 x 8192 x 8192,
+// where the library's own int8 product reaches 2.5); power is a part of it: with
+// operands of zeros the call takes 0.7 of the time.
 #include "common.h"
 #include "lds_dma.h"
 

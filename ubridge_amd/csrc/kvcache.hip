@@ -14,9 +14,9 @@
 //          free page below n; tables and counts follow
 //
 // free and the planning of fork and compact touch a few hundred KiB and are
-// bound by latency (us: free 3, fork's plan 5.5, compact's 3.5); the page copies
-// are bound by HBM, with eight 16-byte loads in flight a thread: 507 pages of 512
-// KiB (530 MB in and out) 109 us, 4.9 TB/s (four in flight 119).  Non-temporal
+// bound by latency (us: free 3.1, fork's check 3.4 and plan 4.7, compact's plan 4.9);
+// the page copies are bound by HBM, with eight 16-byte loads in flight a thread: 507
+// pages of 512 KiB (530 MB in and out) 109 us, 4.9 TB/s (four in flight 119).  Non-temporal
 // access was 4% faster there and 40% slower on fork, whose pages stay in the
 // last-level cache for the attention that reads them next.
 #include "common.h"
@@ -76,8 +76,9 @@ __global__ void __launch_bounds__(256) k_free(int* __restrict__ refs, int* __res
 
 // Workgroup j: len[j], tokens of sample j, and old[j], the page to copy for it (-1:
 // none).  A sample of a row that is not there, of a table with a page in use that is
-// not there, or in a row that holds a page is refused: -1 tokens.  (A launch of its own, about 2 us: the
-// planning workgroup took as long for 4096 entries and 8 us for 16384.)
+// not there, or in a row that holds a page is refused: -1 tokens.  (A launch of its
+// own, 2 us more of a graph: the planning workgroup took as long for 4096 entries
+// and 8 us for 16384.)
 __global__ void __launch_bounds__(256) k_fork_check(const int* __restrict__ lens,
                                                     const int* __restrict__ tables,
                                                     const int* __restrict__ src,
@@ -410,7 +411,8 @@ UB_API int ubridge_kv_compact(const UbridgeKvPool* p, int32_t* n_used, void* str
   int* plan = (int*)ws.get();
   if (!plan) return ub_set_error(UB_ERR_LAUNCH, "%s: no workspace", nm);
   int* map = plan + 2 * (p->P / 2) + 1;
-  // four pages a thread up to 4096: 2048 pages take 3.6 us, 6.6 with sixteen
+  // four pages a thread up to 4096: 2048 pages take 4.9 us (the least of 30 4.0), 5.0
+  // (4.9) with sixteen
   if (p->P <= 4 * PT) k_compact_plan<4><<<1, PT, 0, s>>>(p->refs, p->P, plan, map, n_used);
   else k_compact_plan<16><<<1, PT, 0, s>>>(p->refs, p->P, plan, map, n_used);
   const int b = unit_bytes(p->kv, p->page_bytes);

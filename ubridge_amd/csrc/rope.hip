@@ -22,8 +22,8 @@
 // sine and cosine a pair and token, made by 64 lanes at once and dealt out
 // through LDS, then in registers for all heads.  HBM-bound: the next head's loads
 // are in flight while one is turned, in many wavefronts a SIMD.  8192 tokens of 40
-// heads of 128 in bf16, 168 MB in and out: 33 us (5.1 TB/s, where a copy reaches
-// 5.2); 32 tokens stored into a cache 4.5 us, which is latency.
+// heads of 128 in bf16, 168 MB in and out: 31 us (5.4 TB/s, where copies reach 5.2
+// to 5.5); 32 tokens stored into a cache 4.2 us, which is latency.
 #include "common.h"
 
 namespace {
@@ -165,7 +165,7 @@ struct Two { uint4 a, b; };
 
 // CT: the cache's type (DT or UB_E4M3), -1 without a cache.  WHOLE: every run is
 // whole units (without the code for other runs the kernel needs 20 registers
-// less: 8192 tokens of 40 heads of 128 36.9 us, in the general form 39.7).
+// less: 8192 tokens of 40 heads of 128 36.9 us a call, in the general form 39.7).
 template <int DT, bool INTER, int CT, bool WHOLE>
 __global__ void __launch_bounds__(64 * NW) k_rope(const RopeDev d) {
   typedef typename Elem<DT>::T T;
