@@ -501,6 +501,88 @@ int ubridge_kv_fork(const UbridgeKvPool* pool, const int32_t* src, const int32_t
                     int32_t* new_pages, void* stream);
 int ubridge_kv_compact(const UbridgeKvPool* pool, int32_t* n_used, void* stream);
 
+/* ------------------------------------------------ norm and feed-forward half
+ * No counterpart in the reference's quantized-matmul path. */
+/* Root-mean-square norm of the rows of x [R, C] (rows of up to 64 KiB): h = T(x +
+ * residual), or x without one; y = h w / sqrt(mean(h^2) + eps).  residual [R, C] or
+ * NULL, then h is written (h may be residual or x itself; nothing else overlaps);
+ * w [C] of x's type or f32.  dtype / w_dtype 0 f32, 1 f16, 2 bf16.  out 0: y of
+ * type T; 1: int8 codes [R, C] and f32 scales [R] (amax / 127, 1 for a row of
+ * zeros, NaN with codes 0 for a row that holds an infinity or a NaN); 2: e4m3, the
+ * same with amax / 448; 3 / 4: blocks of 32 as ubridge_mx_quantize writes them
+ * (scale: the bytes), codes 16-byte aligned. */
+typedef struct {
+  const void *x, *residual, *w;
+  void *h, *y, *scale;
+  double eps;
+  int32_t R, C, dtype, w_dtype, out, pad;
+} UbridgeRmsNormArgs;
+int ubridge_rms_norm(const UbridgeRmsNormArgs* args, void* stream);
+/* Its gradient for out 0: h [R, C] as stored, dy [R, C] and dh [R, C] or NULL (the
+ * gradients of y and of h), dx [R, C] (of x, and of residual; dh is added) and dw [C]
+ * of w's type, either NULL if it is not wanted.  Scratch: for dw, at most 2048 C
+ * bytes of f32 partial sums, added in a fixed order. */
+typedef struct {
+  const void *h, *w, *dy, *dh;
+  void *dx, *dw;
+  double eps;
+  int32_t R, C, dtype, w_dtype;
+} UbridgeRmsNormGradArgs;
+int ubridge_rms_norm_grad(const UbridgeRmsNormGradArgs* args, void* stream);
+
+/* Microscaled blocks: 32 consecutive elements of a row under one power of two, byte
+ * 127 + exponent (255: every value NaN); elements e2m1 (format 4, two a byte, the
+ * even one low) or e4m3 (format 8).  A row of C elements is ld = C rounded up to 128
+ * of them: codes [R, ld * format / 8], 16-byte aligned, scales [R, ld / 32], both zero
+ * past C.  quantize: the exponent is floor(log2 amax) - 2 or - 8 (at least -127),
+ * elements to the nearest, ties to even, saturating; a block with an infinity or a NaN
+ * has byte 255 and codes 0.  dtype (of x, y) 0 f32, 1 f16, 2 bf16. */
+int ubridge_mx_quantize(const void* x, int dtype, void* codes, void* scales, int R, int C,
+                        int format, void* stream);
+int ubridge_mx_dequantize(const void* codes, const void* scales, void* y, int dtype, int R, int C,
+                          int format, void* stream);
+/* A weight's codes [N, ld / 2] and scales [N, ld / 32] (format 4, rows of K elements)
+ * into the layout that ubridge_mx_linear reads: w N16 ld / 2 and w_scales N16 ld / 32
+ * bytes, N16 = N rounded up to 16, both 16-byte aligned.  Once a weight; K <= 131072. */
+int ubridge_mx_pack(const void* codes, const void* scales, void* w, void* w_scales, int N, int K,
+                    void* stream);
+/* y[m, n] = T(sum_k a[m, k] w[n, k] + bias[n]): x T [M, K] rounded to blocks of
+ * `format` by the call, or, with x NULL, codes and scales [M, ...] that it has already;
+ * y T [M, N] contiguous, bias f32 [N] or NULL.  Sums are f32.  Scratch beyond 16 tokens,
+ * or where their codes pass a workgroup's 160 KiB: the codes and scales, and 4 M N
+ * bytes a part where long rows are cut (at most 32). */
+typedef struct {
+  const void *x, *codes, *scales, *w, *w_scales;
+  const float* bias;
+  void* y;
+  int32_t M, K, N, dtype, format, pad;
+} UbridgeMxLinearArgs;
+int ubridge_mx_linear(const UbridgeMxLinearArgs* args, void* stream);
+
+/* int8 linear of codes that a norm (or ubridge_int8_linear's rule) made: a int8 [M,
+ * ld], 16-byte aligned, finite in the padding, sa f32 [M]; the rest as
+ * ubridge_int8_linear, whose values it gives.  Scratch: 4 M N bytes a part where long
+ * rows are cut. */
+int ubridge_int8_linear_codes(const int8_t* a, const float* sa, const int8_t* w, const float* sw,
+                              const float* bias, void* y, int dtype, int M, int K, int N, int ld,
+                              void* stream);
+
+/* A mixture-of-experts layer for up to 16 tokens in two launches: top-k of the
+ * softmax of logits [T, E] (logits_dtype 0 f32, 1 f16, 2 bf16; ties to the lowest
+ * expert; an expert whose logit is -inf or NaN is never taken, so a token may have
+ * fewer than k, or none and then zeros), weights f32, divided by their sum if
+ * renormalize; a = T(silu(g) u) of g, u = rows [0, I) and [I, 2 I) of w13 times x; y =
+ * T(sum over the experts of weight * (w2 a)).  w13 [E, 2 I, H] and w2 [E, H, I] of type T
+ * (dtype 1 f16, 2 bf16), or int8 with scales s13 [E, 2 I] and s2 [E, H] of type T
+ * (else NULL).  H and I are multiples of 32, x, w13 and w2 16-byte aligned, k <= 16,
+ * E <= 1024.  y overlaps no input.  Scratch: about T k (2 I + 80) bytes. */
+typedef struct {
+  const void *x, *logits, *w13, *s13, *w2, *s2;
+  void* y;
+  int32_t T, E, k, H, I, dtype, logits_dtype, renormalize;
+} UbridgeMoeDecodeArgs;
+int ubridge_moe_decode(const UbridgeMoeDecodeArgs* args, void* stream);
+
 /* ------------------------------------------------ name-keyed kernel launch
  * Replaces GcuDevice::get_or_load_func(func, module) (src/gcu_device.rs:160-183,
  * DeviceExecutor::get_function src/device_executor.rs:523-531) and

@@ -12,8 +12,9 @@ from .ops import *  # noqa: F401,F403
 from .registry import get_function, has_function  # noqa: F401
 from . import fp8, moe  # noqa: F401
 
-# the attention block, whose compiled binding is loaded when one of them is first used
-_BLOCK = ("attention", "int8", "kvcache", "rope")
+# the attention block, the norm and the feed-forward half, whose compiled binding is
+# loaded when one of them is first used
+_BLOCK = ("attention", "int8", "kvcache", "mx", "norm", "rope")
 
 
 def __getattr__(name):

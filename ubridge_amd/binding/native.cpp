@@ -1,14 +1,13 @@
-// native.cpp -- the host side of the attention block's calls: checks the
-// tensors, allocates results and fills the argument blocks of
-// include/ubridge_hip.h.
+// native.cpp -- the host side of the attention block's calls and of the norm and
+// feed-forward half: checks the tensors, allocates results and fills the argument
+// blocks of include/ubridge_hip.h.
 //
 // A decode step calls these operators a few times a layer, at sizes where the
 // kernels take 5 to 15 us; reading shapes, strides and types of six tensors
 // from Python took 8 to 10 us a call, here about 1 us.  Every refusal is a ValueError, as in
 // the Python modules; a nonzero status of the C entry is returned as an int, for
 // the caller to raise.  Compute stays behind the C ABI, whose entry points
-// attention.py, rope.py, kvcache.py and int8.py hand over (bind) from the library
-// they have loaded.
+// native.py hands over (bind) from the library that it has loaded.
 #include <Python.h>
 #include <cfloat>
 #include <cmath>
@@ -28,6 +27,14 @@ struct {
   decltype(&ubridge_kv_free) free;
   decltype(&ubridge_kv_fork) fork;
   decltype(&ubridge_kv_compact) compact;
+  decltype(&ubridge_int8_linear_codes) linear_codes;
+  decltype(&ubridge_rms_norm) norm;
+  decltype(&ubridge_rms_norm_grad) norm_grad;
+  decltype(&ubridge_mx_quantize) mx_quantize;
+  decltype(&ubridge_mx_dequantize) mx_dequantize;
+  decltype(&ubridge_mx_pack) mx_pack;
+  decltype(&ubridge_mx_linear) mx_linear;
+  decltype(&ubridge_moe_decode) moe_decode;
 } fn;
 
 #define REFUSE(...)                             \
@@ -103,7 +110,7 @@ struct Args {
   }
 
 PyObject* py_bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  COUNT(7)
+  COUNT(15)
   const Args A{args};
   fn.decode = (decltype(fn.decode))A.p(0);
   fn.rope = (decltype(fn.rope))A.p(1);
@@ -112,6 +119,14 @@ PyObject* py_bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   fn.free = (decltype(fn.free))A.p(4);
   fn.fork = (decltype(fn.fork))A.p(5);
   fn.compact = (decltype(fn.compact))A.p(6);
+  fn.linear_codes = (decltype(fn.linear_codes))A.p(7);
+  fn.norm = (decltype(fn.norm))A.p(8);
+  fn.norm_grad = (decltype(fn.norm_grad))A.p(9);
+  fn.mx_quantize = (decltype(fn.mx_quantize))A.p(10);
+  fn.mx_dequantize = (decltype(fn.mx_dequantize))A.p(11);
+  fn.mx_pack = (decltype(fn.mx_pack))A.p(12);
+  fn.mx_linear = (decltype(fn.mx_linear))A.p(13);
+  fn.moe_decode = (decltype(fn.moe_decode))A.p(14);
   if (PyErr_Occurred()) return nullptr;
   Py_RETURN_NONE;
 }
@@ -419,6 +434,326 @@ PyObject* py_compact(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------- norm and feed-forward half
+// Tensors of one call lie on one device.
+bool together(const char* name, std::initializer_list<Ten> ts) {
+  Ten first = nullptr;
+  for (Ten t : ts) {
+    if (!t) continue;
+    if (!first) first = t;
+    if (t->device() != first->device()) {
+      PyErr_Format(PyExc_ValueError, "%s: tensors on several devices", name);
+      return false;
+    }
+  }
+  return true;
+}
+// None, or a tensor (anything else refused)
+bool optional(PyObject* o, Ten& t) { return device_tensor(o, t, true); }
+PyObject* list_of(std::initializer_list<at::Tensor*> ts) {
+  PyObject* l = PyList_New(0);
+  for (at::Tensor* t : ts) {
+    PyObject* o = t->defined() ? THPVariable_Wrap(std::move(*t)) : (Py_INCREF(Py_None), Py_None);
+    if (!l || !o || PyList_Append(l, o)) {
+      Py_XDECREF(l), Py_XDECREF(o);
+      return nullptr;
+    }
+    Py_DECREF(o);
+  }
+  return l;
+}
+int64_t padded(int64_t c) { return (c + 127) / 128 * 128; }
+c10::SmallVector<int64_t, 5> ended(const at::Tensor& x, int64_t last) {
+  c10::SmallVector<int64_t, 5> s(x.sizes().begin(), x.sizes().end());
+  s.back() = last;
+  return s;
+}
+bool same(const at::Tensor& a, const at::Tensor& b) {
+  return a.scalar_type() == b.scalar_type() && a.sizes() == b.sizes();
+}
+
+// x [..., C], w [C], residual | None, residual_out | None, eps, out (0 as x, 1 int8, 2
+// e4m3, 3 fp4 blocks, 4 fp8 blocks), stream -> [y, scale | None, h | None]
+PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  COUNT(7)
+  HANDLE_TH_ERRORS
+  const Args A{args};
+  Ten x, w, res, ho;
+  if (!device_tensor(args[0], x) || !device_tensor(args[1], w) || !optional(args[2], res) || !optional(args[3], ho)) return nullptr;
+  const int dt = code(*x), wt = code(*w);
+  if (dt < 0 || dt > 2 || (wt != dt && wt != 0)) REFUSE("rms_norm takes f32, f16 or bf16 rows and a gain of that type or f32");
+  if (x->dim() == 0 || w->dim() != 1 || w->size(0) != x->size(-1) || !dense(*w)) REFUSE("rms_norm: x [..., C], gain contiguous [C]");
+  const int64_t C = x->size(-1), R = C ? x->numel() / C : 0;
+  if (C == 0 || C * x->element_size() > 65536) REFUSE("rms_norm: rows of %ld (1 element to 64 KiB)", C);
+  if (R >= 1 << 24) REFUSE("rms_norm: %ld rows", R);
+  if (res && !same(*res, *x)) REFUSE("rms_norm: residual must be of x's type and shape");
+  if (ho && (!res || !same(*ho, *x) || !dense(*ho))) REFUSE("rms_norm: residual_out goes with residual, contiguous, of x's type and shape");
+  if (!together("rms_norm", {x, w, res, ho})) return nullptr;
+  const double eps = A.f(4);
+  const int out = (int)A.n(5);
+  if (PyErr_Occurred()) return nullptr;
+  if (!(eps >= 0 && eps <= 3.4e38)) REFUSE("rms_norm: eps must be a float32 of at least 0");
+  at::Tensor xc = dense(*x) ? *x : x->contiguous(), rc, h, y, scale;
+  if (res) {
+    rc = dense(*res) ? *res : res->contiguous();
+    h = ho ? *ho : result(x->sizes(), *x);
+    // (each element is read ahead of its store by the thread that stores it)
+    auto clash = [&](const at::Tensor& t) { return meet(h, t) && h.data_ptr() != t.data_ptr(); };
+    if (clash(*x) || clash(*res) || meet(h, *w)) REFUSE("rms_norm: residual_out overlaps an input in part");
+  }
+  if (out == 0) {
+    y = result(x->sizes(), *x);
+  } else if (out <= 2) {
+    y = result(x->sizes(), *x, out == 1 ? at::kChar : at::kByte);
+    scale = result(x->sizes().slice(0, x->dim() - 1), *x, at::kFloat);
+  } else {
+    y = result(ended(*x, padded(C) / (out == 3 ? 2 : 1)), *x, at::kByte);
+    scale = result(ended(*x, padded(C) / 32), *x, at::kByte);
+  }
+  UbridgeRmsNormArgs p = {};
+  p.x = xc.data_ptr(), p.w = w->data_ptr(), p.y = y.data_ptr(), p.eps = eps;
+  p.residual = res ? rc.data_ptr() : nullptr, p.h = res ? h.data_ptr() : nullptr;
+  p.scale = out ? scale.data_ptr() : nullptr;
+  p.R = R, p.C = C, p.dtype = dt, p.w_dtype = wt, p.out = out;
+  void* stream = A.p(6);
+  if (PyErr_Occurred()) return nullptr;
+  if (const int rc2 = fn.norm(&p, stream)) return PyLong_FromLong(rc2);
+  return list_of({&y, &scale, &h});
+  END_HANDLE_TH_ERRORS
+}
+
+// h [..., C], w, dy, dh | None, eps, whether dx, whether dw, stream -> [dx | None, dw | None]
+PyObject* py_norm_grad(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  COUNT(8)
+  HANDLE_TH_ERRORS
+  const Args A{args};
+  Ten h, w, dy, dh;
+  if (!device_tensor(args[0], h) || !device_tensor(args[1], w) || !device_tensor(args[2], dy) || !optional(args[3], dh)) return nullptr;
+  const int dt = code(*h), wt = code(*w);
+  const int64_t C = h->dim() ? h->size(-1) : 0, R = C ? h->numel() / C : 0;
+  if (dt < 0 || dt > 2 || (wt != dt && wt != 0) || C == 0 || C * h->element_size() > 65536 || R >= 1 << 24 || w->dim() != 1 ||
+      w->size(0) != C || !dense(*w) || !dense(*h) || !same(*dy, *h) || (dh && !same(*dh, *h)))
+    REFUSE("rms_norm's gradient: h, dy and dh [..., C] of one type and shape, gain [C]");
+  if (!together("rms_norm's gradient", {h, w, dy, dh})) return nullptr;
+  at::Tensor dyc = dense(*dy) ? *dy : dy->contiguous(), dhc, dx, dw;
+  if (dh) dhc = dense(*dh) ? *dh : dh->contiguous();
+  if (PyObject_IsTrue(args[5])) dx = result(h->sizes(), *h);
+  if (PyObject_IsTrue(args[6])) dw = result(w->sizes(), *w);
+  UbridgeRmsNormGradArgs p = {};
+  p.h = h->data_ptr(), p.w = w->data_ptr(), p.dy = dyc.data_ptr(), p.dh = dh ? dhc.data_ptr() : nullptr;
+  p.dx = dx.defined() ? dx.data_ptr() : nullptr, p.dw = dw.defined() ? dw.data_ptr() : nullptr;
+  p.eps = A.f(4), p.R = R, p.C = C, p.dtype = dt, p.w_dtype = wt;
+  void* stream = A.p(7);
+  if (PyErr_Occurred()) return nullptr;
+  // (without rows dx has no memory, and there is nothing to run but dw's zeros)
+  if ((p.dx && R) || p.dw)
+    if (const int rc = fn.norm_grad(&p, stream)) return PyLong_FromLong(rc);
+  return list_of({&dx, &dw});
+  END_HANDLE_TH_ERRORS
+}
+
+// x [..., C], format (4, 8), stream -> [codes, scales]
+PyObject* py_mx_quantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  COUNT(3)
+  HANDLE_TH_ERRORS
+  const Args A{args};
+  Ten x;
+  if (!device_tensor(args[0], x)) return nullptr;
+  const int dt = code(*x), f = (int)A.n(1);
+  if (dt < 0 || dt > 2 || x->dim() == 0 || x->size(-1) == 0) REFUSE("mx.quantize takes f32, f16 or bf16 [..., C]");
+  const int64_t C = x->size(-1), R = x->numel() / C;
+  if (!fits(R) || C > 1 << 30 || R * (C + 127) > 1ll << 34) REFUSE("mx.quantize: %ld rows of %ld", R, C);
+  at::Tensor xc = dense(*x) ? *x : x->contiguous();
+  at::Tensor q = result(ended(*x, padded(C) * f / 8), *x, at::kByte), s = result(ended(*x, padded(C) / 32), *x, at::kByte);
+  void* stream = A.p(2);
+  if (PyErr_Occurred()) return nullptr;
+  if (const int rc = fn.mx_quantize(xc.data_ptr(), dt, q.data_ptr(), s.data_ptr(), R, C, f, stream)) return PyLong_FromLong(rc);
+  return list_of({&q, &s});
+  END_HANDLE_TH_ERRORS
+}
+
+// codes and scales of rows of K elements; false: refused
+bool block_rows(const char* name, Ten q, Ten s, int64_t K, int f) {
+  if (K > 0 && K <= 1 << 30 && q->dim() > 0 && s->dim() == q->dim() && q->scalar_type() == at::kByte && s->scalar_type() == at::kByte &&
+      q->size(-1) == padded(K) * f / 8 && s->size(-1) == padded(K) / 32 &&
+      q->sizes().slice(0, q->dim() - 1) == s->sizes().slice(0, s->dim() - 1) && dense(*q) && dense(*s) &&
+      ((uintptr_t)q->data_ptr() & 15) == 0 && ((uintptr_t)s->data_ptr() & 3) == 0)
+    return true;
+  PyErr_Format(PyExc_ValueError, "%s: codes uint8 [..., %ld] and scales uint8 [..., %ld] of rows of %ld, contiguous, aligned to 16 and 4 bytes",
+               name, padded(K) * f / 8, padded(K) / 32, K);
+  return false;
+}
+
+at::ScalarType type_of(int dt) { return dt == 0 ? at::kFloat : dt == 1 ? at::kHalf : at::kBFloat16; }
+
+// codes, scales, C, type code, format, stream -> values [..., C]
+PyObject* py_mx_dequantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  COUNT(6)
+  HANDLE_TH_ERRORS
+  const Args A{args};
+  Ten q, s;
+  if (!device_tensor(args[0], q) || !device_tensor(args[1], s)) return nullptr;
+  const int64_t C = A.n(2);
+  const int dt = (int)A.n(3), f = (int)A.n(4);
+  if (PyErr_Occurred() || !block_rows("mx.dequantize", q, s, C, f) || !together("mx.dequantize", {q, s})) return nullptr;
+  const int64_t R = q->numel() / q->size(-1);
+  if (!fits(R) || R * (C + 127) > 1ll << 34) REFUSE("mx.dequantize: %ld rows of %ld", R, C);
+  at::Tensor y = result(ended(*q, C), *q, type_of(dt));
+  void* stream = A.p(5);
+  if (PyErr_Occurred()) return nullptr;
+  if (const int rc = fn.mx_dequantize(q->data_ptr(), s->data_ptr(), y.data_ptr(), dt, R, C, f, stream)) return PyLong_FromLong(rc);
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// codes [N, ld / 2], scales [N, ld / 32], K, stream -> [w, w_scales]
+PyObject* py_mx_pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  COUNT(4)
+  HANDLE_TH_ERRORS
+  const Args A{args};
+  Ten q, s;
+  if (!device_tensor(args[0], q) || !device_tensor(args[1], s)) return nullptr;
+  const int64_t K = A.n(2);
+  if (PyErr_Occurred() || !block_rows("mx.Linear", q, s, K, 4) || !together("mx.Linear", {q, s})) return nullptr;
+  const int64_t N = q->size(0), N16 = (N + 15) / 16 * 16;
+  if (q->dim() != 2 || !fits(N) || K > 131072) REFUSE("mx.Linear: weight [N, K=%ld] (1..131072)", K);
+  at::Tensor w = result({N16, padded(K) / 2}, *q), ws = result({N16, padded(K) / 32}, *q);
+  void* stream = A.p(3);
+  if (PyErr_Occurred()) return nullptr;
+  if (const int rc = fn.mx_pack(q->data_ptr(), s->data_ptr(), w.data_ptr(), ws.data_ptr(), N, K, stream)) return PyLong_FromLong(rc);
+  return list_of({&w, &ws});
+  END_HANDLE_TH_ERRORS
+}
+
+// first (x [..., K], or codes), scales | None, w, w_scales, bias | None, K, N, format,
+// type code (of y, with codes), out | None, stream
+PyObject* py_mx_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  COUNT(11)
+  HANDLE_TH_ERRORS
+  const Args A{args};
+  Ten x, s, w, ws, b, out;
+  if (!device_tensor(args[0], x) || !optional(args[1], s) || !device_tensor(args[2], w) || !device_tensor(args[3], ws) ||
+      !optional(args[4], b) || !optional(args[9], out))
+    return nullptr;
+  const int64_t K = A.n(5), N = A.n(6);
+  const int f = (int)A.n(7);
+  int dt = (int)A.n(8);
+  if (PyErr_Occurred()) return nullptr;
+  if (s) {
+    if (!block_rows("mx.Linear", x, s, K, f)) return nullptr;
+  } else {
+    dt = code(*x);
+    if (dt < 0 || dt > 2 || x->dim() == 0 || x->size(-1) != K) REFUSE("mx.Linear takes f32, f16 or bf16 activations [..., %ld]", K);
+  }
+  const int64_t N16 = (N + 15) / 16 * 16;
+  if (w->scalar_type() != at::kByte || ws->scalar_type() != at::kByte || !dense(*w) || !dense(*ws) || w->numel() != N16 * padded(K) / 2 ||
+      ws->numel() != N16 * padded(K) / 32 || !vec(b, N))
+    REFUSE("mx.Linear: weight as mx.Linear laid it out, bias contiguous float32 [%ld]", N);
+  if (!together("mx.Linear", {x, s, w, ws, b, out})) return nullptr;
+  const int64_t M = x->numel() / x->size(-1);
+  if (M >= 1 << 22 || M * N >= 1ll << 38 || M * K > 1ll << 34) REFUSE("mx.Linear: %ld rows of %ld to %ld", M, K, N);
+  const auto sizes = ended(*x, N);
+  if (out && (out->scalar_type() != type_of(dt) || out->sizes() != at::IntArrayRef(sizes) || !dense(*out)))
+    REFUSE("mx.Linear: out must be contiguous, of y's type, [..., %ld]", N);
+  if (out && (meet(*out, *x) || (s && meet(*out, *s)) || meet(*out, *w) || meet(*out, *ws) || (b && meet(*out, *b))))
+    REFUSE("mx.Linear: out overlaps an input");
+  at::Tensor y = out ? *out : result(sizes, *x, type_of(dt)), xc = dense(*x) ? *x : x->contiguous();
+  UbridgeMxLinearArgs p = {};
+  if (s) p.codes = xc.data_ptr(), p.scales = s->data_ptr();
+  else p.x = xc.data_ptr();
+  p.w = w->data_ptr(), p.w_scales = ws->data_ptr(), p.bias = ptr(b), p.y = y.data_ptr();
+  p.M = M, p.K = K, p.N = N, p.dtype = dt, p.format = f;
+  void* stream = A.p(10);
+  if (PyErr_Occurred()) return nullptr;
+  if (const int rc = fn.mx_linear(&p, stream)) return PyLong_FromLong(rc);
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// codes int8 [..., ld], scales [...], w [N, ld], w_scale, bias | None, K, type code, out |
+// None, stream
+PyObject* py_linear_codes(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  COUNT(9)
+  HANDLE_TH_ERRORS
+  const Args A{args};
+  Ten q, s, w, sw, b, out;
+  if (!device_tensor(args[0], q) || !device_tensor(args[1], s) || !device_tensor(args[2], w) || !device_tensor(args[3], sw) ||
+      !optional(args[4], b) || !optional(args[7], out))
+    return nullptr;
+  const int64_t K = A.n(5);
+  const int dt = (int)A.n(6);
+  if (PyErr_Occurred()) return nullptr;
+  if (w->scalar_type() != at::kChar || w->dim() != 2 || !dense(*w) || K <= 0 || w->size(1) < K || !vec(sw, w->size(0)) ||
+      !vec(b, w->size(0)))
+    REFUSE("int8.Linear: weight int8 [N, >= %ld], w_scale and bias float32 [N], all contiguous", K);
+  const int64_t N = w->size(0), ld = w->size(1);
+  if (q->scalar_type() != at::kChar || q->dim() == 0 || q->size(-1) != ld || !dense(*q) || ((uintptr_t)q->data_ptr() & 15) ||
+      s->scalar_type() != at::kFloat || s->sizes() != q->sizes().slice(0, q->dim() - 1) || !dense(*s))
+    REFUSE("int8.Linear: codes int8 [..., %ld], aligned to 16 bytes, and scales float32 [...], contiguous", ld);
+  if (!together("int8.Linear", {q, s, w, sw, b, out})) return nullptr;
+  const int64_t M = q->numel() / ld;
+  if (!fits(M)) REFUSE("int8.Linear: %ld rows", M);
+  const auto sizes = ended(*q, N);
+  if (out && (out->scalar_type() != type_of(dt) || out->sizes() != at::IntArrayRef(sizes) || !dense(*out)))
+    REFUSE("int8.Linear: out must be contiguous, of y's type, [..., %ld]", N);
+  if (out && (meet(*out, *q) || meet(*out, *s) || meet(*out, *w) || meet(*out, *sw) || (b && meet(*out, *b))))
+    REFUSE("int8.Linear: out overlaps an input");
+  at::Tensor y = out ? *out : result(sizes, *q, type_of(dt));
+  void* stream = A.p(8);
+  if (PyErr_Occurred()) return nullptr;
+  if (const int rc = fn.linear_codes((const int8_t*)q->data_ptr(), ptr(s), (const int8_t*)w->data_ptr(), ptr(sw), ptr(b), y.data_ptr(), dt, M,
+                                     K, N, ld, stream))
+    return PyLong_FromLong(rc);
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// x [T, H], logits [T, E], w13, s13 | None, w2, s2 | None, k, renormalize, stream
+PyObject* py_moe_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  COUNT(9)
+  HANDLE_TH_ERRORS
+  const Args A{args};
+  Ten x, lg, w13, s13, w2, s2;
+  if (!device_tensor(args[0], x) || !device_tensor(args[1], lg) || !device_tensor(args[2], w13) || !optional(args[3], s13) ||
+      !device_tensor(args[4], w2) || !optional(args[5], s2))
+    return nullptr;
+  const long k = A.n(6);
+  if (PyErr_Occurred()) return nullptr;
+  const int dt = code(*x), lt = code(*lg);
+  if ((dt != 1 && dt != 2) || lt < 0 || lt > 2) REFUSE("FusedMoE.decode takes f16 or bf16 rows and f32, f16 or bf16 logits");
+  if (x->dim() != 2 || lg->dim() != 2 || w13->dim() != 3 || w2->dim() != 3) REFUSE("FusedMoE.decode: x [T, H], logits [T, E], w13 [E, 2 I, H], w2 [E, H, I]");
+  const int64_t T = x->size(0), H = x->size(1), E = w13->size(0), I = w2->size(2);
+  if (lg->size(0) != T || lg->size(1) != E || w13->size(1) != 2 * I || w13->size(2) != H || w2->size(0) != E || w2->size(1) != H)
+    REFUSE("FusedMoE.decode: x [%ld, %ld], logits [%ld, %ld], w13 [%ld, %ld, %ld], w2 [%ld, %ld, %ld] do not fit", T, H, lg->size(0),
+           lg->size(1), E, w13->size(1), w13->size(2), w2->size(0), w2->size(1), I);
+  const bool q8 = w13->scalar_type() == at::kChar;
+  if (w2->scalar_type() != w13->scalar_type() || (!q8 && w13->scalar_type() != x->scalar_type()))
+    REFUSE("FusedMoE.decode: experts are both int8 or both in the activations' dtype");
+  if (q8 != (s13 != nullptr) || q8 != (s2 != nullptr)) REFUSE("FusedMoE.decode: int8 experts, and they alone, have scales");
+  if (q8 && (s13->scalar_type() != x->scalar_type() || s2->scalar_type() != x->scalar_type() || s13->numel() != E * 2 * I ||
+             s2->numel() != E * H || !dense(*s13) || !dense(*s2)))
+    REFUSE("FusedMoE.decode: scales of x's type, [E, 2 I] and [E, H], contiguous");
+  if (!dense(*w13) || !dense(*w2)) REFUSE("FusedMoE.decode: experts must be contiguous");
+  if (T > 16 || k < 1 || k > 16 || k > E || E > 1024 || H == 0 || I == 0 || H % 32 || I % 32 || H > 1 << 20 || I > 1 << 20)
+    REFUSE("FusedMoE.decode: T=%ld (at most 16), topk=%ld (1..16, at most E), E=%ld (at most 1024), H=%ld and I=%ld (multiples of 32)", T, k,
+           E, H, I);
+  if (!together("FusedMoE.decode", {x, lg, w13, s13, w2, s2})) return nullptr;
+  auto whole = [](const at::Tensor& t, int align) { return dense(t) && ((uintptr_t)t.data_ptr() & (align - 1)) == 0; };
+  at::Tensor xc = *x, lc = dense(*lg) ? *lg : lg->contiguous();
+  if (!whole(xc, 16)) xc = xc.clone(at::MemoryFormat::Contiguous);
+  if (!whole(*w13, 16) || !whole(*w2, 16)) REFUSE("FusedMoE.decode: experts not 16-byte aligned");
+  at::Tensor y = result({T, H}, *x);
+  UbridgeMoeDecodeArgs p = {};
+  p.x = xc.data_ptr(), p.logits = lc.data_ptr(), p.w13 = w13->data_ptr(), p.w2 = w2->data_ptr(), p.y = y.data_ptr();
+  p.s13 = q8 ? s13->data_ptr() : nullptr, p.s2 = q8 ? s2->data_ptr() : nullptr;
+  p.T = T, p.E = E, p.k = k, p.H = H, p.I = I, p.dtype = dt, p.logits_dtype = lt, p.renormalize = PyObject_IsTrue(args[7]);
+  void* stream = A.p(8);
+  if (PyErr_Occurred()) return nullptr;
+  if (const int rc = fn.moe_decode(&p, stream)) return PyLong_FromLong(rc);
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"bind", (PyCFunction)(void (*)())py_bind, METH_FASTCALL, "the C entry points, as addresses"},
     {"paged_decode", (PyCFunction)(void (*)())py_decode, METH_FASTCALL, nullptr},
@@ -428,6 +763,14 @@ PyMethodDef methods[] = {
     {"free", (PyCFunction)(void (*)())py_free, METH_FASTCALL, nullptr},
     {"fork", (PyCFunction)(void (*)())py_fork, METH_FASTCALL, nullptr},
     {"compact", (PyCFunction)(void (*)())py_compact, METH_FASTCALL, nullptr},
+    {"linear_codes", (PyCFunction)(void (*)())py_linear_codes, METH_FASTCALL, nullptr},
+    {"norm", (PyCFunction)(void (*)())py_norm, METH_FASTCALL, nullptr},
+    {"norm_grad", (PyCFunction)(void (*)())py_norm_grad, METH_FASTCALL, nullptr},
+    {"mx_quantize", (PyCFunction)(void (*)())py_mx_quantize, METH_FASTCALL, nullptr},
+    {"mx_dequantize", (PyCFunction)(void (*)())py_mx_dequantize, METH_FASTCALL, nullptr},
+    {"mx_pack", (PyCFunction)(void (*)())py_mx_pack, METH_FASTCALL, nullptr},
+    {"mx_linear", (PyCFunction)(void (*)())py_mx_linear, METH_FASTCALL, nullptr},
+    {"moe_decode", (PyCFunction)(void (*)())py_moe_decode, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods};
 

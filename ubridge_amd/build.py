@@ -4,7 +4,8 @@ Every HIP/C++ source under ubridge_amd/csrc is compiled with hipcc in
 parallel and linked into one shared library whose exported symbols are the
 extern "C" entry points declared in include/ubridge_hip.h; then the C++ host
 driver (driver/ub_drive.cpp) is linked against it as lib/ub_drive, and the
-host side of the attention block (binding/native.cpp) becomes _native.so.
+host side of the attention block and of the norm and feed-forward half
+(binding/native.cpp) becomes _native.so.
 
     python ubridge_amd/build.py
 """

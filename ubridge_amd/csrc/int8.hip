@@ -730,6 +730,18 @@ void gemm(Plan plan, const int8_t* q, const float* sa, const int8_t* w, const fl
 #undef UB_RING
 }
 
+// The product of codes a and scales sa, its sums over parts of K (if any) in `sums`.
+template <int DT>
+void product(Plan plan, int parts, const int8_t* a, const float* sa, const int8_t* w, const float* sw, const float* bias,
+             void* y, int* sums, int M, int N, int ld, hipStream_t s) {
+  if (parts > 1) {
+    gemm<kSum>(plan, a, sa, w, sw, bias, sums, M, N, ld, s);
+    k_i8_sum<DT><<<ub_cdiv((long)M * N, 256), 256, 0, s>>>(sums, sa, sw, bias, y, M, N, parts);
+  } else {
+    gemm<DT>(plan, a, sa, w, sw, bias, y, M, N, ld, s);
+  }
+}
+
 template <int DT>
 int linear(const char* nm, const void* x, const int8_t* w, const float* sw, const float* bias, void* y, int M, int K,
            int N, int ld, hipStream_t s) {
@@ -746,13 +758,21 @@ int linear(const char* nm, const void* x, const int8_t* w, const float* sw, cons
   float* sa = (float*)(q + (size_t)M * ld);
   if (!((M >= 512 || ld <= 2048) && quant<DT, 256>(x, q, sa, M, K, ld, s)) && !quant<DT, 1024>(x, q, sa, M, K, ld, s))
     k_quant<DT, 1024, 0><<<M, 1024, 0, s>>>(x, q, sa, K, ld);
-  if (parts > 1) {
-    int* part = (int*)(sa + M);
-    gemm<kSum>(plan, q, sa, w, sw, bias, part, M, N, ld, s);
-    k_i8_sum<DT><<<ub_cdiv((long)M * N, 256), 256, 0, s>>>(part, sa, sw, bias, y, M, N, parts);
-  } else {
-    gemm<DT>(plan, q, sa, w, sw, bias, y, M, N, ld, s);
-  }
+  product<DT>(plan, parts, q, sa, w, sw, bias, y, (int*)(sa + M), M, N, ld, s);
+  return UB_OK;
+}
+
+// Of codes that are there already: the tiles at every size (few tokens too: 16 x 4096
+// x 4096 11.4 us against 10.4 of k_i8_dec, whose quantizing this saves).
+template <int DT>
+int linear_codes(const char* nm, const int8_t* a, const float* sa, const int8_t* w, const float* sw, const float* bias,
+                 void* y, int M, int N, int ld, hipStream_t s) {
+  const Plan plan = plan_for(M, N, ld / 128);
+  const int parts = ub_cdiv(ld / 128, ub_cdiv(ld / 128, plan.parts));
+  const size_t sums = parts > 1 ? sizeof(int) * parts * (size_t)M * N : 0;
+  UbScratch ws(s, sums);
+  if (sums && !ws.get()) return ub_set_error(UB_ERR_LAUNCH, "%s: no workspace", nm);
+  product<DT>(plan, parts, a, sa, w, sw, bias, y, (int*)ws.get(), M, N, ld, s);
   return UB_OK;
 }
 
@@ -773,5 +793,23 @@ UB_API int ubridge_int8_linear(const void* x, int dtype, const int8_t* w, const 
   const int e = dtype == UB_F32   ? linear<UB_F32>(nm, x, w, sw, bias, y, M, K, N, ld, s)
                 : dtype == UB_F16 ? linear<UB_F16>(nm, x, w, sw, bias, y, M, K, N, ld, s)
                                   : linear<UB_BF16>(nm, x, w, sw, bias, y, M, K, N, ld, s);
+  return e ? e : ub_check_launch(nm);
+}
+
+UB_API int ubridge_int8_linear_codes(const int8_t* a, const float* sa, const int8_t* w, const float* sw,
+                                     const float* bias, void* y, int dtype, int M, int K, int N, int ld,
+                                     void* stream) {
+  const char* nm = "ubridge_int8_linear_codes";
+  UB_REQUIRE(dtype == UB_F32 || dtype == UB_F16 || dtype == UB_BF16, "%s: dtype %d", nm, dtype);
+  UB_REQUIRE(M >= 0 && N >= 0 && K > 0 && K <= 132104, "%s: M=%d K=%d (1..132104) N=%d", nm, M, K, N);
+  UB_REQUIRE(ld >= K && ld % 128 == 0 && ld <= 132224, "%s: ld=%d (a multiple of 128, at least K=%d)", nm, ld, K);
+  if ((size_t)M * N == 0) return UB_OK;
+  UB_REQUIRE(a && sa && w && sw && y, "%s: null pointer", nm);
+  UB_REQUIRE((((uintptr_t)a | (uintptr_t)w) & 15) == 0, "%s: codes or weight not 16-byte aligned", nm);
+  UB_REQUIRE(M < 1 << 22 && (int64_t)M * N < 1ll << 38, "%s: M=%d N=%d", nm, M, N);
+  hipStream_t s = ub_stream(stream);
+  const int e = dtype == UB_F32   ? linear_codes<UB_F32>(nm, a, sa, w, sw, bias, y, M, N, ld, s)
+                : dtype == UB_F16 ? linear_codes<UB_F16>(nm, a, sa, w, sw, bias, y, M, N, ld, s)
+                                  : linear_codes<UB_BF16>(nm, a, sa, w, sw, bias, y, M, N, ld, s);
   return e ? e : ub_check_launch(nm);
 }

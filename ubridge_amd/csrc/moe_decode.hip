@@ -1,0 +1,423 @@
+// moe_decode.hip -- a mixture-of-experts layer for up to 16 tokens in two launches
+// (gfx950):
+//
+//   p = softmax(logits[t]),  the k largest (ties to the lowest expert), / their sum
+//   a[t, j] = T(silu(g) u),  g, u = (w13[e] x[t]) rows [0, I), [I, 2 I)
+//   y[t] = T(sum_j p_j (w2[e_j] a[t, j]))
+//
+// int8 weights are exact in T; their scales, the routed weights and all sums are f32.
+// Only a and y are rounded to T: a since it is an operand of the next product.
+//
+// A stream of the weights of the experts in use, read once each: bound by HBM where
+// they are many, by the chain of latencies (logits, weights, sums; twice) for a token
+// or two.  16 tokens are one operand of v_mfma_f32_16x16x32, so no rows are gathered
+// and no list of blocks is built: a product is of 16 weight rows with every token, and
+// an expert's result is kept for the tokens that chose it.
+//  * k_up: every workgroup finds the top-k itself (a wavefront a token; under a
+//    microsecond, against a launch).  An item is 8 columns of an expert: 8 gate rows
+//    and their 8 up rows are the 16 rows of one product.  The workgroups take equal
+//    runs of the items; 8 wavefronts split K, each one run of its rows, two items in
+//    flight.
+//  * k_down: a workgroup owns 8 output columns and adds all experts' parts, so no sums
+//    cross workgroups: 8 rows of each of two experts are the 16 rows of a product,
+//    multiplied by either's activations, and lane half h keeps the one that is its own.
+#include "moe_dev.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kTok = 16, kK = 16, kE = 1024, kUsed = kTok * kK;  // most tokens, top-k, experts; experts in use
+
+// The routing, in scratch memory from k_up to k_down: experts in use, in order, and for
+// each and every token its weight and its slot (-1: not chosen).
+struct Route {
+  int n;
+  int used[kUsed];
+  float w[kUsed][kTok];
+  int8_t slot[kUsed][kTok];
+};
+
+struct DecodeArgs {
+  const void *x, *logits, *w13, *s13, *w2, *s2;
+  void *y, *act;
+  Route* route;
+  int T, E, k, H, I, ldt, norm;
+};
+
+template <int DT>
+__device__ __forceinline__ f32x4 mfma(const uint4& a, const uint4& b, const f32x4& c) {
+  if constexpr (DT == UB_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// 16 bytes of a weight row by the activations that meet them: 16 int8 (two products)
+// or 8 T
+template <int DT, bool Q8>
+__device__ __forceinline__ f32x4 product(const uint4& w, const uint4 (&x)[Q8 ? 2 : 1], f32x4 c) {
+  if constexpr (Q8) {
+    c = mfma<DT>(i8x8_to_t<DT>(w.x, w.y), x[0], c);
+    return mfma<DT>(i8x8_to_t<DT>(w.z, w.w), x[1], c);
+  } else {
+    return mfma<DT>(w, x[0], c);
+  }
+}
+__device__ __forceinline__ uint4 ld16nt(const void* p) {
+  typedef unsigned int u4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(uint4, __builtin_nontemporal_load((const u4*)p));
+}
+
+// OP 0: f32 max, 1: u32 min, 2: f32 sum, over the wavefront
+template <int OP>
+__device__ __forceinline__ uint32_t wave_reduce(uint32_t v) {
+  auto op = [](uint32_t a, uint32_t b) -> uint32_t {
+    if constexpr (OP == 0) return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    else if constexpr (OP == 1) return a < b ? a : b;
+    else return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  };
+#define UB_DPP(c) v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, c, 0xf, 0xf, false))
+  UB_DPP(0xB1);   // quad_perm [1,0,3,2]
+  UB_DPP(0x4E);   // quad_perm [2,3,0,1]
+  UB_DPP(0x141);  // row_half_mirror
+  UB_DPP(0x140);  // row_mirror
+#undef UB_DPP
+  auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = op(a[0], a[1]);
+  auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return op(b[0], b[1]);
+}
+
+// Token t's experts, by one wavefront holding its logits (expert lane + 64 j): f(round,
+// expert, weight) in lane 0.
+template <int NPL, class F>
+__device__ __forceinline__ void top_k(float (&v)[NPL], int k, int norm, F f) {
+  const int lane = threadIdx.x & 63;
+  float m = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < NPL; j++) m = fmaxf(m, v[j]);
+  m = __uint_as_float(wave_reduce<0>(__float_as_uint(m)));
+  if (m == -INFINITY) return;
+  float all = 0.f;
+  if (!norm) {
+#pragma unroll
+    for (int j = 0; j < NPL; j++) all += expf(v[j] - m);
+    all = __uint_as_float(wave_reduce<2>(__float_as_uint(all)));
+  }
+  float picked = -INFINITY;  // lane i: the i-th largest, and its expert
+  int which = 0, got = 0;
+  for (int i = 0; i < k; i++) {
+    float best = v[0];
+    int bj = 0;
+#pragma unroll
+    for (int j = 1; j < NPL; j++)
+      if (v[j] > best) best = v[j], bj = j;
+    const float wb = __uint_as_float(wave_reduce<0>(__float_as_uint(best)));
+    if (wb == -INFINITY) break;
+    const int e = (int)wave_reduce<1>(best == wb ? (uint32_t)(lane + 64 * bj) : 0xffffffffu);
+#pragma unroll
+    for (int j = 0; j < NPL; j++)
+      if (lane + 64 * j == e) v[j] = -INFINITY;
+    if (lane == i) picked = wb, which = e;
+    got++;
+  }
+  const float p = lane < got ? expf(picked - m) : 0.f;
+  if (norm) all = __uint_as_float(wave_reduce<2>(__float_as_uint(p)));
+  if (lane < got) f(lane, which, p / all);
+}
+
+constexpr int W1 = 8;  // wavefronts of k_up
+
+// SP: 64-byte steps of a row that a wavefront takes at once.  MULTI: K in several such
+// pieces, the activations loaded with each; else they stay in registers.
+template <int DT, bool Q8, int NPL, int SP, bool MULTI>
+__global__ void __launch_bounds__(64 * W1) __attribute__((amdgpu_waves_per_eu(SP > 4 ? 2 : 4, SP > 4 ? 2 : 4))) k_up(DecodeArgs a) {
+  constexpr int WB = Q8 ? 1 : 2, EL = 64 / WB, XN = Q8 ? 2 : 1;  // bytes of a weight; elements of a step; operands
+  __shared__ __attribute__((aligned(16))) int8_t slot[kE][kTok];
+  __shared__ uint16_t used[kUsed];
+  __shared__ int nused;
+  __shared__ __attribute__((aligned(16))) float red[2][W1][16][20];
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, h = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int T = a.T, E = a.E, H = a.H, I = a.I;
+  // ---- routing.  Two tokens a wavefront, at most.
+  float lg[2][NPL];
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int t = wave + i * W1;
+#pragma unroll
+    for (int j = 0; j < NPL; j++) {
+      const int e = lane + 64 * j;
+      float v = -INFINITY;
+      if (t < T && e < E) {
+        const size_t at = (size_t)t * E + e;
+        v = a.ldt == UB_F32 ? ((const float*)a.logits)[at] : a.ldt == UB_F16 ? ub_load<UB_F16>(a.logits, at) : ub_load<UB_BF16>(a.logits, at);
+        if (v != v) v = -INFINITY;
+      }
+      lg[i][j] = v;
+    }
+  }
+  // ---- activations of the wavefront's steps: lane (token r, h) takes what meets the
+  // 16 bytes at 64 s + 16 h of a weight row
+  uint4 xf[MULTI ? 1 : SP][XN];
+  const int rowb = H * WB;
+  auto acts = [&](uint4 (&o)[XN], int s) {
+    const int at = s * 64 + 16 * h;  // byte of the row
+#pragma unroll
+    for (int u = 0; u < XN; u++) {
+      o[u] = make_uint4(0, 0, 0, 0);
+      if (r < T && at < rowb) o[u] = *(const uint4*)((const uint16_t*)a.x + (size_t)r * H + at / WB + 8 * u);
+    }
+  };
+  if constexpr (!MULTI) {
+#pragma unroll
+    for (int i = 0; i < SP; i++) acts(xf[i], wave * SP + i);
+  }
+  for (int i = tid; i < E * kTok / 4; i += 64 * W1) ((int*)slot)[i] = -1;
+  __syncthreads();
+  const bool first = blockIdx.x == 0;
+  __shared__ float wts[kTok][kK];
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int t = wave + i * W1;
+    if (t < T)
+      top_k<NPL>(lg[i], a.k, a.norm, [&](int j, int e, float w) {
+        slot[e][t] = (int8_t)j;
+        wts[t][j] = w;
+      });
+  }
+  __syncthreads();
+  if (wave == 0) {
+    int n = 0;
+    for (int e0 = 0; e0 < E; e0 += 64) {
+      const int e = e0 + lane;
+      bool any = false;
+      if (e < E) {
+        const int4 v = *(const int4*)slot[e];
+        any = (v.x & v.y & v.z & v.w) != -1;
+      }
+      const uint64_t m = __ballot(any);
+      if (any) used[n + __popcll(m & ((1ull << lane) - 1))] = (uint16_t)e;
+      n += __popcll(m);
+    }
+    if (lane == 0) nused = n;
+  }
+  __syncthreads();
+  const int nu = __builtin_amdgcn_readfirstlane(nused);
+  if (first) {
+    if (tid == 0) a.route->n = nu;
+    for (int i = tid; i < nu * kTok; i += 64 * W1) {
+      const int e = used[i / kTok], t = i % kTok, j = slot[e][t];
+      if (t == 0) a.route->used[i / kTok] = e;
+      a.route->slot[i / kTok][t] = (int8_t)j;
+      a.route->w[i / kTok][t] = j >= 0 ? wts[t][j] : 0.f;
+    }
+  }
+  // ---- items: (expert in use, 8 columns), equal runs of them
+  const int nc = I / 8, G = gridDim.x;
+  const long items = (long)nu * nc;
+  const int i0 = (int)(items * blockIdx.x / G), i1 = (int)(items * (blockIdx.x + 1) / G);
+  const int pieces = MULTI ? ((rowb + 63) / 64 + W1 * SP - 1) / (W1 * SP) : 1;
+  struct Set {
+    uint4 w[SP];
+    uint4 x[MULTI ? SP : 1][XN];
+  };
+  auto load = [&](Set& b, int it, int p) {
+    const int u = min(it, i1 - 1) / nc, c = min(it, i1 - 1) - u * nc;
+    const int e = used[u];
+    const uint8_t* row = (const uint8_t*)a.w13 + ((size_t)e * 2 * I + (r < 8 ? 8 * c + r : I + 8 * c + r - 8)) * rowb;
+#pragma unroll
+    for (int i = 0; i < SP; i++) {
+      const int s = p * W1 * SP + wave * SP + i, at = s * 64 + 16 * h;
+      b.w[i] = make_uint4(0, 0, 0, 0);
+      if (it < i1 && at < rowb) b.w[i] = ld16nt(row + at);
+      if constexpr (MULTI) acts(b.x[i], s);
+    }
+  };
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  auto mul = [&](Set& b, int it, int p, int buf) {
+#pragma unroll
+    for (int i = 0; i < SP; i++) {
+      if constexpr (MULTI) acc = product<DT, Q8>(b.w[i], b.x[i], acc);
+      else acc = product<DT, Q8>(b.w[i], xf[i], acc);
+    }
+    if (p != pieces - 1) return;
+    // lane (token r, h) holds rows 4 h .. + 3: gate rows for h < 2, up rows above
+    *(f32x4*)&red[buf][wave][r][4 * h] = acc;
+    acc = (f32x4){0.f, 0.f, 0.f, 0.f};
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0); weight loads stay in flight
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (tid < 8 * T) {
+      const int t = tid >> 3, c = tid & 7, u = it / nc, col = (it - u * nc) * 8 + c, e = used[u], j = slot[e][t];
+      if (j >= 0) {
+        float g = 0.f, up = 0.f;
+#pragma unroll
+        for (int w = 0; w < W1; w++) g += red[buf][w][t][c], up += red[buf][w][t][8 + c];
+        if constexpr (Q8) {
+          g *= ub_load<DT>(a.s13, (size_t)e * 2 * I + col);
+          up *= ub_load<DT>(a.s13, (size_t)e * 2 * I + I + col);
+        }
+        ub_store<DT>(a.act, ((size_t)t * a.k + j) * I + col, g / (1.f + expf(-g)) * up);
+      }
+    }
+  };
+  if (i0 >= i1) return;
+  Set b0, b1;
+  const int total = (i1 - i0) * pieces;
+  auto item = [&](int q) { return MULTI ? i0 + q / pieces : i0 + q; };
+  auto piece = [&](int q) { return MULTI ? q % pieces : 0; };
+  load(b0, item(0), piece(0));
+  int done = 0;  // items summed: their buffers alternate
+  for (int q = 0; q < total; q += 2) {
+    load(b1, item(q + 1), piece(q + 1));
+    mul(b0, item(q), piece(q), done & 1);
+    if (piece(q) == pieces - 1) done++;
+    if (q + 1 >= total) break;
+    load(b0, item(q + 2), piece(q + 2));
+    mul(b1, item(q + 1), piece(q + 1), done & 1);
+    if (piece(q + 1) == pieces - 1) done++;
+  }
+}
+
+constexpr int W2 = 16;  // wavefronts of k_down
+
+template <int DT, bool Q8>
+__global__ void __launch_bounds__(64 * W2) k_down(DecodeArgs a) {
+  constexpr int WB = Q8 ? 1 : 2, XN = Q8 ? 2 : 1, P2 = Q8 ? 2 : 4;  // P2: steps in a set
+  __shared__ int used[kUsed];
+  __shared__ float wts[kUsed][kTok];
+  __shared__ int8_t slot[kUsed][kTok];
+  __shared__ __attribute__((aligned(16))) float red[W2][16][20];
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, h = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int T = a.T, H = a.H, I = a.I, k = a.k;
+  const int n = min(a.route->n, kUsed), n0 = blockIdx.x * 8;
+  for (int i = tid; i < n * kTok; i += 64 * W2) {
+    (&wts[0][0])[i] = (&a.route->w[0][0])[i];
+    (&slot[0][0])[i] = (&a.route->slot[0][0])[i];
+    if (i < n) used[i] = a.route->used[i];
+  }
+  __syncthreads();
+  // units: (pair of experts, 64-byte step of their rows), a run of them to a wavefront
+  const int rowb = I * WB, steps = (rowb + 63) / 64, units = (n + 1) / 2 * steps;
+  const int q0 = (int)((long)units * wave / W2), q1 = (int)((long)units * (wave + 1) / W2);
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f}, s0 = sum, s1 = sum;
+  struct Set {
+    uint4 w[P2];
+    uint4 x0[P2][XN], x1[P2][XN];
+  };
+  auto load = [&](Set& b, int q) {
+#pragma unroll
+    for (int i = 0; i < P2; i++) {
+      const int p = (q + i) / steps, s = (q + i) - p * steps, at = s * 64 + 16 * h;
+      b.w[i] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int u = 0; u < XN; u++) b.x0[i][u] = b.x1[i][u] = make_uint4(0, 0, 0, 0);
+      if (q + i < q1 && at < rowb) {
+        const int u = 2 * p + (r >= 8);
+        if (u < n)
+          b.w[i] = ld16nt((const uint8_t*)a.w2 + ((size_t)used[u] * H + n0 + (r & 7)) * rowb + at);
+        const int j0 = r < T ? slot[2 * p][r] : -1, j1 = r < T && 2 * p + 1 < n ? slot[2 * p + 1][r] : -1;
+#pragma unroll
+        for (int v = 0; v < XN; v++) {
+          if (j0 >= 0) b.x0[i][v] = *(const uint4*)((const uint16_t*)a.act + ((size_t)r * k + j0) * I + at / WB + 8 * v);
+          if (j1 >= 0) b.x1[i][v] = *(const uint4*)((const uint16_t*)a.act + ((size_t)r * k + j1) * I + at / WB + 8 * v);
+        }
+      }
+    }
+  };
+  // a pair is done (or the run is): its products to the sums
+  auto fold = [&](int p) {
+    const int u = 2 * p + (h >= 2);
+    if (u < n) {
+      if (slot[u][r] >= 0) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          float f = wts[u][r];
+          if constexpr (Q8) f *= ub_load<DT>(a.s2, (size_t)used[u] * H + n0 + 4 * (h & 1) + i);
+          sum[i] += (h >= 2 ? s1[i] : s0[i]) * f;
+        }
+      }
+    }
+    s0 = s1 = (f32x4){0.f, 0.f, 0.f, 0.f};
+  };
+  auto mul = [&](Set& b, int q) {
+#pragma unroll
+    for (int i = 0; i < P2; i++) {
+      if (q + i >= q1) break;
+      s0 = product<DT, Q8>(b.w[i], b.x0[i], s0);
+      s1 = product<DT, Q8>(b.w[i], b.x1[i], s1);
+      if ((q + i + 1) % steps == 0 || q + i + 1 == q1) fold((q + i) / steps);
+    }
+  };
+  Set b0, b1;
+  load(b0, q0);
+  for (int q = q0; q < q1; q += 2 * P2) {
+    load(b1, q + P2);
+    mul(b0, q);
+    load(b0, q + 2 * P2);
+    mul(b1, q + P2);
+  }
+  *(f32x4*)&red[wave][r][4 * h] = sum;
+  __syncthreads();
+  if (tid < 8 * T) {
+    const int t = tid >> 3, c = tid & 7;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < W2; w++) v += red[w][t][c] + red[w][t][8 + c];
+    ub_store<DT>(a.y, (size_t)t * H + n0 + c, v);
+  }
+}
+
+template <int DT, bool Q8, int NPL>
+void up(const DecodeArgs& a, hipStream_t s) {
+  const int steps = ub_cdiv(a.H * (Q8 ? 1 : 2), 64), per = ub_cdiv(steps, W1);
+  const long items = (long)std::min(a.T * a.k, a.E) * (a.I / 8);
+  const unsigned g = (unsigned)std::min<long>(items, 512);  // two workgroups a CU
+  if (per <= 1) k_up<DT, Q8, NPL, 1, false><<<g, 64 * W1, 0, s>>>(a);
+  else if (per <= 2) k_up<DT, Q8, NPL, 2, false><<<g, 64 * W1, 0, s>>>(a);
+  else if (per <= 4) k_up<DT, Q8, NPL, 4, false><<<g, 64 * W1, 0, s>>>(a);
+  else if (per <= 8) k_up<DT, Q8, NPL, 8, false><<<std::min(g, 256u), 64 * W1, 0, s>>>(a);
+  else k_up<DT, Q8, NPL, 4, true><<<g, 64 * W1, 0, s>>>(a);
+}
+template <int DT, bool Q8>
+void decode(const DecodeArgs& a, hipStream_t s) {
+  if (a.E <= 128) up<DT, Q8, 2>(a, s);
+  else if (a.E <= 256) up<DT, Q8, 4>(a, s);
+  else up<DT, Q8, kE / 64>(a, s);
+  k_down<DT, Q8><<<a.H / 8, 64 * W2, 0, s>>>(a);
+}
+
+}  // namespace
+
+UB_API int ubridge_moe_decode(const UbridgeMoeDecodeArgs* p, void* stream) {
+  const char* nm = "ubridge_moe_decode";
+  UB_REQUIRE(p, "%s: null argument block", nm);
+  UB_REQUIRE(p->dtype == UB_F16 || p->dtype == UB_BF16, "%s: dtype %d", nm, p->dtype);
+  UB_REQUIRE(p->logits_dtype >= UB_F32 && p->logits_dtype <= UB_BF16, "%s: logits of type %d", nm, p->logits_dtype);
+  UB_REQUIRE(p->T >= 0 && p->T <= kTok, "%s: T=%d (at most %d tokens)", nm, p->T, kTok);
+  UB_REQUIRE(p->E > 0 && p->E <= kE && p->k > 0 && p->k <= kK && p->k <= p->E, "%s: E=%d k=%d (E <= %d, 0 < k <= min(E, %d))", nm, p->E,
+             p->k, kE, kK);
+  UB_REQUIRE(p->H > 0 && p->H % 32 == 0 && p->I > 0 && p->I % 32 == 0 && p->H <= 1 << 20 && p->I <= 1 << 20,
+             "%s: H=%d I=%d (multiples of 32)", nm, p->H, p->I);
+  if (p->T == 0) return UB_OK;
+  UB_REQUIRE(p->x && p->logits && p->w13 && p->w2 && p->y, "%s: null pointer", nm);
+  UB_REQUIRE(!p->s13 == !p->s2, "%s: one of two scales", nm);
+  UB_REQUIRE((((uintptr_t)p->x | (uintptr_t)p->w13 | (uintptr_t)p->w2) & 15) == 0, "%s: x or weights not 16-byte aligned", nm);
+  hipStream_t s = ub_stream(stream);
+  const size_t act = ((size_t)p->T * p->k * p->I * 2 + 255) / 256 * 256;
+  UbScratch ws(s, act + sizeof(Route));
+  UB_REQUIRE(ws.get(), "%s: no workspace", nm);
+  const DecodeArgs a = {p->x, p->logits, p->w13, p->s13, p->w2, p->s2, p->y, ws.get(), (Route*)((char*)ws.get() + act),
+                        p->T, p->E, p->k, p->H, p->I, p->logits_dtype, p->renormalize};
+  if (p->s13) p->dtype == UB_F16 ? decode<UB_F16, true>(a, s) : decode<UB_BF16, true>(a, s);
+  else p->dtype == UB_F16 ? decode<UB_F16, false>(a, s) : decode<UB_BF16, false>(a, s);
+  return ub_check_launch(nm);
+}

@@ -5,7 +5,7 @@ device buffers out, stream last).  It has no gradient."""
 import torch
 
 from .native import _native, call
-from .ops import _need_cuda
+from .ops import _DT_CODE, _need_cuda
 
 MAX_K = 132104  # where the int32 sum of K products stays exact
 
@@ -46,3 +46,15 @@ class Linear:
         return call(_native.linear, stream, x, self.w, self.w_scale, self.bias, self.K, out)
 
     __call__ = forward
+
+    def codes(self, a, scales, dtype=torch.bfloat16, out=None, stream=None):
+        """The same of activations that are in codes already: a int8 [..., K] and f32
+        scales [...], as norm.RmsNorm(...)(x, quant="int8") makes them; y is of dtype."""
+        if dtype not in _DT_CODE:
+            raise ValueError(f"int8.Linear: dtype {dtype}")
+        if a.shape[-1:] != (self.K,):
+            raise ValueError(f"int8.Linear: codes must be [..., {self.K}]")
+        if self.ld != self.K:
+            a = torch.nn.functional.pad(a, (0, self.ld - self.K))
+        return call(_native.linear_codes, stream, a, scales, self.w, self.w_scale, self.bias, self.K,
+                    _DT_CODE[dtype], out)

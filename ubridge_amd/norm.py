@@ -1,0 +1,77 @@
+"""Root-mean-square norm of a residual stream: the addition to it, the norm, and
+the rounding that the next product wants, in one launch; differentiable where the
+result keeps its type."""
+import torch
+from torch.autograd.function import once_differentiable
+
+from .native import _native, call
+from .ops import _need_cuda
+
+_OUT = {None: 0, "int8": 1, "e4m3": 2, "fp4": 3, "fp8": 4}
+
+
+class RmsNorm:
+    """y = h * weight / sqrt(mean(h ** 2) + eps), with h = x + residual rounded to
+    x's type (h = x without a residual): the norm is of the stream as it is stored.
+
+    weight [C] f32, or of x's type; x and residual [..., C] f32, f16 or bf16, a row
+    at most 64 KiB.  norm(x) -> y; norm(x, residual) -> (y, h), h in `residual_out` if
+    it is given, which may be residual or x itself.  quant rounds y from f32 for the
+    next product and puts two tensors in its place:
+
+      "int8"        codes int8 [..., C] and f32 scales [...], amax / 127 (1 for a row
+                    of zeros), for int8.Linear.codes
+      "e4m3"        codes uint8 and f32 scales, amax / 448, for fp8.gemm
+      "fp4", "fp8"  microscaled blocks as mx.quantize makes them, for mx.Linear.codes
+
+    A row that holds an infinity or a NaN gives NaN (as int8 and e4m3: the scale; in
+    blocks: the blocks that hold one).  Without quant the call is differentiable, once,
+    in x, residual and weight; with it, or into residual_out, it has no gradient and
+    refuses inputs that ask for one.
+    """
+
+    def __init__(self, weight, eps=1e-6):
+        _need_cuda(weight)
+        self.weight, self.eps = weight, float(eps)
+
+    def forward(self, x, residual=None, quant=None, residual_out=None, stream=None):
+        if quant not in _OUT:
+            raise ValueError(f"RmsNorm: quant {quant!r} (one of {list(_OUT)})")
+        w = self.weight
+        if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad
+                                        or residual is not None and residual.requires_grad):
+            if quant is not None or residual_out is not None:
+                raise ValueError("RmsNorm: no gradient with quant or residual_out")
+            y, h = _Norm.apply(x, residual, w, self.eps, stream)
+            return y if residual is None else (y, h)
+        y, scale, h = call(_native.norm, stream, x, w, residual, residual_out, self.eps, _OUT[quant])
+        r = (y,) if scale is None else (y, scale)
+        if h is not None:
+            r += (h,)
+        return r if len(r) > 1 else y
+
+    __call__ = forward
+
+
+class _Norm(torch.autograd.Function):
+    """(y, h).  The gradient starts from h as it is stored; of x and of residual it
+    is the same."""
+
+    @staticmethod
+    def forward(ctx, x, residual, w, eps, stream):
+        y, _, h = call(_native.norm, stream, x, w, residual, None, eps, 0)
+        ctx.eps, ctx.stream, ctx.added = eps, stream, residual is not None
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x if h is None else h, w)
+        return y, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh):
+        h, w = ctx.saved_tensors
+        need_x, need_res, need_w = ctx.needs_input_grad[:3]
+        if dy is None:  # only h was used
+            dx, dw = dh, torch.zeros_like(w) if need_w else None
+        else:
+            dx, dw = call(_native.norm_grad, None, h.contiguous(), w, dy, dh, ctx.eps, need_x or need_res, need_w)
+        return dx if need_x else None, dx if need_res else None, dw, None, None
