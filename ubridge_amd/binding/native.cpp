@@ -562,7 +562,7 @@ PyObject* py_mx_quantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int dt = code(*x), f = (int)A.n(1);
   if (dt < 0 || dt > 2 || x->dim() == 0 || x->size(-1) == 0) REFUSE("mx.quantize takes f32, f16 or bf16 [..., C]");
   const int64_t C = x->size(-1), R = x->numel() / C;
-  if (!fits(R) || C > 1 << 30 || R * (C + 127) > 1ll << 34) REFUSE("mx.quantize: %ld rows of %ld", R, C);
+  if (!fits(R) || C > 1 << 30 || R * (C + 127) > 1ll << 33) REFUSE("mx.quantize: %ld rows of %ld", R, C);
   at::Tensor xc = dense(*x) ? *x : x->contiguous();
   at::Tensor q = result(ended(*x, padded(C) * f / 8), *x, at::kByte), s = result(ended(*x, padded(C) / 32), *x, at::kByte);
   void* stream = A.p(2);
@@ -597,7 +597,7 @@ PyObject* py_mx_dequantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int dt = (int)A.n(3), f = (int)A.n(4);
   if (PyErr_Occurred() || !block_rows("mx.dequantize", q, s, C, f) || !together("mx.dequantize", {q, s})) return nullptr;
   const int64_t R = q->numel() / q->size(-1);
-  if (!fits(R) || R * (C + 127) > 1ll << 34) REFUSE("mx.dequantize: %ld rows of %ld", R, C);
+  if (!fits(R) || R * (C + 127) > 1ll << 33) REFUSE("mx.dequantize: %ld rows of %ld", R, C);
   at::Tensor y = result(ended(*q, C), *q, type_of(dt));
   void* stream = A.p(5);
   if (PyErr_Occurred()) return nullptr;
@@ -651,7 +651,7 @@ PyObject* py_mx_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     REFUSE("mx.Linear: weight as mx.Linear laid it out, bias contiguous float32 [%ld]", N);
   if (!together("mx.Linear", {x, s, w, ws, b, out})) return nullptr;
   const int64_t M = x->numel() / x->size(-1);
-  if (M >= 1 << 22 || M * N >= 1ll << 38 || M * K > 1ll << 34) REFUSE("mx.Linear: %ld rows of %ld to %ld", M, K, N);
+  if (M >= 1 << 22 || M * N >= 1ll << 38 || (M + 15) * (K + 127) > 1ll << 33) REFUSE("mx.Linear: %ld rows of %ld to %ld", M, K, N);
   const auto sizes = ended(*x, N);
   if (out && (out->scalar_type() != type_of(dt) || out->sizes() != at::IntArrayRef(sizes) || !dense(*out)))
     REFUSE("mx.Linear: out must be contiguous, of y's type, [..., %ld]", N);

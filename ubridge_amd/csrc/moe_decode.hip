@@ -19,8 +19,11 @@
 //    runs of the items; 8 wavefronts split K, each one run of its rows, two items in
 //    flight.
 //  * k_down: a workgroup owns 8 output columns and adds all experts' parts, so no sums
-//    cross workgroups: 8 rows of each of two experts are the 16 rows of a product,
-//    multiplied by either's activations, and lane half h keeps the one that is its own.
+//    cross workgroups.  8 rows of each of two experts are the 16 rows of a product, and
+//    up to 8 tokens of the one and 8 of the other its columns (an expert with more is
+//    listed twice); the two quarters where rows and tokens belong together are kept.
+//  * Scales are asked for ahead of the weights that they go with: loads return in order,
+//    and one asked for at the end of an item would wait for all weights in flight.
 #include "moe_dev.h"
 
 #include <algorithm>
@@ -33,14 +36,17 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTok = 16, kK = 16, kE = 1024, kUsed = kTok * kK;  // most tokens, top-k, experts; experts in use
+constexpr int kEnt = kUsed + kUsed / 8;                          // entries of the list below
 
-// The routing, in scratch memory from k_up to k_down: experts in use, in order, and for
-// each and every token its weight and its slot (-1: not chosen).
+// The routing, in scratch memory from k_up to k_down: experts in use, each with up to 8
+// of its tokens (more: another entry): rows of the activations (t k + j; -1: none),
+// tokens and weights.
 struct Route {
-  int n;
-  int used[kUsed];
-  float w[kUsed][kTok];
-  int8_t slot[kUsed][kTok];
+  int n, pad[3];
+  int expert[kEnt];
+  int16_t row[kEnt][8];
+  int8_t tok[kEnt][8];
+  float w[kEnt][8];
 };
 
 struct DecodeArgs {
@@ -139,8 +145,8 @@ template <int DT, bool Q8, int NPL, int SP, bool MULTI>
 __global__ void __launch_bounds__(64 * W1) __attribute__((amdgpu_waves_per_eu(SP > 4 ? 2 : 4, SP > 4 ? 2 : 4))) k_up(DecodeArgs a) {
   constexpr int WB = Q8 ? 1 : 2, EL = 64 / WB, XN = Q8 ? 2 : 1;  // bytes of a weight; elements of a step; operands
   __shared__ __attribute__((aligned(16))) int8_t slot[kE][kTok];
-  __shared__ uint16_t used[kUsed];
-  __shared__ int nused;
+  __shared__ uint16_t used[kUsed], tokens[kUsed], entry[kUsed];  // experts in use, their tokens (bits), first entries
+  __shared__ int nused, nent;
   __shared__ __attribute__((aligned(16))) float red[2][W1][16][20];
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, h = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -193,43 +199,69 @@ __global__ void __launch_bounds__(64 * W1) __attribute__((amdgpu_waves_per_eu(SP
   }
   __syncthreads();
   if (wave == 0) {
-    int n = 0;
+    int n = 0, m = 0;
     for (int e0 = 0; e0 < E; e0 += 64) {
       const int e = e0 + lane;
-      bool any = false;
+      uint32_t bits = 0;
       if (e < E) {
         const int4 v = *(const int4*)slot[e];
-        any = (v.x & v.y & v.z & v.w) != -1;
+        const int w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int q = 0; q < 4; q++) {  // the sign bits of four bytes, together
+          const uint32_t s = ~(uint32_t)w[q] & 0x80808080u;
+          bits |= ((s >> 7 | s >> 14 | s >> 21 | s >> 28) & 15u) << (4 * q);
+        }
       }
-      const uint64_t m = __ballot(any);
-      if (any) used[n + __popcll(m & ((1ull << lane) - 1))] = (uint16_t)e;
-      n += __popcll(m);
+      const uint64_t one = __ballot(bits != 0), two = __ballot(__popc(bits) > 8), below = (1ull << lane) - 1;
+      if (bits) {
+        const int at = n + __popcll(one & below);
+        used[at] = (uint16_t)e;
+        tokens[at] = (uint16_t)bits;
+        entry[at] = (uint16_t)(m + __popcll(one & below) + __popcll(two & below));
+      }
+      n += __popcll(one);
+      m += __popcll(one) + __popcll(two);
     }
-    if (lane == 0) nused = n;
+    if (lane == 0) nused = n, nent = m;
   }
   __syncthreads();
   const int nu = __builtin_amdgcn_readfirstlane(nused);
   if (first) {
-    if (tid == 0) a.route->n = nu;
-    for (int i = tid; i < nu * kTok; i += 64 * W1) {
-      const int e = used[i / kTok], t = i % kTok, j = slot[e][t];
-      if (t == 0) a.route->used[i / kTok] = e;
-      a.route->slot[i / kTok][t] = (int8_t)j;
-      a.route->w[i / kTok][t] = j >= 0 ? wts[t][j] : 0.f;
+    if (tid == 0) a.route->n = nent;
+    for (int i = tid; i < nu * 16; i += 64 * W1) {
+      const int u = i >> 4, p = i & 15, e = used[u], bits = tokens[u], n = __popc(bits), at = entry[u] + (p >> 3);
+      if (p >= (n > 8 ? 16 : 8)) continue;
+      int b = bits;  // the p-th token of the expert
+      for (int q = 0; q < p; q++) b &= b - 1;
+      const int t = b ? __builtin_ctz(b) : -1, j = t >= 0 ? slot[e][t] : 0;
+      a.route->expert[at] = e;
+      a.route->row[at][p & 7] = (int16_t)(t >= 0 ? t * a.k + j : -1);
+      a.route->tok[at][p & 7] = (int8_t)t;
+      a.route->w[at][p & 7] = t >= 0 ? wts[t][j] : 0.f;
     }
   }
   // ---- items: (expert in use, 8 columns), equal runs of them
   const int nc = I / 8, G = gridDim.x;
   const long items = (long)nu * nc;
-  const int i0 = (int)(items * blockIdx.x / G), i1 = (int)(items * (blockIdx.x + 1) / G);
+  // (of two workgroups of a CU, blocks 256 apart, neighbouring runs: one longer than the
+  // other, if they are not the same)
+  const int run = G == 512 ? ((int)blockIdx.x & 255) * 2 + ((int)blockIdx.x >> 8) : (int)blockIdx.x;
+  const int i0 = (int)(items * run / G), i1 = (int)(items * (run + 1) / G);
   const int pieces = MULTI ? ((rowb + 63) / 64 + W1 * SP - 1) / (W1 * SP) : 1;
   struct Set {
     uint4 w[SP];
     uint4 x[MULTI ? SP : 1][XN];
+    float sg, su;  // scales of the thread's output
   };
+  const int ot = tid >> 3, oc = tid & 7;  // its token and column
   auto load = [&](Set& b, int it, int p) {
     const int u = min(it, i1 - 1) / nc, c = min(it, i1 - 1) - u * nc;
     const int e = used[u];
+    if (Q8 && tid < 8 * T && p == pieces - 1) {
+      const size_t at = (size_t)e * 2 * I + 8 * c + oc;
+      b.sg = ub_load<DT>(a.s13, at);
+      b.su = ub_load<DT>(a.s13, at + I);
+    }
     const uint8_t* row = (const uint8_t*)a.w13 + ((size_t)e * 2 * I + (r < 8 ? 8 * c + r : I + 8 * c + r - 8)) * rowb;
 #pragma unroll
     for (int i = 0; i < SP; i++) {
@@ -239,14 +271,22 @@ __global__ void __launch_bounds__(64 * W1) __attribute__((amdgpu_waves_per_eu(SP
       if constexpr (MULTI) acts(b.x[i], s);
     }
   };
+  const int total = (i1 - i0) * pieces;
+  auto item = [&](int q) { return MULTI ? i0 + q / pieces : i0 + q; };
+  auto piece = [&](int q) { return MULTI ? q % pieces : 0; };
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  auto mul = [&](Set& b, int it, int p, int buf) {
+  // piece q, in b; then piece q + 2's loads
+  auto mul = [&](Set& b, int q, int buf) {
+    const int it = item(q);
 #pragma unroll
     for (int i = 0; i < SP; i++) {
       if constexpr (MULTI) acc = product<DT, Q8>(b.w[i], b.x[i], acc);
       else acc = product<DT, Q8>(b.w[i], xf[i], acc);
     }
-    if (p != pieces - 1) return;
+    const bool last = piece(q) == pieces - 1;
+    const float sg = b.sg, su = b.su;
+    load(b, item(q + 2), piece(q + 2));
+    if (!last) return;
     // lane (token r, h) holds rows 4 h .. + 3: gate rows for h < 2, up rows above
     *(f32x4*)&red[buf][wave][r][4 * h] = acc;
     acc = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -255,33 +295,26 @@ __global__ void __launch_bounds__(64 * W1) __attribute__((amdgpu_waves_per_eu(SP
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     if (tid < 8 * T) {
-      const int t = tid >> 3, c = tid & 7, u = it / nc, col = (it - u * nc) * 8 + c, e = used[u], j = slot[e][t];
+      const int u = it / nc, col = (it - u * nc) * 8 + oc, j = slot[used[u]][ot];
       if (j >= 0) {
         float g = 0.f, up = 0.f;
 #pragma unroll
-        for (int w = 0; w < W1; w++) g += red[buf][w][t][c], up += red[buf][w][t][8 + c];
-        if constexpr (Q8) {
-          g *= ub_load<DT>(a.s13, (size_t)e * 2 * I + col);
-          up *= ub_load<DT>(a.s13, (size_t)e * 2 * I + I + col);
-        }
-        ub_store<DT>(a.act, ((size_t)t * a.k + j) * I + col, g / (1.f + expf(-g)) * up);
+        for (int w = 0; w < W1; w++) g += red[buf][w][ot][oc], up += red[buf][w][ot][8 + oc];
+        if constexpr (Q8) g *= sg, up *= su;
+        ub_store<DT>(a.act, ((size_t)ot * a.k + j) * I + col, g / (1.f + expf(-g)) * up);
       }
     }
   };
   if (i0 >= i1) return;
   Set b0, b1;
-  const int total = (i1 - i0) * pieces;
-  auto item = [&](int q) { return MULTI ? i0 + q / pieces : i0 + q; };
-  auto piece = [&](int q) { return MULTI ? q % pieces : 0; };
   load(b0, item(0), piece(0));
+  load(b1, item(1), piece(1));
   int done = 0;  // items summed: their buffers alternate
   for (int q = 0; q < total; q += 2) {
-    load(b1, item(q + 1), piece(q + 1));
-    mul(b0, item(q), piece(q), done & 1);
+    mul(b0, q, done & 1);
     if (piece(q) == pieces - 1) done++;
     if (q + 1 >= total) break;
-    load(b0, item(q + 2), piece(q + 2));
-    mul(b1, item(q + 1), piece(q + 1), done & 1);
+    mul(b1, q + 1, done & 1);
     if (piece(q + 1) == pieces - 1) done++;
   }
 }
@@ -289,89 +322,104 @@ __global__ void __launch_bounds__(64 * W1) __attribute__((amdgpu_waves_per_eu(SP
 constexpr int W2 = 16;  // wavefronts of k_down
 
 template <int DT, bool Q8>
-__global__ void __launch_bounds__(64 * W2) k_down(DecodeArgs a) {
-  constexpr int WB = Q8 ? 1 : 2, XN = Q8 ? 2 : 1, P2 = Q8 ? 2 : 4;  // P2: steps in a set
-  __shared__ int used[kUsed];
-  __shared__ float wts[kUsed][kTok];
-  __shared__ int8_t slot[kUsed][kTok];
-  __shared__ __attribute__((aligned(16))) float red[W2][16][20];
+__global__ void __launch_bounds__(64 * W2) k_down(DecodeArgs a, int most) {
+  constexpr int WB = Q8 ? 1 : 2, XN = Q8 ? 2 : 1, P = Q8 ? 4 : 6;  // P: steps in a set
+  __shared__ int expert[kEnt + 1];
+  __shared__ int16_t row[kEnt + 1][8];
+  __shared__ int8_t tok[kEnt][8];
+  __shared__ float wts[kEnt][8], sc[kEnt][8];
+  __shared__ float ys[W2][kTok][8];  // a wavefront's sums
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, h = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int T = a.T, H = a.H, I = a.I, k = a.k;
-  const int n = min(a.route->n, kUsed), n0 = blockIdx.x * 8;
-  for (int i = tid; i < n * kTok; i += 64 * W2) {
+  const int T = a.T, H = a.H, I = a.I, n0 = blockIdx.x * 8;
+  const int n = a.route->n;
+  // (entries past n, up to what there can be, are read with the others and not used)
+  for (int i = tid; i < most * 8; i += 64 * W2) {
+    const int u = i >> 3, c = i & 7;
+    (&row[0][0])[i] = (&a.route->row[0][0])[i];
+    (&tok[0][0])[i] = (&a.route->tok[0][0])[i];
     (&wts[0][0])[i] = (&a.route->w[0][0])[i];
-    (&slot[0][0])[i] = (&a.route->slot[0][0])[i];
-    if (i < n) used[i] = a.route->used[i];
+    const int e = a.route->expert[u];
+    if (c == 0) expert[u] = e;
+    if (Q8 && u < n) sc[u][c] = ub_load<DT>(a.s2, (size_t)e * H + n0 + c);
   }
+  for (int i = tid; i < W2 * kTok * 8; i += 64 * W2) (&ys[0][0][0])[i] = 0.f;
   __syncthreads();
-  // units: (pair of experts, 64-byte step of their rows), a run of them to a wavefront
+  if (tid < 8) row[n][tid] = -1;  // the partner of an odd last entry
+  __syncthreads();
+  // units: (pair of entries, 64-byte step of their rows), a run of them to a wavefront
   const int rowb = I * WB, steps = (rowb + 63) / 64, units = (n + 1) / 2 * steps;
   const int q0 = (int)((long)units * wave / W2), q1 = (int)((long)units * (wave + 1) / W2);
-  f32x4 sum = {0.f, 0.f, 0.f, 0.f}, s0 = sum, s1 = sum;
+  const int side = r >> 3, c8 = r & 7;
   struct Set {
-    uint4 w[P2];
-    uint4 x0[P2][XN], x1[P2][XN];
+    uint4 w[P], x[P][XN];
   };
-  auto load = [&](Set& b, int q) {
+  int lq = q0, lp = q0 / steps, ls = q0 - lp * steps;  // the unit to be loaded next
+  auto load = [&](Set& b) {
 #pragma unroll
-    for (int i = 0; i < P2; i++) {
-      const int p = (q + i) / steps, s = (q + i) - p * steps, at = s * 64 + 16 * h;
+    for (int i = 0; i < P; i++) {
       b.w[i] = make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int u = 0; u < XN; u++) b.x0[i][u] = b.x1[i][u] = make_uint4(0, 0, 0, 0);
-      if (q + i < q1 && at < rowb) {
-        const int u = 2 * p + (r >= 8);
-        if (u < n)
-          b.w[i] = ld16nt((const uint8_t*)a.w2 + ((size_t)used[u] * H + n0 + (r & 7)) * rowb + at);
-        const int j0 = r < T ? slot[2 * p][r] : -1, j1 = r < T && 2 * p + 1 < n ? slot[2 * p + 1][r] : -1;
+      for (int v = 0; v < XN; v++) b.x[i][v] = make_uint4(0, 0, 0, 0);
+      const int at = ls * 64 + 16 * h, u = 2 * lp + side;
+      if (lq < q1) {
+        const int ar = row[u][c8];
+        if (at < rowb) {
+          if (u < n) b.w[i] = ld16nt((const uint8_t*)a.w2 + ((size_t)expert[u] * H + n0 + c8) * rowb + at);
+          if (ar >= 0) {
 #pragma unroll
-        for (int v = 0; v < XN; v++) {
-          if (j0 >= 0) b.x0[i][v] = *(const uint4*)((const uint16_t*)a.act + ((size_t)r * k + j0) * I + at / WB + 8 * v);
-          if (j1 >= 0) b.x1[i][v] = *(const uint4*)((const uint16_t*)a.act + ((size_t)r * k + j1) * I + at / WB + 8 * v);
+            for (int v = 0; v < XN; v++) b.x[i][v] = *(const uint4*)((const uint16_t*)a.act + (size_t)ar * I + at / WB + 8 * v);
+          }
         }
+        lq++;
+        if (++ls == steps) ls = 0, lp++;
       }
     }
   };
-  // a pair is done (or the run is): its products to the sums
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  // a pair is done (or the run is): its products to the sums.  Lane (column r, h): rows 4 h
+  // .. + 3, which belong to r's entry if both are of the same half.  The two entries may
+  // share a token: one after the other.
   auto fold = [&](int p) {
-    const int u = 2 * p + (h >= 2);
-    if (u < n) {
-      if (slot[u][r] >= 0) {
+    const int u = 2 * p + side;
+    const bool mine = u < n && (h >> 1) == side && row[u][c8] >= 0;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          float f = wts[u][r];
-          if constexpr (Q8) f *= ub_load<DT>(a.s2, (size_t)used[u] * H + n0 + 4 * (h & 1) + i);
-          sum[i] += (h >= 2 ? s1[i] : s0[i]) * f;
-        }
+    for (int s = 0; s < 2; s++) {
+      if (mine && side == s) {
+        float* y = &ys[wave][tok[u][c8]][4 * (h & 1)];
+#pragma unroll
+        for (int i = 0; i < 4; i++) y[i] += acc[i] * (Q8 ? wts[u][c8] * sc[u][4 * (h & 1) + i] : wts[u][c8]);
       }
+      __builtin_amdgcn_wave_barrier();
+      asm volatile("" ::: "memory");
     }
-    s0 = s1 = (f32x4){0.f, 0.f, 0.f, 0.f};
+    acc = (f32x4){0.f, 0.f, 0.f, 0.f};
   };
-  auto mul = [&](Set& b, int q) {
+  int mq = q0, mp = q0 / steps, ms = q0 - mp * steps;  // the unit to be multiplied next
+  auto mul = [&](Set& b) {
 #pragma unroll
-    for (int i = 0; i < P2; i++) {
-      if (q + i >= q1) break;
-      s0 = product<DT, Q8>(b.w[i], b.x0[i], s0);
-      s1 = product<DT, Q8>(b.w[i], b.x1[i], s1);
-      if ((q + i + 1) % steps == 0 || q + i + 1 == q1) fold((q + i) / steps);
+    for (int i = 0; i < P; i++) {
+      if (mq >= q1) break;
+      acc = product<DT, Q8>(b.w[i], b.x[i], acc);
+      mq++;
+      if (++ms == steps || mq == q1) fold(mp);
+      if (ms == steps) ms = 0, mp++;
     }
+    load(b);
   };
   Set b0, b1;
-  load(b0, q0);
-  for (int q = q0; q < q1; q += 2 * P2) {
-    load(b1, q + P2);
-    mul(b0, q);
-    load(b0, q + 2 * P2);
-    mul(b1, q + P2);
+  load(b0);
+  load(b1);
+  while (mq < q1) {
+    mul(b0);
+    mul(b1);
   }
-  *(f32x4*)&red[wave][r][4 * h] = sum;
   __syncthreads();
   if (tid < 8 * T) {
     const int t = tid >> 3, c = tid & 7;
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < W2; w++) v += red[w][t][c] + red[w][t][8 + c];
+    for (int w = 0; w < W2; w++) v += ys[w][t][c];
     ub_store<DT>(a.y, (size_t)t * H + n0 + c, v);
   }
 }
@@ -392,7 +440,8 @@ void decode(const DecodeArgs& a, hipStream_t s) {
   if (a.E <= 128) up<DT, Q8, 2>(a, s);
   else if (a.E <= 256) up<DT, Q8, 4>(a, s);
   else up<DT, Q8, kE / 64>(a, s);
-  k_down<DT, Q8><<<a.H / 8, 64 * W2, 0, s>>>(a);
+  const int slots = a.T * a.k, most = std::min(slots, a.E) + slots / 9;  // (another entry where an expert has 9 tokens)
+  k_down<DT, Q8><<<a.H / 8, 64 * W2, 0, s>>>(a, most);
 }
 
 }  // namespace

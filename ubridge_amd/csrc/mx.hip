@@ -49,49 +49,34 @@ __device__ __forceinline__ size_t scale_at(size_t row, int b, int nk) {
 }
 
 // ------------------------------------------------------- blocks and back
-// A thread takes units of 16 bytes of x, 256 apart, all loaded before the first is
+// A thread takes U units of 16 bytes of x, 256 apart, all loaded before the first is
 // rounded; the 4 (f32: 8) lanes of a block find its largest by DPP.
-template <int DT, int F, bool PACKED>
+template <int DT, int F, bool PACKED, int U>
 __global__ void __launch_bounds__(256) k_mx_quant(const void* __restrict__ x, uint8_t* __restrict__ q,
-                                                  uint8_t* __restrict__ sc, int64_t units, int C, int nk) {
+                                                  uint8_t* __restrict__ sc, uint32_t units, int C, int nk) {
   typedef typename MxElem<DT>::T T;
-  constexpr int E = MxElem<DT>::E, BL = 32 / E, U = 4;
+  constexpr int E = MxElem<DT>::E, BL = 32 / E;
   const uint32_t per = (uint32_t)nk * (128 / E);  // units a row
   uint4 v[U];
-  const int64_t i0 = (int64_t)blockIdx.x * (256 * U) + threadIdx.x;
+  const uint32_t i0 = blockIdx.x * (256u * U) + threadIdx.x;
 #pragma unroll
   for (int j = 0; j < U; j++) {
-    const int64_t i = i0 + j * 256;
+    const uint32_t i = i0 + j * 256;
     v[j] = make_uint4(0, 0, 0, 0);
     if (i < units) {
-      const int64_t row = i / per;
-      v[j] = mx_unit_at<DT>((const T*)x + row * C, (int)(i - row * per), C);
+      const uint32_t row = i / per;
+      v[j] = mx_unit_at<DT>((const T*)x + (size_t)row * C, (int)(i - row * per), C);
     }
   }
 #pragma unroll
   for (int j = 0; j < U; j++) {
-    const int64_t i = i0 + j * 256;
-    float f[E];
-    uint32_t t = 0;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-      f[e] = mx_get<DT>(v[j], e);
-      t = max(t, __float_as_uint(f[e]) & 0x7fffffffu);
-    }
-    const uint32_t b = mx_byte<F>(mx_top<BL>(t));
+    const uint32_t i = i0 + j * 256;
+    uint32_t o[2];
+    const uint32_t b = mx_round<DT, F>(v[j], o);
     if (i >= units) continue;  // (whole blocks: units is a multiple of theirs)
-    const int64_t row = i / per;
+    const uint32_t row = i / per;
     const int u = (int)(i - row * per), blk = u / BL;
-    uint8_t* o = q + code_at<F, PACKED>(row, blk, nk) + (u % BL) * (E * F / 8);
-    if constexpr (F == MX_FP8) {
-#pragma unroll
-      for (int p = 0; p < E / 4; p++)
-        ((uint32_t*)o)[p] = mx_codes4<F>(f[4 * p], f[4 * p + 1], f[4 * p + 2], f[4 * p + 3], b);
-    } else if constexpr (E == 8) {
-      *(uint32_t*)o = mx_codes4<F>(f[0], f[1], f[2], f[3], b) | mx_codes4<F>(f[4], f[5], f[6], f[7], b) << 16;
-    } else {
-      *(uint16_t*)o = (uint16_t)mx_codes4<F>(f[0], f[1], f[2], f[3], b);
-    }
+    mx_store<DT, F>(q + code_at<F, PACKED>(row, blk, nk) + (u % BL) * (E * F / 8), o);
     if (u % BL == 0) sc[scale_at<PACKED>(row, blk, nk)] = (uint8_t)b;
   }
 }
@@ -99,14 +84,13 @@ __global__ void __launch_bounds__(256) k_mx_quant(const void* __restrict__ x, ui
 // A thread takes 8 elements.
 template <int DT, int F>
 __global__ void __launch_bounds__(256) k_mx_back(const uint8_t* __restrict__ q, const uint8_t* __restrict__ sc,
-                                                 void* __restrict__ y, int64_t units, int C, int nk) {
+                                                 void* __restrict__ y, uint32_t units, int C, int nk) {
   typedef typename MxElem<DT>::T T;
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   constexpr int E = MxElem<DT>::E;
-  const int per = (C + 7) / 8;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const uint32_t per = (uint32_t)(C + 7) / 8, i = blockIdx.x * 256u + threadIdx.x;
   if (i >= units) return;
-  const int64_t row = i / per;
+  const uint32_t row = i / per;
   const int u = (int)(i - row * per);
   const uint8_t* p = q + code_at<F, false>(row, u / 4, nk) + (u & 3) * F;
   const uint32_t b = sc[scale_at<false>(row, u / 4, nk)];
@@ -135,24 +119,24 @@ __global__ void __launch_bounds__(256) k_mx_back(const uint8_t* __restrict__ q, 
 #pragma unroll
   for (int e = 0; e < 8; e++) f[e] *= s;
 #pragma unroll
-  for (int h = 0; h < 8 / E; h++) mx_put<DT>((T*)y + row * C, u * (8 / E) + h, C, mx_pack<DT>(f + h * E));
+  for (int h = 0; h < 8 / E; h++) mx_put<DT>((T*)y + (size_t)row * C, u * (8 / E) + h, C, mx_pack<DT>(f + h * E));
 }
 
 // From rows to the products' layout; rows past R up to a multiple of 16 are zero.
 template <int F>
 __global__ void __launch_bounds__(256) k_mx_pack(const uint8_t* __restrict__ q, const uint8_t* __restrict__ sc,
-                                                 uint8_t* __restrict__ pq, uint32_t* __restrict__ ps, int64_t units, int R,
+                                                 uint8_t* __restrict__ pq, uint32_t* __restrict__ ps, uint32_t units, int R,
                                                  int nk) {
   constexpr int UR = kRowStep<F> / 16;  // 16-byte units of a row's step
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;  // of the result
+  const uint32_t i = blockIdx.x * 256u + threadIdx.x;  // of the result
   if (i >= units) return;
-  const int64_t rs = i / UR;  // (16 rows, step, row)
+  const uint32_t rs = i / UR;  // (16 rows, step, row)
   const int u = (int)(i % UR), r = (int)(rs & 15);
-  const int64_t gs = rs >> 4, row = gs / nk * 16 + r;
-  const int s = (int)(gs % nk);
+  const uint32_t gs = rs >> 4, g = gs / (uint32_t)nk, s = gs - g * nk;
+  const size_t row = (size_t)g * 16 + r;
   uint4 v = make_uint4(0, 0, 0, 0);
   uint32_t w = 0;
-  if (row < R) {
+  if (row < (size_t)R) {
     __builtin_memcpy(&v, q + (row * nk + s) * kRowStep<F> + 16 * u, 16);
     if (u == 0) __builtin_memcpy(&w, sc + (row * nk + s) * 4, 4);
   }
@@ -382,17 +366,22 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
   read_frags(0, std::integral_constant<int, 0>{});
   read_scales(0);
   uint32_t off = 0;
-  constexpr int NR = TN + (F == MX_FP4 ? 1 : 2) * TM;
+  // LDS reads early among the products, so that they are back when those are done
+  auto spread = [&]() {
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // 2 DS reads
+#pragma unroll
+    for (int q = 0; q < TM * TN; q++) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // 1 MFMA
+      __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
   for (int k = 0; k < n; k++) {
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the first product's fragments
     take_scales();
     read_frags(off, std::integral_constant<int, 1>{});
     mul(std::integral_constant<int, 0>{});
-#pragma unroll
-    for (int q = 0; q < TM * TN; q++) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                                // 1 MFMA
-      __builtin_amdgcn_sched_group_barrier(0x100, (NR + TM * TN - 1) / (TM * TN), 0);  // its share of the DS reads
-    }
+    spread();
     __builtin_amdgcn_s_waitcnt(0xC07F);  // the second product's: this step is read
     ub_wait_vmcnt<(NS - 2) * PW>();      // the next step has landed
     ub_barrier();
@@ -401,11 +390,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
     read_frags(off, std::integral_constant<int, 0>{});  // (after the last step: not used)
     read_scales(off);
     mul(std::integral_constant<int, 1>{});
-#pragma unroll
-    for (int q = 0; q < TM * TN; q++) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, (NR + TM + TN + TM * TN - 1) / (TM * TN), 0);
-    }
+    spread();
   }
   __builtin_amdgcn_s_waitcnt(0xC07F);
   ub_wait_vmcnt<0>();
@@ -526,24 +511,9 @@ __global__ void __launch_bounds__(64 * DW) k_mx_dec(MxDecArgs a) {
   } else {
     auto put = [&](const uint4& v, uint32_t i) {  // (called by whole blocks' lanes)
       const uint32_t row = i / per, u = i - row * per;
-      float f[E];
-      uint32_t t = 0;
-#pragma unroll
-      for (int e = 0; e < E; e++) {
-        f[e] = mx_get<DT>(v, e);
-        t = max(t, __float_as_uint(f[e]) & 0x7fffffffu);
-      }
-      const uint32_t b = mx_byte<F>(mx_top<BL>(t));
-      uint8_t* o = ac + row * pitch + u * (E * F / 8);
-      if constexpr (F == MX_FP8) {
-#pragma unroll
-        for (int p = 0; p < E / 4; p++)
-          ((uint32_t*)o)[p] = mx_codes4<F>(f[4 * p], f[4 * p + 1], f[4 * p + 2], f[4 * p + 3], b);
-      } else if constexpr (E == 8) {
-        *(uint32_t*)o = mx_codes4<F>(f[0], f[1], f[2], f[3], b) | mx_codes4<F>(f[4], f[5], f[6], f[7], b) << 16;
-      } else {
-        *(uint16_t*)o = (uint16_t)mx_codes4<F>(f[0], f[1], f[2], f[3], b);
-      }
+      uint32_t o[2];
+      const uint32_t b = mx_round<DT, F>(v, o);
+      mx_store<DT, F>(ac + row * pitch + u * (E * F / 8), o);
       if (u % BL == 0) as[row * spitch + u / BL] = (uint8_t)b;
     };
 #pragma unroll
@@ -620,25 +590,42 @@ void dec(MxDecArgs a, hipStream_t s) {
 // ------------------------------------------------------------- the choice
 template <int F, int DT>
 void quantize(const void* x, uint8_t* q, uint8_t* sc, int R, int C, int nk, bool packed, hipStream_t s) {
-  const int64_t units = (int64_t)R * nk * (128 / MxElem<DT>::E);
-  const unsigned g = (unsigned)((units + 1023) / 1024);
-  if (packed) k_mx_quant<DT, F, true><<<g, 256, 0, s>>>(x, q, sc, units, C, nk);
-  else k_mx_quant<DT, F, false><<<g, 256, 0, s>>>(x, q, sc, units, C, nk);
+  const uint32_t units = (uint32_t)((int64_t)R * nk * (128 / MxElem<DT>::E));
+  auto go = [&](auto u) {
+    constexpr int U = decltype(u)::value;
+    const unsigned g = (units + 256 * U - 1) / (256 * U);
+    if (packed) k_mx_quant<DT, F, true, U><<<g, 256, 0, s>>>(x, q, sc, units, C, nk);
+    else k_mx_quant<DT, F, false, U><<<g, 256, 0, s>>>(x, q, sc, units, C, nk);
+  };
+  // a unit a thread until the CUs are full
+  if (units <= 256 * 2048) go(std::integral_constant<int, 1>{});
+  else go(std::integral_constant<int, 4>{});
 }
 
+// The tile and the number of K parts that take least, by the tile's measured time for
+// a step of K (0.01 us) on a CU that has one workgroup of it, and for each of several
+// (side by side or in turn); parts cost a launch and their sums' way to memory and
+// back.  us, M x K x N, e2m1 (e4m3) activations laid out, on 128 x 256 / 128 x 128 / 64 x
+// 64 / 32 x 128: 64 x 4096 x 6144 23.5 / 12.7 / 9.1 / 9.9 (31 / 17 / 10.5 / 10.5), 201 x
+// 3520 x 9001 24.5 / 13.1 / 13.1 / 12.5 (31 / 16.4 / 16.8 / 14.0), 512 x 4096 x 4096 23.5 /
+// 13.9 / 12.1 / 13.6 (31 / 17 / 14.8 / 15.7), 1024 x 4096 x 14336 42 / 46 / 58 / 80 (55 / 75
+// / 78 / 91); in 4 parts, without their sum, 64 x 4096 x 6144 7.1 / 6.0 / 7.0 on the last
+// three.  The f32 form of e4m3 has too few registers for the first.
 struct Plan { int tile, parts; };
-Plan plan_for(int M, int N, int nk) {
-  static const struct { int m, n, one, each; } t[3] = {{256, 256, 100, 100}, {128, 128, 40, 35}, {64, 64, 25, 20}};
-  Plan best = {0, 1};
+Plan plan_for(int F, bool X, int M, int N, int nk) {
+  static const struct { int m, n, one[2], each[2]; } t[4] = {
+      {128, 256, {63, 87}, {60, 80}}, {128, 128, {30, 42}, {33, 50}}, {64, 64, {18, 23}, {14, 18}}, {32, 128, {22, 23}, {17, 20}}};
+  const int f = F == MX_FP8;
+  Plan best = {-1, 1};
   double least = 0;
-  for (int i = 0; i < 3; i++) {
+  for (int i = X; i < 4; i++) {
     const int64_t tiles = (int64_t)ub_cdiv(M, t[i].m) * ub_cdiv(N, t[i].n);
     for (int p = 1; p <= 32 && p <= nk; p *= 2) {
       if (p > 1 && (tiles * p > 1024 || (int64_t)M * N >= 1 << 26)) break;
       const int64_t per = (tiles * p + kCUs - 1) / kCUs;
-      double cost = (per == 1 ? t[i].one : (double)per * t[i].each) * ub_cdiv(nk, p);
-      if (p > 1) cost += 400 + (double)M * N * 8 * p / 52e3;
-      if ((i == 0 && p == 1) || cost < least) best = {i, p}, least = cost;
+      double cost = (per == 1 ? t[i].one[f] : (double)per * t[i].each[f]) * ub_cdiv(nk, p);
+      if (p > 1) cost += 300 + (double)M * N * 8 * p / 52e3;
+      if (best.tile < 0 || cost < least) best = {i, p}, least = cost;
     }
   }
   return best;
@@ -657,9 +644,12 @@ void gemm(int tile, const MxArgs& a, int parts, hipStream_t s) {
         <<<ub_cdiv(a.M, BM) * ub_cdiv(a.N, BN) * parts, 64 * NW, lds, s>>>(a);                           \
     return;                                                                                              \
   }
-  if (tile == 0) UB_MX(2, 4, 4, 2, (F == MX_FP4 ? 4 : 3), 2)
-  if (tile == 1) UB_MX(2, 2, 2, 2, (F == MX_FP4 ? 4 : 3), 2)
-  UB_MX(2, 2, 1, 1, (F == MX_FP4 ? 6 : 4), 2)
+  // rings as deep as leaves two workgroups of the large tiles to a CU, four of the small
+  if constexpr (!X)
+    if (tile == 0) UB_MX(2, 2, 2, 4, (F == MX_FP4 ? 3 : 2), 2)
+  if (tile <= 1) UB_MX(2, 4, 2, 1, 3, (F == MX_FP4 ? 4 : 2))
+  if (tile == 2) UB_MX(2, 2, 1, 1, (F == MX_FP4 ? 4 : 3), 4)
+  UB_MX(1, 4, 1, 1, (F == MX_FP4 ? 6 : 5), 4)
 #undef UB_MX
 }
 
@@ -674,7 +664,8 @@ int linear(const char* nm, const UbridgeMxLinearArgs& p, hipStream_t s) {
     else dec<F, DT, true>(d, s);
     return UB_OK;
   }
-  const Plan plan = plan_for(M, N, nk);
+  constexpr bool X = F == MX_FP8 && DT == UB_F32;
+  const Plan plan = plan_for(F, X, M, N, nk);
   const int part = ub_cdiv(nk, plan.parts), parts = ub_cdiv(nk, part);  // (none empty)
   const size_t rows = (size_t)ub_cdiv(M, 16) * 16, codes = rows * nk * kRowStep<F>, words = rows * nk * 4;
   const size_t sums = parts > 1 ? sizeof(float) * parts * (size_t)M * N : 0;
@@ -685,10 +676,9 @@ int linear(const char* nm, const UbridgeMxLinearArgs& p, hipStream_t s) {
   if (p.x) {
     quantize<F, DT>(p.x, q, qs, M, p.K, nk, true, s);
   } else {
-    const int64_t units = (int64_t)rows * nk * (kRowStep<F> / 16);
-    k_mx_pack<F><<<(unsigned)((units + 255) / 256), 256, 0, s>>>((const uint8_t*)p.codes, (const uint8_t*)p.scales, q, (uint32_t*)qs, units, M, nk);
+    const uint32_t units = (uint32_t)(rows * nk * (kRowStep<F> / 16));
+    k_mx_pack<F><<<(units + 255) / 256, 256, 0, s>>>((const uint8_t*)p.codes, (const uint8_t*)p.scales, q, (uint32_t*)qs, units, M, nk);
   }
-  constexpr bool X = F == MX_FP8 && DT == UB_F32;
   MxArgs a = {q, w, (const uint32_t*)qs, sw, p.bias, p.y, M, N, nk, part};
   if (parts > 1) {
     a.y = qs + words;
@@ -715,7 +705,7 @@ UB_API int ubridge_mx_quantize(const void* x, int dtype, void* codes, void* scal
   const char* nm = "ubridge_mx_quantize";
   UB_REQUIRE(dtype_ok(dtype), "%s: dtype %d", nm, dtype);
   UB_REQUIRE(format == MX_FP4 || format == MX_FP8, "%s: format %d (4 or 8)", nm, format);
-  UB_REQUIRE(R >= 0 && C > 0 && C <= 1 << 30 && (int64_t)R * (C + 127) <= 1ll << 34, "%s: R=%d C=%d", nm, R, C);  // (2^32 threads a launch)
+  UB_REQUIRE(R >= 0 && C > 0 && C <= 1 << 30 && (int64_t)R * (C + 127) <= 1ll << 33, "%s: R=%d C=%d", nm, R, C);  // (32-bit units)
   if (R == 0) return UB_OK;
   UB_REQUIRE(x && codes && scales, "%s: null pointer", nm);
   UB_REQUIRE(((uintptr_t)codes & 15) == 0, "%s: codes not 16-byte aligned", nm);
@@ -738,13 +728,13 @@ UB_API int ubridge_mx_dequantize(const void* codes, const void* scales, void* y,
   const char* nm = "ubridge_mx_dequantize";
   UB_REQUIRE(dtype_ok(dtype), "%s: dtype %d", nm, dtype);
   UB_REQUIRE(format == MX_FP4 || format == MX_FP8, "%s: format %d (4 or 8)", nm, format);
-  UB_REQUIRE(R >= 0 && C > 0 && C <= 1 << 30 && (int64_t)R * (C + 127) <= 1ll << 34, "%s: R=%d C=%d", nm, R, C);  // (2^32 threads a launch)
+  UB_REQUIRE(R >= 0 && C > 0 && C <= 1 << 30 && (int64_t)R * (C + 127) <= 1ll << 33, "%s: R=%d C=%d", nm, R, C);  // (32-bit units)
   if (R == 0) return UB_OK;
   UB_REQUIRE(y && codes && scales, "%s: null pointer", nm);
   UB_REQUIRE(((uintptr_t)codes & 15) == 0, "%s: codes not 16-byte aligned", nm);
   const int nk = ub_cdiv(C, 128);
-  const int64_t units = (int64_t)R * ub_cdiv(C, 8);
-  const unsigned g = (unsigned)((units + 255) / 256);
+  const uint32_t units = (uint32_t)((int64_t)R * ub_cdiv(C, 8));
+  const unsigned g = (units + 255) / 256;
   hipStream_t s = ub_stream(stream);
   auto go = [&](auto f) {
     constexpr int F = decltype(f)::value;
@@ -761,13 +751,13 @@ UB_API int ubridge_mx_dequantize(const void* codes, const void* scales, void* y,
 UB_API int ubridge_mx_pack(const void* codes, const void* scales, void* w, void* w_scales, int N, int K, void* stream) {
   const char* nm = "ubridge_mx_pack";
   UB_REQUIRE(N >= 0 && K > 0 && K <= kMaxK, "%s: N=%d K=%d (1..%d)", nm, N, K, kMaxK);
-  UB_REQUIRE((int64_t)N * ub_cdiv(K, 128) <= 1ll << 29, "%s: N=%d K=%d", nm, N, K);  // (2^32 threads a launch)
+  UB_REQUIRE((int64_t)N * ub_cdiv(K, 128) <= 1ll << 28, "%s: N=%d K=%d", nm, N, K);  // (32-bit units)
   if (N == 0) return UB_OK;
   UB_REQUIRE(codes && scales && w && w_scales, "%s: null pointer", nm);
   UB_REQUIRE((((uintptr_t)w | (uintptr_t)w_scales) & 15) == 0, "%s: result not 16-byte aligned", nm);
   const int nk = ub_cdiv(K, 128);
-  const int64_t units = (int64_t)ub_cdiv(N, 16) * 16 * nk * 4;
-  k_mx_pack<MX_FP4><<<(unsigned)((units + 255) / 256), 256, 0, ub_stream(stream)>>>(
+  const uint32_t units = (uint32_t)ub_cdiv(N, 16) * 16 * nk * 4;
+  k_mx_pack<MX_FP4><<<(units + 255) / 256, 256, 0, ub_stream(stream)>>>(
       (const uint8_t*)codes, (const uint8_t*)scales, (uint8_t*)w, (uint32_t*)w_scales, units, N, nk);
   return ub_check_launch(nm);
 }
@@ -782,8 +772,8 @@ UB_API int ubridge_mx_linear(const UbridgeMxLinearArgs* p, void* stream) {
   UB_REQUIRE((p->x || (p->codes && p->scales)) && p->w && p->w_scales && p->y, "%s: null pointer", nm);
   UB_REQUIRE((((uintptr_t)p->w | (uintptr_t)p->w_scales) & 15) == 0, "%s: weight not 16-byte aligned", nm);
   UB_REQUIRE(p->x || (((uintptr_t)p->codes & 15) == 0 && ((uintptr_t)p->scales & 3) == 0), "%s: codes not 16-byte, scales not 4-byte aligned", nm);
-  // (2^32 threads a launch)
-  UB_REQUIRE(p->M < 1 << 22 && (int64_t)p->M * p->N < 1ll << 38 && (int64_t)p->M * p->K <= 1ll << 34, "%s: M=%d N=%d K=%d", nm, p->M, p->N, p->K);
+  // (2^32 threads a launch, 32-bit units)
+  UB_REQUIRE(p->M < 1 << 22 && (int64_t)p->M * p->N < 1ll << 38 && ((int64_t)p->M + 15) * (p->K + 127) <= 1ll << 33, "%s: M=%d N=%d K=%d", nm, p->M, p->N, p->K);
   hipStream_t s = ub_stream(stream);
   const int e = p->format == MX_FP4 ? linear<MX_FP4>(nm, *p, s) : linear<MX_FP8>(nm, *p, s);
   return e ? e : ub_check_launch(nm);

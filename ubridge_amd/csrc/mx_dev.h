@@ -131,4 +131,83 @@ __device__ __forceinline__ void mx_put(typename MxElem<DT>::T* p, int i, int C, 
   }
 }
 
+// Rounds the E values of a unit, one of the 4 or 8 neighbouring lanes' that make a
+// block (all of them here): codes in o (e2m1 in o[0]), returns the block's byte.  16-bit
+// values stay packed: the largest magnitude by integer maxima, the elements by the
+// instructions that take pairs, half the operations of going through f32.
+template <int DT, int F>
+__device__ __forceinline__ uint32_t mx_round(const uint4& v, uint32_t (&o)[2]) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  typedef short i16x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  o[0] = o[1] = 0;
+  if constexpr (DT == UB_F32) {
+    float f[4];
+    uint32_t t = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      f[e] = mx_get<DT>(v, e);
+      t = max(t, __float_as_uint(f[e]) & 0x7fffffffu);
+    }
+    const uint32_t b = mx_byte<F>(mx_top<8>(t));
+    o[0] = mx_codes4<F>(f[0], f[1], f[2], f[3], b);
+    return b;
+  } else {
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    u16x2 m = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; i++) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+    const uint32_t top = mx_top<4>(max((uint32_t)m[0], (uint32_t)m[1]));
+    const uint32_t b = mx_byte<F>(DT == UB_BF16 ? top << 16 : __float_as_uint(ub_f16_to_f32((uint16_t)top)));
+    if (b == 255) return b;
+    const float u = mx_unit(b);
+    if constexpr (F == MX_FP8) {  // held to 448 units (f16: to what it has below that)
+      uint32_t lim;
+      if constexpr (DT == UB_BF16) lim = ((b + 8) << 7 | 0x60) * 0x10001u;
+      else lim = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(448.f * u, 448.f * u));
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const u16x2 a = __builtin_elementwise_min(__builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu), __builtin_bit_cast(u16x2, lim));
+        w[i] = __builtin_bit_cast(uint32_t, a) | (w[i] & 0x80008000u);
+      }
+    }
+    auto pair = [&](int i) {
+      if constexpr (DT == UB_BF16) return __builtin_bit_cast(bf16x2, w[i]);
+      else return __builtin_bit_cast(f16x2, w[i]);
+    };
+    if constexpr (F == MX_FP4 && DT == UB_BF16) {
+      o[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(0u, pair(0), u, 0);
+      o[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o[0], pair(1), u, 1);
+      o[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o[0], pair(2), u, 2);
+      o[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o[0], pair(3), u, 3);
+    } else if constexpr (F == MX_FP4) {
+      o[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(0u, pair(0), u, 0);
+      o[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o[0], pair(1), u, 1);
+      o[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o[0], pair(2), u, 2);
+      o[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o[0], pair(3), u, 3);
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        i16x2 c = {0, 0};
+        if constexpr (DT == UB_BF16) {
+          c = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(c, pair(2 * h), u, false);
+          c = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(c, pair(2 * h + 1), u, true);
+        } else {
+          c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(c, pair(2 * h), u, false);
+          c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(c, pair(2 * h + 1), u, true);
+        }
+        o[h] = __builtin_bit_cast(uint32_t, c);
+      }
+    }
+    return b;
+  }
+}
+template <int DT, int F>
+__device__ __forceinline__ void mx_store(uint8_t* p, const uint32_t (&o)[2]) {
+  if constexpr (DT == UB_F32 && F == MX_FP4) *(uint16_t*)p = (uint16_t)o[0];
+  else if constexpr (DT == UB_F32 || F == MX_FP4) *(uint32_t*)p = o[0];
+  else *(uint2*)p = make_uint2(o[0], o[1]);
+}
+
 }  // namespace
