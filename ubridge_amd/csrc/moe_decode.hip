@@ -15,9 +15,9 @@
 // an expert's result is kept for the tokens that chose it.
 //  * k_up: every workgroup finds the top-k itself (a wavefront a token; under a
 //    microsecond, against a launch).  An item is 8 columns of an expert: 8 gate rows
-//    and their 8 up rows are the 16 rows of one product.  The workgroups take equal
-//    runs of the items; 8 wavefronts split K, each one run of its rows, two items in
-//    flight.
+//    and their 8 up rows are the 16 rows of one product.  Groups of 8
+//    wavefronts take the items in turn and split K, each one run of its rows, two items
+//    in flight.
 //  * k_down: a workgroup owns 8 output columns and adds all experts' parts, so no sums
 //    cross workgroups.  8 rows of each of two experts are the 16 rows of a product, and
 //    up to 8 tokens of the one and 8 of the other its columns (an expert with more is
@@ -25,6 +25,7 @@
 //  * Scales are asked for ahead of the weights that they go with: loads return in order,
 //    and one asked for at the end of an item would wait for all weights in flight.
 #include "moe_dev.h"
+#include "wave.h"
 
 #include <algorithm>
 #include <type_traits>
@@ -74,88 +75,76 @@ __device__ __forceinline__ f32x4 product(const uint4& w, const uint4 (&x)[Q8 ? 2
     return mfma<DT>(w, x[0], c);
   }
 }
-__device__ __forceinline__ uint4 ld16nt(const void* p) {
-  typedef unsigned int u4 __attribute__((ext_vector_type(4)));
-  return __builtin_bit_cast(uint4, __builtin_nontemporal_load((const u4*)p));
-}
-
-// OP 0: f32 max, 1: u32 min, 2: f32 sum, over the wavefront
-template <int OP>
-__device__ __forceinline__ uint32_t wave_reduce(uint32_t v) {
-  auto op = [](uint32_t a, uint32_t b) -> uint32_t {
-    if constexpr (OP == 0) return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
-    else if constexpr (OP == 1) return a < b ? a : b;
-    else return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
-  };
-#define UB_DPP(c) v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, c, 0xf, 0xf, false))
-  UB_DPP(0xB1);   // quad_perm [1,0,3,2]
-  UB_DPP(0x4E);   // quad_perm [2,3,0,1]
-  UB_DPP(0x141);  // row_half_mirror
-  UB_DPP(0x140);  // row_mirror
-#undef UB_DPP
-  auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-  v = op(a[0], a[1]);
-  auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-  return op(b[0], b[1]);
+// 16 bytes of a weight row, as one vector (of a struct's four parts the conversions to T
+// make loads byte by byte)
+__device__ __forceinline__ uint4 ld16(const void* p) {
+  typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(uint4, *(const u32x4*)p);
 }
 
 // Token t's experts, by one wavefront holding its logits (expert lane + 64 j): f(round,
-// expert, weight) in lane 0.
+// expert, weight) in lane `round`.  A round is a maximum over the wavefront and, for
+// the lowest expert that has it, a ballot for each j: every workgroup finds the top-k of
+// all tokens, so what counts is the number of instructions.
 template <int NPL, class F>
 __device__ __forceinline__ void top_k(float (&v)[NPL], int k, int norm, F f) {
   const int lane = threadIdx.x & 63;
-  float m = -INFINITY;
-#pragma unroll
-  for (int j = 0; j < NPL; j++) m = fmaxf(m, v[j]);
-  m = __uint_as_float(wave_reduce<0>(__float_as_uint(m)));
-  if (m == -INFINITY) return;
-  float all = 0.f;
-  if (!norm) {
-#pragma unroll
-    for (int j = 0; j < NPL; j++) all += expf(v[j] - m);
-    all = __uint_as_float(wave_reduce<2>(__float_as_uint(all)));
-  }
-  float picked = -INFINITY;  // lane i: the i-th largest, and its expert
+  float m = -INFINITY, all = 0.f, picked = -INFINITY;
   int which = 0, got = 0;
   for (int i = 0; i < k; i++) {
     float best = v[0];
-    int bj = 0;
 #pragma unroll
-    for (int j = 1; j < NPL; j++)
-      if (v[j] > best) best = v[j], bj = j;
-    const float wb = __uint_as_float(wave_reduce<0>(__float_as_uint(best)));
+    for (int j = 1; j < NPL; j++) best = fmaxf(best, v[j]);
+    const float wb = ub_wave_all_max(best);
     if (wb == -INFINITY) break;
-    const int e = (int)wave_reduce<1>(best == wb ? (uint32_t)(lane + 64 * bj) : 0xffffffffu);
+    if (i == 0) {
+      m = wb;
+      if (!norm) {
 #pragma unroll
-    for (int j = 0; j < NPL; j++)
-      if (lane + 64 * j == e) v[j] = -INFINITY;
-    if (lane == i) picked = wb, which = e;
+        for (int j = 0; j < NPL; j++) all += expf(v[j] - m);
+        all = ub_wave_all_sum(all);
+      }
+    }
+    bool found = false;
+#pragma unroll
+    for (int j = 0; j < NPL; j++) {
+      const uint64_t has = __ballot(v[j] == wb);
+      if (!found && has) {  // (the same in every lane)
+        found = true;
+        const int l = __builtin_ctzll(has);
+        if (lane == l) v[j] = -INFINITY;
+        if (lane == i) picked = wb, which = l + 64 * j;
+      }
+    }
     got++;
   }
+  if (got == 0) return;
   const float p = lane < got ? expf(picked - m) : 0.f;
-  if (norm) all = __uint_as_float(wave_reduce<2>(__float_as_uint(p)));
+  if (norm) all = ub_wave_all_sum(p);
   if (lane < got) f(lane, which, p / all);
 }
 
-constexpr int W1 = 8;  // wavefronts of k_up
+constexpr int W1 = 8;  // wavefronts to an item in k_up
 
 // SP: 64-byte steps of a row that a wavefront takes at once.  MULTI: K in several such
-// pieces, the activations loaded with each; else they stay in registers.
-template <int DT, bool Q8, int NPL, int SP, bool MULTI>
-__global__ void __launch_bounds__(64 * W1) __attribute__((amdgpu_waves_per_eu(SP > 4 ? 2 : 4, SP > 4 ? 2 : 4))) k_up(DecodeArgs a) {
+// pieces, the activations loaded with each; else they stay in registers.  NG: groups of
+// wavefronts with an item each, so that the routing is found once a CU.
+template <int DT, bool Q8, int NPL, int SP, bool MULTI, int NG>
+__global__ void __launch_bounds__(64 * W1 * NG) __attribute__((amdgpu_waves_per_eu(2 * NG, 2 * NG))) k_up(DecodeArgs a) {
+  constexpr int NT = 64 * W1 * NG, TW = kTok / (W1 * NG);  // threads; tokens of a wavefront
   constexpr int WB = Q8 ? 1 : 2, EL = 64 / WB, XN = Q8 ? 2 : 1;  // bytes of a weight; elements of a step; operands
   __shared__ __attribute__((aligned(16))) int8_t slot[kE][kTok];
   __shared__ uint16_t used[kUsed], tokens[kUsed], entry[kUsed];  // experts in use, their tokens (bits), first entries
   __shared__ int nused, nent;
-  __shared__ __attribute__((aligned(16))) float red[2][W1][16][20];
+  __shared__ __attribute__((aligned(16))) float red[2][NG][W1][16][20];
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, h = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), wave = wv % W1, grp = wv / W1;
   const int T = a.T, E = a.E, H = a.H, I = a.I;
-  // ---- routing.  Two tokens a wavefront, at most.
-  float lg[2][NPL];
+  // ---- routing
+  float lg[TW][NPL];
 #pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int t = wave + i * W1;
+  for (int i = 0; i < TW; i++) {
+    const int t = wv + i * W1 * NG;
 #pragma unroll
     for (int j = 0; j < NPL; j++) {
       const int e = lane + 64 * j;
@@ -184,13 +173,13 @@ __global__ void __launch_bounds__(64 * W1) __attribute__((amdgpu_waves_per_eu(SP
 #pragma unroll
     for (int i = 0; i < SP; i++) acts(xf[i], wave * SP + i);
   }
-  for (int i = tid; i < E * kTok / 4; i += 64 * W1) ((int*)slot)[i] = -1;
+  for (int i = tid; i < E * kTok / 4; i += NT) ((int*)slot)[i] = -1;
   __syncthreads();
   const bool first = blockIdx.x == 0;
   __shared__ float wts[kTok][kK];
 #pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int t = wave + i * W1;
+  for (int i = 0; i < TW; i++) {
+    const int t = wv + i * W1 * NG;
     if (t < T)
       top_k<NPL>(lg[i], a.k, a.norm, [&](int j, int e, float w) {
         slot[e][t] = (int8_t)j;
@@ -198,7 +187,7 @@ __global__ void __launch_bounds__(64 * W1) __attribute__((amdgpu_waves_per_eu(SP
       });
   }
   __syncthreads();
-  if (wave == 0) {
+  if (wv == 0) {
     int n = 0, m = 0;
     for (int e0 = 0; e0 < E; e0 += 64) {
       const int e = e0 + lane;
@@ -228,7 +217,7 @@ __global__ void __launch_bounds__(64 * W1) __attribute__((amdgpu_waves_per_eu(SP
   const int nu = __builtin_amdgcn_readfirstlane(nused);
   if (first) {
     if (tid == 0) a.route->n = nent;
-    for (int i = tid; i < nu * 16; i += 64 * W1) {
+    for (int i = tid; i < nu * 16; i += NT) {
       const int u = i >> 4, p = i & 15, e = used[u], bits = tokens[u], n = __popc(bits), at = entry[u] + (p >> 3);
       if (p >= (n > 8 ? 16 : 8)) continue;
       int b = bits;  // the p-th token of the expert
@@ -240,24 +229,21 @@ __global__ void __launch_bounds__(64 * W1) __attribute__((amdgpu_waves_per_eu(SP
       a.route->w[at][p & 7] = t >= 0 ? wts[t][j] : 0.f;
     }
   }
-  // ---- items: (expert in use, 8 columns), equal runs of them
-  const int nc = I / 8, G = gridDim.x;
-  const long items = (long)nu * nc;
-  // (of two workgroups of a CU, blocks 256 apart, neighbouring runs: one longer than the
-  // other, if they are not the same)
-  const int run = G == 512 ? ((int)blockIdx.x & 255) * 2 + ((int)blockIdx.x >> 8) : (int)blockIdx.x;
-  const int i0 = (int)(items * run / G), i1 = (int)(items * (run + 1) / G);
+  // ---- items
+  // (expert in use, 8 columns); all groups walk along one front, which memory likes better
+  // than runs of their own
+  const int nc = I / 8, G = gridDim.x * NG, run = blockIdx.x + grp * gridDim.x;
+  const int items = nu * nc, longest = (items + G - 1) / G;  // the groups meet at one barrier an item
   const int pieces = MULTI ? ((rowb + 63) / 64 + W1 * SP - 1) / (W1 * SP) : 1;
   struct Set {
     uint4 w[SP];
     uint4 x[MULTI ? SP : 1][XN];
     float sg, su;  // scales of the thread's output
   };
-  const int ot = tid >> 3, oc = tid & 7;  // its token and column
+  const int gt = tid - grp * 64 * W1, ot = gt >> 3, oc = gt & 7;  // its token and column
   auto load = [&](Set& b, int it, int p) {
-    const int u = min(it, i1 - 1) / nc, c = min(it, i1 - 1) - u * nc;
-    const int e = used[u];
-    if (Q8 && tid < 8 * T && p == pieces - 1) {
+    const int at0 = min(it, items - 1), u = at0 / nc, c = at0 - u * nc, e = used[u];
+    if (Q8 && gt < 8 * T && p == pieces - 1) {
       const size_t at = (size_t)e * 2 * I + 8 * c + oc;
       b.sg = ub_load<DT>(a.s13, at);
       b.su = ub_load<DT>(a.s13, at + I);
@@ -267,12 +253,12 @@ __global__ void __launch_bounds__(64 * W1) __attribute__((amdgpu_waves_per_eu(SP
     for (int i = 0; i < SP; i++) {
       const int s = p * W1 * SP + wave * SP + i, at = s * 64 + 16 * h;
       b.w[i] = make_uint4(0, 0, 0, 0);
-      if (it < i1 && at < rowb) b.w[i] = ld16nt(row + at);
+      if (it < items && at < rowb) b.w[i] = ld16(row + at);
       if constexpr (MULTI) acts(b.x[i], s);
     }
   };
-  const int total = (i1 - i0) * pieces;
-  auto item = [&](int q) { return MULTI ? i0 + q / pieces : i0 + q; };
+  const int total = longest * pieces;
+  auto item = [&](int q) { return (MULTI ? q / pieces : q) * G + run; };
   auto piece = [&](int q) { return MULTI ? q % pieces : 0; };
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   // piece q, in b; then piece q + 2's loads
@@ -288,24 +274,24 @@ __global__ void __launch_bounds__(64 * W1) __attribute__((amdgpu_waves_per_eu(SP
     load(b, item(q + 2), piece(q + 2));
     if (!last) return;
     // lane (token r, h) holds rows 4 h .. + 3: gate rows for h < 2, up rows above
-    *(f32x4*)&red[buf][wave][r][4 * h] = acc;
+    *(f32x4*)&red[buf][grp][wave][r][4 * h] = acc;
     acc = (f32x4){0.f, 0.f, 0.f, 0.f};
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0); weight loads stay in flight
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (tid < 8 * T) {
+    if (gt < 8 * T && it < items) {
       const int u = it / nc, col = (it - u * nc) * 8 + oc, j = slot[used[u]][ot];
       if (j >= 0) {
         float g = 0.f, up = 0.f;
 #pragma unroll
-        for (int w = 0; w < W1; w++) g += red[buf][w][ot][oc], up += red[buf][w][ot][8 + oc];
+        for (int w = 0; w < W1; w++) g += red[buf][grp][w][ot][oc], up += red[buf][grp][w][ot][8 + oc];
         if constexpr (Q8) g *= sg, up *= su;
         ub_store<DT>(a.act, ((size_t)ot * a.k + j) * I + col, g / (1.f + expf(-g)) * up);
       }
     }
   };
-  if (i0 >= i1) return;
+  if (items == 0) return;
   Set b0, b1;
   load(b0, item(0), piece(0));
   load(b1, item(1), piece(1));
@@ -323,7 +309,7 @@ constexpr int W2 = 16;  // wavefronts of k_down
 
 template <int DT, bool Q8>
 __global__ void __launch_bounds__(64 * W2) k_down(DecodeArgs a, int most) {
-  constexpr int WB = Q8 ? 1 : 2, XN = Q8 ? 2 : 1, P = Q8 ? 4 : 6;  // P: steps in a set
+  constexpr int WB = Q8 ? 1 : 2, XN = Q8 ? 2 : 1, P = 4;  // P: steps of a unit
   __shared__ int expert[kEnt + 1];
   __shared__ int16_t row[kEnt + 1][8];
   __shared__ int8_t tok[kEnt][8];
@@ -347,41 +333,42 @@ __global__ void __launch_bounds__(64 * W2) k_down(DecodeArgs a, int most) {
   __syncthreads();
   if (tid < 8) row[n][tid] = -1;  // the partner of an odd last entry
   __syncthreads();
-  // units: (pair of entries, 64-byte step of their rows), a run of them to a wavefront
-  const int rowb = I * WB, steps = (rowb + 63) / 64, units = (n + 1) / 2 * steps;
-  const int q0 = (int)((long)units * wave / W2), q1 = (int)((long)units * (wave + 1) / W2);
+  // units: P 64-byte steps of the rows of a pair of entries, dealt out in turn, so that
+  // all workgroups walk through the experts together
+  const int rowb = I * WB, per = ((rowb + 63) / 64 + P - 1) / P, units = (n + 1) / 2 * per;
   const int side = r >> 3, c8 = r & 7;
   struct Set {
     uint4 w[P], x[P][XN];
   };
-  int lq = q0, lp = q0 / steps, ls = q0 - lp * steps;  // the unit to be loaded next
-  auto load = [&](Set& b) {
+  auto load = [&](Set& b, int q) {
+    const int p = q / per, u = 2 * p + side, at0 = (q - p * per) * (64 * P) + 16 * h;
+    const bool any = q < units;  // (the same in every lane)
+    const int ar = any ? row[u][c8] : -1;
+    const uint8_t* pw = (const uint8_t*)a.w2 + ((size_t)(any && u < n ? expert[u] : 0) * H + n0 + c8) * rowb + at0;
+    const uint16_t* px = (const uint16_t*)a.act + (size_t)max(ar, 0) * I + at0 / WB;
 #pragma unroll
     for (int i = 0; i < P; i++) {
       b.w[i] = make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int v = 0; v < XN; v++) b.x[i][v] = make_uint4(0, 0, 0, 0);
-      const int at = ls * 64 + 16 * h, u = 2 * lp + side;
-      if (lq < q1) {
-        const int ar = row[u][c8];
-        if (at < rowb) {
-          if (u < n) b.w[i] = ld16nt((const uint8_t*)a.w2 + ((size_t)expert[u] * H + n0 + c8) * rowb + at);
-          if (ar >= 0) {
+      if (any && at0 + 64 * i < rowb) {
+        if (u < n) b.w[i] = ld16(pw + 64 * i);
+        if (ar >= 0) {
 #pragma unroll
-            for (int v = 0; v < XN; v++) b.x[i][v] = *(const uint4*)((const uint16_t*)a.act + (size_t)ar * I + at / WB + 8 * v);
-          }
+          for (int v = 0; v < XN; v++) b.x[i][v] = *(const uint4*)(px + 64 * i / WB + 8 * v);
         }
-        lq++;
-        if (++ls == steps) ls = 0, lp++;
       }
     }
   };
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  // a pair is done (or the run is): its products to the sums.  Lane (column r, h): rows 4 h
-  // .. + 3, which belong to r's entry if both are of the same half.  The two entries may
-  // share a token: one after the other.
-  auto fold = [&](int p) {
-    const int u = 2 * p + side;
+  // Unit q's products, to the sums.  Lane (column r, h): rows 4 h .. + 3, which belong to
+  // r's entry if both are of the same half.  The two entries may share a token: one after
+  // the other.
+  auto mul = [&](Set& b, int q) {
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < P; i++) acc = product<DT, Q8>(b.w[i], b.x[i], acc);
+    load(b, q + 2 * W2);
+    const int u = 2 * (q / per) + side;
     const bool mine = u < n && (h >> 1) == side && row[u][c8] >= 0;
 #pragma unroll
     for (int s = 0; s < 2; s++) {
@@ -393,26 +380,13 @@ __global__ void __launch_bounds__(64 * W2) k_down(DecodeArgs a, int most) {
       __builtin_amdgcn_wave_barrier();
       asm volatile("" ::: "memory");
     }
-    acc = (f32x4){0.f, 0.f, 0.f, 0.f};
-  };
-  int mq = q0, mp = q0 / steps, ms = q0 - mp * steps;  // the unit to be multiplied next
-  auto mul = [&](Set& b) {
-#pragma unroll
-    for (int i = 0; i < P; i++) {
-      if (mq >= q1) break;
-      acc = product<DT, Q8>(b.w[i], b.x[i], acc);
-      mq++;
-      if (++ms == steps || mq == q1) fold(mp);
-      if (ms == steps) ms = 0, mp++;
-    }
-    load(b);
   };
   Set b0, b1;
-  load(b0);
-  load(b1);
-  while (mq < q1) {
-    mul(b0);
-    mul(b1);
+  load(b0, wave);
+  load(b1, wave + W2);
+  for (int q = wave; q < units; q += 2 * W2) {
+    mul(b0, q);
+    if (q + W2 < units) mul(b1, q + W2);
   }
   __syncthreads();
   if (tid < 8 * T) {
@@ -428,12 +402,19 @@ template <int DT, bool Q8, int NPL>
 void up(const DecodeArgs& a, hipStream_t s) {
   const int steps = ub_cdiv(a.H * (Q8 ? 1 : 2), 64), per = ub_cdiv(steps, W1);
   const long items = (long)std::min(a.T * a.k, a.E) * (a.I / 8);
-  const unsigned g = (unsigned)std::min<long>(items, 512);  // two workgroups a CU
-  if (per <= 1) k_up<DT, Q8, NPL, 1, false><<<g, 64 * W1, 0, s>>>(a);
-  else if (per <= 2) k_up<DT, Q8, NPL, 2, false><<<g, 64 * W1, 0, s>>>(a);
-  else if (per <= 4) k_up<DT, Q8, NPL, 4, false><<<g, 64 * W1, 0, s>>>(a);
-  else if (per <= 8) k_up<DT, Q8, NPL, 8, false><<<std::min(g, 256u), 64 * W1, 0, s>>>(a);
-  else k_up<DT, Q8, NPL, 4, true><<<g, 64 * W1, 0, s>>>(a);
+  auto go = [&](auto sp, auto multi, auto ng) {
+    constexpr int SP = decltype(sp)::value, NG = decltype(ng)::value;
+    const unsigned g = (unsigned)std::min<long>((items + NG - 1) / NG, 256);  // a workgroup a CU
+    k_up<DT, Q8, NPL, SP, decltype(multi)::value, NG><<<g, 64 * W1 * NG, 0, s>>>(a);
+  };
+  using std::integral_constant;
+  integral_constant<int, 2> two;
+  std::false_type once;
+  if (per <= 1) go(integral_constant<int, 1>{}, once, two);
+  else if (per <= 2) go(two, once, two);
+  else if (per <= 4) go(integral_constant<int, 4>{}, once, two);
+  else if (per <= 8) go(integral_constant<int, 8>{}, once, integral_constant<int, Q8 ? 1 : 2>{});  // (registers)
+  else go(integral_constant<int, 4>{}, std::true_type{}, two);
 }
 template <int DT, bool Q8>
 void decode(const DecodeArgs& a, hipStream_t s) {

@@ -18,6 +18,7 @@
 // registers of the workgroup (or, short, of the wavefront) that owns it: x and
 // residual are read once, h and y written once.
 #include "mx_dev.h"
+#include "wave.h"
 
 #include <type_traits>
 
@@ -53,14 +54,9 @@ __device__ __forceinline__ void gain(const void* w, int wf32, int i, int C, floa
 // Sum (or maximum of bit patterns) over the NT threads of a row.  `part` is one
 // of the workgroup's LDS arrays; each call takes its own, so that one barrier a
 // call suffices.
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
 template <int NT>
 __device__ __forceinline__ double row_sum(double v, double* part) {
-  v = wave_sum(v);
+  v = ub_wave_all_sum(v);
   if constexpr (NT > 64) {
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
     __syncthreads();
@@ -72,8 +68,7 @@ __device__ __forceinline__ double row_sum(double v, double* part) {
 }
 template <int NT>
 __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* part) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
+  v = ub_wave_all_max(v);
   if constexpr (NT > 64) {
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
     __syncthreads();
@@ -261,8 +256,8 @@ __global__ void __launch_bounds__(NT) k_norm_grad(NormGradArgs a) {
         ss = __builtin_fma(f, f, ss);
         gh = __builtin_fma((double)(mx_get<DT>(d[j], e) * w[j][e]), f, gh);
       }
-    ss = wave_sum(ss);
-    gh = wave_sum(gh);
+    ss = ub_wave_all_sum(ss);
+    gh = ub_wave_all_sum(gh);
     if ((tid & 63) == 0) s0[turn][tid >> 6] = ss, s1[turn][tid >> 6] = gh;
     __syncthreads();
     ss = gh = 0.0;
@@ -326,7 +321,9 @@ void with_shape(int R, int ld, F f) {
   if (R >= 1024 && units <= 128) UB_NORM(64, 2);
   if (units <= 256) UB_NORM(256, 1);
   if (R >= 512 && units <= 512) UB_NORM(256, 2);
+  if (R >= 512 && units <= 768) UB_NORM(256, 3);
   if (R >= 512 && units <= 1024) UB_NORM(256, 4);
+  if (units <= 512) UB_NORM(512, 1);
   if (units <= 1024) UB_NORM(1024, 1);
   if (units <= 2048) UB_NORM(1024, 2);
   UB_NORM(1024, 4);
