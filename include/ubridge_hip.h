@@ -503,12 +503,12 @@ int ubridge_kv_compact(const UbridgeKvPool* pool, int32_t* n_used, void* stream)
 
 /* ------------------------------------------------ norm and feed-forward half
  * No counterpart in the reference's quantized-matmul path. */
-/* Root-mean-square norm of the rows of x [R, C] (rows of up to 64 KiB): h = T(x +
+/* Root-mean-square norm of the rows of x [R, C] (R < 2^22, rows of up to 64 KiB): h = T(x +
  * residual), or x without one; y = h w / sqrt(mean(h^2) + eps).  residual [R, C] or
  * NULL, then h is written (h may be residual or x itself; nothing else overlaps);
  * w [C] of x's type or f32.  dtype / w_dtype 0 f32, 1 f16, 2 bf16.  out 0: y of
  * type T; 1: int8 codes [R, C] and f32 scales [R] (amax / 127, 1 for a row of
- * zeros, NaN with codes 0 for a row that holds an infinity or a NaN); 2: e4m3, the
+ * zeros, NaN with codes 0 where a row's h holds an infinity or a NaN); 2: e4m3, the
  * same with amax / 448; 3 / 4: blocks of 32 as ubridge_mx_quantize writes them
  * (scale: the bytes), codes 16-byte aligned. */
 typedef struct {
@@ -560,7 +560,7 @@ typedef struct {
 int ubridge_mx_linear(const UbridgeMxLinearArgs* args, void* stream);
 
 /* int8 linear of codes that a norm (or ubridge_int8_linear's rule) made: a int8 [M,
- * ld], 16-byte aligned, finite in the padding, sa f32 [M]; the rest as
+ * ld], -127 .. 127, 16-byte aligned, anything in the padding, sa f32 [M]; the rest as
  * ubridge_int8_linear, whose values it gives.  Scratch: 4 M N bytes a part where long
  * rows are cut. */
 int ubridge_int8_linear_codes(const int8_t* a, const float* sa, const int8_t* w, const float* sw,

@@ -1,11 +1,16 @@
 """CPU checks of the norm's and the feed-forward half's C entries: each refuses what
 it cannot take before it touches a device, and the argument blocks have the layout
 that the header gives them."""
+import os
 import struct
+import subprocess
+import sys
 
 import pytest
 
 import ubridge_amd
+from conftest import ROOT
+from test_launch_limits import STAND_IN
 from ubridge_amd import int8, mx, norm  # noqa: F401  (they register the entries)
 
 lib = ubridge_amd._lib.lib
@@ -33,7 +38,7 @@ def test_rms_norm():
     refused(call(out=5), 1, b"out 5")
     refused(call(out=-1), 1, b"out -1")
     refused(call(R=-1), 1, b"R=-1")
-    refused(call(R=1 << 24), 1, b"R=16777216")
+    refused(call(R=1 << 22), 1, b"R=4194304")
     refused(call(C=0), 1, b"C=0")
     refused(call(C=32769), 1, b"C=32769")
     refused(call(C=16385, dt=0, wt=0), 1, b"C=16385")
@@ -143,3 +148,36 @@ def test_moe_decode():
     refused(call(s13=P), 1, b"one of two scales")
     refused(call(w2=P + 8), 1, b"not 16-byte aligned")
     assert call(T=0) == 0
+
+
+LIMITS = r"""
+import ctypes, struct, sys
+shim = ctypes.CDLL(sys.argv[1], ctypes.RTLD_GLOBAL)
+lib = ctypes.CDLL(sys.argv[2])
+mx = struct.Struct("@7P6i")
+for device in (0, 1, 0):
+    shim.stand_in_device(device)
+    for f in (4, 8):
+        for dt in range(3):
+            for M, K, N, pre in ((1, 14336, 4096, 0), (16, 8192, 512, 0), (16, 8192, 512, 1), (16, 14336, 64, 0),
+                                 (40, 4096, 4096, 0), (64, 16384, 450, 1), (201, 3520, 9001, 0), (1024, 2048, 2048, 0),
+                                 (4096, 4096, 14336, 0)):
+                a = mx.pack(0 if pre else 4096, *[4096] * 4, 0, 4096, M, K, N, dt, f, 0)
+                rc = lib.ubridge_mx_linear(a, None)
+                assert rc == 0, (f, dt, M, K, N, rc)
+"""
+
+
+def test_lds_limits_of_two_devices(tmp_path):
+    # (the HIP runtime's calls answered by a stand-in: nothing is run)
+    src, shim = tmp_path / "stand_in.cpp", tmp_path / "stand_in.so"
+    src.write_text(STAND_IN)
+    subprocess.run(["g++", "-O1", "-shared", "-fPIC", "-std=c++17", "-o", str(shim), str(src)], check=True)
+    lib = os.path.join(ROOT, "ubridge_amd", "lib", "libubridge_hip.so")
+    r = subprocess.run([sys.executable, "-c", LIMITS, str(shim), lib], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr
+    lines = [[int(x) for x in line.split()[1::2]] for line in r.stdout.splitlines()]
+    for device, kernel, lds, limit in lines:
+        assert lds <= limit <= 160 * 1024, (device, kernel, lds, limit)
+    big = [{k for d, k, lds, _ in lines if d == device and lds > 65536} for device in (0, 1)]
+    assert big[0] == big[1] and len(big[0]) >= 2 * 3 * 2  # few tokens, and the largest tiles, of each type

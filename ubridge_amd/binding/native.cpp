@@ -485,7 +485,7 @@ PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (x->dim() == 0 || w->dim() != 1 || w->size(0) != x->size(-1) || !dense(*w)) REFUSE("rms_norm: x [..., C], gain contiguous [C]");
   const int64_t C = x->size(-1), R = C ? x->numel() / C : 0;
   if (C == 0 || C * x->element_size() > 65536) REFUSE("rms_norm: rows of %ld (1 element to 64 KiB)", C);
-  if (R >= 1 << 24) REFUSE("rms_norm: %ld rows", R);
+  if (R >= 1 << 22) REFUSE("rms_norm: %ld rows", R);
   if (res && !same(*res, *x)) REFUSE("rms_norm: residual must be of x's type and shape");
   if (ho && (!res || !same(*ho, *x) || !dense(*ho))) REFUSE("rms_norm: residual_out goes with residual, contiguous, of x's type and shape");
   if (!together("rms_norm", {x, w, res, ho})) return nullptr;
@@ -531,7 +531,7 @@ PyObject* py_norm_grad(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!device_tensor(args[0], h) || !device_tensor(args[1], w) || !device_tensor(args[2], dy) || !optional(args[3], dh)) return nullptr;
   const int dt = code(*h), wt = code(*w);
   const int64_t C = h->dim() ? h->size(-1) : 0, R = C ? h->numel() / C : 0;
-  if (dt < 0 || dt > 2 || (wt != dt && wt != 0) || C == 0 || C * h->element_size() > 65536 || R >= 1 << 24 || w->dim() != 1 ||
+  if (dt < 0 || dt > 2 || (wt != dt && wt != 0) || C == 0 || C * h->element_size() > 65536 || R >= 1 << 22 || w->dim() != 1 ||
       w->size(0) != C || !dense(*w) || !dense(*h) || !same(*dy, *h) || (dh && !same(*dh, *h)))
     REFUSE("rms_norm's gradient: h, dy and dh [..., C] of one type and shape, gain [C]");
   if (!together("rms_norm's gradient", {h, w, dy, dh})) return nullptr;

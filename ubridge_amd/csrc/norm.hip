@@ -5,7 +5,8 @@
 //   y = h r w,   r = 1 / sqrt(mean(h^2) + eps)
 //
 // y goes out in T, as int8 or e4m3 codes with one f32 scale a row (amax / 127,
-// amax / 448; 1 for a row of zeros), or in blocks of 32 (mx_dev.h).  The norm is
+// amax / 448; 1 for a row of zeros; NaN, codes 0, where a value is not finite), or in
+// blocks of 32 (mx_dev.h).  The norm is
 // taken of h as it is stored, so that every later reader of the residual stream
 // sees the values that were normed.  The sum of squares and r are formed in 64
 // bits, which hold the square of every f32 (the additions hide behind the loads);
@@ -352,8 +353,9 @@ void norm_grad(const NormGradArgs& a, int groups, hipStream_t s) {
 
 constexpr int kRow = 65536;  // bytes of a row, at most
 
+// (2^32 threads a launch)
 bool sizes_ok(int R, int C, int dt) {
-  return R >= 0 && R < 1 << 24 && C > 0 && (int64_t)C * (dt == UB_F32 ? 4 : 2) <= kRow;
+  return R >= 0 && R < 1 << 22 && C > 0 && (int64_t)C * (dt == UB_F32 ? 4 : 2) <= kRow;
 }
 
 }  // namespace

@@ -24,8 +24,9 @@ class RmsNorm:
       "e4m3"        codes uint8 and f32 scales, amax / 448, for fp8.gemm
       "fp4", "fp8"  microscaled blocks as mx.quantize makes them, for mx.Linear.codes
 
-    A row that holds an infinity or a NaN gives NaN (as int8 and e4m3: the scale; in
-    blocks: the blocks that hold one).  Without quant the call is differentiable, once,
+    A NaN makes its row NaN; an infinity is NaN in its place, and the rest of its row
+    zeros.  Codes of such a row are 0 under a scale of NaN; of blocks, those that hold
+    a NaN are NaN.  At most 2 ** 22 - 1 rows.  Without quant the call is differentiable, once,
     in x, residual and weight; with it, or into residual_out, it has no gradient and
     refuses inputs that ask for one.
     """
