@@ -12,6 +12,7 @@
 #include <cfloat>
 #include <cmath>
 #include <ATen/core/Tensor.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -450,15 +451,17 @@ bool together(const char* name, std::initializer_list<Ten> ts) {
 }
 // None, or a tensor (anything else refused)
 bool optional(PyObject* o, Ten& t) { return device_tensor(o, t, true); }
-PyObject* list_of(std::initializer_list<at::Tensor*> ts) {
-  PyObject* l = PyList_New(0);
+// a tuple of them, None for one that is not there
+PyObject* tuple_of(std::initializer_list<at::Tensor*> ts) {
+  PyObject* l = PyTuple_New(ts.size());
+  Py_ssize_t i = 0;
   for (at::Tensor* t : ts) {
     PyObject* o = t->defined() ? THPVariable_Wrap(std::move(*t)) : (Py_INCREF(Py_None), Py_None);
-    if (!l || !o || PyList_Append(l, o)) {
+    if (!l || !o) {
       Py_XDECREF(l), Py_XDECREF(o);
       return nullptr;
     }
-    Py_DECREF(o);
+    PyTuple_SET_ITEM(l, i++, o);
   }
   return l;
 }
@@ -473,7 +476,8 @@ bool same(const at::Tensor& a, const at::Tensor& b) {
 }
 
 // x [..., C], w [C], residual | None, residual_out | None, eps, out (0 as x, 1 int8, 2
-// e4m3, 3 fp4 blocks, 4 fp8 blocks), stream -> [y, scale | None, h | None]
+// e4m3, 3 fp4 blocks, 4 fp8 blocks), stream -> y, or (y, scale), (y, h), (y, scale, h);
+// None where a gradient is asked for (refused with quant or residual_out)
 PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   COUNT(7)
   HANDLE_TH_ERRORS
@@ -489,6 +493,10 @@ PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (res && !same(*res, *x)) REFUSE("rms_norm: residual must be of x's type and shape");
   if (ho && (!res || !same(*ho, *x) || !dense(*ho))) REFUSE("rms_norm: residual_out goes with residual, contiguous, of x's type and shape");
   if (!together("rms_norm", {x, w, res, ho})) return nullptr;
+  if (at::GradMode::is_enabled() && (x->requires_grad() || w->requires_grad() || (res && res->requires_grad()))) {
+    if (A.n(5) || ho) REFUSE("rms_norm: no gradient with quant or residual_out");
+    Py_RETURN_NONE;
+  }
   const double eps = A.f(4);
   const int out = (int)A.n(5);
   if (PyErr_Occurred()) return nullptr;
@@ -518,11 +526,13 @@ PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   void* stream = A.p(6);
   if (PyErr_Occurred()) return nullptr;
   if (const int rc2 = fn.norm(&p, stream)) return PyLong_FromLong(rc2);
-  return list_of({&y, &scale, &h});
+  if (out && res) return tuple_of({&y, &scale, &h});
+  if (out || res) return tuple_of({&y, out ? &scale : &h});
+  return THPVariable_Wrap(std::move(y));
   END_HANDLE_TH_ERRORS
 }
 
-// h [..., C], w, dy, dh | None, eps, whether dx, whether dw, stream -> [dx | None, dw | None]
+// h [..., C], w, dy, dh | None, eps, whether dx, whether dw, stream -> (dx | None, dw | None)
 PyObject* py_norm_grad(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   COUNT(8)
   HANDLE_TH_ERRORS
@@ -548,11 +558,11 @@ PyObject* py_norm_grad(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   // (without rows dx has no memory, and there is nothing to run but dw's zeros)
   if ((p.dx && R) || p.dw)
     if (const int rc = fn.norm_grad(&p, stream)) return PyLong_FromLong(rc);
-  return list_of({&dx, &dw});
+  return tuple_of({&dx, &dw});
   END_HANDLE_TH_ERRORS
 }
 
-// x [..., C], format (4, 8), stream -> [codes, scales]
+// x [..., C], format (4, 8), stream -> (codes, scales)
 PyObject* py_mx_quantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   COUNT(3)
   HANDLE_TH_ERRORS
@@ -568,7 +578,7 @@ PyObject* py_mx_quantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   void* stream = A.p(2);
   if (PyErr_Occurred()) return nullptr;
   if (const int rc = fn.mx_quantize(xc.data_ptr(), dt, q.data_ptr(), s.data_ptr(), R, C, f, stream)) return PyLong_FromLong(rc);
-  return list_of({&q, &s});
+  return tuple_of({&q, &s});
   END_HANDLE_TH_ERRORS
 }
 
@@ -606,7 +616,7 @@ PyObject* py_mx_dequantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// codes [N, ld / 2], scales [N, ld / 32], K, stream -> [w, w_scales]
+// codes [N, ld / 2], scales [N, ld / 32], K, stream -> (w, w_scales)
 PyObject* py_mx_pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   COUNT(4)
   HANDLE_TH_ERRORS
@@ -621,7 +631,7 @@ PyObject* py_mx_pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   void* stream = A.p(3);
   if (PyErr_Occurred()) return nullptr;
   if (const int rc = fn.mx_pack(q->data_ptr(), s->data_ptr(), w.data_ptr(), ws.data_ptr(), N, K, stream)) return PyLong_FromLong(rc);
-  return list_of({&w, &ws});
+  return tuple_of({&w, &ws});
   END_HANDLE_TH_ERRORS
 }
 

@@ -49,13 +49,15 @@ __device__ __forceinline__ size_t scale_at(size_t row, int b, int nk) {
 }
 
 // ------------------------------------------------------- blocks and back
-// A thread takes U units of 16 bytes of x, 256 apart, all loaded before the first is
-// rounded; the 4 (f32: 8) lanes of a block find its largest by DPP.
-template <int DT, int F, bool PACKED, int U>
+// A thread takes two units of 16 bytes of x, 256 apart, both loaded before the first is
+// rounded; the 4 (f32: 8) lanes of a block find its largest by DPP.  us, bf16 to e2m1 laid
+// out, 1 / 2 / 4 units a thread: 201 x 3520 3.6 / 3.6 / 3.7, 4096 x 4096 9.4 / 9.7 / 9.9,
+// and in rows 14336 x 4096 27.9 / 26.2 / 26.5 (5.7 TB/s).
+template <int DT, int F, bool PACKED>
 __global__ void __launch_bounds__(256) k_mx_quant(const void* __restrict__ x, uint8_t* __restrict__ q,
                                                   uint8_t* __restrict__ sc, uint32_t units, int C, int nk) {
   typedef typename MxElem<DT>::T T;
-  constexpr int E = MxElem<DT>::E, BL = 32 / E;
+  constexpr int E = MxElem<DT>::E, BL = 32 / E, U = 2;
   const uint32_t per = (uint32_t)nk * (128 / E);  // units a row
   uint4 v[U];
   const uint32_t i0 = blockIdx.x * (256u * U) + threadIdx.x;
@@ -591,30 +593,27 @@ void dec(MxDecArgs a, hipStream_t s) {
 template <int F, int DT>
 void quantize(const void* x, uint8_t* q, uint8_t* sc, int R, int C, int nk, bool packed, hipStream_t s) {
   const uint32_t units = (uint32_t)((int64_t)R * nk * (128 / MxElem<DT>::E));
-  auto go = [&](auto u) {
-    constexpr int U = decltype(u)::value;
-    const unsigned g = (units + 256 * U - 1) / (256 * U);
-    if (packed) k_mx_quant<DT, F, true, U><<<g, 256, 0, s>>>(x, q, sc, units, C, nk);
-    else k_mx_quant<DT, F, false, U><<<g, 256, 0, s>>>(x, q, sc, units, C, nk);
-  };
-  // a unit a thread until the CUs are full
-  if (units <= 256 * 2048) go(std::integral_constant<int, 1>{});
-  else go(std::integral_constant<int, 4>{});
+  const unsigned g = (units + 511) / 512;
+  if (packed) k_mx_quant<DT, F, true><<<g, 256, 0, s>>>(x, q, sc, units, C, nk);
+  else k_mx_quant<DT, F, false><<<g, 256, 0, s>>>(x, q, sc, units, C, nk);
 }
 
-// The tile and the number of K parts that take least, by the tile's measured time for
-// a step of K (0.01 us) on a CU that has one workgroup of it, and for each of several
-// (side by side or in turn); parts cost a launch and their sums' way to memory and
-// back.  us, M x K x N, e2m1 (e4m3) activations laid out, on 128 x 256 / 128 x 128 / 64 x
-// 64 / 32 x 128: 64 x 4096 x 6144 23.5 / 12.7 / 9.1 / 9.9 (31 / 17 / 10.5 / 10.5), 201 x
-// 3520 x 9001 24.5 / 13.1 / 13.1 / 12.5 (31 / 16.4 / 16.8 / 14.0), 512 x 4096 x 4096 23.5 /
-// 13.9 / 12.1 / 13.6 (31 / 17 / 14.8 / 15.7), 1024 x 4096 x 14336 42 / 46 / 58 / 80 (55 / 75
-// / 78 / 91); in 4 parts, without their sum, 64 x 4096 x 6144 7.1 / 6.0 / 7.0 on the last
-// three.  The f32 form of e4m3 has too few registers for the first.
+// The tile and the number of K parts that take least, by measured times (0.01 us): a
+// step of K on a CU that has one workgroup of the tile, the same for each of several
+// (side by side or in turn), and what a tile takes beside its steps; parts cost a
+// launch and their sums' way to memory and back.  us, M x K x N, e2m1 (e4m3) activations
+// laid out, on 128 x 256 / 128 x 128 / 64 x 64 / 32 x 128: 64 x 4096 x 6144 23.5 / 12.7 / 9.1 /
+// 9.9 (31 / 17 / 10.5 / 10.5), 201 x 3520 x 9001 24.5 / 13.1 / 13.1 / 12.5 (31 / 16.4 / 16.8 /
+// 14.0), 512 x 4096 x 4096 23.5 / 13.9 / 12.1 / 13.6 (31 / 17 / 14.8 / 15.7), 1646 x 5413 x 4856
+// 35 / 27 / 41 / -, 1024 x 4096 x 14336 42 / 46 / 58 / 80 (55 / 75 / 78 / 91); 160 x 10304 x 436
+// in 8 parts 8.6 on the last two.  The f32 form of e4m3 has too few registers for the
+// first.
 struct Plan { int tile, parts; };
 Plan plan_for(int F, bool X, int M, int N, int nk) {
-  static const struct { int m, n, one[2], each[2]; } t[4] = {
-      {128, 256, {63, 87}, {60, 80}}, {128, 128, {30, 42}, {33, 50}}, {64, 64, {18, 23}, {14, 18}}, {32, 128, {22, 23}, {17, 20}}};
+  static const struct { int m, n, tile, one[2], each[2]; } t[4] = {{128, 256, 390, {63, 75}, {50, 70}},
+                                                                   {128, 128, 150, {25, 38}, {28, 51}},
+                                                                   {64, 64, 60, {17, 22}, {12, 16}},
+                                                                   {32, 128, 60, {20, 22}, {15, 18}}};
   const int f = F == MX_FP8;
   Plan best = {-1, 1};
   double least = 0;
@@ -623,7 +622,7 @@ Plan plan_for(int F, bool X, int M, int N, int nk) {
     for (int p = 1; p <= 32 && p <= nk; p *= 2) {
       if (p > 1 && (tiles * p > 1024 || (int64_t)M * N >= 1 << 26)) break;
       const int64_t per = (tiles * p + kCUs - 1) / kCUs;
-      double cost = (per == 1 ? t[i].one[f] : (double)per * t[i].each[f]) * ub_cdiv(nk, p);
+      double cost = (double)per * (t[i].tile + (per == 1 ? t[i].one[f] : t[i].each[f]) * ub_cdiv(nk, p));
       if (p > 1) cost += 300 + (double)M * N * 8 * p / 52e3;
       if (best.tile < 0 || cost < least) best = {i, p}, least = cost;
     }

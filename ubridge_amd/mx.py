@@ -24,7 +24,7 @@ def quantize(x, fmt="fp4", stream=None):
     floor(log2 amax) - 2 ("fp8": - 8), at least -127; values go to the nearest
     element, ties to even, those past the largest (6, 448 times the power) to it.  A
     block that holds an infinity or a NaN becomes NaN."""
-    return tuple(call(_native.mx_quantize, stream, x, _bits(fmt)))
+    return call(_native.mx_quantize, stream, x, _bits(fmt))
 
 
 def dequantize(codes, scales, C, dtype=torch.bfloat16, stream=None):

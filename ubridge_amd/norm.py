@@ -38,18 +38,11 @@ class RmsNorm:
     def forward(self, x, residual=None, quant=None, residual_out=None, stream=None):
         if quant not in _OUT:
             raise ValueError(f"RmsNorm: quant {quant!r} (one of {list(_OUT)})")
-        w = self.weight
-        if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad
-                                        or residual is not None and residual.requires_grad):
-            if quant is not None or residual_out is not None:
-                raise ValueError("RmsNorm: no gradient with quant or residual_out")
-            y, h = _Norm.apply(x, residual, w, self.eps, stream)
+        r = call(_native.norm, stream, x, self.weight, residual, residual_out, self.eps, _OUT[quant])
+        if r is None:  # a gradient is asked for
+            y, h = _Norm.apply(x, residual, self.weight, self.eps, stream)
             return y if residual is None else (y, h)
-        y, scale, h = call(_native.norm, stream, x, w, residual, residual_out, self.eps, _OUT[quant])
-        r = (y,) if scale is None else (y, scale)
-        if h is not None:
-            r += (h,)
-        return r if len(r) > 1 else y
+        return r
 
     __call__ = forward
 
@@ -60,7 +53,8 @@ class _Norm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, residual, w, eps, stream):
-        y, _, h = call(_native.norm, stream, x, w, residual, None, eps, 0)
+        r = call(_native.norm, stream, x, w, residual, None, eps, 0)
+        y, h = (r, None) if residual is None else r
         ctx.eps, ctx.stream, ctx.added = eps, stream, residual is not None
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x if h is None else h, w)
