@@ -310,8 +310,8 @@ constexpr int W2 = 16;  // wavefronts of k_down
 template <int DT, bool Q8>
 __global__ void __launch_bounds__(64 * W2) k_down(DecodeArgs a, int most) {
   constexpr int WB = Q8 ? 1 : 2, XN = Q8 ? 2 : 1, P = 4;  // P: steps of a unit
-  __shared__ int expert[kEnt + 1];
-  __shared__ int16_t row[kEnt + 1][8];
+  __shared__ int expert[kEnt];
+  __shared__ int16_t row[kEnt][8];
   __shared__ int8_t tok[kEnt][8];
   __shared__ float wts[kEnt][8], sc[kEnt][8];
   __shared__ float ys[W2][kTok][8];  // a wavefront's sums
@@ -319,20 +319,6 @@ __global__ void __launch_bounds__(64 * W2) k_down(DecodeArgs a, int most) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int T = a.T, H = a.H, I = a.I, n0 = blockIdx.x * 8;
   const int n = a.route->n;
-  // (entries past n, up to what there can be, are read with the others and not used)
-  for (int i = tid; i < most * 8; i += 64 * W2) {
-    const int u = i >> 3, c = i & 7;
-    (&row[0][0])[i] = (&a.route->row[0][0])[i];
-    (&tok[0][0])[i] = (&a.route->tok[0][0])[i];
-    (&wts[0][0])[i] = (&a.route->w[0][0])[i];
-    const int e = a.route->expert[u];
-    if (c == 0) expert[u] = e;
-    if (Q8 && u < n) sc[u][c] = ub_load<DT>(a.s2, (size_t)e * H + n0 + c);
-  }
-  for (int i = tid; i < W2 * kTok * 8; i += 64 * W2) (&ys[0][0][0])[i] = 0.f;
-  __syncthreads();
-  if (tid < 8) row[n][tid] = -1;  // the partner of an odd last entry
-  __syncthreads();
   // units: P 64-byte steps of the rows of a pair of entries, dealt out in turn, so that
   // all workgroups walk through the experts together
   const int rowb = I * WB, per = ((rowb + 63) / 64 + P - 1) / P, units = (n + 1) / 2 * per;
@@ -340,11 +326,15 @@ __global__ void __launch_bounds__(64 * W2) k_down(DecodeArgs a, int most) {
   struct Set {
     uint4 w[P], x[P][XN];
   };
-  auto load = [&](Set& b, int q) {
+  // Unit q's weights and activations.  FIRST: where they lie is read from scratch memory
+  // itself, not from LDS, which is being filled meanwhile.
+  auto load = [&](Set& b, int q, auto first) {
+    constexpr bool FIRST = decltype(first)::value;
     const int p = q / per, u = 2 * p + side, at0 = (q - p * per) * (64 * P) + 16 * h;
-    const bool any = q < units;  // (the same in every lane)
-    const int ar = any ? row[u][c8] : -1;
-    const uint8_t* pw = (const uint8_t*)a.w2 + ((size_t)(any && u < n ? expert[u] : 0) * H + n0 + c8) * rowb + at0;
+    const bool any = q < units && u < n;
+    int ar = -1, e = 0;
+    if (any) ar = FIRST ? a.route->row[u][c8] : row[u][c8], e = FIRST ? a.route->expert[u] : expert[u];
+    const uint8_t* pw = (const uint8_t*)a.w2 + ((size_t)e * H + n0 + c8) * rowb + at0;
     const uint16_t* px = (const uint16_t*)a.act + (size_t)max(ar, 0) * I + at0 / WB;
 #pragma unroll
     for (int i = 0; i < P; i++) {
@@ -352,7 +342,7 @@ __global__ void __launch_bounds__(64 * W2) k_down(DecodeArgs a, int most) {
 #pragma unroll
       for (int v = 0; v < XN; v++) b.x[i][v] = make_uint4(0, 0, 0, 0);
       if (any && at0 + 64 * i < rowb) {
-        if (u < n) b.w[i] = ld16(pw + 64 * i);
+        b.w[i] = ld16(pw + 64 * i);
         if (ar >= 0) {
 #pragma unroll
           for (int v = 0; v < XN; v++) b.x[i][v] = *(const uint4*)(px + 64 * i / WB + 8 * v);
@@ -367,7 +357,7 @@ __global__ void __launch_bounds__(64 * W2) k_down(DecodeArgs a, int most) {
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < P; i++) acc = product<DT, Q8>(b.w[i], b.x[i], acc);
-    load(b, q + 2 * W2);
+    load(b, q + 2 * W2, std::false_type{});
     const int u = 2 * (q / per) + side;
     const bool mine = u < n && (h >> 1) == side && row[u][c8] >= 0;
 #pragma unroll
@@ -382,8 +372,20 @@ __global__ void __launch_bounds__(64 * W2) k_down(DecodeArgs a, int most) {
     }
   };
   Set b0, b1;
-  load(b0, wave);
-  load(b1, wave + W2);
+  // (entries past n, up to what there can be, are read with the others and not used)
+  for (int i = tid; i < most * 8; i += 64 * W2) {
+    (&row[0][0])[i] = (&a.route->row[0][0])[i];
+    (&tok[0][0])[i] = (&a.route->tok[0][0])[i];
+    (&wts[0][0])[i] = (&a.route->w[0][0])[i];
+    if ((i & 7) == 0) expert[i >> 3] = a.route->expert[i >> 3];
+  }
+  load(b0, wave, std::true_type{});
+  load(b1, wave + W2, std::true_type{});
+  if constexpr (Q8)
+    for (int i = tid; i < n * 8; i += 64 * W2)
+      sc[i >> 3][i & 7] = ub_load<DT>(a.s2, (size_t)a.route->expert[i >> 3] * H + n0 + (i & 7));
+  for (int i = tid; i < W2 * kTok * 8; i += 64 * W2) (&ys[0][0][0])[i] = 0.f;
+  __syncthreads();
   for (int q = wave; q < units; q += 2 * W2) {
     mul(b0, q);
     if (q + W2 < units) mul(b1, q + W2);
