@@ -11,7 +11,8 @@
  *     quantized matmul_* / ubridge_w4a16_gemm beyond 1024 tokens (uint8
  *     4-bit: from 640), and the f32 partials (at most 8 x M x N x 4 bytes)
  *     of the pipelined GEMMs when they split K over workgroups, and what the
- *     attention block's entries (below) say of theirs.  That
+ *     entries of the attention block and of the norm and feed-forward half
+ *     (below) say of theirs.  That
  *     scratch comes from the allocator the caller registers with
  *     ubridge_set_workspace_allocator (taken and handed back on the call's
  *     stream, as the reference's topsaten workspaces are), else from a
@@ -548,9 +549,10 @@ int ubridge_mx_pack(const void* codes, const void* scales, void* w, void* w_scal
                     void* stream);
 /* y[m, n] = T(sum_k a[m, k] w[n, k] + bias[n]): x T [M, K] rounded to blocks of
  * `format` by the call, or, with x NULL, codes and scales [M, ...] that it has already;
- * y T [M, N] contiguous, bias f32 [N] or NULL.  Sums are f32.  Scratch beyond 16 tokens,
- * or where their codes pass a workgroup's 160 KiB: the codes and scales, and 4 M N
- * bytes a part where long rows are cut (at most 32). */
+ * y T [M, N] contiguous, bias f32 [N] or NULL.  Sums are f32.  Scratch beyond 16 tokens
+ * or M K = 61440, where the call rounds: the codes and scales; and, beyond 16 tokens or
+ * where their codes pass a workgroup's 160 KiB, the codes laid out, and 4 M N bytes a part
+ * where long rows are cut (at most 32). */
 typedef struct {
   const void *x, *codes, *scales, *w, *w_scales;
   const float* bias;

@@ -180,3 +180,24 @@ def test_graph(dev, T):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("q8", [True, False])
+def test_weights_past_32_bits(dev, q8):
+    # the last experts of 4.3e9 weights give what a layer of these alone gives
+    E, H, I = (64, 16384, 2048) if q8 else (40, 16384, 2048)
+    g = torch.Generator(device=dev).manual_seed(1)
+    kw = dict(device=dev, generator=g)
+    if q8:
+        w13, w2 = (torch.randint(-127, 128, s, dtype=torch.int8, **kw) for s in ((E, 2 * I, H), (E, H, I)))
+        s13, s2 = (torch.rand(*s, **kw).half() * 1e-3 for s in ((E, 2 * I), (E, H)))
+    else:
+        w13, w2 = (torch.empty(*s, device=dev, dtype=torch.float16).normal_(generator=g).mul_(s[-1] ** -0.5)
+                   for s in ((E, 2 * I, H), (E, H, I)))
+        s13 = s2 = None
+    x = torch.randn(3, H, **kw).half()
+    lg = torch.full((3, E), -math.inf, device=dev)
+    lg[:, -4:] = torch.randn(3, 4, **kw)
+    y = moe.FusedMoE(w13, w2, s13, s2, topk=2).decode(x, lg)
+    part = [t if t is None else t[-4:].contiguous() for t in (w13, w2, s13, s2)]
+    assert torch.equal(y, moe.FusedMoE(*part, topk=2).decode(x, lg[:, -4:]))

@@ -279,3 +279,29 @@ def test_graph_and_bits(dev, M):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, w)
+
+
+def test_rows_past_32_bits(dev):
+    # 2.3e9 elements in, and as many out: the last rows are those of a call of their own
+    x = torch.empty(70000, 32768, device=dev, dtype=torch.bfloat16).normal_()
+    for fmt in ("fp4", "fp8"):
+        q, s = mx.quantize(x, fmt)
+        want = mx.quantize(x[-3:], fmt)
+        assert torch.equal(q[-3:], want[0]) and torch.equal(s[-3:], want[1])
+        y = mx.dequantize(q, s, 32768)
+        assert torch.equal(y[-3:], mx.dequantize(*want, 32768))
+        del y
+    x = x[:, :64].contiguous()
+    i, neg, s = weight(32768, 64)
+    lin = mx.Linear(pack(i, neg, "fp4").to(dev), s.to(dev), 64)
+    y = lin(x)  # (64 products of e2m1: the sums are exact, in whatever order)
+    assert torch.equal(y[-3:], lin(x[-3:])) and torch.equal(y[:3], lin(x[:3]))
+
+
+@pytest.mark.parametrize("act", ["fp4", "fp8"])
+@pytest.mark.parametrize("M,K", [(15, 4096), (16, 4096), (4, 15360), (5, 15360), (16, 9000)])
+def test_where_few_tokens_are_rounded(dev, M, K, act):
+    # both sides of the number of values from which a launch of its own rounds them
+    x, lin, y, size = both(dev, M, K, 200, torch.float16, act, True)
+    near(lin(x), y, size, K, act)
+    assert torch.equal(lin.codes(*mx.quantize(x, act), torch.float16), lin(x))

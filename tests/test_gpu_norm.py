@@ -359,3 +359,47 @@ def test_fp8_gemm_takes_the_codes(dev):
     q, s = n(x, quant="e4m3")
     want = fp8.gemm(*fp8.quantize_rows(n(x)), wq, ws)
     assert torch.equal(fp8.gemm(q, s, wq, ws), want)
+
+
+def test_rows_past_32_bits(dev):
+    # 2.3e9 elements: the last rows are those of a call of their own
+    n = norm.RmsNorm(torch.rand(32768, device=dev), EPS)
+    x = torch.empty(70000, 32768, device=dev, dtype=torch.bfloat16).normal_()
+    y, h = n(x, x)
+    want = n(x[-3:], x[-3:])
+    assert torch.equal(y[-3:], want[0]) and torch.equal(h[-3:], want[1])
+    del h
+    leaf = x.requires_grad_()
+    (dx,) = torch.autograd.grad(n(leaf), [leaf], y)
+    last = x.detach()[-3:].clone().requires_grad_()
+    (want,) = torch.autograd.grad(n(last), [last], y[-3:])
+    assert torch.equal(dx[-3:], want)
+
+
+def test_gradient_in_a_graph(dev):
+    x, res, w = (t.requires_grad_() for t in make(dev, 40, 1000, torch.bfloat16))
+    dy, dh = (torch.randn(40, 1000, device=dev).bfloat16() for _ in "yh")
+    n = norm.RmsNorm(w, EPS)
+
+    def run():
+        y, h = n(x, res)
+        return [y.detach(), h.detach(), *torch.autograd.grad([y, h], [x, res, w], [dy, dh])]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for seed in range(3):
+        with torch.no_grad():
+            for t, v in zip((x, res, w), make(dev, 40, 1000, torch.bfloat16, seed=seed + 1)):
+                t.copy_(v)
+            dy.normal_(), dh.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in got]
+        want = run()
+        assert all(torch.equal(a, b) for a, b in zip(kept, want))

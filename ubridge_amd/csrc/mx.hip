@@ -419,8 +419,9 @@ __global__ void __launch_bounds__(256) k_mx_sum(const float* __restrict__ part, 
 // operand, 2 P steps in flight; lane (r, h) holds block h of row r, and ends with
 // columns 4 h .. + 3 of token r.  The activations' codes lie in LDS for the whole
 // launch (rows 16 bytes further apart than they are long, for the banks); each
-// workgroup makes them itself while its first weights are on their way.  The
-// wavefronts' sums meet in LDS in their order.
+// workgroup makes them itself while its first weights are on their way, up to kRound
+// values; beyond, a launch of its own makes them once.  The wavefronts' sums meet in LDS
+// in their order.
 constexpr int DW = 16, RP = 20;  // wavefronts; floats of a token's row of sums
 
 struct MxDecArgs {
@@ -571,6 +572,12 @@ __global__ void __launch_bounds__(64 * DW) k_mx_dec(MxDecArgs a) {
   }
 }
 
+// us, rounding in every workgroup / in a launch ahead / the tiles (M x K x N): 4 x 4096 x
+// 4096 6.0 / 7.4 / 9.0, 4 x 14336 x 4096 10.5 / 10.8 / 11.7, 16 x 4096 x 4096 9.1 / 7.8 / 9.3, 16
+// x 4096 x 28672 15.4 / 15.1 / 16.2, 16 x 8192 x 8192 15.7 / 11.9 / 13.8, 16 x 14336 x 4096 21.7 /
+// 12.2 / 12.2; of codes that are there 5.2, 8.5, 5.4, 12.7, 9.3, 9.6.  1 x 28672 x 8192 22 (5.6
+// TB/s).
+constexpr int kRound = 60 * 1024;
 constexpr int kCUs = 256, kLds = 160 * 1024;
 size_t dec_lds(int F, int M, int nk) {
   return sizeof(float) * DW * 16 * RP + (size_t)M * (nk * 128 * F / 8 + 16 + nk * 4 + 4) + 16;
@@ -659,8 +666,19 @@ int linear(const char* nm, const UbridgeMxLinearArgs& p, hipStream_t s) {
   const uint32_t* sw = (const uint32_t*)p.w_scales;
   if (M <= 16 && dec_lds(F, M, nk) <= kLds) {
     MxDecArgs d = {p.x, (const uint8_t*)p.codes, (const uint8_t*)p.scales, w, sw, p.bias, p.y, M, p.K, N, nk, 0, 0, 0};
-    if (p.x) dec<F, DT, false>(d, s);
-    else dec<F, DT, true>(d, s);
+    if (p.x && (int64_t)M * p.K <= kRound) {
+      dec<F, DT, false>(d, s);
+      return UB_OK;
+    }
+    const size_t codes = p.x ? (size_t)M * nk * kRowStep<F> : 0;
+    UbScratch ws(s, codes + (p.x ? (size_t)M * nk * 4 : 0));
+    if (p.x) {
+      uint8_t* q = (uint8_t*)ws.get();
+      if (!q) return ub_set_error(UB_ERR_LAUNCH, "%s: no workspace", nm);
+      quantize<F, DT>(p.x, q, q + codes, M, p.K, nk, false, s);
+      d.x = nullptr, d.q = q, d.qs = q + codes;
+    }
+    dec<F, DT, true>(d, s);
     return UB_OK;
   }
   constexpr bool X = F == MX_FP8 && DT == UB_F32;
