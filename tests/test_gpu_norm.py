@@ -345,6 +345,17 @@ def test_int8_linear_takes_the_codes(dev, M, K):
     assert torch.equal(got, want)
     out = torch.empty(M, 96, device=dev, dtype=torch.bfloat16)
     assert torch.equal(lin.codes(q, s, out=out), want.bfloat16())
+    side = torch.cuda.Stream()
+    for _ in range(5):  # all of the call is the stream's, a copy to padded rows too
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            late = torch.empty_like(q).fill_(0)
+            torch.ones(4096, 4096, device=dev).matmul(torch.ones(4096, 4096, device=dev))
+            late.copy_(q)
+        got = lin.codes(late, s, torch.float32, stream=side)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(got, want)
+        late.record_stream(torch.cuda.current_stream())
     for call in (lambda: lin.codes(q.float(), s), lambda: lin.codes(q[:, :4], s), lambda: lin.codes(q, s[:0]),
                  lambda: lin.codes(q, s, torch.float64), lambda: lin.codes(q, s, torch.float32, out=out)):
         with pytest.raises(ValueError):

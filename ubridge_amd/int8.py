@@ -55,6 +55,7 @@ class Linear:
         if a.shape[-1:] != (self.K,):
             raise ValueError(f"int8.Linear: codes must be [..., {self.K}]")
         if self.ld != self.K:
-            a = torch.nn.functional.pad(a, (0, self.ld - self.K))
+            with torch.cuda.stream(stream):
+                a = torch.nn.functional.pad(a, (0, self.ld - self.K))
         return call(_native.linear_codes, stream, a, scales, self.w, self.w_scale, self.bias, self.K,
                     _DT_CODE[dtype], out)
