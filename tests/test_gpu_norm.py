@@ -149,6 +149,25 @@ def test_scales_of_extreme_rows(dev):
     assert int(s[4, 0]) == 255 and int(s[5, 0]) == 255 and bool((s[5] == 255).all())
 
 
+@pytest.mark.parametrize("gain", [2.0**-100, 2.0**-62, 2.0**-57, 2.0**55, 2.0**60, 2.0**100])
+@pytest.mark.parametrize("C", [200, 5003])
+def test_codes_at_extreme_scales(dev, C, gain):
+    # the result's own quotients, bit for bit, also where residuals of a division would
+    # underflow (the gains' own spread puts scales on both sides of 2^-60 and 2^60)
+    x, _, w = make(dev, 9, C, torch.float32, residual=False)
+    n = norm.RmsNorm(w * gain, EPS)
+    y = n(x * torch.exp2(torch.arange(9.0, device=dev) - 4)[:, None])
+    q, s = n(x * torch.exp2(torch.arange(9.0, device=dev) - 4)[:, None], quant="int8")
+    yc, sc = y.cpu(), s.cpu()
+    assert torch.equal(sc, yc.abs().amax(1) / 127.0)
+    assert torch.equal(q.cpu(), torch.round(yc / sc[:, None]).clamp(-127, 127).to(torch.int8))
+    q, s = n(x * torch.exp2(torch.arange(9.0, device=dev) - 4)[:, None], quant="e4m3")
+    sc = s.cpu()
+    assert torch.equal(sc, yc.abs().amax(1) / 448.0)
+    want = (yc / sc[:, None]).clamp(-448, 448).to(torch.float8_e4m3fn)
+    assert torch.equal(q.cpu().view(torch.uint8), want.view(torch.uint8))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_in_place_strides_and_shapes(dev, dtype):
     x, res, w = make(dev, 24, 520, dtype)
@@ -213,6 +232,16 @@ def gradients(x, res, w, dy, dh):
                                  (40, 8200), (3, 16384)])
 @pytest.mark.parametrize("residual", [True, False])
 def test_gradients(dev, R, C, dtype, residual):
+    gradients_hold(dev, R, C, dtype, residual)
+
+
+@pytest.mark.parametrize("dtype,C", [(torch.bfloat16, 32768), (torch.float16, 20001), (torch.bfloat16, 16392), (torch.float32, 8196)])
+@pytest.mark.parametrize("residual", [True, False])
+def test_gradients_of_long_rows(dev, C, dtype, residual):
+    gradients_hold(dev, 600, C, dtype, residual)
+
+
+def gradients_hold(dev, R, C, dtype, residual):
     x, res, w = make(dev, R, C, dtype, torch.float32 if C % 2 else dtype, residual)
     g = torch.Generator().manual_seed(R * C)
     dy = torch.randn(R, C, generator=g).to(dtype).to(dev)
