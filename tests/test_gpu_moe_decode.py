@@ -94,6 +94,15 @@ def test_decode_large(dev, T, E, k, H, I, q8):
     check(x, lg, layer, layer.decode(x, lg))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,E,k,H,I,q8", [(16, 48, 3, 4128, 224, False), (16, 40, 4, 4160, 256, True), (9, 64, 8, 5152, 192, False),
+                                          (2, 32, 16, 6176, 288, True), (7, 48, 8, 4128, 224, False), (11, 6, 3, 3552, 160, False),
+                                          (16, 6, 3, 2080, 160, False), (13, 6, 3, 4064, 160, True)])
+def test_decode_rows_in_pieces(dev, T, E, k, H, I, q8, dtype):
+    x, lg, layer = make(dev, T, E, k, H, I, dtype, q8)
+    check(x, lg, layer, layer.decode(x, lg))
+
+
 @pytest.mark.parametrize("logits", [torch.float32, torch.float16, torch.bfloat16])
 def test_against_forward(dev, logits):
     # the same layer by its three launches, whose gate, up, weights and rows are rounded

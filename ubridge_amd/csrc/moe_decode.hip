@@ -13,17 +13,17 @@
 // or two.  16 tokens are one operand of v_mfma_f32_16x16x32, so no rows are gathered
 // and no list of blocks is built: a product is of 16 weight rows with every token, and
 // an expert's result is kept for the tokens that chose it.
-//  * k_up: every workgroup finds the top-k itself (a wavefront a token; under a
-//    microsecond, against a launch).  An item is 8 columns of an expert: 8 gate rows
-//    and their 8 up rows are the 16 rows of one product.  Groups of 8
-//    wavefronts take the items in turn and split K, each one run of its rows, two items
-//    in flight.
+//  * k_up: every workgroup finds the top-k itself (a wavefront a token; 2.6 us of the
+//    call, against a launch).  An item is 8 columns of an expert: 8 gate rows and their 8
+//    up rows are the 16 rows of one product.  Groups of 8 or 16 wavefronts take the items
+//    in turn and split K, each one run of its rows, two items in flight.
 //  * k_down: a workgroup owns 8 output columns and adds all experts' parts, so no sums
 //    cross workgroups.  8 rows of each of two experts are the 16 rows of a product, and
 //    up to 8 tokens of the one and 8 of the other its columns (an expert with more is
 //    listed twice); the two quarters where rows and tokens belong together are kept.
 //  * Scales are asked for ahead of the weights that they go with: loads return in order,
 //    and one asked for at the end of an item would wait for all weights in flight.
+#include "lds_dma.h"
 #include "moe_dev.h"
 #include "wave.h"
 
@@ -124,38 +124,33 @@ __device__ __forceinline__ void top_k(float (&v)[NPL], int k, int norm, F f) {
   if (lane < got) f(lane, which, p / all);
 }
 
-constexpr int W1 = 8;  // wavefronts to an item in k_up
-
 // SP: 64-byte steps of a row that a wavefront takes at once.  MULTI: K in several such
-// pieces, the activations loaded with each; else they stay in registers.  NG: groups of
-// wavefronts with an item each, so that the routing is found once a CU.
-template <int DT, bool Q8, int NPL, int SP, bool MULTI, int NG>
-__global__ void __launch_bounds__(64 * W1 * NG) __attribute__((amdgpu_waves_per_eu(2 * NG, 2 * NG))) k_up(DecodeArgs a) {
-  constexpr int NT = 64 * W1 * NG, TW = kTok / (W1 * NG);  // threads; tokens of a wavefront
+// pieces, the activations loaded with each; else they stay in registers.  NG groups of
+// W1 wavefronts, 16 in all, have an item each: the routing is found once a CU.  NI: items
+// side by side, taken together.
+template <int DT, bool Q8, int NPL, int SP, bool MULTI, int NG, int NI>
+__global__ void __launch_bounds__(1024) k_up(DecodeArgs a) {
+  constexpr int NT = 1024, W1 = 16 / NG, NB = NI == 1 ? 2 : 1, CI = 8 * NI;  // CI: columns of an item and its neighbours
   constexpr int WB = Q8 ? 1 : 2, EL = 64 / WB, XN = Q8 ? 2 : 1;  // bytes of a weight; elements of a step; operands
   __shared__ __attribute__((aligned(16))) int8_t slot[kE][kTok];
   __shared__ uint16_t used[kUsed], tokens[kUsed], entry[kUsed];  // experts in use, their tokens (bits), first entries
   __shared__ int nused, nent;
-  __shared__ __attribute__((aligned(16))) float red[2][NG][W1][16][20];
+  __shared__ __attribute__((aligned(16))) float red[NB][NG][NI][W1][16][20];
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, h = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), wave = wv % W1, grp = wv / W1;
   const int T = a.T, E = a.E, H = a.H, I = a.I;
   // ---- routing
-  float lg[TW][NPL];
+  float lg[NPL];  // of token wv
 #pragma unroll
-  for (int i = 0; i < TW; i++) {
-    const int t = wv + i * W1 * NG;
-#pragma unroll
-    for (int j = 0; j < NPL; j++) {
-      const int e = lane + 64 * j;
-      float v = -INFINITY;
-      if (t < T && e < E) {
-        const size_t at = (size_t)t * E + e;
-        v = a.ldt == UB_F32 ? ((const float*)a.logits)[at] : a.ldt == UB_F16 ? ub_load<UB_F16>(a.logits, at) : ub_load<UB_BF16>(a.logits, at);
-        if (v != v) v = -INFINITY;
-      }
-      lg[i][j] = v;
+  for (int j = 0; j < NPL; j++) {
+    const int e = lane + 64 * j;
+    float v = -INFINITY;
+    if (wv < T && e < E) {
+      const size_t at = (size_t)wv * E + e;
+      v = a.ldt == UB_F32 ? ((const float*)a.logits)[at] : a.ldt == UB_F16 ? ub_load<UB_F16>(a.logits, at) : ub_load<UB_BF16>(a.logits, at);
+      if (v != v) v = -INFINITY;
     }
+    lg[j] = v;
   }
   // ---- activations of the wavefront's steps: lane (token r, h) takes what meets the
   // 16 bytes at 64 s + 16 h of a weight row
@@ -177,15 +172,11 @@ __global__ void __launch_bounds__(64 * W1 * NG) __attribute__((amdgpu_waves_per_
   __syncthreads();
   const bool first = blockIdx.x == 0;
   __shared__ float wts[kTok][kK];
-#pragma unroll
-  for (int i = 0; i < TW; i++) {
-    const int t = wv + i * W1 * NG;
-    if (t < T)
-      top_k<NPL>(lg[i], a.k, a.norm, [&](int j, int e, float w) {
-        slot[e][t] = (int8_t)j;
-        wts[t][j] = w;
-      });
-  }
+  if (wv < T)
+    top_k<NPL>(lg, a.k, a.norm, [&](int j, int e, float w) {
+      slot[e][wv] = (int8_t)j;
+      wts[wv][j] = w;
+    });
   __syncthreads();
   if (wv == 0) {
     int n = 0, m = 0;
@@ -232,63 +223,77 @@ __global__ void __launch_bounds__(64 * W1 * NG) __attribute__((amdgpu_waves_per_
   // ---- items
   // (expert in use, 8 columns); all groups walk along one front, which memory likes better
   // than runs of their own
-  const int nc = I / 8, G = gridDim.x * NG, run = blockIdx.x + grp * gridDim.x;
+  const int nc = I / CI, G = gridDim.x * NG, run = blockIdx.x + grp * gridDim.x;
   const int items = nu * nc, longest = (items + G - 1) / G;  // the groups meet at one barrier an item
   const int pieces = MULTI ? ((rowb + 63) / 64 + W1 * SP - 1) / (W1 * SP) : 1;
   struct Set {
-    uint4 w[SP];
+    uint4 w[SP][NI];
     uint4 x[MULTI ? SP : 1][XN];
     float sg, su;  // scales of the thread's output
   };
-  const int gt = tid - grp * 64 * W1, ot = gt >> 3, oc = gt & 7;  // its token and column
+  const int gt = tid - grp * 64 * W1, ot = gt / CI, oc = gt % CI;  // its token and column
   auto load = [&](Set& b, int it, int p) {
     const int at0 = min(it, items - 1), u = at0 / nc, c = at0 - u * nc, e = used[u];
-    if (Q8 && gt < 8 * T && p == pieces - 1) {
-      const size_t at = (size_t)e * 2 * I + 8 * c + oc;
+    if (Q8 && gt < CI * T && p == pieces - 1) {
+      const size_t at = (size_t)e * 2 * I + CI * c + oc;
       b.sg = ub_load<DT>(a.s13, at);
       b.su = ub_load<DT>(a.s13, at + I);
     }
-    const uint8_t* row = (const uint8_t*)a.w13 + ((size_t)e * 2 * I + (r < 8 ? 8 * c + r : I + 8 * c + r - 8)) * rowb;
+    const uint8_t* row = (const uint8_t*)a.w13 + ((size_t)e * 2 * I + (r < 8 ? CI * c + r : I + CI * c + r - 8)) * rowb;
 #pragma unroll
     for (int i = 0; i < SP; i++) {
       const int s = p * W1 * SP + wave * SP + i, at = s * 64 + 16 * h;
-      b.w[i] = make_uint4(0, 0, 0, 0);
-      if (it < items && at < rowb) b.w[i] = ld16(row + at);
+#pragma unroll
+      for (int n = 0; n < NI; n++) b.w[i][n] = make_uint4(0, 0, 0, 0);
+      if (it < items && at < rowb) {
+#pragma unroll
+        for (int n = 0; n < NI; n++) b.w[i][n] = ld16(row + (size_t)n * 8 * rowb + at);
+      }
       if constexpr (MULTI) acts(b.x[i], s);
     }
   };
   const int total = longest * pieces;
   auto item = [&](int q) { return (MULTI ? q / pieces : q) * G + run; };
   auto piece = [&](int q) { return MULTI ? q % pieces : 0; };
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  f32x4 acc[NI];
+#pragma unroll
+  for (int n = 0; n < NI; n++) acc[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
   // piece q, in b; then piece q + 2's loads
   auto mul = [&](Set& b, int q, int buf) {
     const int it = item(q);
 #pragma unroll
-    for (int i = 0; i < SP; i++) {
-      if constexpr (MULTI) acc = product<DT, Q8>(b.w[i], b.x[i], acc);
-      else acc = product<DT, Q8>(b.w[i], xf[i], acc);
-    }
+    for (int i = 0; i < SP; i++)
+#pragma unroll
+      for (int n = 0; n < NI; n++) {
+        if constexpr (MULTI) acc[n] = product<DT, Q8>(b.w[i][n], b.x[i], acc[n]);
+        else acc[n] = product<DT, Q8>(b.w[i][n], xf[i], acc[n]);
+      }
     const bool last = piece(q) == pieces - 1;
     const float sg = b.sg, su = b.su;
     load(b, item(q + 2), piece(q + 2));
     if (!last) return;
     // lane (token r, h) holds rows 4 h .. + 3: gate rows for h < 2, up rows above
-    *(f32x4*)&red[buf][grp][wave][r][4 * h] = acc;
-    acc = (f32x4){0.f, 0.f, 0.f, 0.f};
+    if (NB == 1) buf = 0;
+#pragma unroll
+    for (int n = 0; n < NI; n++) {
+      *(f32x4*)&red[buf][grp][n][wave][r][4 * h] = acc[n];
+      acc[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0); weight loads stay in flight
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (gt < 8 * T && it < items) {
-      const int u = it / nc, col = (it - u * nc) * 8 + oc, j = slot[used[u]][ot];
+    ub_barrier();
+    if (gt < CI * T && it < items) {
+      const int u = it / nc, col = (it - u * nc) * CI + oc, j = slot[used[u]][ot];
       if (j >= 0) {
         float g = 0.f, up = 0.f;
 #pragma unroll
-        for (int w = 0; w < W1; w++) g += red[buf][grp][w][ot][oc], up += red[buf][grp][w][ot][8 + oc];
+        for (int w = 0; w < W1; w++) g += red[buf][grp][oc >> 3][w][ot][oc & 7], up += red[buf][grp][oc >> 3][w][ot][8 + (oc & 7)];
         if constexpr (Q8) g *= sg, up *= su;
         ub_store<DT>(a.act, ((size_t)ot * a.k + j) * I + col, g / (1.f + expf(-g)) * up);
       }
+    }
+    if constexpr (NB == 1) {  // (two of them by turns need no second barrier)
+      __builtin_amdgcn_s_waitcnt(0xC07F);
+      ub_barrier();
     }
   };
   if (items == 0) return;
@@ -402,21 +407,37 @@ __global__ void __launch_bounds__(64 * W2) k_down(DecodeArgs a, int most) {
 
 template <int DT, bool Q8, int NPL>
 void up(const DecodeArgs& a, hipStream_t s) {
-  const int steps = ub_cdiv(a.H * (Q8 ? 1 : 2), 64), per = ub_cdiv(steps, W1);
+  const int steps = ub_cdiv(a.H * (Q8 ? 1 : 2), 64);
   const long items = (long)std::min(a.T * a.k, a.E) * (a.I / 8);
-  auto go = [&](auto sp, auto multi, auto ng) {
-    constexpr int SP = decltype(sp)::value, NG = decltype(ng)::value;
-    const unsigned g = (unsigned)std::min<long>((items + NG - 1) / NG, 256);  // a workgroup a CU
-    k_up<DT, Q8, NPL, SP, decltype(multi)::value, NG><<<g, 64 * W1 * NG, 0, s>>>(a);
+  auto go = [&](auto sp, auto multi, auto ng, auto ni) {
+    constexpr int SP = decltype(sp)::value, NG = decltype(ng)::value, NI = decltype(ni)::value;
+    const unsigned g = (unsigned)std::min<long>((items / NI + NG - 1) / NG, 256);  // a workgroup a CU
+    k_up<DT, Q8, NPL, SP, decltype(multi)::value, NG, NI><<<g, 1024, 0, s>>>(a);
   };
-  using std::integral_constant;
-  integral_constant<int, 2> two;
+  // As few steps a wavefront as hold the row, with two items to a workgroup up to 4 (more
+  // bytes in flight; 8 of int8 are too many registers for 16 wavefronts).  Longer rows in
+  // pieces: four items side by side, so that activations are loaded a quarter as often,
+  // where there are enough items and those loads weigh something: int8, whose are twice the
+  // weights' bytes, or half of the tokens at least.  us of the layer, E 64, k 8, one by one /
+  // four, bf16 7168 x 512: T 4 137 / 140, 8 220 / 209, 16 318 / 277; int8: T 2 60 / 54, 16
+  // 230 / 172.
+  std::integral_constant<int, 1> one;
+  std::integral_constant<int, 2> two;
+  std::integral_constant<int, 4> four;
+  std::integral_constant<int, 8> eight;
   std::false_type once;
-  if (per <= 1) go(integral_constant<int, 1>{}, once, two);
-  else if (per <= 2) go(two, once, two);
-  else if (per <= 4) go(integral_constant<int, 4>{}, once, two);
-  else if (per <= 8) go(integral_constant<int, 8>{}, once, integral_constant<int, Q8 ? 1 : 2>{});  // (registers)
-  else go(integral_constant<int, 4>{}, std::true_type{}, two);
+  if (steps <= 8) return go(one, once, two, one);
+  if (steps <= 16) return go(two, once, two, one);
+  if (steps <= 32) return go(four, once, two, one);
+  if constexpr (Q8) {
+    if (steps <= 64) return go(four, once, one, one);
+  } else {
+    if (steps <= 64) return go(eight, once, two, one);
+    if (steps <= 128) return go(eight, once, one, one);
+  }
+  std::true_type multi;
+  if (items / 4 >= 256 && (Q8 || a.T >= 8)) return go(one, multi, one, four);
+  go(four, multi, two, one);
 }
 template <int DT, bool Q8>
 void decode(const DecodeArgs& a, hipStream_t s) {
