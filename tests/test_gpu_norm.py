@@ -319,6 +319,26 @@ def test_gradient_paths(dev):
     assert x.grad.data_ptr() != res.grad.data_ptr() and torch.equal(x.grad, res.grad)
 
 
+def test_the_gradient_is_of_the_calls_stream(dev):
+    # forward on a side stream that is busy, its backward asked for from another: it comes
+    # after, without a wait of the caller's
+    x, res, w = (t.requires_grad_() for t in make(dev, 64, 4096, torch.bfloat16))
+    n = norm.RmsNorm(w, EPS)
+    dy = torch.randn(64, 4096, device=dev).bfloat16()
+    want = torch.autograd.grad(n(x, res), (x, res, w), (dy, dy))
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            a = torch.ones(4096, 4096, device=dev)
+            for _ in range(8):
+                a = a.matmul(a).clamp(max=1)
+        y, h = n(x, res, stream=side)
+        got = torch.autograd.grad((y, h), (x, res, w), (dy, dy))
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+        torch.cuda.current_stream().wait_stream(side)
+
+
 def test_repeats_its_bits_and_streams(dev):
     x, res, w = make(dev, 1500, 1000, torch.bfloat16)
     w.requires_grad_()

@@ -6,6 +6,7 @@ from torch.autograd.function import once_differentiable
 
 from .native import _native, call
 from .ops import _need_cuda
+from .rope import _stored
 
 _OUT = {None: 0, "int8": 1, "e4m3": 2, "fp4": 3, "fp8": 4}
 
@@ -40,7 +41,8 @@ class RmsNorm:
             raise ValueError(f"RmsNorm: quant {quant!r} (one of {list(_OUT)})")
         r = call(_native.norm, stream, x, self.weight, residual, residual_out, self.eps, _OUT[quant])
         if r is None:  # a gradient is asked for
-            y, h = _Norm.apply(x, residual, self.weight, self.eps, stream)
+            with torch.cuda.stream(stream):  # the backward pass is of the same stream
+                y, h = _Norm.apply(x, residual, self.weight, self.eps)
             return y if residual is None else (y, h)
         return r
 
@@ -52,10 +54,10 @@ class _Norm(torch.autograd.Function):
     is the same."""
 
     @staticmethod
-    def forward(ctx, x, residual, w, eps, stream):
-        r = call(_native.norm, stream, x, w, residual, None, eps, 0)
+    def forward(ctx, x, residual, w, eps):
+        r = call(_native.norm, None, x, w, residual, None, eps, 0)
         y, h = (r, None) if residual is None else r
-        ctx.eps, ctx.stream, ctx.added = eps, stream, residual is not None
+        ctx.eps = eps
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x if h is None else h, w)
         return y, h
@@ -68,5 +70,6 @@ class _Norm(torch.autograd.Function):
         if dy is None:  # only h was used
             dx, dw = dh, torch.zeros_like(w) if need_w else None
         else:
-            dx, dw = call(_native.norm_grad, None, h.contiguous(), w, dy, dh, ctx.eps, need_x or need_res, need_w)
-        return dx if need_x else None, dx if need_res else None, dw, None, None
+            dx, dw = call(_native.norm_grad, None, h.contiguous(), w, _stored(dy), _stored(dh), ctx.eps,
+                          need_x or need_res, need_w)
+        return dx if need_x else None, dx if need_res else None, dw, None
