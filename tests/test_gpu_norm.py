@@ -10,6 +10,7 @@ import pytest
 import torch
 
 from ubridge_amd import fp8, int8, mx, norm
+from ubridge_amd.native import _native
 
 pytestmark = pytest.mark.gpu
 
@@ -319,6 +320,16 @@ def test_gradient_paths(dev):
     assert x.grad.data_ptr() != res.grad.data_ptr() and torch.equal(x.grad, res.grad)
 
 
+def test_forward_mode_is_refused(dev):
+    x, res, w = make(dev, 4, 64, torch.float32)
+    with torch.autograd.forward_ad.dual_level():
+        d = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: norm.RmsNorm(w, EPS)(d), lambda: norm.RmsNorm(w, EPS)(x, d), lambda: norm.RmsNorm(d[0], EPS)(x, quant="int8")):
+            with pytest.raises(ValueError, match="forward mode"):
+                call()
+        near(norm.RmsNorm(w, EPS)(x), plain(x, None, w)[1])
+
+
 def test_the_gradient_is_of_the_calls_stream(dev):
     # forward on a side stream that is busy, its backward asked for from another: it comes
     # after, without a wait of the caller's
@@ -434,6 +445,28 @@ def test_rows_past_32_bits(dev):
     last = x.detach()[-3:].clone().requires_grad_()
     (want,) = torch.autograd.grad(n(last), [last], y[-3:])
     assert torch.equal(dx[-3:], want)
+
+
+def test_a_captured_gradient_refuses_leaves_of_a_living_eager_graph(dev):
+    x, res, w = make(dev, 8, 256, torch.bfloat16)
+    w.requires_grad_()
+    n = norm.RmsNorm(w, EPS)
+    y = n(x, res)[0]  # lives, on the default stream
+    assert _native.default_stream_leaf(x, None, w) and not _native.default_stream_leaf(x, res)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(ValueError, match="lives"):
+            n(x, res)
+        with torch.no_grad():
+            z = n(x, res)[0]  # without a gradient: as ever
+    graph.replay()
+    assert torch.equal(z, y)
+    del y
+    assert not _native.default_stream_leaf(x, w)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        y = n(x, res)[0]
+    assert not _native.default_stream_leaf(x, w)
 
 
 def test_gradient_in_a_graph(dev):

@@ -14,7 +14,9 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include "../../include/ubridge_hip.h"
 
@@ -532,6 +534,23 @@ PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// Whether one of the tensors (or None) is a leaf whose gradient is accumulated on the
+// default stream, by a graph that lives already: a backward pass that is being captured
+// would wait for that stream, which ends the capture and with it the process.
+PyObject* py_default_stream_leaf(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  for (Py_ssize_t i = 0; i < nargs; i++) {
+    Ten t;
+    if (!optional(args[i], t)) return nullptr;
+    if (!t || !t->requires_grad() || t->grad_fn()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto stream = node ? node->stream() : std::nullopt;
+    if (stream && stream->id() == 0) Py_RETURN_TRUE;
+  }
+  Py_RETURN_FALSE;
+  END_HANDLE_TH_ERRORS
+}
+
 // h [..., C], w, dy, dh | None, eps, whether dx, whether dw, stream -> (dx | None, dw | None)
 PyObject* py_norm_grad(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   COUNT(8)
@@ -775,6 +794,7 @@ PyMethodDef methods[] = {
     {"compact", (PyCFunction)(void (*)())py_compact, METH_FASTCALL, nullptr},
     {"linear_codes", (PyCFunction)(void (*)())py_linear_codes, METH_FASTCALL, nullptr},
     {"norm", (PyCFunction)(void (*)())py_norm, METH_FASTCALL, nullptr},
+    {"default_stream_leaf", (PyCFunction)(void (*)())py_default_stream_leaf, METH_FASTCALL, nullptr},
     {"norm_grad", (PyCFunction)(void (*)())py_norm_grad, METH_FASTCALL, nullptr},
     {"mx_quantize", (PyCFunction)(void (*)())py_mx_quantize, METH_FASTCALL, nullptr},
     {"mx_dequantize", (PyCFunction)(void (*)())py_mx_dequantize, METH_FASTCALL, nullptr},

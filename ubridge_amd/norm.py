@@ -2,11 +2,12 @@
 the rounding that the next product wants, in one launch; differentiable where the
 result keeps its type."""
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .native import _native, call
 from .ops import _need_cuda
-from .rope import _stored
+from .rope import _level, _stored
 
 _OUT = {None: 0, "int8": 1, "e4m3": 2, "fp4": 3, "fp8": 4}
 
@@ -29,7 +30,9 @@ class RmsNorm:
     zeros.  Codes of such a row are 0 under a scale of NaN; of blocks, those that hold
     a NaN are NaN.  At most 2 ** 22 - 1 rows.  Without quant the call is differentiable, once,
     in x, residual and weight; with it, or into residual_out, it has no gradient and
-    refuses inputs that ask for one.
+    refuses inputs that ask for one; inputs with a tangent (forward mode) are always refused.  A call that
+    is captured for its gradient is refused while results of an eager one of the same
+    leaves live that was on the default stream.
     """
 
     def __init__(self, weight, eps=1e-6):
@@ -39,9 +42,15 @@ class RmsNorm:
     def forward(self, x, residual=None, quant=None, residual_out=None, stream=None):
         if quant not in _OUT:
             raise ValueError(f"RmsNorm: quant {quant!r} (one of {list(_OUT)})")
+        if _level() >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                 for t in (x, residual, self.weight)):
+            raise ValueError("RmsNorm: no forward mode")
         r = call(_native.norm, stream, x, self.weight, residual, residual_out, self.eps, _OUT[quant])
         if r is None:  # a gradient is asked for
             with torch.cuda.stream(stream):  # the backward pass is of the same stream
+                if torch.cuda.is_current_stream_capturing() and _native.default_stream_leaf(x, residual, self.weight):
+                    raise ValueError("RmsNorm: captured with a gradient while an eager graph of the same leaves lives: "
+                                     "delete its results first, or make them on another stream than the default one")
                 y, h = _Norm.apply(x, residual, self.weight, self.eps)
             return y if residual is None else (y, h)
         return r
