@@ -70,7 +70,9 @@ const char* ubridge_version(void);
  * buffer of (current device, stream), including buffers graphs captured on
  * it still name (do not replay those graphs afterwards).  Call it before
  * destroying a stream the library has used.  Fails (1) while the stream
- * captures.  topsaten_release_graph_workspace_pool does the same.
+ * captures.  (Graphs captured on one stream share its buffer: replay them one
+ * after the other.  Calls of the norm and feed-forward half have buffers of
+ * each capture's own.)  topsaten_release_graph_workspace_pool does the same.
  *
  * ubridge_workspace_stats: pool buffers allocated and not yet freed (count,
  * bytes, all devices and streams) and caller-allocator blocks not yet handed

@@ -142,3 +142,49 @@ def test_main(dev, capsys, monkeypatch):
                                      "--topk", "2", "--vocab", "100"])
     example.main()
     assert "tokens" in capsys.readouterr().out
+
+
+def test_graphs_of_one_stream_side_by_side(dev):
+    # two graphs captured on one stream have scratch of their own each: replayed on two
+    # streams at once, beside eager calls, all keep their bits
+    from ubridge_amd import ops
+    g = torch.Generator().manual_seed(5)
+    halves, head = example.build(2, 256, 96, 16, 4, 100, g)
+    layer = halves[1][1].layer
+    lin = mx.Linear(*mx.quantize(torch.randn(200, 2000, generator=g).to(dev)), 2000)
+    n = norm.RmsNorm(torch.rand(2000, generator=g).to(dev).requires_grad_())
+
+    def run(x, lg, big, dy):
+        w = n.weight
+        return [layer.decode(x, lg), lin(big), torch.autograd.grad(n(big), [w], dy)[0]]
+    E = layer.E
+    ins = [[torch.randn(m, 256, generator=g).bfloat16().to(dev), torch.randn(m, E, generator=g).to(dev),
+            torch.randn(300, 2000, generator=g).bfloat16().to(dev), torch.randn(300, 2000, generator=g).bfloat16().to(dev)]
+           for m in (16, 16, 16)]
+    want = [run(*i) for i in ins]
+    want = [[t.clone() for t in w] for w in want]
+    capture = torch.cuda.Stream()
+    ops.release_workspace(capture)
+    live = [ops.workspace_stats()[0]]
+    graphs, outs = [], []
+    for i in ins[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=capture):
+            outs.append(run(*i))
+        graphs.append(graph)
+        live.append(ops.workspace_stats()[0])
+    assert live[0] < live[1] < live[2], live
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        with torch.cuda.stream(capture):
+            got = run(*ins[2])
+        torch.cuda.synchronize()
+        for o, w in zip([*outs, got], want):
+            assert all(torch.equal(a, b) for a, b in zip(o, w))
+    del graphs, outs
+    ops.release_workspace(capture)
+    assert ops.workspace_stats()[0] == live[0]

@@ -54,10 +54,12 @@ int ub_tune(int knob);
 // per-(device, stream) pool (ubridge_release_workspace frees it).  Works while
 // s captures a graph (the allocation is made outside the capture), so the
 // route a call takes never depends on whether an eager call came first;
-// get() is null only when the allocation itself fails.
+// get() is null only when the allocation itself fails.  per_graph: a call that is
+// captured draws on buffers of that graph's own, so that graphs captured on one
+// stream may be replayed side by side on others.
 class UbScratch {
  public:
-  UbScratch(hipStream_t s, size_t bytes);
+  UbScratch(hipStream_t s, size_t bytes, bool per_graph = false);
   ~UbScratch();
   UbScratch(const UbScratch&) = delete;
   UbScratch& operator=(const UbScratch&) = delete;

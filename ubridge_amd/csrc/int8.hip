@@ -770,7 +770,7 @@ int linear_codes(const char* nm, const int8_t* a, const float* sa, const int8_t*
   const Plan plan = plan_for(M, N, ld / 128);
   const int parts = ub_cdiv(ld / 128, ub_cdiv(ld / 128, plan.parts));
   const size_t sums = parts > 1 ? sizeof(int) * parts * (size_t)M * N : 0;
-  UbScratch ws(s, sums);
+  UbScratch ws(s, sums, true);
   if (sums && !ws.get()) return ub_set_error(UB_ERR_LAUNCH, "%s: no workspace", nm);
   product<DT>(plan, parts, a, sa, w, sw, bias, y, (int*)ws.get(), M, N, ld, s);
   return UB_OK;

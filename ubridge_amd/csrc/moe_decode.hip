@@ -469,7 +469,7 @@ UB_API int ubridge_moe_decode(const UbridgeMoeDecodeArgs* p, void* stream) {
   UB_REQUIRE((((uintptr_t)p->x | (uintptr_t)p->w13 | (uintptr_t)p->w2) & 15) == 0, "%s: x or weights not 16-byte aligned", nm);
   hipStream_t s = ub_stream(stream);
   const size_t act = ((size_t)p->T * p->k * p->I * 2 + 255) / 256 * 256;
-  UbScratch ws(s, act + sizeof(Route));
+  UbScratch ws(s, act + sizeof(Route), true);
   UB_REQUIRE(ws.get(), "%s: no workspace", nm);
   const DecodeArgs a = {p->x, p->logits, p->w13, p->s13, p->w2, p->s2, p->y, ws.get(), (Route*)((char*)ws.get() + act),
                         p->T, p->E, p->k, p->H, p->I, p->logits_dtype, p->renormalize};

@@ -678,7 +678,7 @@ int linear(const char* nm, const UbridgeMxLinearArgs& p, hipStream_t s) {
       return UB_OK;
     }
     const size_t codes = p.x ? (size_t)M * nk * kRowStep<F> : 0;
-    UbScratch ws(s, codes + (p.x ? (size_t)M * nk * 4 : 0));
+    UbScratch ws(s, codes + (p.x ? (size_t)M * nk * 4 : 0), true);
     if (p.x) {
       uint8_t* q = (uint8_t*)ws.get();
       if (!q) return ub_set_error(UB_ERR_LAUNCH, "%s: no workspace", nm);
@@ -693,7 +693,7 @@ int linear(const char* nm, const UbridgeMxLinearArgs& p, hipStream_t s) {
   const int part = ub_cdiv(nk, plan.parts), parts = ub_cdiv(nk, part);  // (none empty)
   const size_t rows = (size_t)ub_cdiv(M, 16) * 16, codes = rows * nk * kRowStep<F>, words = rows * nk * 4;
   const size_t sums = parts > 1 ? sizeof(float) * parts * (size_t)M * N : 0;
-  UbScratch ws(s, codes + words + sums);
+  UbScratch ws(s, codes + words + sums, true);
   uint8_t* q = (uint8_t*)ws.get();
   if (!q) return ub_set_error(UB_ERR_LAUNCH, "%s: no workspace", nm);
   uint8_t* qs = q + codes;

@@ -433,7 +433,7 @@ UB_API int ubridge_rms_norm_grad(const UbridgeRmsNormGradArgs* p, void* stream) 
   if (p->R == 0 && !p->dw) return UB_OK;
   hipStream_t s = ub_stream(stream);
   const int groups = p->R < kGradGroups ? p->R : kGradGroups;
-  UbScratch ws(s, p->dw ? sizeof(float) * (size_t)groups * p->C : 0);
+  UbScratch ws(s, p->dw ? sizeof(float) * (size_t)groups * p->C : 0, true);
   UB_REQUIRE(!p->dw || groups == 0 || ws.get(), "%s: no workspace", nm);
   const NormGradArgs a = {p->h, p->w, p->dy, p->dh, p->dx, p->dw ? ws.get() : nullptr, p->R, p->C, p->w_dtype == UB_F32, p->eps};
   if (groups) {

@@ -120,7 +120,9 @@ UB_API int ubridge_tune_get(const char* name) {
 //    it outgrows is retired: freed once an event recorded after its last use
 //    has completed, unless it was handed out while the stream captured a
 //    graph (graphs keep its address: it then lives until
-//    ubridge_release_workspace).  ubridge_release_workspace(stream)
+//    ubridge_release_workspace).  Calls that ask for it draw, while they are
+//    captured, on buffers of that capture alone, which live as long.
+//    ubridge_release_workspace(stream)
 //    synchronizes the stream and frees all of that stream's buffers.
 // Growth during a graph capture allocates with the capture mode relaxed, so
 // calls take the same route (and give the same bits) captured or eager.
@@ -133,6 +135,7 @@ struct WsBuf {
   void* p = nullptr;
   size_t bytes = 0;
   bool graph = false;  // handed out during a capture
+  unsigned long long capture = 0;  // the one capture that it belongs to (0: any)
 };
 struct WsRetired {
   WsBuf b;
@@ -157,6 +160,17 @@ bool capturing(hipStream_t s) {
     return false;
   }
   return st != hipStreamCaptureStatusNone;
+}
+
+// The capture's own number, or 0 (not known: the stream's shared buffer serves).
+unsigned long long capture_id(hipStream_t s) {
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo(s, &st, &id) != hipSuccess) {
+    (void)hipGetLastError();
+    return 0;
+  }
+  return st == hipStreamCaptureStatusActive ? id : 0;
 }
 
 void ws_free(const WsBuf& b) {
@@ -199,40 +213,59 @@ void ws_sweep(WsPool& pool, hipStream_t s) {
   }
 }
 
-void* ws_pool_get(hipStream_t s, size_t bytes) {
+// A new buffer (caller holds g_ws_mu); p null: none to be had.
+WsBuf ws_new(size_t bytes) {
+  WsBuf b;
+  const size_t sz = bytes < ((size_t)1 << 20) ? ((size_t)1 << 20) : bytes;
+  hipError_t e;
+  {
+    UbRelaxCapture relax;
+    e = hipMalloc(&b.p, sz);
+  }
+  if (e != hipSuccess) {
+    (void)hipGetLastError();
+    b.p = nullptr;
+    return b;
+  }
+  g_ws_live_n++;
+  g_ws_live_bytes += sz;
+  b.bytes = sz;
+  return b;
+}
+
+void* ws_pool_get(hipStream_t s, size_t bytes, bool per_graph) {
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess) return nullptr;
   const bool cap = capturing(s);
   std::lock_guard<std::mutex> lk(g_ws_mu);
   WsPool& pool = g_ws[{dev, s}];
   if (!cap && !pool.retired.empty()) ws_sweep(pool, s);
+  if (const unsigned long long id = cap && per_graph ? capture_id(s) : 0) {
+    for (const WsRetired& r : pool.retired)
+      if (r.b.capture == id && r.b.bytes >= bytes) return r.b.p;
+    WsBuf b = ws_new(bytes);
+    if (!b.p) return nullptr;
+    b.graph = true, b.capture = id;
+    pool.retired.push_back(WsRetired{b, nullptr});
+    return b.p;
+  }
   if (pool.cur.bytes >= bytes) {
     pool.cur.graph |= cap;
     return pool.cur.p;
   }
-  void* p = nullptr;
-  const size_t sz = bytes < ((size_t)1 << 20) ? ((size_t)1 << 20) : bytes;
-  hipError_t e;
-  {
-    UbRelaxCapture relax;
-    e = hipMalloc(&p, sz);
-  }
-  if (e != hipSuccess) {
-    (void)hipGetLastError();
-    return nullptr;
-  }
-  g_ws_live_n++;
-  g_ws_live_bytes += sz;
+  WsBuf b = ws_new(bytes);
+  if (!b.p) return nullptr;
   if (pool.cur.p) {
     pool.retired.push_back(WsRetired{pool.cur, nullptr});
     if (!cap) ws_sweep(pool, s);  // orders it behind the work already on s
   }
-  pool.cur = WsBuf{p, sz, cap};
-  return p;
+  b.graph = cap;
+  pool.cur = b;
+  return b.p;
 }
 }  // namespace
 
-UbScratch::UbScratch(hipStream_t s, size_t bytes) : s_(s) {
+UbScratch::UbScratch(hipStream_t s, size_t bytes, bool per_graph) : s_(s) {
   if (bytes == 0) return;
   ubridge_ws_alloc_fn fa;
   void* ctx;
@@ -251,7 +284,7 @@ UbScratch::UbScratch(hipStream_t s, size_t bytes) : s_(s) {
     }
     return;
   }
-  p_ = ws_pool_get(s, bytes);
+  p_ = ws_pool_get(s, bytes, per_graph);
 }
 
 UbScratch::~UbScratch() {
