@@ -554,12 +554,15 @@ int ubridge_mx_pack(const void* codes, const void* scales, void* w, void* w_scal
  * y T [M, N] contiguous, bias f32 [N] or NULL.  Sums are f32.  Scratch beyond 16 tokens
  * or M K = 61440, where the call rounds: the codes and scales; and, beyond 16 tokens or
  * where their codes pass a workgroup's 160 KiB, the codes laid out, and 4 M N bytes a part
- * where long rows are cut (at most 32). */
+ * where long rows are cut (at most 32).  one_product (else 0), of format 8 with f16 or
+ * bf16 results beyond 16 tokens: one matrix product in place of two, which drops what
+ * lies 2^-13 below the largest of neighbouring products, at most 2^-10 of the sum of
+ * magnitudes. */
 typedef struct {
   const void *x, *codes, *scales, *w, *w_scales;
   const float* bias;
   void* y;
-  int32_t M, K, N, dtype, format, pad;
+  int32_t M, K, N, dtype, format, one_product;
 } UbridgeMxLinearArgs;
 int ubridge_mx_linear(const UbridgeMxLinearArgs* args, void* stream);
 

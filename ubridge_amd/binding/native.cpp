@@ -655,9 +655,9 @@ PyObject* py_mx_pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 // first (x [..., K], or codes), scales | None, w, w_scales, bias | None, K, N, format,
-// type code (of y, with codes), out | None, stream
+// type code (of y, with codes), out | None, whether one product, stream
 PyObject* py_mx_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  COUNT(11)
+  COUNT(12)
   HANDLE_TH_ERRORS
   const Args A{args};
   Ten x, s, w, ws, b, out;
@@ -691,8 +691,8 @@ PyObject* py_mx_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (s) p.codes = xc.data_ptr(), p.scales = s->data_ptr();
   else p.x = xc.data_ptr();
   p.w = w->data_ptr(), p.w_scales = ws->data_ptr(), p.bias = ptr(b), p.y = y.data_ptr();
-  p.M = M, p.K = K, p.N = N, p.dtype = dt, p.format = f;
-  void* stream = A.p(10);
+  p.M = M, p.K = K, p.N = N, p.dtype = dt, p.format = f, p.one_product = PyObject_IsTrue(args[10]);
+  void* stream = A.p(11);
   if (PyErr_Occurred()) return nullptr;
   if (const int rc = fn.mx_linear(&p, stream)) return PyLong_FromLong(rc);
   return THPVariable_Wrap(std::move(y));

@@ -9,10 +9,13 @@
 //
 // Of e4m3 the matrix unit aligns the products of neighbouring elements to the largest
 // exponent among them and drops what lies more than 13 bits below it (measured: 2^-9
-// is kept beside 2^4 and lost beside 2^5; e2m1's own products span less).  On values
-// like hidden states that leaves 6e-6 of a result, far below a 16-bit result's
-// rounding.  For f32 results a is cut in two by magnitude, at 2, and multiplied twice
-// (X below): either part's products lie within 14 bits, so nothing is dropped.
+// is kept beside 2^4 and lost beside 2^5; e2m1's own products span less): up to 2^-10 of
+// the sum of magnitudes, where large values cancel more than a result's rounding, 6e-6
+// of it on values like hidden states.  So a is cut in two by magnitude, at 2, and
+// multiplied twice (X, kSide, kTurn, kCut below): either part's products lie within 14
+// bits, and nothing is dropped.  A caller may take one product instead (one_product) for
+// 16-bit results of more than 16 tokens, where the second costs most: 4096 x 4096 x 14336
+// (M K N) 300 us against 195, 201 x 3520 x 9001 24 against 17.
 //
 // Rows are padded with zero codes to a step of 128 elements.  Outside, codes and
 // scales lie in rows; a weight is laid out once, activations by the kernel that
@@ -156,17 +159,21 @@ struct MxArgs {
 };
 
 __device__ __forceinline__ i32x8 wide(const i32x4& v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
-// e4m3 codes of magnitude 2 and more (HI), or below (bit 6 of a code tells), zeros
-// elsewhere
-template <bool HI>
-__device__ __forceinline__ i32x8 cut(const i32x8& v) {
-  i32x8 o;
+// e4m3 codes of magnitude 2 and more in `hi`, those below in `lo` (bit 6 of a code
+// tells), zeros elsewhere.  v_perm fills bytes with the sign of bytes 1 and 3 of either
+// operand: of v << 9 (codes 0 and 2) and of v << 1 (1 and 3).
+__device__ __forceinline__ uint32_t cut(uint32_t v, uint32_t& lo) {
+  const uint32_t m = __builtin_amdgcn_perm(v << 1, v << 9, 0x0b090a08u);
+  lo = v & ~m;
+  return v & m;
+}
+__device__ __forceinline__ void cut(const i32x8& v, i32x8& lo, i32x8& hi) {
 #pragma unroll
   for (int i = 0; i < 8; i++) {
-    const uint32_t t = (uint32_t)v[i] & 0x40404040u, m = ((t << 1) - (t >> 6)) | t << 1;
-    o[i] = (int)(HI ? (uint32_t)v[i] & m : (uint32_t)v[i] & ~m);
+    uint32_t l;
+    hi[i] = (int)cut((uint32_t)v[i], l);
+    lo[i] = (int)l;
   }
-  return o;
 }
 
 // Outputs of a wavefront, 32 TM x 32 TN, through its part of LDS in rows, so that
@@ -245,10 +252,10 @@ __device__ __forceinline__ int xcd_run(int i, int total) {
 // word shifted by 16 kh.  Fragments are in registers, two sets: those of one
 // product are read while the other's multiply.
 // Measured, e2m1 x e2m1, 4096 x 4096 x 14336 (M K N): 141 us, 3.4 PFLOP/s (3.9 at 8192^3); with
-// e4m3 activations 187.  From registers the unit reaches 7.7: the clock falls to 1.9 GHz, the
+// e4m3 activations 187, in two parts 290.  From registers the unit reaches 7.7: the clock falls to 1.9 GHz, the
 // fill of LDS alone takes two thirds of the time (17 TB/s out of L2), its reads and the
 // products as long each.  Small tiles are bound by that fill: 201 x 3520 x 9001 with e4m3
-// 14.6 us, 176 MB.
+// 14.6 us, 176 MB (in two parts 21).
 template <int F, int DT, bool X, int WM, int WN, int TM, int TN, int NS, int OCC>
 __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(OCC, OCC))) k_mx_gemm(MxArgs a) {
   constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN, NW = WM * WN, RB = kRowStep<F>;
@@ -346,20 +353,30 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
   };
   auto mul = [&](auto J) {
     constexpr int j = decltype(J)::value;
+    auto add = [&](int m, int n, const i32x8& v) {
+      acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(wf[j][n]), v, acc[m][n], 4, F == MX_FP4 ? 4 : 0, j,
+                                                                  (int)sw[n], j, (int)sa[m]);
+    };
+    auto act = [&](int m) {
+      if constexpr (F == MX_FP4) return wide(af[j][m]);
+      else return __builtin_shufflevector(af[j][m], ag[j][m], 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    if constexpr (X) {
 #pragma unroll
-    for (int n = 0; n < TN; n++)
+      for (int m = 0; m < TM; m++) {  // (cut once for all columns)
+        i32x8 lo, hi;
+        cut(act(m), lo, hi);
 #pragma unroll
-      for (int m = 0; m < TM; m++) {
-        i32x8 act;
-        if constexpr (F == MX_FP4) act = wide(af[j][m]);
-        else act = __builtin_shufflevector(af[j][m], ag[j][m], 0, 1, 2, 3, 4, 5, 6, 7);
-        auto add = [&](const i32x8& v) {
-          acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(wf[j][n]), v, acc[m][n], 4, F == MX_FP4 ? 4 : 0, j,
-                                                                      (int)sw[n], j, (int)sa[m]);
-        };
-        if constexpr (X) add(cut<false>(act)), add(cut<true>(act));
-        else add(act);
+        for (int n = 0; n < TN; n++) add(m, n, lo);
+#pragma unroll
+        for (int n = 0; n < TN; n++) add(m, n, hi);
       }
+    } else {
+#pragma unroll
+      for (int n = 0; n < TN; n++)
+#pragma unroll
+        for (int m = 0; m < TM; m++) add(m, n, act(m));
+    }
   };
   constexpr int PW = NL + SL;  // loads of a step in a wavefront
   const int k0 = kp * a.part, n = min(a.part, nk - k0);
@@ -422,13 +439,14 @@ __global__ void __launch_bounds__(256) k_mx_sum(const float* __restrict__ part, 
 // its steps: the tile's codes are consecutive in memory, and so are a wavefront's.
 // Weights go straight to the registers of v_mfma_scale_f32_16x16x128 as its left
 // operand, 2 P steps in flight; lane (r, h) holds block h of row r, and ends with
-// columns 4 h .. + 3 of token r.  The activations' codes lie in LDS for the whole
-// launch (rows 16 bytes further apart than they are long, for the banks); each
-// workgroup makes them itself while its first weights are on their way, up to kRound
-// values; beyond, a launch of its own makes them once.  The wavefronts' sums meet in LDS
-// in their order.
-// HBM bounds it where the weight is large, launch and first latency else: 1 x 14336 x 4096
-// (M K N) 7.8 us (31 MB, 4 TB/s), 16 x 4096 x 28672 12.6 (64 MB, 5 TB/s).
+// columns 4 h .. + 3 of token r.  The activations' codes (of e4m3 both parts, where they
+// fit) lie in LDS for the whole launch (rows 16 bytes further apart than they are long,
+// for the banks); each workgroup makes them itself while its first weights are on their
+// way, up to kRound values; beyond, a launch of its own makes them once.  The wavefronts'
+// sums meet in LDS in their order.
+// HBM bounds it where the weight is large, launch and first latency else.  us of codes that
+// are there, e2m1 / e4m3 (M x K x N): 1 x 14336 x 4096 7.5 / 8.2 (31 MB, 4 TB/s), 8 x 4096 x 28672
+// 11.0 / 11.5 (64 MB, 5.8 TB/s), 16 x 4096 x 28672 11.4 / 13.6 (one product alone 11.8).
 constexpr int DW = 16, RP = 20;  // wavefronts; floats of a token's row of sums
 
 struct MxDecArgs {
@@ -440,17 +458,24 @@ struct MxDecArgs {
   int M, K, N, nk, tiles, ks, per;  // per: steps of a wavefront
 };
 
-template <int F, int DT, bool PRE>
+// Where the two parts of e4m3 activations (`cut`) are: of e2m1 none; cut in registers by
+// every wavefront; or both in LDS, and multiplied as columns 0-7 and 8-15 of one product
+// (up to 8 tokens), or in turn.  us, 16 x 4096 x 28672, in turn / in registers: 13.6 / 16.9.
+enum { kWhole, kCut, kSide, kTurn };
+
+template <int F, int DT, bool PRE, int PARTS>
 __global__ void __launch_bounds__(64 * DW) k_mx_dec(MxDecArgs a) {
   typedef typename MxElem<DT>::T T;
   constexpr int E = MxElem<DT>::E, BL = 32 / E, XU = 8, P = 4, RB = kRowStep<F>;
+  constexpr bool TWO = PARTS == kSide || PARTS == kTurn;
+  static_assert((PARTS == kWhole) == (F == MX_FP4), "the parts of e4m3");
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, h = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nk = a.nk, M = a.M, pitch = nk * RB + 16, spitch = nk * 4 + 4;
   float* red = (float*)lds;                       // [16 wavefronts][16 tokens][RP]
-  uint8_t* ac = lds + sizeof(float) * DW * 16 * RP;  // codes [M][pitch]
-  uint8_t* as = ac + M * pitch;                   // scale bytes [M][spitch]
+  uint8_t* ac = lds + sizeof(float) * DW * 16 * RP;  // codes [M][pitch], TWO: the lower parts behind them
+  uint8_t* as = ac + (TWO ? 2 : 1) * M * pitch;  // scale bytes [M][spitch]
   const int nt = (a.N + 15) / 16, tl = wave / a.ks, kp = wave - tl * a.ks;
   const int s0 = kp * a.per, s1 = min(nk, s0 + a.per);
   const int pieces = (a.per + P - 1) / P;
@@ -510,7 +535,14 @@ __global__ void __launch_bounds__(64 * DW) k_mx_dec(MxDecArgs a) {
     const uint32_t rowu = (uint32_t)nk * UR;
     auto put = [&](const uint4& v, uint32_t i) {
       const uint32_t row = i / rowu;
-      *(uint4*)(ac + row * pitch + (i - row * rowu) * 16) = v;
+      uint8_t* p = ac + row * pitch + (i - row * rowu) * 16;
+      if constexpr (TWO) {
+        uint4 lo;
+        *(uint4*)p = make_uint4(cut(v.x, lo.x), cut(v.y, lo.y), cut(v.z, lo.z), cut(v.w, lo.w));
+        *(uint4*)(p + M * pitch) = lo;
+      } else {
+        *(uint4*)p = v;
+      }
     };
 #pragma unroll
     for (int j = 0; j < XU; j++)
@@ -523,7 +555,13 @@ __global__ void __launch_bounds__(64 * DW) k_mx_dec(MxDecArgs a) {
       const uint32_t row = i / per, u = i - row * per;
       uint32_t o[2];
       const uint32_t b = mx_round<DT, F>(v, o);
-      mx_store<DT, F>(ac + row * pitch + u * (E * F / 8), o);
+      uint8_t* p = ac + row * pitch + u * (E * F / 8);
+      if constexpr (TWO) {
+        uint32_t lo[2];
+        o[0] = cut(o[0], lo[0]), o[1] = cut(o[1], lo[1]);
+        mx_store<DT, F>(p + M * pitch, lo);
+      }
+      mx_store<DT, F>(p, o);
       if (u % BL == 0) as[row * spitch + u / BL] = (uint8_t)b;
     };
 #pragma unroll
@@ -535,24 +573,37 @@ __global__ void __launch_bounds__(64 * DW) k_mx_dec(MxDecArgs a) {
     }
   }
   __syncthreads();
-  const int tok = min(r, M - 1);  // (tokens past M: not used)
-  const uint8_t* ar = ac + tok * pitch + 16 * h;
+  const int tok = min(PARTS == kSide ? r & 7 : r, M - 1);  // (tokens past M: not used)
+  const uint8_t* ar = ac + (PARTS == kSide && r >= 8 ? M + tok : tok) * pitch + 16 * h;
   const uint8_t* sr = as + tok * spitch + h;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   auto work = [&](Set& b, Scales& sc) {
+    auto steps = [&](const uint8_t* ar) {
 #pragma unroll
-    for (int i = 0; i < P; i++) {
-      const int s = min(s0 + c * P + i, nk - 1);  // (past the run: times zeros)
-      const uint32_t sa = s0 + c * P + i < s1 ? sr[4 * s] : 0;  // (and no NaN of another's block)
-      i32x8 act;
-      if constexpr (F == MX_FP4) act = wide(*(const i32x4*)(ar + s * RB));
-      else act = __builtin_shufflevector(*(const i32x4*)(ar + s * RB), *(const i32x4*)(ar + s * RB + 64), 0, 1, 2, 3, 4, 5, 6, 7);
-      auto add = [&](const i32x8& v) {
-        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(b[i]), v, acc, 4, F == MX_FP4 ? 4 : 0, 0, (int)sc[i], 0,
-                                                               (int)sa);
-      };
-      if constexpr (F == MX_FP8 && DT == UB_F32) add(cut<false>(act)), add(cut<true>(act));
-      else add(act);
+      for (int i = 0; i < P; i++) {
+        const int s = min(s0 + c * P + i, nk - 1);  // (past the run: times zeros)
+        const uint32_t sa = s0 + c * P + i < s1 ? sr[4 * s] : 0;  // (and no NaN of another's block)
+        i32x8 act;
+        if constexpr (F == MX_FP4) act = wide(*(const i32x4*)(ar + s * RB));
+        else act = __builtin_shufflevector(*(const i32x4*)(ar + s * RB), *(const i32x4*)(ar + s * RB + 64), 0, 1, 2, 3, 4, 5, 6, 7);
+        auto add = [&](const i32x8& v) {
+          acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(b[i]), v, acc, 4, F == MX_FP4 ? 4 : 0, 0, (int)sc[i], 0,
+                                                                 (int)sa);
+        };
+        if constexpr (PARTS == kCut) {
+          i32x8 lo, hi;
+          cut(act, lo, hi);
+          add(lo), add(hi);
+        } else {
+          add(act);
+        }
+      }
+    };
+    if constexpr (PARTS == kTurn) {
+#pragma unroll 1  // (of both parts at once the operands spill)
+      for (int p = 1; p >= 0; p--) steps(ar + p * M * pitch);
+    } else {
+      steps(ar);
     }
     load(b, sc, gn, cn);
     next(gn, cn);
@@ -564,7 +615,10 @@ __global__ void __launch_bounds__(64 * DW) k_mx_dec(MxDecArgs a) {
       for (int i = tid; i < a.tiles * M * 16; i += 64 * DW) {
         const int j = i & 15, mt = i >> 4, t = mt / M, m = mt - t * M, n = (g * a.tiles + t) * 16 + j;
         float v = 0.f;
-        for (int p = 0; p < a.ks; p++) v += red[((t * a.ks + p) * 16 + m) * RP + j];
+        for (int p = 0; p < a.ks; p++) {
+          v += red[((t * a.ks + p) * 16 + m) * RP + j];
+          if constexpr (PARTS == kSide) v += red[((t * a.ks + p) * 16 + m + 8) * RP + j];
+        }
         if (n < a.N) ub_store<DT>(a.y, (size_t)m * a.N + n, v + (a.bias ? a.bias[n] : 0.f));
       }
       __builtin_amdgcn_s_waitcnt(0xC07F);
@@ -586,21 +640,29 @@ __global__ void __launch_bounds__(64 * DW) k_mx_dec(MxDecArgs a) {
 // TB/s).
 constexpr int kRound = 60 * 1024;
 constexpr int kCUs = 256, kLds = 160 * 1024;
-size_t dec_lds(int F, int M, int nk) {
-  return sizeof(float) * DW * 16 * RP + (size_t)M * (nk * 128 * F / 8 + 16 + nk * 4 + 4) + 16;
+size_t dec_lds(int F, int M, int nk, bool two) {
+  return sizeof(float) * DW * 16 * RP + (size_t)M * ((two ? 2 : 1) * (nk * 128 * F / 8 + 16) + nk * 4 + 4) + 16;
 }
 
-template <int F, int DT, bool PRE>
-void dec(MxDecArgs a, hipStream_t s) {
+template <int F, int DT, bool PRE, int PARTS>
+void dec_as(MxDecArgs a, hipStream_t s) {
   static UbLdsLimit limit;
-  limit.raise((const void*)k_mx_dec<F, DT, PRE>, kLds);
+  limit.raise((const void*)k_mx_dec<F, DT, PRE, PARTS>, kLds);
   const int nt = ub_cdiv(a.N, 16);
   // a group of tiles for every CU, as many wavefronts to a tile as that leaves
   a.tiles = nt <= kCUs ? 1 : nt <= kCUs * DW ? ub_cdiv(nt, kCUs) : DW;
   a.ks = DW / a.tiles;
   a.per = ub_cdiv(a.nk, a.ks);
   const int groups = ub_cdiv(nt, a.tiles);
-  k_mx_dec<F, DT, PRE><<<groups < kCUs ? groups : kCUs, 64 * DW, dec_lds(F, a.M, a.nk), s>>>(a);
+  k_mx_dec<F, DT, PRE, PARTS><<<groups < kCUs ? groups : kCUs, 64 * DW, dec_lds(F, a.M, a.nk, PARTS >= kSide), s>>>(a);
+}
+
+template <int F, int DT, bool PRE>
+void dec(const MxDecArgs& a, hipStream_t s) {
+  if constexpr (F == MX_FP4) dec_as<F, DT, PRE, kWhole>(a, s);
+  else if (dec_lds(F, a.M, a.nk, true) > kLds) dec_as<F, DT, PRE, kCut>(a, s);
+  else if (a.M <= 8) dec_as<F, DT, PRE, kSide>(a, s);
+  else dec_as<F, DT, PRE, kTurn>(a, s);
 }
 
 // ------------------------------------------------------------- the choice
@@ -620,18 +682,20 @@ void quantize(const void* x, uint8_t* q, uint8_t* sc, int R, int C, int nk, bool
 // 9.9 (31 / 17 / 10.5 / 10.5), 201 x 3520 x 9001 24.5 / 13.1 / 13.1 / 12.5 (31 / 16.4 / 16.8 /
 // 14.0), 512 x 4096 x 4096 23.5 / 13.9 / 12.1 / 13.6 (31 / 17 / 14.8 / 15.7), 1646 x 5413 x 4856
 // 35 / 27 / 41 / -, 1024 x 4096 x 14336 42 / 46 / 58 / 80 (55 / 75 / 78 / 91); 160 x 10304 x 436
-// in 8 parts 8.6 on the last two.  The f32 form of e4m3 has too few registers for the
-// first.
+// in 8 parts 8.6 on the last two.  e4m3 in two parts, the call with codes that are there,
+// on the same tiles: 64 x 4096 x 6144 - / 31 / 19 / 19, 201 x 3520 x 9001 52 / 30 / 29 / 24, 512 x
+// 4096 x 4096 56 / 34 / 28 / 27, 1646 x 5413 x 4856 80 / 86 / 102 / -, 1024 x 4096 x 14336 89 / 120 /
+// 127 / -.
 struct Plan { int tile, parts; };
 Plan plan_for(int F, bool X, int M, int N, int nk) {
-  static const struct { int m, n, tile, one[2], each[2]; } t[4] = {{128, 256, 390, {63, 75}, {50, 70}},
-                                                                   {128, 128, 150, {25, 38}, {28, 51}},
-                                                                   {64, 64, 60, {17, 22}, {12, 16}},
-                                                                   {32, 128, 60, {20, 22}, {15, 18}}};
-  const int f = F == MX_FP8;
+  static const struct { int m, n, tile, one[3], each[3]; } t[4] = {{128, 256, 390, {63, 75, 124}, {50, 70, 122}},
+                                                                   {128, 128, 150, {25, 38, 63}, {28, 51, 78}},
+                                                                   {64, 64, 60, {17, 22, 37}, {12, 16, 26}},
+                                                                   {32, 128, 60, {20, 22, 37}, {15, 18, 28}}};
+  const int f = F == MX_FP4 ? 0 : X ? 2 : 1;
   Plan best = {-1, 1};
   double least = 0;
-  for (int i = X; i < 4; i++) {
+  for (int i = 0; i < 4; i++) {
     const int64_t tiles = (int64_t)ub_cdiv(M, t[i].m) * ub_cdiv(N, t[i].n);
     for (int p = 1; p <= 32 && p <= nk; p *= 2) {
       if (p > 1 && (tiles * p > 1024 || (int64_t)M * N >= 1 << 26)) break;
@@ -658,9 +722,12 @@ void gemm(int tile, const MxArgs& a, int parts, hipStream_t s) {
     return;                                                                                              \
   }
   // rings as deep as leaves two workgroups of the large tiles to a CU, four of the small
-  if constexpr (!X)
-    if (tile == 0) UB_MX(2, 2, 2, 4, (F == MX_FP4 ? 3 : 2), 2)
-  if (tile <= 1) UB_MX(2, 4, 2, 1, 3, (F == MX_FP4 ? 4 : 2))
+  if (tile == 0) UB_MX(2, 2, 2, 4, (F == MX_FP4 ? 3 : 2), 2)
+  if constexpr (X) {
+    if (tile == 1) UB_MX(4, 2, 1, 2, 3, 2)
+  } else {
+    if (tile == 1) UB_MX(2, 4, 2, 1, 3, (F == MX_FP4 ? 4 : 2))
+  }
   if (tile == 2) UB_MX(2, 2, 1, 1, (F == MX_FP4 ? 4 : 3), 4)
   UB_MX(1, 4, 1, 1, (F == MX_FP4 ? 6 : 5), 4)
 #undef UB_MX
@@ -671,7 +738,7 @@ int linear(const char* nm, const UbridgeMxLinearArgs& p, hipStream_t s) {
   const int nk = ub_cdiv(p.K, 128), M = p.M, N = p.N;
   const uint8_t* w = (const uint8_t*)p.w;
   const uint32_t* sw = (const uint32_t*)p.w_scales;
-  if (M <= 16 && dec_lds(F, M, nk) <= kLds) {
+  if (M <= 16 && dec_lds(F, M, nk, false) <= kLds) {
     MxDecArgs d = {p.x, (const uint8_t*)p.codes, (const uint8_t*)p.scales, w, sw, p.bias, p.y, M, p.K, N, nk, 0, 0, 0};
     if (p.x && (int64_t)M * p.K <= kRound) {
       dec<F, DT, false>(d, s);
@@ -688,8 +755,10 @@ int linear(const char* nm, const UbridgeMxLinearArgs& p, hipStream_t s) {
     dec<F, DT, true>(d, s);
     return UB_OK;
   }
-  constexpr bool X = F == MX_FP8 && DT == UB_F32;
-  const Plan plan = plan_for(F, X, M, N, nk);
+  // (of f32 results always: the rounding of 16 bits does not cover what one product drops)
+  constexpr bool X = F == MX_FP8;
+  const bool exact = X && (DT == UB_F32 || M <= 16 || !p.one_product);
+  const Plan plan = plan_for(F, exact, M, N, nk);
   const int part = ub_cdiv(nk, plan.parts), parts = ub_cdiv(nk, part);  // (none empty)
   const size_t rows = (size_t)ub_cdiv(M, 16) * 16, codes = rows * nk * kRowStep<F>, words = rows * nk * 4;
   const size_t sums = parts > 1 ? sizeof(float) * parts * (size_t)M * N : 0;
@@ -704,13 +773,19 @@ int linear(const char* nm, const UbridgeMxLinearArgs& p, hipStream_t s) {
     k_mx_pack<F><<<(units + 255) / 256, 256, 0, s>>>((const uint8_t*)p.codes, (const uint8_t*)p.scales, q, (uint32_t*)qs, units, M, nk);
   }
   MxArgs a = {q, w, (const uint32_t*)qs, sw, p.bias, p.y, M, N, nk, part};
+  auto product = [&](auto dt, int np) {
+    constexpr int D = decltype(dt)::value;
+    if constexpr (X && DT == UB_F32) gemm<F, D, true>(plan.tile, a, np, s);
+    else if (exact) gemm<F, D, X>(plan.tile, a, np, s);
+    else gemm<F, D, false>(plan.tile, a, np, s);
+  };
   if (parts > 1) {
     a.y = qs + words;
-    gemm<F, kSum, X>(plan.tile, a, parts, s);
+    product(std::integral_constant<int, kSum>{}, parts);
     const int64_t all = (int64_t)M * N;
     k_mx_sum<DT><<<(unsigned)((all + 255) / 256), 256, 0, s>>>((const float*)a.y, p.bias, p.y, all, N, parts);
   } else {
-    gemm<F, DT, X>(plan.tile, a, 1, s);
+    product(std::integral_constant<int, DT>{}, 1);
   }
   return UB_OK;
 }

@@ -42,15 +42,17 @@ class Linear:
     of quantize(x, activations), "fp4" or "fp8".
 
     x is f32, f16 or bf16 [..., K] and y [..., N] has its type; sums are f32, bias f32
-    [N] or None.  `out`, if given, overlaps no input.  A block of NaN, in a row of x or
+    [N] or None.  exact=False, of 8-bit activations, f16 or bf16 results and more than 16
+    tokens: one matrix product in place of two, which drops addends 2 ** -13 below the
+    largest of their neighbours (at most 2 ** -10 of the sum of magnitudes).  `out`, if given, overlaps no input.  A block of NaN, in a row of x or
     of w, makes that row's results NaN.  The weight is laid out once: the tensors given
     are not kept.  codes(a, scales, dtype) takes activations that are in blocks already
     (norm.RmsNorm's), and gives y of dtype.
     """
 
-    def __init__(self, codes, scales, K, bias=None, activations="fp4"):
+    def __init__(self, codes, scales, K, bias=None, activations="fp4", exact=True):
         _need_cuda(codes, scales, bias)
-        self.bits = _bits(activations)
+        self.bits, self.exact = _bits(activations), exact
         if codes.dim() != 2:
             raise ValueError("mx.Linear takes a weight [N, K] in blocks")
         self.N, self.K = codes.shape[0], K
@@ -61,7 +63,7 @@ class Linear:
 
     def forward(self, x, out=None, stream=None):
         return call(_native.mx_linear, stream, x, None, self.w, self.w_scales, self.bias, self.K, self.N, self.bits,
-                    0, out)
+                    0, out, not self.exact)
 
     __call__ = forward
 
@@ -69,4 +71,4 @@ class Linear:
         if dtype not in _DT_CODE:
             raise ValueError(f"mx.Linear: dtype {dtype}")
         return call(_native.mx_linear, stream, a, scales, self.w, self.w_scales, self.bias, self.K, self.N, self.bits,
-                    _DT_CODE[dtype], out)
+                    _DT_CODE[dtype], out, not self.exact)
