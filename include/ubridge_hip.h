@@ -578,11 +578,12 @@ int ubridge_int8_linear_codes(const int8_t* a, const float* sa, const int8_t* w,
  * softmax of logits [T, E] (logits_dtype 0 f32, 1 f16, 2 bf16; ties to the lowest
  * expert; an expert whose logit is -inf or NaN is never taken, so a token may have
  * fewer than k, or none and then zeros), weights f32, divided by their sum if
- * renormalize; a = T(silu(g) u) of g, u = rows [0, I) and [I, 2 I) of w13 times x; y =
+ * renormalize; a = silu(g) u of g, u = rows [0, I) and [I, 2 I) of w13 times x (to 2^-17,
+ * over the range of f32); y =
  * T(sum over the experts of weight * (w2 a)).  w13 [E, 2 I, H] and w2 [E, H, I] of type T
  * (dtype 1 f16, 2 bf16), or int8 with scales s13 [E, 2 I] and s2 [E, H] of type T
  * (else NULL).  H and I are multiples of 32, x, w13 and w2 16-byte aligned, k <= 16,
- * E <= 1024.  y overlaps no input.  Scratch: 2 T k I bytes and 17 KiB. */
+ * E <= 1024.  y overlaps no input.  Scratch: 4 T k I bytes and 9 KiB. */
 typedef struct {
   const void *x, *logits, *w13, *s13, *w2, *s2;
   void* y;

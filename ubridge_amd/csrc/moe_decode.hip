@@ -2,11 +2,14 @@
 // (gfx950):
 //
 //   p = softmax(logits[t]),  the k largest (ties to the lowest expert), / their sum
-//   a[t, j] = T(silu(g) u),  g, u = (w13[e] x[t]) rows [0, I), [I, 2 I)
+//   a[t, j] = silu(g) u,     g, u = (w13[e] x[t]) rows [0, I), [I, 2 I)
 //   y[t] = T(sum_j p_j (w2[e_j] a[t, j]))
 //
 // int8 weights are exact in T; their scales, the routed weights and all sums are f32.
-// Only a and y are rounded to T: a since it is an operand of the next product.
+// Only y is rounded to T.  a, an operand of the next product, is the sum of two bf16, its
+// rounding and what that leaves: 2^-17 of it, over the range of f32 (one f16 would be
+// infinite from 65520 on, where y need not be).  So the second product is of bf16: int8
+// weights are exact there too, an f16 weight is the sum of two.
 //
 // A stream of the weights of the experts in use, read once each: bound by HBM where
 // they are many, by the chain of latencies (logits, weights, sums; twice) for a token
@@ -19,8 +22,9 @@
 //    in turn and split K, each one run of its rows, two items in flight.
 //  * k_down: a workgroup owns 8 output columns and adds all experts' parts, so no sums
 //    cross workgroups.  8 rows of each of two experts are the 16 rows of a product, and
-//    up to 8 tokens of the one and 8 of the other its columns (an expert with more is
-//    listed twice); the two quarters where rows and tokens belong together are kept.
+//    up to 4 tokens of the one and 4 of the other its columns, both parts of a each (an
+//    expert with more is listed again); the two quarters where rows and tokens belong
+//    together are kept.
 //  * Scales are asked for ahead of the weights that they go with: loads return in order,
 //    and one asked for at the end of an item would wait for all weights in flight.
 // Measured, k_up + k_down: 16 tokens, 8 of 128 int8 experts of 2048 x 768 52 + 31 us (4.9 and
@@ -40,22 +44,23 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTok = 16, kK = 16, kE = 1024, kUsed = kTok * kK;  // most tokens, top-k, experts; experts in use
-constexpr int kEnt = kUsed + kUsed / 8;                          // entries of the list below
+// tokens of an entry of the list below, and entries (at most one a token and expert)
+constexpr int kPer = 4, kEnt = kUsed;
 
-// The routing, in scratch memory from k_up to k_down: experts in use, each with up to 8
-// of its tokens (more: another entry): rows of the activations (t k + j; -1: none),
+// The routing, in scratch memory from k_up to k_down: experts in use, each with up to
+// kPer of its tokens (more: another entry): rows of the activations (t k + j; -1: none),
 // tokens and weights.
 struct Route {
   int n, pad[3];
   int expert[kEnt];
-  int16_t row[kEnt][8];
-  int8_t tok[kEnt][8];
-  float w[kEnt][8];
+  int16_t row[kEnt][kPer];
+  int8_t tok[kEnt][kPer];
+  float w[kEnt][kPer];
 };
 
 struct DecodeArgs {
   const void *x, *logits, *w13, *s13, *w2, *s2;
-  void *y, *act;
+  void *y, *act;  // act: bf16 [2][T k][I], a rounded and the rest
   Route* route;
   int T, E, k, H, I, ldt, norm;
 };
@@ -76,6 +81,25 @@ __device__ __forceinline__ f32x4 product(const uint4& w, const uint4 (&x)[Q8 ? 2
     return mfma<DT>(i8x8_to_t<DT>(w.z, w.w), x[1], c);
   } else {
     return mfma<DT>(w, x[0], c);
+  }
+}
+// The same for the second product, of bf16: 16 int8, 8 bf16, or 8 f16 as the first 8 of
+// their 11 bits and the rest
+template <int DT, bool Q8>
+__device__ __forceinline__ f32x4 product_bf16(const uint4& w, const uint4 (&x)[Q8 ? 2 : 1], f32x4 c) {
+  if constexpr (Q8 || DT == UB_BF16) return product<UB_BF16, Q8>(w, x, c);
+  else {
+    const uint32_t p[4] = {w.x, w.y, w.z, w.w};
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float a = ub_f16_to_f32((uint16_t)p[i]), b = ub_f16_to_f32((uint16_t)(p[i] >> 16));
+      const uint32_t ha = __float_as_uint(a) & 0xffff0000u, hb = __float_as_uint(b) & 0xffff0000u;
+      hi[i] = ha >> 16 | hb;
+      lo[i] = __float_as_uint(a - __uint_as_float(ha)) >> 16 | (__float_as_uint(b - __uint_as_float(hb)) & 0xffff0000u);
+    }
+    c = mfma<UB_BF16>(make_uint4(lo[0], lo[1], lo[2], lo[3]), x[0], c);
+    return mfma<UB_BF16>(make_uint4(hi[0], hi[1], hi[2], hi[3]), x[0], c);
   }
 }
 // 16 bytes of a weight row, as one vector (of a struct's four parts the conversions to T
@@ -195,15 +219,22 @@ __global__ void __launch_bounds__(1024) k_up(DecodeArgs a) {
           bits |= ((s >> 7 | s >> 14 | s >> 21 | s >> 28) & 15u) << (4 * q);
         }
       }
-      const uint64_t one = __ballot(bits != 0), two = __ballot(__popc(bits) > 8), below = (1ull << lane) - 1;
+      const uint64_t one = __ballot(bits != 0), below = (1ull << lane) - 1;
+      int ahead = 0, all = 0;  // entries of the lanes below, and of all
+#pragma unroll
+      for (int q = 0; q < kTok; q += kPer) {
+        const uint64_t more = __ballot(__popc(bits) > q);
+        ahead += __popcll(more & below);
+        all += __popcll(more);
+      }
       if (bits) {
         const int at = n + __popcll(one & below);
         used[at] = (uint16_t)e;
         tokens[at] = (uint16_t)bits;
-        entry[at] = (uint16_t)(m + __popcll(one & below) + __popcll(two & below));
+        entry[at] = (uint16_t)(m + ahead);
       }
       n += __popcll(one);
-      m += __popcll(one) + __popcll(two);
+      m += all;
     }
     if (lane == 0) nused = n, nent = m;
   }
@@ -212,15 +243,15 @@ __global__ void __launch_bounds__(1024) k_up(DecodeArgs a) {
   if (first) {
     if (tid == 0) a.route->n = nent;
     for (int i = tid; i < nu * 16; i += NT) {
-      const int u = i >> 4, p = i & 15, e = used[u], bits = tokens[u], n = __popc(bits), at = entry[u] + (p >> 3);
-      if (p >= (n > 8 ? 16 : 8)) continue;
+      const int u = i >> 4, p = i & 15, e = used[u], bits = tokens[u], n = __popc(bits), at = entry[u] + p / kPer, i4 = p % kPer;
+      if (p >= (n + kPer - 1) / kPer * kPer) continue;
       int b = bits;  // the p-th token of the expert
       for (int q = 0; q < p; q++) b &= b - 1;
       const int t = b ? __builtin_ctz(b) : -1, j = t >= 0 ? slot[e][t] : 0;
       a.route->expert[at] = e;
-      a.route->row[at][p & 7] = (int16_t)(t >= 0 ? t * a.k + j : -1);
-      a.route->tok[at][p & 7] = (int8_t)t;
-      a.route->w[at][p & 7] = t >= 0 ? wts[t][j] : 0.f;
+      a.route->row[at][i4] = (int16_t)(t >= 0 ? t * a.k + j : -1);
+      a.route->tok[at][i4] = (int8_t)t;
+      a.route->w[at][i4] = t >= 0 ? wts[t][j] : 0.f;
     }
   }
   // ---- items
@@ -291,7 +322,12 @@ __global__ void __launch_bounds__(1024) k_up(DecodeArgs a) {
 #pragma unroll
         for (int w = 0; w < W1; w++) g += red[buf][grp][oc >> 3][w][ot][oc & 7], up += red[buf][grp][oc >> 3][w][ot][8 + (oc & 7)];
         if constexpr (Q8) g *= sg, up *= su;
-        ub_store<DT>(a.act, ((size_t)ot * a.k + j) * I + col, g / (1.f + expf(-g)) * up);
+        const float v = g / (1.f + expf(-g)) * up;
+        const uint16_t hi = ub_f32_to_bf16(v);
+        const float f = ub_bf16_to_f32(hi);
+        uint16_t* at = (uint16_t*)a.act + ((size_t)ot * a.k + j) * I + col;
+        at[0] = hi;
+        at[(size_t)T * a.k * I] = ub_f32_to_bf16(__builtin_isinf(f) ? 0.f : v - f);
       }
     }
     if constexpr (NB == 1) {  // (two of them by turns need no second barrier)
@@ -317,9 +353,9 @@ template <int DT, bool Q8, int W2>
 __global__ void __launch_bounds__(64 * W2) __attribute__((amdgpu_waves_per_eu(4, 4))) k_down(DecodeArgs a, int most) {
   constexpr int WB = Q8 ? 1 : 2, XN = Q8 ? 2 : 1, P = 4;  // P: steps of a unit
   __shared__ int expert[kEnt];
-  __shared__ int16_t row[kEnt][8];
-  __shared__ int8_t tok[kEnt][8];
-  __shared__ float wts[kEnt][8], sc[kEnt][8];
+  __shared__ int16_t row[kEnt][kPer];
+  __shared__ int8_t tok[kEnt][kPer];
+  __shared__ float wts[kEnt][kPer], sc[kEnt][8];
   __shared__ float ys[W2][kTok][8];  // a wavefront's sums
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, h = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -328,7 +364,10 @@ __global__ void __launch_bounds__(64 * W2) __attribute__((amdgpu_waves_per_eu(4,
   // units: P 64-byte steps of the rows of a pair of entries, dealt out in turn, so that
   // all workgroups walk through the experts together
   const int rowb = I * WB, per = ((rowb + 63) / 64 + P - 1) / P, units = (n + 1) / 2 * per;
-  const int side = r >> 3, c8 = r & 7;
+  // columns 0-3 of a side are the first parts of its tokens, 4-7 the second, backwards (so
+  // that the two are a half row's mirror images)
+  const int side = r >> 3, c8 = r & 7, rest = c8 >> 2, c4 = rest ? 7 - c8 : c8;
+  const uint16_t* act = (const uint16_t*)a.act + (rest ? (size_t)T * a.k * I : 0);
   struct Set {
     uint4 w[P], x[P][XN];
   };
@@ -339,9 +378,9 @@ __global__ void __launch_bounds__(64 * W2) __attribute__((amdgpu_waves_per_eu(4,
     const int p = q / per, u = 2 * p + side, at0 = (q - p * per) * (64 * P) + 16 * h;
     const bool any = q < units && u < n;
     int ar = -1, e = 0;
-    if (any) ar = FIRST ? a.route->row[u][c8] : row[u][c8], e = FIRST ? a.route->expert[u] : expert[u];
+    if (any) ar = FIRST ? a.route->row[u][c4] : row[u][c4], e = FIRST ? a.route->expert[u] : expert[u];
     const uint8_t* pw = (const uint8_t*)a.w2 + ((size_t)e * H + n0 + c8) * rowb + at0;
-    const uint16_t* px = (const uint16_t*)a.act + (size_t)max(ar, 0) * I + at0 / WB;
+    const uint16_t* px = act + (size_t)max(ar, 0) * I + at0 / WB;
 #pragma unroll
     for (int i = 0; i < P; i++) {
       b.w[i] = make_uint4(0, 0, 0, 0);
@@ -362,16 +401,21 @@ __global__ void __launch_bounds__(64 * W2) __attribute__((amdgpu_waves_per_eu(4,
   auto mul = [&](Set& b, int q) {
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < P; i++) acc = product<DT, Q8>(b.w[i], b.x[i], acc);
+    for (int i = 0; i < P; i++) acc = product_bf16<DT, Q8>(b.w[i], b.x[i], acc);
     load(b, q + 2 * W2, std::false_type{});
     const int u = 2 * (q / per) + side;
-    const bool mine = u < n && (h >> 1) == side && row[u][c8] >= 0;
+    const bool mine = u < n && (h >> 1) == side && !rest && row[u][c4] >= 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {  // the other part of the token's (row_half_mirror)
+      const float v = acc[i];
+      acc[i] = v + __uint_as_float(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x141, 0xf, 0xf, false));
+    }
 #pragma unroll
     for (int s = 0; s < 2; s++) {
       if (mine && side == s) {
-        float* y = &ys[wave][tok[u][c8]][4 * (h & 1)];
+        float* y = &ys[wave][tok[u][c4]][4 * (h & 1)];
 #pragma unroll
-        for (int i = 0; i < 4; i++) y[i] += acc[i] * (Q8 ? wts[u][c8] * sc[u][4 * (h & 1) + i] : wts[u][c8]);
+        for (int i = 0; i < 4; i++) y[i] += acc[i] * (Q8 ? wts[u][c4] * sc[u][4 * (h & 1) + i] : wts[u][c4]);
       }
       __builtin_amdgcn_wave_barrier();
       asm volatile("" ::: "memory");
@@ -379,11 +423,11 @@ __global__ void __launch_bounds__(64 * W2) __attribute__((amdgpu_waves_per_eu(4,
   };
   Set b0, b1;
   // (entries past n, up to what there can be, are read with the others and not used)
-  for (int i = tid; i < most * 8; i += 64 * W2) {
+  for (int i = tid; i < most * kPer; i += 64 * W2) {
     (&row[0][0])[i] = (&a.route->row[0][0])[i];
     (&tok[0][0])[i] = (&a.route->tok[0][0])[i];
     (&wts[0][0])[i] = (&a.route->w[0][0])[i];
-    if ((i & 7) == 0) expert[i >> 3] = a.route->expert[i >> 3];
+    if (i % kPer == 0) expert[i / kPer] = a.route->expert[i / kPer];
   }
   load(b0, wave, std::true_type{});
   load(b1, wave + W2, std::true_type{});
@@ -445,7 +489,8 @@ void decode(const DecodeArgs& a, hipStream_t s) {
   if (a.E <= 128) up<DT, Q8, 2>(a, s);
   else if (a.E <= 256) up<DT, Q8, 4>(a, s);
   else up<DT, Q8, kE / 64>(a, s);
-  const int slots = a.T * a.k, most = std::min(slots, a.E) + slots / 9;  // (another entry where an expert has 9 tokens)
+  // entries, at most: one an expert in use, another for each kPer tokens past the first kPer
+  const int slots = a.T * a.k, used = std::min(slots, a.E), most = used + (slots - used) / kPer;
   // 16 wavefronts while every workgroup has a CU of its own; else 4, four workgroups to a
   // CU: no round waits for the start and end of the one before it.  us of the layer, E 64, k 8,
   // one token, 16 / 4 wavefronts, bf16 (int8): 2048 x 768 23.6 / 25.0 (18.5 / 19.5), 7168 x 512
@@ -471,7 +516,7 @@ UB_API int ubridge_moe_decode(const UbridgeMoeDecodeArgs* p, void* stream) {
   UB_REQUIRE(!p->s13 == !p->s2, "%s: one of two scales", nm);
   UB_REQUIRE((((uintptr_t)p->x | (uintptr_t)p->w13 | (uintptr_t)p->w2) & 15) == 0, "%s: x or weights not 16-byte aligned", nm);
   hipStream_t s = ub_stream(stream);
-  const size_t act = ((size_t)p->T * p->k * p->I * 2 + 255) / 256 * 256;
+  const size_t act = ((size_t)p->T * p->k * p->I * 4 + 255) / 256 * 256;
   UbScratch ws(s, act + sizeof(Route), true);
   UB_REQUIRE(ws.get(), "%s: no workspace", nm);
   const DecodeArgs a = {p->x, p->logits, p->w13, p->s13, p->w2, p->s2, p->y, ws.get(), (Route*)((char*)ws.get() + act),

@@ -326,9 +326,9 @@ class FusedMoE:
         """The layer for up to 16 tokens in two launches, with the weights of the experts
         in use read once: x [T, H], router_logits [T, E] (f32, f16 or bf16) -> [T, H].
 
-        The values of forward() but for roundings: routed weights, gate, up and the
-        experts' results stay f32, and only the gated activations and y are rounded to
-        x's type.  Ties go to the lowest expert; one whose logit is -inf or NaN is never
+        The values of forward() but for roundings: routed weights, gate, up, the gated
+        activations (to 2 ** -17) and the experts' results stay f32, and only y is
+        rounded to x's type.  Ties go to the lowest expert; one whose logit is -inf or NaN is never
         chosen, and a token that is left with none gives zeros.  H and I are multiples of
         32, topk at most 16, E at most 1024.  It has no gradient."""
         from .native import _native, call
