@@ -97,6 +97,11 @@ bool meet(const at::Tensor& x, const at::Tensor& y) {
   };
   return (const char*)x.data_ptr() < end(y) && (const char*)y.data_ptr() < end(x);
 }
+// After a caller's tensor (or null) has been written: graphs that saved it notice.
+void written(Ten t) {
+  if (t && !t->is_inference()) torch::autograd::impl::bump_version(*t);
+}
+bool records(Ten t) { return t && at::GradMode::is_enabled() && t->requires_grad(); }
 bool fits(int64_t x) { return x >= 0 && x <= 0x7fffffff; }
 
 // args: count and place checks
@@ -193,6 +198,7 @@ PyObject* py_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   void* stream = A.p(13);
   if (PyErr_Occurred()) return nullptr;
   if (const int rc = fn.decode(&p, stream)) return PyLong_FromLong(rc);
+  written(out);
   PyObject* po = THPVariable_Wrap(std::move(o));
   return with_lse ? Py_BuildValue("[NN]", po, THPVariable_Wrap(std::move(l))) : po;
   END_HANDLE_TH_ERRORS
@@ -356,6 +362,7 @@ PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (PyErr_Occurred()) return nullptr;
   if (const int rc = fn.linear(xp, dt, (const int8_t*)w->data_ptr(), ptr(sw), ptr(b), y.data_ptr(), M, K, N, ld, stream))
     return PyLong_FromLong(rc);
+  written(out);
   return THPVariable_Wrap(std::move(y));
   END_HANDLE_TH_ERRORS
 }
@@ -495,7 +502,7 @@ PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (res && !same(*res, *x)) REFUSE("rms_norm: residual must be of x's type and shape");
   if (ho && (!res || !same(*ho, *x) || !dense(*ho))) REFUSE("rms_norm: residual_out goes with residual, contiguous, of x's type and shape");
   if (!together("rms_norm", {x, w, res, ho})) return nullptr;
-  if (at::GradMode::is_enabled() && (x->requires_grad() || w->requires_grad() || (res && res->requires_grad()))) {
+  if (records(x) || records(w) || records(res) || records(ho)) {
     if (A.n(5) || ho) REFUSE("rms_norm: no gradient with quant or residual_out");
     Py_RETURN_NONE;
   }
@@ -528,6 +535,7 @@ PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   void* stream = A.p(6);
   if (PyErr_Occurred()) return nullptr;
   if (const int rc2 = fn.norm(&p, stream)) return PyLong_FromLong(rc2);
+  written(ho);
   if (out && res) return tuple_of({&y, &scale, &h});
   if (out || res) return tuple_of({&y, out ? &scale : &h});
   return THPVariable_Wrap(std::move(y));
@@ -684,6 +692,7 @@ PyObject* py_mx_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const auto sizes = ended(*x, N);
   if (out && (out->scalar_type() != type_of(dt) || out->sizes() != at::IntArrayRef(sizes) || !dense(*out)))
     REFUSE("mx.Linear: out must be contiguous, of y's type, [..., %ld]", N);
+  if (records(out)) REFUSE("mx.Linear: no gradient, and out asks for one");
   if (out && (meet(*out, *x) || (s && meet(*out, *s)) || meet(*out, *w) || meet(*out, *ws) || (b && meet(*out, *b))))
     REFUSE("mx.Linear: out overlaps an input");
   at::Tensor y = out ? *out : result(sizes, *x, type_of(dt)), xc = dense(*x) ? *x : x->contiguous();
@@ -695,6 +704,7 @@ PyObject* py_mx_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   void* stream = A.p(11);
   if (PyErr_Occurred()) return nullptr;
   if (const int rc = fn.mx_linear(&p, stream)) return PyLong_FromLong(rc);
+  written(out);
   return THPVariable_Wrap(std::move(y));
   END_HANDLE_TH_ERRORS
 }
@@ -725,6 +735,7 @@ PyObject* py_linear_codes(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const auto sizes = ended(*q, N);
   if (out && (out->scalar_type() != type_of(dt) || out->sizes() != at::IntArrayRef(sizes) || !dense(*out)))
     REFUSE("int8.Linear: out must be contiguous, of y's type, [..., %ld]", N);
+  if (records(out)) REFUSE("int8.Linear: no gradient, and out asks for one");
   if (out && (meet(*out, *q) || meet(*out, *s) || meet(*out, *w) || meet(*out, *sw) || (b && meet(*out, *b))))
     REFUSE("int8.Linear: out overlaps an input");
   at::Tensor y = out ? *out : result(sizes, *q, type_of(dt));
@@ -733,6 +744,7 @@ PyObject* py_linear_codes(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (const int rc = fn.linear_codes((const int8_t*)q->data_ptr(), ptr(s), (const int8_t*)w->data_ptr(), ptr(sw), ptr(b), y.data_ptr(), dt, M,
                                      K, N, ld, stream))
     return PyLong_FromLong(rc);
+  written(out);
   return THPVariable_Wrap(std::move(y));
   END_HANDLE_TH_ERRORS
 }

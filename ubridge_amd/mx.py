@@ -44,7 +44,7 @@ class Linear:
     x is f32, f16 or bf16 [..., K] and y [..., N] has its type; sums are f32, bias f32
     [N] or None.  exact=False, of 8-bit activations, f16 or bf16 results and more than 16
     tokens: one matrix product in place of two, which drops addends 2 ** -13 below the
-    largest of their neighbours (at most 2 ** -10 of the sum of magnitudes).  `out`, if given, overlaps no input.  A block of NaN, in a row of x or
+    largest of their neighbours (at most 2 ** -10 of the sum of magnitudes).  `out`, if given, overlaps no input and asks for no gradient.  A block of NaN, in a row of x or
     of w, makes that row's results NaN.  The weight is laid out once: the tensors given
     are not kept.  codes(a, scales, dtype) takes activations that are in blocks already
     (norm.RmsNorm's), and gives y of dtype.

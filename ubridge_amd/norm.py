@@ -30,7 +30,8 @@ class RmsNorm:
     zeros.  Codes of such a row are 0 under a scale of NaN; of blocks, those that hold
     a NaN are NaN.  At most 2 ** 22 - 1 rows.  Without quant the call is differentiable, once,
     in x, residual and weight; with it, or into residual_out, it has no gradient and
-    refuses inputs that ask for one; inputs with a tangent (forward mode) are always refused.  A call that
+    refuses inputs, or a residual_out, that ask for one; inputs with a tangent (forward
+    mode) are always refused.  residual_out's version rises, as after any write in place.  A call that
     is captured for its gradient is refused while results of an eager one of the same
     leaves live that was on the default stream.
     """
