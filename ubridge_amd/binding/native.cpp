@@ -13,6 +13,7 @@
 #include <cmath>
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/AutogradState.h>
 #include <ATen/ops/empty.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -458,6 +459,18 @@ bool together(const char* name, std::initializer_list<Ten> ts) {
   }
   return true;
 }
+// Whether a gradient is asked for that the operator does not have: of an input that
+// records, or one with a tangent (forward mode).  Refused: a result without it would be
+// silently cut off.
+bool without_gradient(const char* name, std::initializer_list<Ten> ts) {
+  const bool forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  for (Ten t : ts)
+    if (records(t) || (t && forward && t->_fw_grad(/*level=*/0).defined())) {
+      PyErr_Format(PyExc_ValueError, "%s: no gradient, and an input asks for one (detach it, or call under no_grad)", name);
+      return false;
+    }
+  return true;
+}
 // None, or a tensor (anything else refused)
 bool optional(PyObject* o, Ten& t) { return device_tensor(o, t, true); }
 // a tuple of them, None for one that is not there
@@ -598,6 +611,7 @@ PyObject* py_mx_quantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!device_tensor(args[0], x)) return nullptr;
   const int dt = code(*x), f = (int)A.n(1);
   if (dt < 0 || dt > 2 || x->dim() == 0 || x->size(-1) == 0) REFUSE("mx.quantize takes f32, f16 or bf16 [..., C]");
+  if (!without_gradient("mx.quantize", {x})) return nullptr;
   const int64_t C = x->size(-1), R = x->numel() / C;
   if (!fits(R) || C > 1 << 30 || R * (C + 127) > 1ll << 33) REFUSE("mx.quantize: %ld rows of %ld", R, C);
   at::Tensor xc = dense(*x) ? *x : x->contiguous();
@@ -692,7 +706,7 @@ PyObject* py_mx_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const auto sizes = ended(*x, N);
   if (out && (out->scalar_type() != type_of(dt) || out->sizes() != at::IntArrayRef(sizes) || !dense(*out)))
     REFUSE("mx.Linear: out must be contiguous, of y's type, [..., %ld]", N);
-  if (records(out)) REFUSE("mx.Linear: no gradient, and out asks for one");
+  if (!without_gradient("mx.Linear", {x, b, out})) return nullptr;
   if (out && (meet(*out, *x) || (s && meet(*out, *s)) || meet(*out, *w) || meet(*out, *ws) || (b && meet(*out, *b))))
     REFUSE("mx.Linear: out overlaps an input");
   at::Tensor y = out ? *out : result(sizes, *x, type_of(dt)), xc = dense(*x) ? *x : x->contiguous();
@@ -735,7 +749,7 @@ PyObject* py_linear_codes(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const auto sizes = ended(*q, N);
   if (out && (out->scalar_type() != type_of(dt) || out->sizes() != at::IntArrayRef(sizes) || !dense(*out)))
     REFUSE("int8.Linear: out must be contiguous, of y's type, [..., %ld]", N);
-  if (records(out)) REFUSE("int8.Linear: no gradient, and out asks for one");
+  if (!without_gradient("int8.Linear", {s, sw, b, out})) return nullptr;
   if (out && (meet(*out, *q) || meet(*out, *s) || meet(*out, *w) || meet(*out, *sw) || (b && meet(*out, *b))))
     REFUSE("int8.Linear: out overlaps an input");
   at::Tensor y = out ? *out : result(sizes, *q, type_of(dt));
@@ -779,6 +793,7 @@ PyObject* py_moe_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     REFUSE("FusedMoE.decode: T=%ld (at most 16), topk=%ld (1..16, at most E), E=%ld (at most 1024), H=%ld and I=%ld (multiples of 32)", T, k,
            E, H, I);
   if (!together("FusedMoE.decode", {x, lg, w13, s13, w2, s2})) return nullptr;
+  if (!without_gradient("FusedMoE.decode", {x, lg, w13, s13, w2, s2})) return nullptr;
   auto whole = [](const at::Tensor& t, int align) { return dense(t) && ((uintptr_t)t.data_ptr() & (align - 1)) == 0; };
   at::Tensor xc = *x, lc = dense(*lg) ? *lg : lg->contiguous();
   if (!whole(xc, 16)) xc = xc.clone(at::MemoryFormat::Contiguous);

@@ -49,7 +49,8 @@ class Linear:
 
     def codes(self, a, scales, dtype=torch.bfloat16, out=None, stream=None):
         """The same of activations that are in codes already: a int8 [..., K] (-127 .. 127),
-        contiguous, and f32 scales [...], as norm.RmsNorm(...)(x, quant="int8") makes them; y is of dtype."""
+        contiguous, and f32 scales [...], as norm.RmsNorm(...)(x, quant="int8") makes them; y is of dtype.
+        Inputs that ask for a gradient, or have a tangent, are refused."""
         if dtype not in _DT_CODE:
             raise ValueError(f"int8.Linear: dtype {dtype}")
         if a.shape[-1:] != (self.K,):

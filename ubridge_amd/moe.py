@@ -330,7 +330,8 @@ class FusedMoE:
         activations (to 2 ** -17) and the experts' results stay f32, and only y is
         rounded to x's type.  Ties go to the lowest expert; one whose logit is -inf or NaN is never
         chosen, and a token that is left with none gives zeros.  H and I are multiples of
-        32, topk at most 16, E at most 1024.  It has no gradient."""
+        32, topk at most 16, E at most 1024.  It has no gradient: inputs that ask
+        for one, or have a tangent, are refused."""
         from .native import _native, call
         return call(_native.moe_decode, stream, x, router_logits, self.w13, self.s13, self.w2, self.s2, self.topk,
                     self.renormalize)

@@ -1,6 +1,6 @@
 """Microscaled blocks: 32 consecutive values under one power of two, elements of 4
 bits (e2m1, "fp4") or 8 (e4m3, "fp8"); a linear whose weight is held in 4-bit blocks.
-None of it has a gradient.
+None of it has a gradient: inputs that ask for one, or have a tangent, are refused.
 
 Rows of C elements are stored as ld = C rounded up to 128 of them, zero past C:
 codes uint8 [..., ld / 2] (two a byte, the even one low; "fp8": [..., ld]) and
