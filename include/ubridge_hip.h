@@ -74,6 +74,11 @@ const char* ubridge_version(void);
  * after the other.  Calls of the norm and feed-forward half have buffers of
  * each capture's own.)  topsaten_release_graph_workspace_pool does the same.
  *
+ * Threads: calls may come from several threads, on one stream too.  A call that
+ * takes pool scratch enqueues its kernels together: another thread's that
+ * wants scratch of the same stream, or releases it, waits until then.
+ * ubridge_set_workspace_allocator is for when no call is going on.
+ *
  * ubridge_workspace_stats: pool buffers allocated and not yet freed (count,
  * bytes, all devices and streams) and caller-allocator blocks not yet handed
  * back (0 between calls). */

@@ -54,7 +54,8 @@ int ub_tune(int knob);
 // per-(device, stream) pool (ubridge_release_workspace frees it).  Works while
 // s captures a graph (the allocation is made outside the capture), so the
 // route a call takes never depends on whether an eager call came first;
-// get() is null only when the allocation itself fails.  per_graph: a call that is
+// get() is null only when the allocation itself fails.  While it lives, other threads'
+// scratch of the same stream waits: a call's launches stay together.  per_graph: a call that is
 // captured draws on buffers of that graph's own, so that graphs captured on one
 // stream may be replayed side by side on others.
 class UbScratch {
@@ -68,6 +69,7 @@ class UbScratch {
  private:
   void* p_ = nullptr;
   hipStream_t s_ = nullptr;
+  void* pool_ = nullptr;  // the library's, held until the end
   bool caller_ = false;
 };
 

@@ -116,7 +116,9 @@ UB_API int ubridge_tune_get(const char* name) {
 //    call that needs scratch takes it from that allocator on its stream and
 //    hands it back on the same stream once its kernels are enqueued; the
 //    library then holds no device memory of its own;
-//  * otherwise a per-(device, stream) pool buffer, grown on demand.  A buffer
+//  * otherwise a per-(device, stream) pool buffer, grown on demand, of one call at a
+//    time: another thread's call on the stream waits until the first has
+//    enqueued its kernels.  A buffer
 //    it outgrows is retired: freed once an event recorded after its last use
 //    has completed, unless it was handed out while the stream captured a
 //    graph (graphs keep its address: it then lives until
@@ -142,11 +144,15 @@ struct WsRetired {
   hipEvent_t ev = nullptr;  // completes after the buffer's last eager use
 };
 struct WsPool {
+  // Held by a call from its first scratch to its last launch: its kernels lie together
+  // on the stream, with no other call's on the same buffer in between and no buffer
+  // outgrown (and freed) under it.  (recursive: a call may take several.)
+  std::recursive_mutex call;
   WsBuf cur;
   std::vector<WsRetired> retired;  // ev null: not yet ordered (see sweep)
 };
 std::mutex g_ws_mu;
-std::map<std::pair<int, hipStream_t>, WsPool> g_ws;
+std::map<std::pair<int, hipStream_t>, WsPool> g_ws;  // (never erased from: calls wait on them)
 size_t g_ws_live_n = 0, g_ws_live_bytes = 0;  // pool buffers allocated, not freed
 long g_ws_caller_out = 0;                     // caller-allocator blocks not yet handed back
 ubridge_ws_alloc_fn g_ws_alloc = nullptr;
@@ -233,12 +239,17 @@ WsBuf ws_new(size_t bytes) {
   return b;
 }
 
-void* ws_pool_get(hipStream_t s, size_t bytes, bool per_graph) {
+WsPool* ws_pool(hipStream_t s) {
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess) return nullptr;
+  std::lock_guard<std::mutex> lk(g_ws_mu);
+  return &g_ws[{dev, s}];
+}
+
+// (the caller holds pool.call)
+void* ws_pool_get(WsPool& pool, hipStream_t s, size_t bytes, bool per_graph) {
   const bool cap = capturing(s);
   std::lock_guard<std::mutex> lk(g_ws_mu);
-  WsPool& pool = g_ws[{dev, s}];
   if (!cap && !pool.retired.empty()) ws_sweep(pool, s);
   if (const unsigned long long id = cap && per_graph ? capture_id(s) : 0) {
     for (const WsRetired& r : pool.retired)
@@ -284,10 +295,19 @@ UbScratch::UbScratch(hipStream_t s, size_t bytes, bool per_graph) : s_(s) {
     }
     return;
   }
-  p_ = ws_pool_get(s, bytes, per_graph);
+  try {
+    WsPool* pool = ws_pool(s);
+    if (!pool) return;
+    pool->call.lock();
+    pool_ = pool;
+    p_ = ws_pool_get(*pool, s, bytes, per_graph);
+  } catch (...) {  // (out of host memory: as without device memory)
+    p_ = nullptr;
+  }
 }
 
 UbScratch::~UbScratch() {
+  if (pool_) ((WsPool*)pool_)->call.unlock();
   if (!caller_) return;
   ubridge_ws_free_fn ff;
   void* ctx;
@@ -323,19 +343,21 @@ UB_API int ubridge_release_workspace(void* stream) {
   if (capturing(s))
     return ub_set_error(UB_ERR_INVALID_ARG,
                         "ubridge_release_workspace: the stream is capturing a graph");
-  std::lock_guard<std::mutex> lk(g_ws_mu);
-  auto it = g_ws.find({dev, s});
-  if (it == g_ws.end()) return UB_OK;
+  WsPool* pool = ws_pool(s);
+  if (!pool) return ub_set_error(UB_ERR_LAUNCH, "no device");
+  std::lock_guard<std::recursive_mutex> call(pool->call);  // (another thread's call ends first)
   if (hipStreamSynchronize(s) != hipSuccess) {
     const hipError_t e = hipGetLastError();
     return ub_set_error(UB_ERR_LAUNCH, "ubridge_release_workspace: %s", hipGetErrorString(e));
   }
-  for (WsRetired& r : it->second.retired) {
+  std::lock_guard<std::mutex> lk(g_ws_mu);
+  for (WsRetired& r : pool->retired) {
     if (r.ev) (void)hipEventDestroy(r.ev);
     ws_free(r.b);
   }
-  ws_free(it->second.cur);
-  g_ws.erase(it);
+  pool->retired.clear();
+  ws_free(pool->cur);
+  pool->cur = WsBuf{};
   return UB_OK;
 }
 
