@@ -36,6 +36,7 @@ int hipStreamSynchronize(void*) { say("synchronize", 0); usleep(500); return 0; 
 int hipStreamIsCapturing(void*, int* st) { *st = 0; return 0; }
 int hipThreadExchangeStreamCaptureMode(int*) { return 0; }
 int hipGetLastError() { return 0; }
+int hipblasLtCreate(void**) { return 1; }  // (no library products)
 int __hipPushCallConfiguration(dim3 g, dim3 b, size_t lds, void* s) { cfg = {g, b, lds, s}; return 0; }
 int __hipPopCallConfiguration(dim3* g, dim3* b, size_t* lds, void** s) {
   *g = cfg.g, *b = cfg.b, *lds = cfg.lds, *s = cfg.s;
@@ -131,3 +132,25 @@ def test_a_call_s_launches_lie_together(shim, one, other):
                 inside = None
         return True
     assert fits(threads) or fits(threads[::-1]), both
+
+
+LEVELS = r"""
+import ctypes, sys
+shim = ctypes.CDLL(sys.argv[1], ctypes.RTLD_GLOBAL)
+lib = ctypes.CDLL(sys.argv[2])
+V, odd = ctypes.c_void_p(4096), ctypes.c_void_p(4098)
+for a in (V, odd):  # 72 x 4096 x 1544: parts of K
+    print("call", flush=True)
+    assert lib.ubridge_tune_set(b"w4a16_path", 3) == 0  # (not through the library product)
+    assert lib.ubridge_w4a16_gemm(a, V, V, V, V, 72, 4096, 1544, 128, 2, None) == 0
+"""
+
+
+def test_two_pieces_of_one_call(shim):
+    # an aligned call takes one buffer; the misaligned one a second, beside it
+    lib = os.path.join(ROOT, "ubridge_amd", "lib", "libubridge_hip.so")
+    r = subprocess.run([sys.executable, "-c", LEVELS, shim, lib], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr
+    aligned, odd = [[line.split()[1] for line in part.splitlines()] for part in r.stdout.split("call\n")[1:]]
+    assert aligned.count("alloc") == 1 and odd.count("alloc") == 1, r.stdout
+    assert "free" not in aligned + odd and odd.count("launch") == aligned.count("launch") + 1, r.stdout

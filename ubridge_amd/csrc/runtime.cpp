@@ -116,7 +116,8 @@ UB_API int ubridge_tune_get(const char* name) {
 //    call that needs scratch takes it from that allocator on its stream and
 //    hands it back on the same stream once its kernels are enqueued; the
 //    library then holds no device memory of its own;
-//  * otherwise a per-(device, stream) pool buffer, grown on demand, of one call at a
+//  * otherwise a per-(device, stream) pool buffer (one for each that a call holds at
+//    once), grown on demand, of one call at a
 //    time: another thread's call on the stream waits until the first has
 //    enqueued its kernels.  A buffer
 //    it outgrows is retired: freed once an event recorded after its last use
@@ -138,6 +139,7 @@ struct WsBuf {
   size_t bytes = 0;
   bool graph = false;  // handed out during a capture
   unsigned long long capture = 0;  // the one capture that it belongs to (0: any)
+  size_t level = 0;                // there: scratch that its call held already
 };
 struct WsRetired {
   WsBuf b;
@@ -148,7 +150,10 @@ struct WsPool {
   // on the stream, with no other call's on the same buffer in between and no buffer
   // outgrown (and freed) under it.  (recursive: a call may take several.)
   std::recursive_mutex call;
-  WsBuf cur;
+  // By how many the call holds already: a call that takes a second scratch while it
+  // holds the first (a copy of misaligned activations, then parts of K) gets another.
+  std::vector<WsBuf> cur;
+  size_t held = 0;
   std::vector<WsRetired> retired;  // ev null: not yet ordered (see sweep)
 };
 std::mutex g_ws_mu;
@@ -251,27 +256,30 @@ void* ws_pool_get(WsPool& pool, hipStream_t s, size_t bytes, bool per_graph) {
   const bool cap = capturing(s);
   std::lock_guard<std::mutex> lk(g_ws_mu);
   if (!cap && !pool.retired.empty()) ws_sweep(pool, s);
+  const size_t level = pool.held - 1;
   if (const unsigned long long id = cap && per_graph ? capture_id(s) : 0) {
     for (const WsRetired& r : pool.retired)
-      if (r.b.capture == id && r.b.bytes >= bytes) return r.b.p;
+      if (r.b.capture == id && r.b.level == level && r.b.bytes >= bytes) return r.b.p;
     WsBuf b = ws_new(bytes);
     if (!b.p) return nullptr;
-    b.graph = true, b.capture = id;
+    b.graph = true, b.capture = id, b.level = level;
     pool.retired.push_back(WsRetired{b, nullptr});
     return b.p;
   }
-  if (pool.cur.bytes >= bytes) {
-    pool.cur.graph |= cap;
-    return pool.cur.p;
+  if (pool.cur.size() <= level) pool.cur.resize(level + 1);
+  WsBuf& cur = pool.cur[level];
+  if (cur.bytes >= bytes) {
+    cur.graph |= cap;
+    return cur.p;
   }
   WsBuf b = ws_new(bytes);
   if (!b.p) return nullptr;
-  if (pool.cur.p) {
-    pool.retired.push_back(WsRetired{pool.cur, nullptr});
+  if (cur.p) {
+    pool.retired.push_back(WsRetired{cur, nullptr});
     if (!cap) ws_sweep(pool, s);  // orders it behind the work already on s
   }
   b.graph = cap;
-  pool.cur = b;
+  cur = b;
   return b.p;
 }
 }  // namespace
@@ -300,6 +308,7 @@ UbScratch::UbScratch(hipStream_t s, size_t bytes, bool per_graph) : s_(s) {
     if (!pool) return;
     pool->call.lock();
     pool_ = pool;
+    pool->held++;
     p_ = ws_pool_get(*pool, s, bytes, per_graph);
   } catch (...) {  // (out of host memory: as without device memory)
     p_ = nullptr;
@@ -307,7 +316,10 @@ UbScratch::UbScratch(hipStream_t s, size_t bytes, bool per_graph) : s_(s) {
 }
 
 UbScratch::~UbScratch() {
-  if (pool_) ((WsPool*)pool_)->call.unlock();
+  if (WsPool* pool = (WsPool*)pool_) {
+    pool->held--;
+    pool->call.unlock();
+  }
   if (!caller_) return;
   ubridge_ws_free_fn ff;
   void* ctx;
@@ -356,8 +368,8 @@ UB_API int ubridge_release_workspace(void* stream) {
     ws_free(r.b);
   }
   pool->retired.clear();
-  ws_free(pool->cur);
-  pool->cur = WsBuf{};
+  for (const WsBuf& b : pool->cur) ws_free(b);
+  pool->cur.clear();
   return UB_OK;
 }
 
