@@ -72,7 +72,8 @@ const char* ubridge_version(void);
  * destroying a stream the library has used.  Fails (1) while the stream
  * captures.  (Graphs captured on one stream share its buffer: replay them one
  * after the other.  Calls of the norm and feed-forward half have buffers of
- * each capture's own.)  topsaten_release_graph_workspace_pool does the same.
+ * each capture's own, which serve others once the graph and its executables
+ * are destroyed.)  topsaten_release_graph_workspace_pool does the same.
  *
  * Threads: calls may come from several threads, on one stream too.  A call that
  * takes pool scratch enqueues its kernels together: another thread's that

@@ -1,6 +1,7 @@
-"""Calls of two threads on one stream: the launches of a call that takes scratch lie
-together, so that no other call's use of the stream's buffer, and no growth of it,
-falls between them.  The HIP runtime's calls are answered by a stand-in: nothing is run."""
+"""The library's scratch.  Calls of two threads on one stream: the launches of a call that
+takes scratch lie together, so that no other call's use of the stream's buffer, and no
+growth of it, falls between them.  A call's several pieces.  Buffers of captured
+graphs.  The HIP runtime's calls are answered by a stand-in: nothing is run."""
 import itertools
 import os
 import subprocess
@@ -33,7 +34,30 @@ int hipEventRecord(void*, void*) { return 0; }
 int hipEventQuery(void*) { return 0; }
 int hipEventDestroy(void*) { return 0; }
 int hipStreamSynchronize(void*) { say("synchronize", 0); usleep(500); return 0; }
-int hipStreamIsCapturing(void*, int* st) { *st = 0; return 0; }
+static int status;
+static unsigned long long capture;
+static int graphs[64];                                    // a graph is the address of one
+static struct { void (*end)(void*); void* p; } kept[64];  // by graph
+static void* object[2];
+void stand_in_capture(int on) { status = on; capture += on; }
+void stand_in_destroy(int graph) { if (kept[graph].end) kept[graph].end(kept[graph].p); }
+int hipStreamIsCapturing(void*, int* st) { *st = status; return 0; }
+int hipStreamGetCaptureInfo(void*, int* st, unsigned long long* id) { *st = status, *id = capture; return 0; }
+int hipStreamGetCaptureInfo_v2(void*, int* st, unsigned long long* id, void** graph, const void** deps, size_t* n) {
+  *st = status, *id = capture, *deps = 0, *n = 0;
+  *graph = &graphs[capture];
+  return 0;
+}
+int hipUserObjectCreate(void** o, void* p, void (*end)(void*), unsigned, unsigned) {
+  object[0] = (void*)end, object[1] = p;
+  *o = object;
+  return 0;
+}
+int hipGraphRetainUserObject(void* g, void*, unsigned, unsigned) {
+  kept[(int*)g - graphs] = {(void (*)(void*))object[0], object[1]};
+  return 0;
+}
+int hipUserObjectRelease(void*, unsigned) { return 0; }
 int hipThreadExchangeStreamCaptureMode(int*) { return 0; }
 int hipGetLastError() { return 0; }
 int hipblasLtCreate(void**) { return 1; }  // (no library products)
@@ -154,3 +178,48 @@ def test_two_pieces_of_one_call(shim):
     aligned, odd = [[line.split()[1] for line in part.splitlines()] for part in r.stdout.split("call\n")[1:]]
     assert aligned.count("alloc") == 1 and odd.count("alloc") == 1, r.stdout
     assert "free" not in aligned + odd and odd.count("launch") == aligned.count("launch") + 1, r.stdout
+
+
+GRAPHS = r"""
+import ctypes, struct, sys
+shim = ctypes.CDLL(sys.argv[1], ctypes.RTLD_GLOBAL)
+lib = ctypes.CDLL(sys.argv[2])
+mx = struct.Struct("@7P6i")
+P = 4096
+def linear(M, K, N):
+    assert lib.ubridge_mx_linear(mx.pack(P, 0, 0, P, P, 0, P, M, K, N, 2, 4, 0), None) == 0
+def live():
+    n, b, c = ctypes.c_size_t(), ctypes.c_size_t(), ctypes.c_long()
+    assert lib.ubridge_workspace_stats(ctypes.byref(n), ctypes.byref(b), ctypes.byref(c)) == 0
+    return n.value
+def capture(M):
+    shim.stand_in_capture(1)
+    linear(M, 4096, 512)
+    linear(M, 2048, 512)
+    shim.stand_in_capture(0)
+linear(40, 4096, 512)
+assert live() == 1
+for graph in range(1, 11):  # captured and destroyed in turn: one buffer serves all
+    capture(200 if graph % 2 else 40)
+    assert live() == 2, (graph, live())
+    shim.stand_in_destroy(graph)
+capture(40)  # graph 11 lives on
+capture(40)  # 12 has its own beside it
+assert live() == 3
+shim.stand_in_destroy(12)
+linear(40, 4096, 512)  # an eager call gives the ended one's back, and no other
+assert live() == 2
+capture(4000)  # 13: larger than what there is
+assert live() == 3
+assert lib.ubridge_release_workspace(None) == 0 and live() == 0
+shim.stand_in_destroy(11)  # (graphs that end after the release)
+shim.stand_in_destroy(13)
+linear(40, 4096, 512)
+assert live() == 1
+"""
+
+
+def test_buffers_of_ended_graphs_serve_others(shim):
+    lib = os.path.join(ROOT, "ubridge_amd", "lib", "libubridge_hip.so")
+    r = subprocess.run([sys.executable, "-c", GRAPHS, shim, lib], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr

@@ -117,15 +117,15 @@ UB_API int ubridge_tune_get(const char* name) {
 //    hands it back on the same stream once its kernels are enqueued; the
 //    library then holds no device memory of its own;
 //  * otherwise a per-(device, stream) pool buffer (one for each that a call holds at
-//    once), grown on demand, of one call at a
-//    time: another thread's call on the stream waits until the first has
-//    enqueued its kernels.  A buffer
+//    once), grown on demand, of one call at a time: another thread's call on the
+//    stream waits until the first has enqueued its kernels.  A buffer
 //    it outgrows is retired: freed once an event recorded after its last use
 //    has completed, unless it was handed out while the stream captured a
 //    graph (graphs keep its address: it then lives until
 //    ubridge_release_workspace).  Calls that ask for it draw, while they are
-//    captured, on buffers of that capture alone, which live as long.
-//    ubridge_release_workspace(stream)
+//    captured, on buffers of that capture alone, which are free again, for another
+//    capture or at the next eager call, once its graph and the executables of it
+//    are destroyed.  ubridge_release_workspace(stream)
 //    synchronizes the stream and frees all of that stream's buffers.
 // Growth during a graph capture allocates with the capture mode relaxed, so
 // calls take the same route (and give the same bits) captured or eager.
@@ -134,12 +134,27 @@ UB_API int ubridge_tune_get(const char* name) {
 #include <utility>
 #include <vector>
 namespace {
+// What a buffer and the graph that names it share: the graph retains it as a user
+// object, whose end is the end of the graph, of the executables made from it and of
+// their launches.  That call may come on any thread, after the pool is gone too.
+struct WsTie {
+  std::atomic<bool> ended{false};
+  std::atomic<int> refs{2};
+  void drop() {
+    if (refs.fetch_sub(1) == 1) delete this;
+  }
+  static void end(void* p) {
+    ((WsTie*)p)->ended = true;
+    ((WsTie*)p)->drop();
+  }
+};
 struct WsBuf {
   void* p = nullptr;
   size_t bytes = 0;
   bool graph = false;  // handed out during a capture
   unsigned long long capture = 0;  // the one capture that it belongs to (0: any)
   size_t level = 0;                // there: scratch that its call held already
+  WsTie* tie = nullptr;            // and its graph (null: not known, it lives until released)
 };
 struct WsRetired {
   WsBuf b;
@@ -173,18 +188,47 @@ bool capturing(hipStream_t s) {
   return st != hipStreamCaptureStatusNone;
 }
 
-// The capture's own number, or 0 (not known: the stream's shared buffer serves).
-unsigned long long capture_id(hipStream_t s) {
+// The capture's own number and graph, or 0 (not known: the stream's shared buffer serves).
+unsigned long long capture_id(hipStream_t s, hipGraph_t* graph) {
   hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
   unsigned long long id = 0;
-  if (hipStreamGetCaptureInfo(s, &st, &id) != hipSuccess) {
+  const hipGraphNode_t* deps = nullptr;
+  size_t n = 0;
+  *graph = nullptr;
+  if (hipStreamGetCaptureInfo_v2(s, &st, &id, graph, &deps, &n) != hipSuccess) {
     (void)hipGetLastError();
     return 0;
   }
   return st == hipStreamCaptureStatusActive ? id : 0;
 }
 
-void ws_free(const WsBuf& b) {
+// Ties a buffer to the graph being captured; null: it could not be.
+WsTie* ws_tie(hipGraph_t graph) {
+  if (!graph) return nullptr;
+  WsTie* t = new WsTie;
+  UbRelaxCapture relax;
+  hipUserObject_t o = nullptr;
+  if (hipUserObjectCreate(&o, t, WsTie::end, 1, hipUserObjectNoDestructorSync) != hipSuccess) {
+    (void)hipGetLastError();
+    delete t;
+    return nullptr;
+  }
+  if (hipGraphRetainUserObject(graph, o, 1, hipGraphUserObjectMove) != hipSuccess) {
+    (void)hipGetLastError();
+    (void)hipUserObjectRelease(o, 1);  // (drops the graph's reference)
+    t->drop();
+    return nullptr;
+  }
+  return t;
+}
+
+void ws_untie(WsBuf& b) {
+  if (b.tie) b.tie->drop();
+  b.tie = nullptr;
+}
+
+void ws_free(WsBuf& b) {
+  ws_untie(b);
   if (!b.p) return;
   (void)hipFree(b.p);
   (void)hipGetLastError();
@@ -195,10 +239,14 @@ void ws_free(const WsBuf& b) {
 // Retired buffers of a pool (s not capturing, caller holds g_ws_mu): order
 // the unordered ones behind an event recorded now (everything that used them
 // is already on s), free those whose event has completed.  Graph-held
-// buffers stay until released.
+// buffers stay until their graph has ended, or until released.
 void ws_sweep(WsPool& pool, hipStream_t s) {
   for (size_t i = 0; i < pool.retired.size();) {
     WsRetired& r = pool.retired[i];
+    if (r.b.tie && r.b.tie->ended) {
+      ws_untie(r.b);
+      r.b.graph = false;
+    }
     if (r.b.graph) {
       i++;
       continue;
@@ -257,13 +305,24 @@ void* ws_pool_get(WsPool& pool, hipStream_t s, size_t bytes, bool per_graph) {
   std::lock_guard<std::mutex> lk(g_ws_mu);
   if (!cap && !pool.retired.empty()) ws_sweep(pool, s);
   const size_t level = pool.held - 1;
-  if (const unsigned long long id = cap && per_graph ? capture_id(s) : 0) {
+  hipGraph_t graph = nullptr;
+  if (const unsigned long long id = cap && per_graph ? capture_id(s, &graph) : 0) {
     for (const WsRetired& r : pool.retired)
       if (r.b.capture == id && r.b.level == level && r.b.bytes >= bytes) return r.b.p;
-    WsBuf b = ws_new(bytes);
-    if (!b.p) return nullptr;
-    b.graph = true, b.capture = id, b.level = level;
-    pool.retired.push_back(WsRetired{b, nullptr});
+    // one whose graph has ended, the smallest that suffices, or a new one
+    size_t at = pool.retired.size();
+    for (size_t i = 0; i < pool.retired.size(); i++) {
+      const WsBuf& b = pool.retired[i].b;
+      if (b.tie && b.tie->ended && b.bytes >= bytes && (at == pool.retired.size() || b.bytes < pool.retired[at].b.bytes)) at = i;
+    }
+    if (at == pool.retired.size()) {
+      WsBuf b = ws_new(bytes);
+      if (!b.p) return nullptr;
+      pool.retired.push_back(WsRetired{b, nullptr});
+    }
+    WsBuf& b = pool.retired[at].b;
+    ws_untie(b);
+    b.graph = true, b.capture = id, b.level = level, b.tie = ws_tie(graph);
     return b.p;
   }
   if (pool.cur.size() <= level) pool.cur.resize(level + 1);
@@ -368,7 +427,7 @@ UB_API int ubridge_release_workspace(void* stream) {
     ws_free(r.b);
   }
   pool->retired.clear();
-  for (const WsBuf& b : pool->cur) ws_free(b);
+  for (WsBuf& b : pool->cur) ws_free(b);
   pool->cur.clear();
   return UB_OK;
 }
