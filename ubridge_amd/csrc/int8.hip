@@ -762,8 +762,11 @@ int linear(const char* nm, const void* x, const int8_t* w, const float* sw, cons
   return UB_OK;
 }
 
-// Of codes that are there already: the tiles at every size (few tokens too: 16 x 4096
-// x 4096 11.4 us against 10.4 of k_i8_dec, whose quantizing this saves).
+// Of codes that are there already: the tiles at every size.  us of the call, of codes / of
+// x, which is rounded (M x K x N): 1 x 4096 x 4096 9.3 / 7.0, 8 9.2 / 7.8, 16 9.1 / 10.2, 200
+// 12.1 / 15.8, 1 x 14336 x 4096 12.7 / 13.8, 16 13.1 / 16.6, 1 x 4096 x 28672 19.8 / 21.0, 16
+// 20.1 / 24.1.  Up to about 10 tokens of a small weight k_i8_dec, one launch that rounds by
+// itself, takes less: these have codes for the norm's sake only.
 template <int DT>
 int linear_codes(const char* nm, const int8_t* a, const float* sa, const int8_t* w, const float* sw, const float* bias,
                  void* y, int M, int N, int ld, hipStream_t s) {
