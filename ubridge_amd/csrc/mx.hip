@@ -15,7 +15,7 @@
 // multiplied twice (X, kSide, kTurn, kCut below): either part's products lie within 14
 // bits, and nothing is dropped.  A caller may take one product instead (one_product) for
 // 16-bit results of more than 16 tokens, where the second costs most: 4096 x 4096 x 14336
-// (M K N) 300 us against 195, 201 x 3520 x 9001 24 against 17.
+// (M K N) 300 us against 195, 201 x 3520 x 9001 19 against 16.
 //
 // Rows are padded with zero codes to a step of 128 elements.  Outside, codes and
 // scales lie in rows; a weight is laid out once, activations by the kernel that
@@ -39,10 +39,12 @@ constexpr int kSum = 100;  // "type" of the f32 sums over a part of K
 // bytes of a row's step of 128 elements
 template <int F> constexpr int kRowStep = 128 * F / 8;
 
-// Places of block b of a row, in rows or laid out for the products.
-template <int F, bool PACKED>
+// Places of block b of a row, in rows or laid out for the products (TWO: in two parts, the
+// lower kLower bytes behind the higher, in every 16 rows of a step).
+constexpr int kLower = 16 * kRowStep<MX_FP8>;
+template <int F, bool PACKED, bool TWO = false>
 __device__ __forceinline__ size_t code_at(size_t row, int b, int nk) {
-  if constexpr (PACKED) return (((row >> 4) * nk + (b >> 2)) * 16 + (row & 15)) * kRowStep<F> + (b & 3) * (kRowStep<F> / 4);
+  if constexpr (PACKED) return (((row >> 4) * nk + (b >> 2)) * (TWO ? 32 : 16) + (row & 15)) * kRowStep<F> + (b & 3) * (kRowStep<F> / 4);
   else return row * (size_t)nk * kRowStep<F> + (size_t)b * (kRowStep<F> / 4);
 }
 template <bool PACKED>
@@ -51,12 +53,30 @@ __device__ __forceinline__ size_t scale_at(size_t row, int b, int nk) {
   else return row * (size_t)nk * 4 + b;
 }
 
+// e4m3 codes of magnitude 2 and more in `hi`, those below in `lo` (bit 6 of a code
+// tells), zeros elsewhere.  v_perm fills bytes with the sign of bytes 1 and 3 of either
+// operand: of v << 9 (codes 0 and 2) and of v << 1 (1 and 3).
+__device__ __forceinline__ uint32_t cut(uint32_t v, uint32_t& lo) {
+  const uint32_t m = __builtin_amdgcn_perm(v << 1, v << 9, 0x0b090a08u);
+  lo = v & ~m;
+  return v & m;
+}
+__device__ __forceinline__ void cut(const i32x8& v, i32x8& lo, i32x8& hi) {
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    uint32_t l;
+    hi[i] = (int)cut((uint32_t)v[i], l);
+    lo[i] = (int)l;
+  }
+}
+
 // ------------------------------------------------------- blocks and back
 // A thread takes two units of 16 bytes of x, 256 apart, both loaded before the first is
 // rounded; the 4 (f32: 8) lanes of a block find its largest by DPP.  us, bf16 to e2m1 laid
 // out, 1 / 2 / 4 units a thread: 201 x 3520 3.6 / 3.6 / 3.7, 4096 x 4096 9.4 / 9.7 / 9.9,
 // and in rows 14336 x 4096 27.9 / 26.2 / 26.5 (5.7 TB/s).
-template <int DT, int F, bool PACKED>
+// TWO: codes of e4m3 in their two parts (`cut`).
+template <int DT, int F, bool PACKED, bool TWO>
 __global__ void __launch_bounds__(256) k_mx_quant(const void* __restrict__ x, uint8_t* __restrict__ q,
                                                   uint8_t* __restrict__ sc, uint32_t units, int C, int nk) {
   typedef typename MxElem<DT>::T T;
@@ -81,7 +101,13 @@ __global__ void __launch_bounds__(256) k_mx_quant(const void* __restrict__ x, ui
     if (i >= units) continue;  // (whole blocks: units is a multiple of theirs)
     const uint32_t row = i / per;
     const int u = (int)(i - row * per), blk = u / BL;
-    mx_store<DT, F>(q + code_at<F, PACKED>(row, blk, nk) + (u % BL) * (E * F / 8), o);
+    uint8_t* p = q + code_at<F, PACKED, TWO>(row, blk, nk) + (u % BL) * (E * F / 8);
+    if constexpr (TWO) {
+      uint32_t lo[2];
+      o[0] = cut(o[0], lo[0]), o[1] = cut(o[1], lo[1]);
+      mx_store<DT, F>(p + kLower, lo);
+    }
+    mx_store<DT, F>(p, o);
     if (u % BL == 0) sc[scale_at<PACKED>(row, blk, nk)] = (uint8_t)b;
   }
 }
@@ -128,7 +154,7 @@ __global__ void __launch_bounds__(256) k_mx_back(const uint8_t* __restrict__ q, 
 }
 
 // From rows to the products' layout; rows past R up to a multiple of 16 are zero.
-template <int F>
+template <int F, bool TWO = false>
 __global__ void __launch_bounds__(256) k_mx_pack(const uint8_t* __restrict__ q, const uint8_t* __restrict__ sc,
                                                  uint8_t* __restrict__ pq, uint32_t* __restrict__ ps, uint32_t units, int R,
                                                  int nk) {
@@ -145,7 +171,13 @@ __global__ void __launch_bounds__(256) k_mx_pack(const uint8_t* __restrict__ q, 
     __builtin_memcpy(&v, q + (row * nk + s) * kRowStep<F> + 16 * u, 16);
     if (u == 0) __builtin_memcpy(&w, sc + (row * nk + s) * 4, 4);
   }
-  ((uint4*)pq)[i] = v;
+  uint4* p = (uint4*)pq + (TWO ? i + (i / (16 * UR)) * (16 * UR) : i);
+  if constexpr (TWO) {
+    uint4 lo;
+    v = make_uint4(cut(v.x, lo.x), cut(v.y, lo.y), cut(v.z, lo.z), cut(v.w, lo.w));
+    p[kLower / 16] = lo;
+  }
+  *p = v;
   if (u == 0) ps[rs] = w;
 }
 
@@ -158,24 +190,13 @@ struct MxArgs {
   int M, N, nk, part;      // steps of K in all, and of a part
 };
 
-__device__ __forceinline__ i32x8 wide(const i32x4& v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
-// e4m3 codes of magnitude 2 and more in `hi`, those below in `lo` (bit 6 of a code
-// tells), zeros elsewhere.  v_perm fills bytes with the sign of bytes 1 and 3 of either
-// operand: of v << 9 (codes 0 and 2) and of v << 1 (1 and 3).
-__device__ __forceinline__ uint32_t cut(uint32_t v, uint32_t& lo) {
-  const uint32_t m = __builtin_amdgcn_perm(v << 1, v << 9, 0x0b090a08u);
-  lo = v & ~m;
-  return v & m;
-}
-__device__ __forceinline__ void cut(const i32x8& v, i32x8& lo, i32x8& hi) {
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    uint32_t l;
-    hi[i] = (int)cut((uint32_t)v[i], l);
-    lo[i] = (int)l;
-  }
-}
+// e4m3 activations on the tiles: one product; two parts, cut by each wavefront; or two
+// parts in memory, on tiles of 32 rows, which four wavefronts would cut again each, 7 of
+// 23 us of 201 x 3520 x 9001: cut / in memory 23.1 / 19.5, 64 x 4096 x 6144 18.5 / 14.7 (64
+// x 64 tiles 18.8 / 20.3, 128 x 128 30.3 / 29.1).
+enum { kOne, kCuts, kParts };
 
+__device__ __forceinline__ i32x8 wide(const i32x4& v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
 // Outputs of a wavefront, 32 TM x 32 TN, through its part of LDS in rows, so that
 // a store instruction writes whole runs of a row.  The weights are the products'
 // left operand: lane (c, kh) holds row m = c and columns 8 q + 4 kh .. + 3 of a 32 x
@@ -255,11 +276,12 @@ __device__ __forceinline__ int xcd_run(int i, int total) {
 // e4m3 activations 187, in two parts 290.  From registers the unit reaches 7.7: the clock falls to 1.9 GHz, the
 // fill of LDS alone takes two thirds of the time (17 TB/s out of L2), its reads and the
 // products as long each.  Small tiles are bound by that fill: 201 x 3520 x 9001 with e4m3
-// 14.6 us, 176 MB (in two parts 21).
-template <int F, int DT, bool X, int WM, int WN, int TM, int TN, int NS, int OCC>
+// 14.6 us, 176 MB.
+template <int F, int DT, int X, int WM, int WN, int TM, int TN, int NS, int OCC>
 __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(OCC, OCC))) k_mx_gemm(MxArgs a) {
   constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN, NW = WM * WN, RB = kRowStep<F>;
-  constexpr int CA = BM * RB / 1024, CB = BN * 64 / 1024, NL = (CA + CB + NW - 1) / NW;  // load instructions
+  constexpr int PA = X == kParts ? 2 : 1, CA = PA * BM * RB / 1024, CB = BN * 64 / 1024;  // parts of a; chunks of 1 KiB
+  constexpr int NL = (CA + CB + NW - 1) / NW;                                           // load instructions
   constexpr int SAR = BM < 64 ? 64 : BM, SL = ((SAR + BN) / 64 + NW - 1) / NW;           // and of scales
   constexpr int SO = NL * NW * 1024, ST = SO + SL * NW * 256;  // offset of the scales; bytes of a step
   typedef MxOut<DT, TM, TN> Out;
@@ -275,7 +297,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
   const int m0 = tile_m * BM, n0 = tile_n * BN;
   // groups of 16 rows past the end lie past the buffers: zeros
   const int gm = min(BM, a.M - m0 + 15) / 16, gn = min(BN, a.N - n0 + 15) / 16;
-  const ub_u32x4 ra = ub_desc(a.a + (size_t)(m0 / 16) * nk * 16 * RB, (uint64_t)gm * nk * 16 * RB);
+  const ub_u32x4 ra = ub_desc(a.a + (size_t)(m0 / 16) * nk * 16 * RB * PA, (uint64_t)gm * nk * 16 * RB * PA);
   const ub_u32x4 rb = ub_desc(a.w + (size_t)(n0 / 16) * nk * 1024, (uint64_t)gn * nk * 1024);
   const ub_u32x4 rsa = ub_desc(a.sa + (size_t)(m0 / 16) * nk * 16, (uint64_t)gm * nk * 64);
   const ub_u32x4 rsb = ub_desc(a.sw + (size_t)(n0 / 16) * nk * 16, (uint64_t)gn * nk * 64);
@@ -285,9 +307,10 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
   for (int i = 0; i < NL; i++) {
     const int c = i * NW + wave;  // chunk of 1 KiB: A's, then the weight's, then none
     const int r4 = lane >> 2, u4 = (lane & 3) ^ ((r4 >> 2) & 3);
-    if (c < CA && F == MX_FP8) {
-      const int r = 8 * (c & 1) + (lane >> 3), u = (lane & 7) ^ ((r >> 1) & 7);
-      v[i] = (uint32_t)(c >> 1) * nk * 2048 + r * 128 + u * 16;
+    if (c < CA && F == MX_FP8) {  // (in LDS all rows' higher parts, then the lower)
+      const int p = c * PA / CA, cr = c - p * (CA / PA);
+      const int r = 8 * (cr & 1) + (lane >> 3), u = (lane & 7) ^ ((r >> 1) & 7);
+      v[i] = (uint32_t)(cr >> 1) * nk * 2048 * PA + p * kLower + r * 128 + u * 16;
     } else {
       v[i] = c < CA + CB ? (uint32_t)(c < CA ? c : c - CA) * nk * 1024 + r4 * 64 + u4 * 16 : kDmaOOB;
     }
@@ -301,7 +324,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
 #pragma unroll
     for (int i = 0; i < NL; i++) {
       const int c = i * NW + wave;
-      ub_lds_load16_at(c < CA ? ra : rb, base + off + c * 1024, v[i], (uint32_t)k * (c < CA ? 16 * RB : 1024));
+      ub_lds_load16_at(c < CA ? ra : rb, base + off + c * 1024, v[i], (uint32_t)k * (c < CA ? 16 * RB * PA : 1024));
     }
 #pragma unroll
     for (int i = 0; i < SL; i++) {
@@ -318,6 +341,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
       for (int r = 0; r < 16; r++) acc[i][j][r] = 0.f;
   const int l32 = lane & 31, kh = lane >> 5;
   i32x4 wf[2][TN], af[2][TM], ag[2][TM];  // (ag: the second half of e4m3)
+  i32x4 lf[X == kParts ? 2 : 1][TM], lg[X == kParts ? 2 : 1][TM];  // (of the lower parts)
   uint32_t sw[TN], sa[TM], sw2[TN], sa2[TM];
   auto read_frags = [&](uint32_t off, auto J) {
     constexpr int j = decltype(J)::value;
@@ -335,6 +359,10 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
       for (int m = 0; m < TM; m++) {
         af[j][m] = *(const i32x4*)(pa + m * 32 * 128 + u0);
         ag[j][m] = *(const i32x4*)(pa + m * 32 * 128 + u1);
+        if constexpr (X == kParts) {
+          lf[j][m] = *(const i32x4*)(pa + CA * 512 + m * 32 * 128 + u0);
+          lg[j][m] = *(const i32x4*)(pa + CA * 512 + m * 32 * 128 + u1);
+        }
       }
     }
   };
@@ -361,11 +389,12 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
       if constexpr (F == MX_FP4) return wide(af[j][m]);
       else return __builtin_shufflevector(af[j][m], ag[j][m], 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    if constexpr (X) {
+    if constexpr (X != kOne) {
 #pragma unroll
       for (int m = 0; m < TM; m++) {  // (cut once for all columns)
         i32x8 lo, hi;
-        cut(act(m), lo, hi);
+        if constexpr (X == kCuts) cut(act(m), lo, hi);
+        else lo = __builtin_shufflevector(lf[j][m], lg[j][m], 0, 1, 2, 3, 4, 5, 6, 7), hi = act(m);
 #pragma unroll
         for (int n = 0; n < TN; n++) add(m, n, lo);
 #pragma unroll
@@ -666,12 +695,15 @@ void dec(const MxDecArgs& a, hipStream_t s) {
 }
 
 // ------------------------------------------------------------- the choice
+// (two: the codes in parts, packed)
 template <int F, int DT>
-void quantize(const void* x, uint8_t* q, uint8_t* sc, int R, int C, int nk, bool packed, hipStream_t s) {
+void quantize(const void* x, uint8_t* q, uint8_t* sc, int R, int C, int nk, bool packed, bool two, hipStream_t s) {
   const uint32_t units = (uint32_t)((int64_t)R * nk * (128 / MxElem<DT>::E));
   const unsigned g = (units + 511) / 512;
-  if (packed) k_mx_quant<DT, F, true><<<g, 256, 0, s>>>(x, q, sc, units, C, nk);
-  else k_mx_quant<DT, F, false><<<g, 256, 0, s>>>(x, q, sc, units, C, nk);
+  if constexpr (F == MX_FP8)
+    if (two) return k_mx_quant<DT, F, true, true><<<g, 256, 0, s>>>(x, q, sc, units, C, nk);
+  if (packed) k_mx_quant<DT, F, true, false><<<g, 256, 0, s>>>(x, q, sc, units, C, nk);
+  else k_mx_quant<DT, F, false, false><<<g, 256, 0, s>>>(x, q, sc, units, C, nk);
 }
 
 // The tile and the number of K parts that take least, by measured times (0.01 us): a
@@ -683,15 +715,15 @@ void quantize(const void* x, uint8_t* q, uint8_t* sc, int R, int C, int nk, bool
 // 14.0), 512 x 4096 x 4096 23.5 / 13.9 / 12.1 / 13.6 (31 / 17 / 14.8 / 15.7), 1646 x 5413 x 4856
 // 35 / 27 / 41 / -, 1024 x 4096 x 14336 42 / 46 / 58 / 80 (55 / 75 / 78 / 91); 160 x 10304 x 436
 // in 8 parts 8.6 on the last two.  e4m3 in two parts, the call with codes that are there,
-// on the same tiles: 64 x 4096 x 6144 - / 31 / 19 / 19, 201 x 3520 x 9001 52 / 30 / 29 / 24, 512 x
-// 4096 x 4096 56 / 34 / 28 / 27, 1646 x 5413 x 4856 80 / 86 / 102 / -, 1024 x 4096 x 14336 89 / 120 /
+// on the same tiles: 64 x 4096 x 6144 - / 30 / 19 / 15, 201 x 3520 x 9001 52 / 31 / 29 / 19.5, 512 x
+// 4096 x 4096 55 / 33 / 28 / 23, 1646 x 5413 x 4856 80 / 86 / 102 / -, 1024 x 4096 x 14336 89 / 120 /
 // 127 / -.
 struct Plan { int tile, parts; };
 Plan plan_for(int F, bool X, int M, int N, int nk) {
   static const struct { int m, n, tile, one[3], each[3]; } t[4] = {{128, 256, 390, {63, 75, 124}, {50, 70, 122}},
                                                                    {128, 128, 150, {25, 38, 63}, {28, 51, 78}},
                                                                    {64, 64, 60, {17, 22, 37}, {12, 16, 26}},
-                                                                   {32, 128, 60, {20, 22, 37}, {15, 18, 28}}};
+                                                                   {32, 128, 60, {20, 22, 28}, {15, 18, 22}}};
   const int f = F == MX_FP4 ? 0 : X ? 2 : 1;
   Plan best = {-1, 1};
   double least = 0;
@@ -708,12 +740,12 @@ Plan plan_for(int F, bool X, int M, int N, int nk) {
   return best;
 }
 
-template <int F, int DT, bool X>
+template <int F, int DT, int X>
 void gemm(int tile, const MxArgs& a, int parts, hipStream_t s) {
 #define UB_MX(WM, WN, TM, TN, NS, OCC)                                                                   \
   {                                                                                                      \
     constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN, NW = WM * WN;                                    \
-    constexpr int nl = (BM * kRowStep<F> / 1024 + BN / 16 + NW - 1) / NW, sl = (((BM < 64 ? 64 : BM) + BN) / 64 + NW - 1) / NW; \
+    constexpr int nl = (BM * kRowStep<F> / 1024 * (X == kParts ? 2 : 1) + BN / 16 + NW - 1) / NW, sl = (((BM < 64 ? 64 : BM) + BN) / 64 + NW - 1) / NW; \
     constexpr int lds = NS * NW * (nl * 1024 + sl * 256);                                                \
     static UbLdsLimit limit;                                                                             \
     limit.raise((const void*)k_mx_gemm<F, DT, X, WM, WN, TM, TN, NS, OCC>, lds);                            \
@@ -722,14 +754,18 @@ void gemm(int tile, const MxArgs& a, int parts, hipStream_t s) {
     return;                                                                                              \
   }
   // rings as deep as leaves two workgroups of the large tiles to a CU, four of the small
-  if (tile == 0) UB_MX(2, 2, 2, 4, (F == MX_FP4 ? 3 : 2), 2)
-  if constexpr (X) {
-    if (tile == 1) UB_MX(4, 2, 1, 2, 3, 2)
+  if constexpr (X == kParts) {
+    UB_MX(1, 4, 1, 1, 3, 3)
   } else {
-    if (tile == 1) UB_MX(2, 4, 2, 1, 3, (F == MX_FP4 ? 4 : 2))
+    if (tile == 0) UB_MX(2, 2, 2, 4, (F == MX_FP4 ? 3 : 2), 2)
+    if constexpr (X == kCuts) {
+      if (tile == 1) UB_MX(4, 2, 1, 2, 3, 2)
+    } else {
+      if (tile == 1) UB_MX(2, 4, 2, 1, 3, (F == MX_FP4 ? 4 : 2))
+    }
+    if (tile == 2) UB_MX(2, 2, 1, 1, (F == MX_FP4 ? 4 : 3), 4)
+    if constexpr (X == kOne) UB_MX(1, 4, 1, 1, (F == MX_FP4 ? 6 : 5), 4)
   }
-  if (tile == 2) UB_MX(2, 2, 1, 1, (F == MX_FP4 ? 4 : 3), 4)
-  UB_MX(1, 4, 1, 1, (F == MX_FP4 ? 6 : 5), 4)
 #undef UB_MX
 }
 
@@ -749,7 +785,7 @@ int linear(const char* nm, const UbridgeMxLinearArgs& p, hipStream_t s) {
     if (p.x) {
       uint8_t* q = (uint8_t*)ws.get();
       if (!q) return ub_set_error(UB_ERR_LAUNCH, "%s: no workspace", nm);
-      quantize<F, DT>(p.x, q, q + codes, M, p.K, nk, false, s);
+      quantize<F, DT>(p.x, q, q + codes, M, p.K, nk, false, false, s);
       d.x = nullptr, d.q = q, d.qs = q + codes;
     }
     dec<F, DT, true>(d, s);
@@ -760,24 +796,29 @@ int linear(const char* nm, const UbridgeMxLinearArgs& p, hipStream_t s) {
   const bool exact = X && (DT == UB_F32 || M <= 16 || !p.one_product);
   const Plan plan = plan_for(F, exact, M, N, nk);
   const int part = ub_cdiv(nk, plan.parts), parts = ub_cdiv(nk, part);  // (none empty)
-  const size_t rows = (size_t)ub_cdiv(M, 16) * 16, codes = rows * nk * kRowStep<F>, words = rows * nk * 4;
+  const bool two = exact && plan.tile == 3;
+  const size_t rows = (size_t)ub_cdiv(M, 16) * 16, codes = rows * nk * kRowStep<F> * (two ? 2 : 1), words = rows * nk * 4;
   const size_t sums = parts > 1 ? sizeof(float) * parts * (size_t)M * N : 0;
   UbScratch ws(s, codes + words + sums, true);
   uint8_t* q = (uint8_t*)ws.get();
   if (!q) return ub_set_error(UB_ERR_LAUNCH, "%s: no workspace", nm);
   uint8_t* qs = q + codes;
   if (p.x) {
-    quantize<F, DT>(p.x, q, qs, M, p.K, nk, true, s);
+    quantize<F, DT>(p.x, q, qs, M, p.K, nk, true, two, s);
   } else {
-    const uint32_t units = (uint32_t)(rows * nk * (kRowStep<F> / 16));
-    k_mx_pack<F><<<(units + 255) / 256, 256, 0, s>>>((const uint8_t*)p.codes, (const uint8_t*)p.scales, q, (uint32_t*)qs, units, M, nk);
+    const uint32_t units = (uint32_t)(rows * nk * (kRowStep<F> / 16)), g = (units + 255) / 256;
+    const uint8_t *c = (const uint8_t*)p.codes, *cs = (const uint8_t*)p.scales;
+    if (two) k_mx_pack<F, F == MX_FP8><<<g, 256, 0, s>>>(c, cs, q, (uint32_t*)qs, units, M, nk);
+    else k_mx_pack<F><<<g, 256, 0, s>>>(c, cs, q, (uint32_t*)qs, units, M, nk);
   }
   MxArgs a = {q, w, (const uint32_t*)qs, sw, p.bias, p.y, M, N, nk, part};
   auto product = [&](auto dt, int np) {
     constexpr int D = decltype(dt)::value;
-    if constexpr (X && DT == UB_F32) gemm<F, D, true>(plan.tile, a, np, s);
-    else if (exact) gemm<F, D, X>(plan.tile, a, np, s);
-    else gemm<F, D, false>(plan.tile, a, np, s);
+    if constexpr (X) {
+      if (two) return gemm<F, D, kParts>(plan.tile, a, np, s);
+      if (exact) return gemm<F, D, kCuts>(plan.tile, a, np, s);
+    }
+    if constexpr (!X || DT != UB_F32) gemm<F, D, kOne>(plan.tile, a, np, s);
   };
   if (parts > 1) {
     a.y = qs + words;
@@ -813,9 +854,9 @@ UB_API int ubridge_mx_quantize(const void* x, int dtype, void* codes, void* scal
   uint8_t *q = (uint8_t*)codes, *sc = (uint8_t*)scales;
   auto go = [&](auto f) {
     constexpr int F = decltype(f)::value;
-    if (dtype == UB_F32) quantize<F, UB_F32>(x, q, sc, R, C, nk, false, s);
-    else if (dtype == UB_F16) quantize<F, UB_F16>(x, q, sc, R, C, nk, false, s);
-    else quantize<F, UB_BF16>(x, q, sc, R, C, nk, false, s);
+    if (dtype == UB_F32) quantize<F, UB_F32>(x, q, sc, R, C, nk, false, false, s);
+    else if (dtype == UB_F16) quantize<F, UB_F16>(x, q, sc, R, C, nk, false, false, s);
+    else quantize<F, UB_BF16>(x, q, sc, R, C, nk, false, false, s);
   };
   if (format == MX_FP4) go(std::integral_constant<int, MX_FP4>{});
   else go(std::integral_constant<int, MX_FP8>{});
