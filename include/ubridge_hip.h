@@ -589,7 +589,7 @@ int ubridge_int8_linear_codes(const int8_t* a, const float* sa, const int8_t* w,
  * T(sum over the experts of weight * (w2 a)).  w13 [E, 2 I, H] and w2 [E, H, I] of type T
  * (dtype 1 f16, 2 bf16), or int8 with scales s13 [E, 2 I] and s2 [E, H] of type T
  * (else NULL).  H and I are multiples of 32, x, w13 and w2 16-byte aligned, k <= 16,
- * E <= 1024.  y overlaps no input.  Scratch: 4 T k I bytes and 9 KiB. */
+ * E <= 1024.  y overlaps no input.  Scratch: 4 T k I bytes and 16 KiB. */
 typedef struct {
   const void *x, *logits, *w13, *s13, *w2, *s2;
   void* y;

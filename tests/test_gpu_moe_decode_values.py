@@ -80,3 +80,13 @@ def test_infinite_results_stay_with_their_token(dev):
     assert torch.equal(got[keep], clean[keep])
     y = check(x[keep], lg[keep], layer, got[keep])
     assert y.shape == (5, 128) and bool(torch.isinf(got[3]).any()) and not bool(torch.isnan(got[3]).any())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("q8", [True, False])
+@pytest.mark.parametrize("T,E,k,H,I", [(16, 6, 3, 2560, 96), (13, 3, 1, 4096, 160), (16, 16, 16, 2080, 32), (1, 8, 8, 4096, 224),
+                                       (16, 2, 1, 7168, 32), (9, 64, 8, 2592, 96), (16, 4, 4, 5120, 64), (16, 1, 1, 4096, 32)])
+def test_wide_results(dev, T, E, k, H, I, q8, dtype):
+    # on both sides of where a workgroup takes 16 columns and 8 tokens of one expert
+    x, lg, layer = make(dev, T, E, k, H, I, dtype, q8)
+    check(x, lg, layer, layer.decode(x, lg))

@@ -20,11 +20,11 @@
 //    call, against a launch).  An item is 8 columns of an expert: 8 gate rows and their 8
 //    up rows are the 16 rows of one product.  Groups of 8 or 16 wavefronts take the items
 //    in turn and split K, each one run of its rows, two items in flight.
-//  * k_down: a workgroup owns 8 output columns and adds all experts' parts, so no sums
-//    cross workgroups.  8 rows of each of two experts are the 16 rows of a product, and
-//    up to 4 tokens of the one and 4 of the other its columns, both parts of a each (an
-//    expert with more is listed again); the two quarters where rows and tokens belong
-//    together are kept.
+//  * k_down: a workgroup owns 8 or 16 output columns and adds all experts' parts, so no
+//    sums cross workgroups.  16 rows of an expert are the rows of a product, both parts of
+//    up to 8 tokens' a its columns (an expert with more is listed again).  Or, while there
+//    are too few columns to give every CU 16, 8 rows of each of two experts, and up to 4
+//    tokens of either: the two quarters where rows and tokens belong together are kept.
 //  * Scales are asked for ahead of the weights that they go with: loads return in order,
 //    and one asked for at the end of an item would wait for all weights in flight.
 // Measured, k_up + k_down: 16 tokens, 8 of 128 int8 experts of 2048 x 768 52 + 31 us (4.9 and
@@ -44,25 +44,24 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTok = 16, kK = 16, kE = 1024, kUsed = kTok * kK;  // most tokens, top-k, experts; experts in use
-// tokens of an entry of the list below, and entries (at most one a token and expert)
-constexpr int kPer = 4, kEnt = kUsed;
+constexpr int kEnt = kUsed;  // entries of the list below: at most one a token and expert
 
-// The routing, in scratch memory from k_up to k_down: experts in use, each with up to
-// kPer of its tokens (more: another entry): rows of the activations (t k + j; -1: none),
-// tokens and weights.
+// The routing, in scratch memory from k_up to k_down: experts in use, each with up to 4 or
+// 8 (`per`) of its tokens (more: another entry): rows of the activations (t k + j; -1:
+// none), tokens and weights, `per` to an entry.
 struct Route {
   int n, pad[3];
   int expert[kEnt];
-  int16_t row[kEnt][kPer];
-  int8_t tok[kEnt][kPer];
-  float w[kEnt][kPer];
+  int16_t row[kEnt * 8];
+  int8_t tok[kEnt * 8];
+  float w[kEnt * 8];
 };
 
 struct DecodeArgs {
   const void *x, *logits, *w13, *s13, *w2, *s2;
-  void *y, *act;  // act: bf16 [2][T k][I], a rounded and the rest
+  void *y, *act;  // act: bf16 [T k][I / 8][2][8], a rounded and the rest
   Route* route;
-  int T, E, k, H, I, ldt, norm;
+  int T, E, k, H, I, ldt, norm, per;
 };
 
 template <int DT>
@@ -221,8 +220,7 @@ __global__ void __launch_bounds__(1024) k_up(DecodeArgs a) {
       }
       const uint64_t one = __ballot(bits != 0), below = (1ull << lane) - 1;
       int ahead = 0, all = 0;  // entries of the lanes below, and of all
-#pragma unroll
-      for (int q = 0; q < kTok; q += kPer) {
+      for (int q = 0; q < kTok; q += a.per) {
         const uint64_t more = __ballot(__popc(bits) > q);
         ahead += __popcll(more & below);
         all += __popcll(more);
@@ -242,16 +240,17 @@ __global__ void __launch_bounds__(1024) k_up(DecodeArgs a) {
   const int nu = __builtin_amdgcn_readfirstlane(nused);
   if (first) {
     if (tid == 0) a.route->n = nent;
-    for (int i = tid; i < nu * 16; i += NT) {
-      const int u = i >> 4, p = i & 15, e = used[u], bits = tokens[u], n = __popc(bits), at = entry[u] + p / kPer, i4 = p % kPer;
-      if (p >= (n + kPer - 1) / kPer * kPer) continue;
+    for (int l = tid; l < nu * 16; l += NT) {
+      const int u = l >> 4, p = l & 15, e = used[u], bits = tokens[u], n = __popc(bits), at = entry[u] + p / a.per;
+      if (p >= (n + a.per - 1) / a.per * a.per) continue;
       int b = bits;  // the p-th token of the expert
       for (int q = 0; q < p; q++) b &= b - 1;
       const int t = b ? __builtin_ctz(b) : -1, j = t >= 0 ? slot[e][t] : 0;
+      const int i = at * a.per + p % a.per;
       a.route->expert[at] = e;
-      a.route->row[at][i4] = (int16_t)(t >= 0 ? t * a.k + j : -1);
-      a.route->tok[at][i4] = (int8_t)t;
-      a.route->w[at][i4] = t >= 0 ? wts[t][j] : 0.f;
+      a.route->row[i] = (int16_t)(t >= 0 ? t * a.k + j : -1);
+      a.route->tok[i] = (int8_t)t;
+      a.route->w[i] = t >= 0 ? wts[t][j] : 0.f;
     }
   }
   // ---- items
@@ -325,9 +324,9 @@ __global__ void __launch_bounds__(1024) k_up(DecodeArgs a) {
         const float v = g / (1.f + expf(-g)) * up;
         const uint16_t hi = ub_f32_to_bf16(v);
         const float f = ub_bf16_to_f32(hi);
-        uint16_t* at = (uint16_t*)a.act + ((size_t)ot * a.k + j) * I + col;
+        uint16_t* at = (uint16_t*)a.act + (((size_t)ot * a.k + j) * I + (col & ~7)) * 2 + (col & 7);
         at[0] = hi;
-        at[(size_t)T * a.k * I] = ub_f32_to_bf16(__builtin_isinf(f) ? 0.f : v - f);
+        at[8] = ub_f32_to_bf16(__builtin_isinf(f) ? 0.f : v - f);
       }
     }
     if constexpr (NB == 1) {  // (two of them by turns need no second barrier)
@@ -349,25 +348,27 @@ __global__ void __launch_bounds__(1024) k_up(DecodeArgs a) {
   }
 }
 
-template <int DT, bool Q8, int W2>
+// NC output columns a workgroup: 16 of one expert, or 8 of each of two (above).
+constexpr int W2 = 8;  // wavefronts
+template <int DT, bool Q8, int NC>
 __global__ void __launch_bounds__(64 * W2) __attribute__((amdgpu_waves_per_eu(4, 4))) k_down(DecodeArgs a, int most) {
   constexpr int WB = Q8 ? 1 : 2, XN = Q8 ? 2 : 1, P = 4;  // P: steps of a unit
+  constexpr int PER = NC / 2, SIDES = 16 / NC;            // tokens of an entry, entries of a unit
   __shared__ int expert[kEnt];
-  __shared__ int16_t row[kEnt][kPer];
-  __shared__ int8_t tok[kEnt][kPer];
-  __shared__ float wts[kEnt][kPer], sc[kEnt][8];
-  __shared__ float ys[W2][kTok][8];  // a wavefront's sums
+  __shared__ int16_t row[kEnt * PER];
+  __shared__ int8_t tok[kEnt * PER];
+  __shared__ float wts[kEnt * PER], sc[kEnt * NC];
+  __shared__ float ys[W2][kTok][NC];  // a wavefront's sums
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, h = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int T = a.T, H = a.H, I = a.I, n0 = blockIdx.x * 8;
+  const int T = a.T, H = a.H, I = a.I, n0 = blockIdx.x * NC;
   const int n = a.route->n;
-  // units: P 64-byte steps of the rows of a pair of entries, dealt out in turn, so that
+  // units: P 64-byte steps of the rows of an entry, or a pair, dealt out in turn, so that
   // all workgroups walk through the experts together
-  const int rowb = I * WB, per = ((rowb + 63) / 64 + P - 1) / P, units = (n + 1) / 2 * per;
-  // columns 0-3 of a side are the first parts of its tokens, 4-7 the second, backwards (so
-  // that the two are a half row's mirror images)
-  const int side = r >> 3, c8 = r & 7, rest = c8 >> 2, c4 = rest ? 7 - c8 : c8;
-  const uint16_t* act = (const uint16_t*)a.act + (rest ? (size_t)T * a.k * I : 0);
+  const int rowb = I * WB, per = ((rowb + 63) / 64 + P - 1) / P, units = (n + SIDES - 1) / SIDES * per;
+  // the first half of a side's columns are the first parts of its tokens, the other half
+  // the second, backwards (so that the two are mirror images in a row of lanes, or half one)
+  const int side = r / NC, c = r % NC, rest = c / PER, ct = rest ? NC - 1 - c : c;
   struct Set {
     uint4 w[P], x[P][XN];
   };
@@ -375,12 +376,13 @@ __global__ void __launch_bounds__(64 * W2) __attribute__((amdgpu_waves_per_eu(4,
   // itself, not from LDS, which is being filled meanwhile.
   auto load = [&](Set& b, int q, auto first) {
     constexpr bool FIRST = decltype(first)::value;
-    const int p = q / per, u = 2 * p + side, at0 = (q - p * per) * (64 * P) + 16 * h;
+    const int p = q / per, u = SIDES * p + side, at0 = (q - p * per) * (64 * P) + 16 * h;
     const bool any = q < units && u < n;
     int ar = -1, e = 0;
-    if (any) ar = FIRST ? a.route->row[u][c4] : row[u][c4], e = FIRST ? a.route->expert[u] : expert[u];
-    const uint8_t* pw = (const uint8_t*)a.w2 + ((size_t)e * H + n0 + c8) * rowb + at0;
-    const uint16_t* px = act + (size_t)max(ar, 0) * I + at0 / WB;
+    if (any) ar = FIRST ? a.route->row[u * PER + ct] : row[u * PER + ct], e = FIRST ? a.route->expert[u] : expert[u];
+    const uint8_t* pw = (const uint8_t*)a.w2 + ((size_t)e * H + n0 + c) * rowb + at0;
+    // (bytes: at most 256 rows of 2^20 values)
+    const uint32_t px = (uint32_t)max(ar, 0) * I * 4 + at0 / WB * 4 + 16 * rest;
 #pragma unroll
     for (int i = 0; i < P; i++) {
       b.w[i] = make_uint4(0, 0, 0, 0);
@@ -390,32 +392,31 @@ __global__ void __launch_bounds__(64 * W2) __attribute__((amdgpu_waves_per_eu(4,
         b.w[i] = ld16(pw + 64 * i);
         if (ar >= 0) {
 #pragma unroll
-          for (int v = 0; v < XN; v++) b.x[i][v] = *(const uint4*)(px + 64 * i / WB + 8 * v);
+          for (int v = 0; v < XN; v++) b.x[i][v] = *(const uint4*)((const uint8_t*)a.act + px + (64 * i / WB + 8 * v) * 4);
         }
       }
     }
   };
-  // Unit q's products, to the sums.  Lane (column r, h): rows 4 h .. + 3, which belong to
-  // r's entry if both are of the same half.  The two entries may share a token: one after
-  // the other.
+  // Unit q's products, to the sums.  Lane (column r, h): rows 4 h .. + 3, of two entries
+  // r's own if both are of the same half.  The two may share a token: one after the other.
   auto mul = [&](Set& b, int q) {
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < P; i++) acc = product_bf16<DT, Q8>(b.w[i], b.x[i], acc);
     load(b, q + 2 * W2, std::false_type{});
-    const int u = 2 * (q / per) + side;
-    const bool mine = u < n && (h >> 1) == side && !rest && row[u][c4] >= 0;
+    const int u = SIDES * (q / per) + side, at = u * PER + ct, out = (4 * h) % NC;
+    const bool mine = u < n && (SIDES == 1 || (h >> 1) == side) && !rest && row[at] >= 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {  // the other part of the token's (row_half_mirror)
+    for (int i = 0; i < 4; i++) {  // the other part of the token's (row_mirror, row_half_mirror)
       const float v = acc[i];
-      acc[i] = v + __uint_as_float(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x141, 0xf, 0xf, false));
+      acc[i] = v + __uint_as_float(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), NC == 16 ? 0x140 : 0x141, 0xf, 0xf, false));
     }
 #pragma unroll
-    for (int s = 0; s < 2; s++) {
+    for (int s = 0; s < SIDES; s++) {
       if (mine && side == s) {
-        float* y = &ys[wave][tok[u][c4]][4 * (h & 1)];
+        float* y = &ys[wave][tok[at]][out];
 #pragma unroll
-        for (int i = 0; i < 4; i++) y[i] += acc[i] * (Q8 ? wts[u][c4] * sc[u][4 * (h & 1) + i] : wts[u][c4]);
+        for (int i = 0; i < 4; i++) y[i] += acc[i] * (Q8 ? wts[at] * sc[u * NC + out + i] : wts[at]);
       }
       __builtin_amdgcn_wave_barrier();
       asm volatile("" ::: "memory");
@@ -423,30 +424,30 @@ __global__ void __launch_bounds__(64 * W2) __attribute__((amdgpu_waves_per_eu(4,
   };
   Set b0, b1;
   // (entries past n, up to what there can be, are read with the others and not used)
-  for (int i = tid; i < most * kPer; i += 64 * W2) {
-    (&row[0][0])[i] = (&a.route->row[0][0])[i];
-    (&tok[0][0])[i] = (&a.route->tok[0][0])[i];
-    (&wts[0][0])[i] = (&a.route->w[0][0])[i];
-    if (i % kPer == 0) expert[i / kPer] = a.route->expert[i / kPer];
+  for (int i = tid; i < most * PER; i += 64 * W2) {
+    row[i] = a.route->row[i];
+    tok[i] = a.route->tok[i];
+    wts[i] = a.route->w[i];
+    if (i % PER == 0) expert[i / PER] = a.route->expert[i / PER];
   }
   load(b0, wave, std::true_type{});
   load(b1, wave + W2, std::true_type{});
   if constexpr (Q8)
-    for (int i = tid; i < n * 8; i += 64 * W2)
-      sc[i >> 3][i & 7] = ub_load<DT>(a.s2, (size_t)a.route->expert[i >> 3] * H + n0 + (i & 7));
-  for (int i = tid; i < W2 * kTok * 8; i += 64 * W2) (&ys[0][0][0])[i] = 0.f;
+    for (int i = tid; i < n * NC; i += 64 * W2)
+      sc[i] = ub_load<DT>(a.s2, (size_t)a.route->expert[i / NC] * H + n0 + i % NC);
+  for (int i = tid; i < W2 * kTok * NC; i += 64 * W2) (&ys[0][0][0])[i] = 0.f;
   __syncthreads();
   for (int q = wave; q < units; q += 2 * W2) {
     mul(b0, q);
     if (q + W2 < units) mul(b1, q + W2);
   }
   __syncthreads();
-  if (tid < 8 * T) {
-    const int t = tid >> 3, c = tid & 7;
+  if (tid < NC * T) {
+    const int t = tid / NC, o = tid % NC;
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < W2; w++) v += ys[w][t][c];
-    ub_store<DT>(a.y, (size_t)t * H + n0 + c, v);
+    for (int w = 0; w < W2; w++) v += ys[w][t][o];
+    ub_store<DT>(a.y, (size_t)t * H + n0 + o, v);
   }
 }
 
@@ -485,18 +486,23 @@ void up(const DecodeArgs& a, hipStream_t s) {
   go(four, multi, two, one);
 }
 template <int DT, bool Q8>
-void decode(const DecodeArgs& a, hipStream_t s) {
+void decode(DecodeArgs a, hipStream_t s) {
+  // 16 columns a workgroup, unless that gives some CU more than 8 would.  us of the layer, 8 /
+  // 16 columns, E 64, k 8, I 512, one token bf16 (16 int8): 2048 16.8 / 18.8 (47 / 56), 2560 20.8 /
+  // 20.8 (68 / 64), 4096 - (88 / 81), 5120 30.2 / 30.6, 6144 32.8 / 32.8 (146 / 148), 7168 37.7 /
+  // 35.3 (173 / 161); 16 tokens, 2 of 8 experts, 4096 x 1024 bf16 47.9 / 41.4, 4096 x 4096 int8 111 /
+  // 94.  8 wavefronts: 4 or 16 are up to 10% slower where workgroups and CUs are as many, 4
+  // up to 6% faster for one token where workgroups are many.
+  const int narrow = ub_cdiv(a.H / 8, 256), wides = 2 * ub_cdiv(a.H / 16, 256);
+  const bool wide = wides <= narrow;
+  a.per = wide ? 8 : 4;
   if (a.E <= 128) up<DT, Q8, 2>(a, s);
   else if (a.E <= 256) up<DT, Q8, 4>(a, s);
   else up<DT, Q8, kE / 64>(a, s);
-  // entries, at most: one an expert in use, another for each kPer tokens past the first kPer
-  const int slots = a.T * a.k, used = std::min(slots, a.E), most = used + (slots - used) / kPer;
-  // 16 wavefronts while every workgroup has a CU of its own; else 4, four workgroups to a
-  // CU: no round waits for the start and end of the one before it.  us of the layer, E 64, k 8,
-  // one token, 16 / 4 wavefronts, bf16 (int8): 2048 x 768 23.6 / 25.0 (18.5 / 19.5), 7168 x 512
-  // 48.2 / 40.4 (39.5 / 31.9), 16 tokens, 4096 x 512 142 / 135 (87.7 / 84.9).
-  if (a.H / 8 <= 256) k_down<DT, Q8, 16><<<a.H / 8, 64 * 16, 0, s>>>(a, most);
-  else k_down<DT, Q8, 4><<<a.H / 8, 64 * 4, 0, s>>>(a, most);
+  // entries, at most: one an expert in use, another for each `per` tokens past the first
+  const int slots = a.T * a.k, used = std::min(slots, a.E), most = used + (slots - used) / a.per;
+  if (wide) k_down<DT, Q8, 16><<<a.H / 16, 64 * W2, 0, s>>>(a, most);
+  else k_down<DT, Q8, 8><<<a.H / 8, 64 * W2, 0, s>>>(a, most);
 }
 
 }  // namespace
