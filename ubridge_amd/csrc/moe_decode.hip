@@ -27,9 +27,9 @@
 //    tokens of either: the two quarters where rows and tokens belong together are kept.
 //  * Scales are asked for ahead of the weights that they go with: loads return in order,
 //    and one asked for at the end of an item would wait for all weights in flight.
-// Measured, k_up + k_down: 16 tokens, 8 of 128 int8 experts of 2048 x 768 52 + 31 us (4.9 and
-// 4.1 TB/s), 5 tokens, 6 of 64 f16 ones of 2048 x 1408 53 + 30 (5.3, 4.9), one token of the
-// former 11 + 6.
+// Measured (medians), k_up + k_down: 16 tokens, 8 of 128 int8 experts of 2048 x 768 57 + 37 us
+// (4.5 and 3.5 TB/s), 5 tokens, 6 of 64 f16 ones of 2048 x 1408 55 + 34 (5.2, 4.2), one token
+// of the former 12 + 7.
 #include "lds_dma.h"
 #include "moe_dev.h"
 #include "wave.h"

@@ -272,8 +272,8 @@ __device__ __forceinline__ int xcd_run(int i, int total) {
 // block, bytes 16 kh .. of blocks j and 2 + j), and its scale is byte j of the row's
 // word shifted by 16 kh.  Fragments are in registers, two sets: those of one
 // product are read while the other's multiply.
-// Measured, e2m1 x e2m1, 4096 x 4096 x 14336 (M K N): 141 us, 3.4 PFLOP/s (3.9 at 8192^3); with
-// e4m3 activations 187, in two parts 290.  From registers the unit reaches 7.7: the clock falls to 1.9 GHz, the
+// Measured, e2m1 x e2m1, 4096 x 4096 x 14336 (M K N): 141 us at best, 3.4 PFLOP/s (3.9 at 8192^3),
+// among other work up to 171; with e4m3 activations 187, in two parts 290.  From registers the unit reaches 7.7: the clock falls to 1.9 GHz, the
 // fill of LDS alone takes two thirds of the time (17 TB/s out of L2), its reads and the
 // products as long each.  Small tiles are bound by that fill: 201 x 3520 x 9001 with e4m3
 // 14.6 us, 176 MB.
@@ -473,8 +473,8 @@ __global__ void __launch_bounds__(256) k_mx_sum(const float* __restrict__ part, 
 // for the banks); each workgroup makes them itself while its first weights are on their
 // way, up to kRound values; beyond, a launch of its own makes them once.  The wavefronts'
 // sums meet in LDS in their order.
-// HBM bounds it where the weight is large, launch and first latency else.  us of codes that
-// are there, e2m1 / e4m3 (M x K x N): 1 x 14336 x 4096 7.5 / 8.2 (31 MB, 4 TB/s), 8 x 4096 x 28672
+// HBM bounds it where the weight is large, launch and first latency else.  us of a call
+// among others with codes that are there, e2m1 / e4m3 (M x K x N): 1 x 14336 x 4096 7.5 / 8.2 (31 MB, 4 TB/s), 8 x 4096 x 28672
 // 11.0 / 11.5 (64 MB, 5.8 TB/s), 16 x 4096 x 28672 11.4 / 13.6 (one product alone 11.8).
 constexpr int DW = 16, RP = 20;  // wavefronts; floats of a token's row of sums
 

@@ -17,8 +17,8 @@
 //
 // Bound by HBM for many rows, by one launch's latency for few.  A row stays in the
 // registers of the workgroup (or, short, of the wavefront) that owns it: x and
-// residual are read once, h and y written once.  us: 8 x 4096 with residual to e4m3 4.2;
-// 8192 x 4096 bf16 with residual 51 (5.2 TB/s), its gradient 52 + 4 (5.2 TB/s); 2047 x
+// residual are read once, h and y written once.  us: 8 x 4096 with residual to e4m3 4.4;
+// 8192 x 4096 bf16 with residual 51 (5.2 TB/s), its gradient 51 + 4 (5.2 TB/s); 2047 x
 // 5003 f16 from odd places, f32 gain, 12.4.
 #include "mx_dev.h"
 #include "wave.h"
