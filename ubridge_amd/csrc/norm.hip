@@ -93,7 +93,7 @@ __device__ __forceinline__ float scale_of(uint32_t top, float most) {
 // v / s, correctly rounded: v r (r = 1 / s) corrected twice by its exact residual
 // (Markstein's division), 5 operations where the IEEE divide takes 11
 // (bf16 with residual, 2048 x 4096 to e4m3: 15.4 us, with the divide 16.5).  PLAIN, the divide:
-// for s outside [2^-60, 2^60], where residuals underflow.
+// for s outside [2^-60, 2^60], where residuals underflow.  (A zero comes out as +0.)
 template <bool PLAIN>
 __device__ __forceinline__ float quotient(float v, float s, float r) {
   if constexpr (PLAIN) return __fdiv_rn(v, s);
@@ -101,13 +101,16 @@ __device__ __forceinline__ float quotient(float v, float s, float r) {
   q = __builtin_fmaf(__builtin_fmaf(-q, s, v), r, q);
   return __builtin_fmaf(__builtin_fmaf(-q, s, v), r, q);
 }
-// Codes of four values, int8 or e4m3.
+// Codes of four values, int8 or e4m3 (whose zeros keep their sign, as in blocks and in
+// ubridge_fp8_quantize_rows).
 template <bool PLAIN, bool I8>
 __device__ __forceinline__ uint32_t codes4(const float* v, float s, float r) {
   float q[4];
 #pragma unroll
-  for (int e = 0; e < 4; e++)
+  for (int e = 0; e < 4; e++) {
     q[e] = __builtin_amdgcn_fmed3f(quotient<PLAIN>(v[e], s, r), I8 ? -127.f : -448.f, I8 ? 127.f : 448.f);
+    if constexpr (!I8 && !PLAIN) q[e] = copysignf(q[e], v[e]);
+  }
   if constexpr (I8) {
     uint32_t o = 0;
 #pragma unroll
