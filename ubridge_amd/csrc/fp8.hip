@@ -20,6 +20,7 @@
 // K-step ahead, between the MFMAs.
 #include "common.h"
 #include "lds_dma.h"
+#include "quotient.h"
 
 #include <type_traits>
 
@@ -488,13 +489,9 @@ __global__ void __launch_bounds__(256) k_quant_rows_fp8(const void* __restrict__
 // keeps NV 16-byte units of the row in registers (all loads in flight at
 // once, the row read once), the amax is a wave shuffle and one LDS exchange,
 // and a unit's codes leave as one 8- (16-bit x) or 4-byte (f32) store.
-// The quotient is x * (1/s) corrected twice by its exact residual
-// x - q s (Markstein's division: with 1/s correctly rounded, the second
-// correction of an already faithful q gives the correctly rounded x / s), 5
-// operations instead of the ~11 of the IEEE divide, with the sign of x put
-// back for zeros.  A quotient below 2^-11 gives code 0 whatever its last bits,
-// and for s in [2^-60, 2^60] the residuals of larger ones do not underflow;
-// rows with another s (also inf) divide.
+// The quotient is ub_quotient's, with the sign of x put back for zeros.  One below
+// 2^-11 gives code 0 whatever its last bits, and for s in [2^-60, 2^60] the
+// residuals of larger ones do not underflow; rows with another s (also inf) divide.
 // HBM-bound at many rows, latency-bound at few (hence 1024 threads there).
 // bf16 rows of 8192, us, one element per lane / this form: 1 row 31.9 / 2.6,
 // 16 rows 37.6 / 2.9, 1024 rows 67 / 5.3, 4096 rows 76 / 17.3 (5.8 TB/s); f32
@@ -548,14 +545,9 @@ __global__ void __launch_bounds__(NT) k_quant_rows_fp8_v(const uint4* __restrict
       else ((int2*)q)[row + i] = make_int2(o[0], o[1]);
     }
   };
-  if (s >= 0x1p-60f && s <= 0x1p60f) {  // uniform over the row
+  if (ub_exact_scale(s)) {  // uniform over the row
     const float r = __fdiv_rn(1.0f, s);
-    store([&](float v) {
-      float d = v * r;
-      d = __builtin_fmaf(__builtin_fmaf(-d, s, v), r, d);
-      d = __builtin_fmaf(__builtin_fmaf(-d, s, v), r, d);
-      return copysignf(d, v);
-    });
+    store([&](float v) { return copysignf(ub_quotient(v, s, r), v); });
   } else {
     store([&](float v) { return __fdiv_rn(v, s); });
   }

@@ -22,6 +22,7 @@
 // operands of zeros the call takes 0.7 of the time.
 #include "common.h"
 #include "lds_dma.h"
+#include "quotient.h"
 
 #include <type_traits>
 
@@ -67,12 +68,9 @@ __device__ __forceinline__ float scale_of(uint32_t top) {
   return top >= 0x7f800000u ? __builtin_nanf("") : top == 0 ? 1.0f : __fdiv_rn(__uint_as_float(top), 127.0f);
 }
 
-// The code of v under scale s, in the low byte.  The quotient is v r (r = 1 / s)
-// corrected twice by its exact residual v - q s (Markstein's division: the
-// second correction gives the correctly rounded v / s), 5 operations where the
-// IEEE divide takes 11.  Adding 1.5 2^23 rounds to an integer, ties to even, in
-// the low bits.  PLAIN, for s outside [2^-60, 2^60], where residuals underflow:
-// the divide; and a clamp, since |v / s| <= 127 but for a denormal s, whose own
+// The code of v under scale s, in the low byte.  Adding 1.5 2^23 rounds to an integer,
+// ties to even, in the low bits.  PLAIN, for s out of ub_quotient's range: the
+// divide; and a clamp, since |v / s| <= 127 but for a denormal s, whose own
 // rounding is as large as s.  A NaN or zero s has codes 0.
 template <bool PLAIN>
 __device__ __forceinline__ uint32_t code(float v, float s, float r) {
@@ -81,9 +79,7 @@ __device__ __forceinline__ uint32_t code(float v, float s, float r) {
     q = __fdiv_rn(v, s);
     q = q == q ? fminf(fmaxf(q, -127.f), 127.f) : 0.f;
   } else {
-    q = v * r;
-    q = __builtin_fmaf(__builtin_fmaf(-q, s, v), r, q);
-    q = __builtin_fmaf(__builtin_fmaf(-q, s, v), r, q);
+    q = ub_quotient(v, s, r);
   }
   return __float_as_uint(q + 12582912.f);
 }
@@ -101,7 +97,7 @@ __device__ __forceinline__ void codes(const uint4& u, float s, float r, uint32_t
 }
 // (the same in every lane, as s is)
 __device__ __forceinline__ bool plain_scale(float s) {
-  return __builtin_amdgcn_readfirstlane(!(s >= 0x1p-60f && s <= 0x1p60f));
+  return __builtin_amdgcn_readfirstlane(!ub_exact_scale(s));
 }
 
 // One workgroup of NT threads a row; a thread keeps NV units of it in registers,
@@ -227,13 +223,6 @@ struct Epilogue {
   }
 };
 
-// Workgroup i runs on XCD i % 8: its place in an order of `total` of which every
-// XCD, each with its own L2, takes one contiguous run.
-__device__ __forceinline__ int xcd_run(int i, int total) {
-  const int x = i % 8;
-  return x * (total / 8) + min(x, total % 8) + i / 8;
-}
-
 // WM x WN wavefronts of 32 TM x 32 TN outputs each, v_mfma_i32_32x32x32_i8.  The
 // operands reach LDS by direct loads in a ring of NS 64-byte K-steps, each row of
 // 64 bytes swizzled in 16-byte units (unit u of row r at u ^ ((r >> 2) & 3)) so
@@ -356,7 +345,7 @@ k_i8_gemm(const int8_t* __restrict__ A, const float* __restrict__ sa, const int8
   const int b = (int)blockIdx.x;
   int tile_m, tile_n;
   if (TM == 1 || b < full) {
-    ub_tile_at(xcd_run(b, full), 0, tm, tn, 8, tile_m, tile_n);
+    ub_tile_at(ub_xcd_run(b, full), 0, tm, tn, 8, tile_m, tile_n);
     i8_tile<DT, WM, WN, TM, TN, NS>(A, sa, B, sw, bias, y, M, N, ld, tile_m * BM, tile_n * BN, lds);
   } else if constexpr (TM > 1) {
     ub_tile_at(full + ((b - full) >> 1), 0, tm, tn, 8, tile_m, tile_n);
@@ -385,7 +374,7 @@ k_i8_ring(const int8_t* __restrict__ A, const float* __restrict__ sa, const int8
   const int wm = wave / WN, wn = wave % WN;
   int tile_m, tile_n;
   const int tm = (M + BM - 1) / BM, tn = (N + BN - 1) / BN;
-  const int id = xcd_run((int)blockIdx.x, (int)gridDim.x), kp = id / (tm * tn);  // part kp of K
+  const int id = ub_xcd_run((int)blockIdx.x, (int)gridDim.x), kp = id / (tm * tn);  // part kp of K
   ub_tile_at(id - kp * tm * tn, 0, tm, tn, 8, tile_m, tile_n);
   // rows and columns even over the tiles: what a tile does not need, it does not
   // load (rows past the end lie past the buffers: zeros)

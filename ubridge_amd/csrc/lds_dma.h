@@ -122,6 +122,12 @@ __device__ __forceinline__ void ub_barrier() {
 // itself walks groups of `gm` tile rows column by column, so the tiles
 // resident at one time share a few A row-panels and B column-panels
 // instead of sweeping whole rows of B.
+// ub_xcd_run: workgroup i's place in an order of `total` of which every XCD takes one
+// contiguous run, for any total.
+__device__ __forceinline__ int ub_xcd_run(int i, int total) {
+  const int x = i % 8;
+  return x * (total / 8) + min(x, total % 8) + i / 8;
+}
 // ub_tile_at: tile number `pid` of that order, after the regrouping of `dealt`
 // tiles (0: none, the caller's own).
 __device__ __forceinline__ void ub_tile_at(int pid, int dealt, int tm, int tn, int gm, int& im, int& in_) {

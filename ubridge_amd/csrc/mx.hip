@@ -256,13 +256,6 @@ struct MxOut {
   }
 };
 
-// Workgroup i runs on XCD i % 8: its place in an order of `total` of which every
-// XCD, each with its own L2, takes one contiguous run.
-__device__ __forceinline__ int xcd_run(int i, int total) {
-  const int x = i % 8;
-  return x * (total / 8) + min(x, total % 8) + i / 8;
-}
-
 // WM x WN wavefronts of 32 TM x 32 TN outputs, 128 elements of K a step.  Codes and
 // scale words reach LDS by direct loads into a ring of NS steps, NS - 1 in flight.
 // A row's step is 4 (e4m3: 8) units of 16 bytes, unit u of row r at u ^ ((r >> 2) &
@@ -292,7 +285,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
   const int wm = wave / WN, wn = wave % WN, nk = a.nk;
   int tile_m, tile_n;
   const int tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN;
-  const int id = xcd_run((int)blockIdx.x, (int)gridDim.x), kp = id / (tm * tn);  // part kp of K
+  const int id = ub_xcd_run((int)blockIdx.x, (int)gridDim.x), kp = id / (tm * tn);  // part kp of K
   ub_tile_at(id - kp * tm * tn, 0, tm, tn, 8, tile_m, tile_n);
   const int m0 = tile_m * BM, n0 = tile_n * BN;
   // groups of 16 rows past the end lie past the buffers: zeros

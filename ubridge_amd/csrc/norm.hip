@@ -21,6 +21,7 @@
 // 8192 x 4096 bf16 with residual 51 (5.2 TB/s), its gradient 51 + 4 (5.2 TB/s); 2047 x
 // 5003 f16 from odd places, f32 gain, 12.4.
 #include "mx_dev.h"
+#include "quotient.h"
 #include "wave.h"
 
 #include <type_traits>
@@ -90,25 +91,16 @@ __device__ __forceinline__ float scale_of(uint32_t top, float most) {
   if (top == 0) return 1.f;
   return fmaxf(__fdiv_rn(__uint_as_float(top), most), 0x1p-149f);
 }
-// v / s, correctly rounded: v r (r = 1 / s) corrected twice by its exact residual
-// (Markstein's division), 5 operations where the IEEE divide takes 11
-// (bf16 with residual, 2048 x 4096 to e4m3: 15.4 us, with the divide 16.5).  PLAIN, the divide:
-// for s outside [2^-60, 2^60], where residuals underflow.  (A zero comes out as +0.)
-template <bool PLAIN>
-__device__ __forceinline__ float quotient(float v, float s, float r) {
-  if constexpr (PLAIN) return __fdiv_rn(v, s);
-  float q = v * r;
-  q = __builtin_fmaf(__builtin_fmaf(-q, s, v), r, q);
-  return __builtin_fmaf(__builtin_fmaf(-q, s, v), r, q);
-}
 // Codes of four values, int8 or e4m3 (whose zeros keep their sign, as in blocks and in
-// ubridge_fp8_quantize_rows).
+// ubridge_fp8_quantize_rows).  PLAIN: s is out of ub_quotient's range (bf16 with residual,
+// 2048 x 4096 to e4m3: 15.4 us, with the divide for every row 16.5).
 template <bool PLAIN, bool I8>
 __device__ __forceinline__ uint32_t codes4(const float* v, float s, float r) {
   float q[4];
 #pragma unroll
   for (int e = 0; e < 4; e++) {
-    q[e] = __builtin_amdgcn_fmed3f(quotient<PLAIN>(v[e], s, r), I8 ? -127.f : -448.f, I8 ? 127.f : 448.f);
+    q[e] = PLAIN ? __fdiv_rn(v[e], s) : ub_quotient(v[e], s, r);
+    q[e] = __builtin_amdgcn_fmed3f(q[e], I8 ? -127.f : -448.f, I8 ? 127.f : 448.f);
     if constexpr (!I8 && !PLAIN) q[e] = copysignf(q[e], v[e]);
   }
   if constexpr (I8) {
@@ -189,7 +181,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) k_norm(NormArgs a) {
     if (tid == 0) ((float*)a.scale)[row] = s;
     uint8_t* q = (uint8_t*)a.y + row * C;
     // (the same in a wavefront, whose lanes have one row)
-    const bool none = __builtin_amdgcn_readfirstlane(s != s), plain = __builtin_amdgcn_readfirstlane(!(s >= 0x1p-60f && s <= 0x1p60f));
+    const bool none = __builtin_amdgcn_readfirstlane(s != s), plain = __builtin_amdgcn_readfirstlane(!ub_exact_scale(s));
     const float rs = plain ? 0.f : __fdiv_rn(1.f, s);
     auto all = [&](auto pl, auto i) {
 #pragma unroll
@@ -386,6 +378,12 @@ void norm(const NormArgs& a, hipStream_t s) {
 
 constexpr int kGradGroups = 512;  // workgroups, at most: dw's partial sums stay small beside the rows
 
+// Threads a row: 256 up to 4 units each.  us of the call with dx and dw, bf16 with dh, on 64 / 128 /
+// 256 / 512 / 1024 threads: 65536 x 128 192 / 221 / 224 / 280 / 549, 8192 x 512 21 / 26 / 26 / 38 / 75, 1024
+// 29 / 28 / 28 / 38 / 75, 2048 40 / 36 / 31 / 39 / 74, 4096 - / 59 / 51 / 52 / 78, 8192 - / - / 107 / 111
+// / 111; 4096 x 16384 - / - / - / 119 / 116; 64 x 8192 - / - / 9.4 / 8.7 / 9.1; f32 8192 x 4096 - / - / 102 /
+// 105 / 108.  (Rows under 1024 values would take 15-20% less on a wavefront each, and are far
+// from HBM's time either way.)
 template <int DT>
 void norm_grad(const NormGradArgs& a, int groups, hipStream_t s) {
   const int units = ub_cdiv(a.C, MxElem<DT>::E);
